@@ -12,12 +12,12 @@
 //    mask words (4 words per request); active tile ids are compacted per
 //    builder block of kBuilderTiles tiles. Skipped in dense mode.
 //  * tc_projection_kernel: one persistent CTA per SM, 10 warps.
-//      warp 0      one lane issues TMA loads of the W tile (128 rows x 64 K,
-//                  128-byte swizzle) and of h (Npad rows x 64 K) into a ring of
-//                  shared-memory stages;
+//      warp 0      one lane issues TMA loads of the W tile (128 rows x 128 bytes
+//                  of K, 128-byte swizzle) and of h (Npad rows x 128 bytes) into
+//                  a ring of shared-memory stages;
 //      warp 1      allocates TMEM; one lane issues tcgen05.mma (M=128 vocabulary
-//                  rows, N = batch padded to a multiple of 32, K = 16 per
-//                  instruction) into one of 4 TMEM accumulators (2 when
+//                  rows, N = batch padded to a multiple of 32, 32 bytes of K per
+//                  instruction: kind::f16, or kind::i8 for int8 operands) into one of 4 TMEM accumulators (2 when
 //                  N > 128), committing each stage back to the producer and
 //                  each tile to the epilogue;
 //      warps 2-9   epilogue, two warps per TMEM lane quadrant splitting the
@@ -42,6 +42,13 @@
 //
 // Every wait is bounded; a timed-out wait sets the workspace error word and the
 // kernel drains its copies and tensor-core work before returning.
+//
+// T is __half or __nv_bfloat16 (operands and logits of one type), or
+// Int8Rows<Out>: int8 operands accumulated exactly in int32 TMEM columns, the
+// epilogue applying the request's and the vocabulary row's scale. Each
+// including source instantiates launch_block_gemm_typed for its types.
+#pragma once
+
 #include <cuda.h>
 
 #include <algorithm>
@@ -59,7 +66,7 @@ namespace gsp {
 namespace {
 
 constexpr int kTileRows = 128;
-constexpr int kTileK = 64;  // K elements per stage: one 128-byte swizzle row
+constexpr int kTileKBytes = 128;  // K bytes per stage: one swizzle row (64 half-precision, 128 int8 elements)
 constexpr int kEpilogueWarps = 8;  // two per TMEM lane quadrant
 constexpr int kGemmThreads = 32 * (2 + kEpilogueWarps);
 constexpr int kMaxNpad = 256;
@@ -67,12 +74,12 @@ constexpr int kMaxAcc = 4;          // TMEM accumulators (4 when npad <= 128, el
 constexpr int kMaxUnits = kMaxNpad / 64;  // 32-column units per epilogue warp
 constexpr int kMaxStages = 8;
 constexpr int kMaxMine = 64;  // tiles per CTA that the set-up can list in shared memory
-constexpr uint32_t kABytes = kTileRows * kTileK * 2;  // 16 KB
+constexpr uint32_t kABytes = kTileRows * kTileKBytes;  // 16 KB
 
 struct GemmConfig {
   int npad;      // batch padded to a multiple of 32 (<= 256)
   int stages;
-  int kblocks;   // ceil(H / 64)
+  int kblocks;   // ceil(K bytes of a row / 128)
   int ntiles;    // ceil(V / 128)
   int nbuild;    // builder blocks (block mode)
   int acc_shift; // log2 of the accumulator count
@@ -93,14 +100,14 @@ __host__ __device__ inline GemmLayout gemm_layout(int npad, int stages, int nbui
   l.a = off;
   off += (size_t)stages * kABytes;
   l.b = align_to(off, 1024);
-  off = l.b + (size_t)stages * npad * kTileK * 2;
+  off = l.b + (size_t)stages * npad * kTileKBytes;
   l.bars = align_to(off, 16);
   off = l.bars + 8 * (2 * (size_t)stages + 2 * kMaxAcc);
   l.tmem = align_to(off, 16);
   off = l.tmem + 16;
   l.keys = align_to(off, 16);
   off = l.keys + 8 * (size_t)kMaxNpad;
-  l.skeys = align_to(off, 16);  // sampler: the CTA's winning perturbed key per request
+  l.skeys = align_to(off, 16);  // sampler: the CTA's winning perturbed key per request; int8: the requests' scales
   off = l.skeys + 8 * (size_t)kMaxNpad;
   l.stats = align_to(off, 16);  // sampler: the CTA's (max, sum) pair per request
   off = l.stats + 8 * (size_t)kMaxNpad;
@@ -140,9 +147,11 @@ template <typename T>
 __device__ __forceinline__ void fill_inactive_tiles(const BlockGemmParams& p, int ntiles, int cta, int G, int ew,
                                                     int lane) {
   const int V = p.vocab, nw = p.nw, B = p.batch;
-  const uint16_t ninf = DTypeTraits<T>::kNegInfBits;
-  const uint32_t x = (uint32_t)ninf | ((uint32_t)ninf << 16);
-  const bool vec_ok = ((reinterpret_cast<uintptr_t>(p.logits) & 15) == 0) && (p.logits_stride % 8 == 0);
+  using OutBits = typename DTypeTraits<T>::OutBits;
+  constexpr int kOutVec = 16 / (int)sizeof(OutBits);  // logits per 16-byte store
+  const OutBits ninf = DTypeTraits<T>::kNegInfBits;
+  const uint32_t x = sizeof(OutBits) == 2 ? (uint32_t)ninf | ((uint32_t)ninf << 16) : (uint32_t)ninf;
+  const bool vec_ok = ((reinterpret_cast<uintptr_t>(p.logits) & 15) == 0) && (p.logits_stride % kOutVec == 0);
   for (int t = cta + ew * G; t < ntiles; t += kEpilogueWarps * G) {
     uint32_t any = 0u;
     for (int b = lane; b < B; b += 32) {
@@ -155,11 +164,13 @@ __device__ __forceinline__ void fill_inactive_tiles(const BlockGemmParams& p, in
     }
     if (__any_sync(FULL_MASK, any != 0u)) continue;
     const int r0 = t * kTileRows;
-    uint16_t* base = static_cast<uint16_t*>(p.logits) + r0;
+    OutBits* base = static_cast<OutBits*>(p.logits) + r0;
     if (vec_ok && r0 + kTileRows <= V) {
       // 256 B per request: lanes 0-15 take request b, lanes 16-31 request b + 1
-      for (int b = lane >> 4; b < B; b += 2)
-        reinterpret_cast<uint4*>(base + (int64_t)b * p.logits_stride)[lane & 15] = make_uint4(x, x, x, x);
+      // (512 B of fp32 logits: the whole warp one request)
+      constexpr int kLanes = kTileRows / kOutVec;
+      for (int b = lane / kLanes; b < B; b += 32 / kLanes)
+        reinterpret_cast<uint4*>(base + (int64_t)b * p.logits_stride)[lane % kLanes] = make_uint4(x, x, x, x);
     } else {
       for (int b = 0; b < B; ++b)
         for (int r = lane; r < kTileRows && r0 + r < V; r += 32) base[(int64_t)b * p.logits_stride + r] = ninf;
@@ -194,6 +205,34 @@ __device__ __forceinline__ unsigned long long merge_unit_key(unsigned long long 
       top1_key(DTypeTraits<T>::bits_to_float((uint16_t)bits), (uint64_t)(row_base + (int64_t)r));
   return key > running ? key : running;
 }
+
+// Warp-local keys by logit width: 32 bits for 16-bit logits (above), 64 bits
+// (order-preserving fp32 bits, then 0xffffffff - lane) for fp32 logits.
+template <typename T>
+using WarpKey = std::conditional_t<sizeof(typename DTypeTraits<T>::OutBits) == 2, uint32_t, unsigned long long>;
+
+template <typename T>
+__device__ __forceinline__ WarpKey<T> warp_key(typename DTypeTraits<T>::OutBits bits, int lane) {
+  if constexpr (sizeof(bits) == 2)
+    return warp_key16(bits, 0xffffu - (uint32_t)lane);
+  else
+    return top1_key(__uint_as_float(bits), (uint64_t)lane);
+}
+
+template <typename T>
+__device__ __forceinline__ unsigned long long merge_warp_key(unsigned long long running, WarpKey<T> k,
+                                                             int64_t row_base) {
+  if constexpr (sizeof(WarpKey<T>) == 4) {
+    return merge_unit_key<T>(running, k, row_base);
+  } else {
+    if (k == 0ull) return running;
+    const unsigned long long key = top1_key(key_value(k), (uint64_t)(row_base + key_index(k)));
+    return key > running ? key : running;
+  }
+}
+
+__device__ __forceinline__ uint32_t shfl_xor_key(uint32_t k, int m) { return __shfl_xor_sync(FULL_MASK, k, m); }
+__device__ __forceinline__ unsigned long long shfl_xor_key(unsigned long long k, int m) { return shfl_xor_u64(k, m); }
 
 // Sampler state of one epilogue unit (kSample kernels): its requests' seeds and
 // the CTA's per-request accumulators in shared memory, all offset to the
@@ -239,40 +278,53 @@ __device__ __forceinline__ void sample_column(const UnitSampler& su, int jj, boo
   }
 }
 
+// One accumulator column's logit: the fp32 sum, or (int8 operands) the exact
+// integer sum times the request's scale times the vocabulary row's.
+template <typename T>
+__device__ __forceinline__ float column_logit(uint32_t acc, const float* s_hscale, int jj, float row_scale) {
+  if constexpr (IsInt8Rows<T>::value)
+    return __fmul_rn(__fmul_rn((float)(int)acc, s_hscale[jj]), row_scale);
+  else
+    return __uint_as_float(acc);
+}
+
 // One epilogue unit: kCols accumulator columns (requests b0 .. b0 + kCols - 1)
 // of this warp's 32 TMEM lanes (one vocabulary row per thread). Rounds to the
 // logits dtype, applies the mask bit (word_l: this lane's mask word for
 // request b0 + lane % kCols), stores the row's logits (-inf where illegal) and
-// returns in lane l < kCols the warp_key16 maximum over the 32 rows for
+// returns in lane l < kCols the warp_key maximum over the 32 rows for
 // request b0 + l. With kSample, also feeds every column to sample_column.
+// s_hscale (the unit's requests) and row_scale: int8 operands only.
 template <typename T, int kCols, bool kSample>
-__device__ __forceinline__ uint32_t epilogue_unit(uint32_t taddr, uint32_t word_l, int b0, int B, bool row_ok,
-                                                  bool store, uint16_t* out, int64_t stride, int lane,
-                                                  const UnitSampler& su) {
+__device__ __forceinline__ WarpKey<T> epilogue_unit(uint32_t taddr, uint32_t word_l, int b0, int B, bool row_ok,
+                                                    bool store, typename DTypeTraits<T>::OutBits* out, int64_t stride,
+                                                    int lane, const UnitSampler& su, const float* s_hscale,
+                                                    float row_scale) {
+  using OutBits = typename DTypeTraits<T>::OutBits;
+  using Key = WarpKey<T>;
   uint32_t v[kCols];
   if constexpr (kCols == 32) tmem_ld32(taddr, v);
   else tmem_ld16(taddr, v);
   tmem_ld_wait();
-  const uint16_t ninf = DTypeTraits<T>::kNegInfBits;
+  const OutBits ninf = DTypeTraits<T>::kNegInfBits;
   const uint32_t lanebit = row_ok ? (1u << lane) : 0u;
-  const uint32_t low = 0xffffu - (uint32_t)lane;
-  uint32_t key[kCols];
+  Key key[kCols];
   if (b0 + kCols <= B) {
 #pragma unroll
     for (int jj = 0; jj < kCols; ++jj) {
       const bool legal = (__shfl_sync(FULL_MASK, word_l, jj) & lanebit) != 0u;
-      const uint16_t bits = legal ? DTypeTraits<T>::round_bits(__uint_as_float(v[jj])) : ninf;
+      const OutBits bits = legal ? DTypeTraits<T>::round_bits(column_logit<T>(v[jj], s_hscale, jj, row_scale)) : ninf;
       if (store) out[jj * stride] = bits;
-      key[jj] = legal ? warp_key16(bits, low) : 0u;
+      key[jj] = legal ? warp_key<T>(bits, lane) : Key(0);
       if constexpr (kSample) sample_column<T>(su, jj, legal, bits);
     }
   } else {
 #pragma unroll
     for (int jj = 0; jj < kCols; ++jj) {
       const bool legal = (__shfl_sync(FULL_MASK, word_l, jj) & lanebit) != 0u;  // word is 0 past B
-      const uint16_t bits = legal ? DTypeTraits<T>::round_bits(__uint_as_float(v[jj])) : ninf;
+      const OutBits bits = legal ? DTypeTraits<T>::round_bits(column_logit<T>(v[jj], s_hscale, jj, row_scale)) : ninf;
       if (store && b0 + jj < B) out[jj * stride] = bits;
-      key[jj] = legal ? warp_key16(bits, low) : 0u;
+      key[jj] = legal ? warp_key<T>(bits, lane) : Key(0);
       if constexpr (kSample) sample_column<T>(su, jj, legal, bits);
     }
   }
@@ -283,14 +335,14 @@ __device__ __forceinline__ uint32_t epilogue_unit(uint32_t taddr, uint32_t word_
     const bool upper = (lane & h) != 0;
 #pragma unroll
     for (int j = 0; j < h; ++j) {
-      const uint32_t send = upper ? key[j] : key[j + h];
-      const uint32_t keep = upper ? key[j + h] : key[j];
-      const uint32_t recv = __shfl_xor_sync(FULL_MASK, send, h);
+      const Key send = upper ? key[j] : key[j + h];
+      const Key keep = upper ? key[j + h] : key[j];
+      const Key recv = shfl_xor_key(send, h);
       key[j] = keep > recv ? keep : recv;
     }
   }
   if constexpr (kCols == 16) {
-    const uint32_t other = __shfl_xor_sync(FULL_MASK, key[0], 16);
+    const Key other = shfl_xor_key(key[0], 16);
     key[0] = key[0] > other ? key[0] : other;
   }
   return key[0];
@@ -317,6 +369,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   unsigned long long* s_keys = reinterpret_cast<unsigned long long*>(smem + L.keys);
   unsigned long long* s_skeys = reinterpret_cast<unsigned long long*>(smem + L.skeys);
   unsigned long long* s_stats = reinterpret_cast<unsigned long long*>(smem + L.stats);
+  float* s_hscale = reinterpret_cast<float*>(smem + L.skeys);  // int8 kernels never sample
   int* s_pref = reinterpret_cast<int*>(smem + L.pref);
   int* s_mine = reinterpret_cast<int*>(smem + L.mine);
   int* s_misc = reinterpret_cast<int*>(smem + L.misc);  // [0] abort, [1] last-CTA flag
@@ -357,6 +410,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   // Everything above overlaps the tile builder; from here on its outputs (and
   // the inactive-tile -inf fill) are complete and visible.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr bool kInt8 = IsInt8Rows<T>::value;
+  constexpr int kTileK = kTileKBytes / (int)sizeof(typename DTypeTraits<T>::Bits);  // K elements per stage
+  if constexpr (kInt8) {
+    for (int i = tid; i < kMaxNpad; i += kGemmThreads) s_hscale[i] = i < B ? __ldg(p.hidden_scales + i) : 0.f;
+  }
   if (!p.dense && c.stage_list && warp != 2) {
     // The whole compacted list into shared memory, in the same round trip as
     // the counts that warp 2 reads (the A stages are idle until the
@@ -442,9 +500,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             *abort_flag = 1;
             break;
           }
-          mbar_arrive_expect_tx(full + s, kABytes + (uint32_t)c.npad * kTileK * 2u);
+          mbar_arrive_expect_tx(full + s, kABytes + (uint32_t)(c.npad * kTileKBytes));
           tma_load_2d(s_a + (size_t)s * kABytes, &tmap_w, kb * kTileK, tile * kTileRows, full + s);
-          tma_load_2d(s_b + (size_t)s * c.npad * kTileK * 2, &tmap_h, kb * kTileK, 0, full + s);
+          tma_load_2d(s_b + (size_t)s * c.npad * kTileKBytes, &tmap_h, kb * kTileK, 0, full + s);
         }
       }
       // Let every issued copy land before the CTA can exit: the stage ring is
@@ -483,10 +541,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
           tc_fence_after_sync();
           const uint64_t ad = tc_desc_sw128(s_a + (size_t)s * kABytes);
-          const uint64_t bd = tc_desc_sw128(s_b + (size_t)s * c.npad * kTileK * 2);
+          const uint64_t bd = tc_desc_sw128(s_b + (size_t)s * c.npad * kTileKBytes);
 #pragma unroll
-          for (int k = 0; k < kTileK / 16; ++k)
-            tc_mma_f16(d, ad + 2ull * k, bd + 2ull * k, c.idesc, (kb | k) != 0);
+          for (int k = 0; k < kTileKBytes / 32; ++k) {
+            if constexpr (kInt8)
+              tc_mma_i8(d, ad + 2ull * k, bd + 2ull * k, c.idesc, (kb | k) != 0);
+            else
+              tc_mma_f16(d, ad + 2ull * k, bd + 2ull * k, c.idesc, (kb | k) != 0);
+          }
           tc_commit(empty + s);  // stage s is free once these MMAs complete
           last_stage = s;
           last_use = use;
@@ -530,6 +592,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           else if (word_idx < p.nw) words[u] = __ldg(p.mask + (int64_t)b * p.mask_stride + word_idx);
         }
       }
+      float row_scale = 0.f;
+      if constexpr (kInt8) row_scale = row0 + lane < V ? __ldg(p.weight_scales + row0 + lane) : 0.f;
       const bool ok = mbar_wait(tfull + acc, ause & 1u, abort_flag);
       __syncwarp();
       if (!ok) {
@@ -541,15 +605,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const bool row_ok = row < V;
       const bool store = row_ok && p.logits != nullptr;
       const uint32_t tcol = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * c.npad);
-      uint16_t* out = static_cast<uint16_t*>(p.logits) + row;
+      typename DTypeTraits<T>::OutBits* out = static_cast<typename DTypeTraits<T>::OutBits*>(p.logits) + row;
       if constexpr (narrow) {
         const int b0 = 16 * half;
         UnitSampler su{};
         if constexpr (kSample)
           su = UnitSampler{p.seeds + b0, s_skeys + b0, s_stats + b0, p.offset, p.inv_temp, p.vocab_offset + row};
-        const uint32_t k = epilogue_unit<T, 16, kSample>(tcol + (uint32_t)b0, words[0], b0, B, row_ok, store,
-                                                 out + (int64_t)b0 * p.logits_stride, p.logits_stride, lane, su);
-        running[0] = merge_unit_key<T>(running[0], k, p.vocab_offset + row0);
+        const WarpKey<T> k = epilogue_unit<T, 16, kSample>(tcol + (uint32_t)b0, words[0], b0, B, row_ok, store,
+                                                           out + (int64_t)b0 * p.logits_stride, p.logits_stride, lane,
+                                                           su, s_hscale + b0, row_scale);
+        running[0] = merge_warp_key<T>(running[0], k, p.vocab_offset + row0);
       } else {
 #pragma unroll
         for (int u = 0; u < kMaxUnits; ++u) {
@@ -558,9 +623,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             UnitSampler su{};
             if constexpr (kSample)
               su = UnitSampler{p.seeds + b0, s_skeys + b0, s_stats + b0, p.offset, p.inv_temp, p.vocab_offset + row};
-            const uint32_t k = epilogue_unit<T, 32, kSample>(tcol + (uint32_t)b0, words[u], b0, B, row_ok, store,
-                                                     out + (int64_t)b0 * p.logits_stride, p.logits_stride, lane, su);
-            running[u] = merge_unit_key<T>(running[u], k, p.vocab_offset + row0);
+            const WarpKey<T> k = epilogue_unit<T, 32, kSample>(tcol + (uint32_t)b0, words[u], b0, B, row_ok, store,
+                                                               out + (int64_t)b0 * p.logits_stride, p.logits_stride,
+                                                               lane, su, s_hscale + b0, row_scale);
+            running[u] = merge_warp_key<T>(running[u], k, p.vocab_offset + row0);
           }
         }
       }
@@ -720,18 +786,26 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// 2-D K-major tensor map [rows, H] with a (64 x box_rows) box and 128-byte swizzle.
-bool make_map(CUtensorMap* map, const void* base, int bf16, uint64_t rows, uint64_t cols, uint64_t row_stride_elems,
+template <typename T>
+constexpr CUtensorMapDataType tensor_map_type() {
+  if (std::is_same<T, __half>::value) return CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (std::is_same<T, __nv_bfloat16>::value) return CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return CU_TENSOR_MAP_DATA_TYPE_UINT8;
+}
+
+// 2-D K-major tensor map [rows, H] with a (128 bytes x box_rows) box and 128-byte swizzle.
+template <typename T>
+bool make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t row_stride_elems,
               uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
+  constexpr int kSize = (int)sizeof(typename DTypeTraits<T>::Bits);
   const cuuint64_t dims[2] = {cols, rows};
-  const cuuint64_t strides[1] = {row_stride_elems * 2};
-  const cuuint32_t box[2] = {(cuuint32_t)kTileK, box_rows};
+  const cuuint64_t strides[1] = {row_stride_elems * kSize};
+  const cuuint32_t box[2] = {(cuuint32_t)(kTileKBytes / kSize), box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  return fn(map, tensor_map_type<T>(), 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -742,10 +816,22 @@ int smem_optin(int dev) {
   return v;
 }
 
+// GSP_DTYPE_* code of an Int8Rows type's logits.
+template <typename T>
+struct Int8OutCode;
+template <>
+struct Int8OutCode<Int8Rows<__half>> { static constexpr int value = 0; };
+template <>
+struct Int8OutCode<Int8Rows<__nv_bfloat16>> { static constexpr int value = 1; };
+template <>
+struct Int8OutCode<Int8Rows<float>> { static constexpr int value = 2; };
+
 template <typename T>
 cudaError_t launch_chunk(const BlockGemmParams& p, int dev, cudaStream_t stream) {
   GemmConfig c;
   c.npad = ((p.batch + 31) / 32) * 32;
+  constexpr bool kInt8 = IsInt8Rows<T>::value;
+  constexpr int kTileK = kTileKBytes / (int)sizeof(typename DTypeTraits<T>::Bits);
   c.kblocks = (p.hidden_dim + kTileK - 1) / kTileK;
   c.ntiles = (p.vocab + kTileRows - 1) / kTileRows;
   c.nbuild = (c.ntiles + kBuilderTiles - 1) / kBuilderTiles;
@@ -755,9 +841,10 @@ cudaError_t launch_chunk(const BlockGemmParams& p, int dev, cudaStream_t stream)
   uint32_t cols = 32;
   while (cols < ((uint32_t)c.npad << c.acc_shift)) cols <<= 1;
   c.tmem_cols = cols;
-  c.idesc = tc_idesc_f16((uint32_t)c.npad, sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value);
+  c.idesc = kInt8 ? tc_idesc_i8((uint32_t)c.npad)
+                  : tc_idesc_f16((uint32_t)c.npad, std::is_same<T, __nv_bfloat16>::value);
   c.stage_list = 0;
-  const size_t stage_bytes = kABytes + (size_t)c.npad * kTileK * 2;
+  const size_t stage_bytes = kABytes + (size_t)c.npad * kTileKBytes;
   const size_t fixed = gemm_layout(c.npad, 0, c.nbuild).total + 1024 + 2048;
   c.stages = (int)std::min<size_t>(kMaxStages, ((size_t)smem_optin(dev) - fixed) / stage_bytes);
   if (c.stages < 2) return cudaErrorInvalidConfiguration;
@@ -766,11 +853,10 @@ cudaError_t launch_chunk(const BlockGemmParams& p, int dev, cudaStream_t stream)
   // the whole list fits the A stages and each CTA's share fits s_mine
   c.stage_list = (size_t)c.ntiles * 4 <= (size_t)c.stages * kABytes && (c.ntiles + G - 1) / G <= kMaxMine;
 
-  const int bf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   CUtensorMap tw, th;
-  if (!make_map(&tw, p.weight, bf16, (uint64_t)p.vocab, (uint64_t)p.hidden_dim, (uint64_t)p.weight_stride, kTileRows) ||
-      !make_map(&th, p.hidden, bf16, (uint64_t)p.batch, (uint64_t)p.hidden_dim, (uint64_t)p.hidden_stride,
-                (uint32_t)c.npad))
+  if (!make_map<T>(&tw, p.weight, (uint64_t)p.vocab, (uint64_t)p.hidden_dim, (uint64_t)p.weight_stride, kTileRows) ||
+      !make_map<T>(&th, p.hidden, (uint64_t)p.batch, (uint64_t)p.hidden_dim, (uint64_t)p.hidden_stride,
+                   (uint32_t)c.npad))
     return cudaErrorInvalidValue;
 
   cudaError_t err;
@@ -779,8 +865,12 @@ cudaError_t launch_chunk(const BlockGemmParams& p, int dev, cudaStream_t stream)
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
   }
   const bool sample = p.sample_index != nullptr;
-  auto k = c.npad == 32 ? (sample ? tc_projection_kernel<T, true, true> : tc_projection_kernel<T, true, false>)
-                        : (sample ? tc_projection_kernel<T, false, true> : tc_projection_kernel<T, false, false>);
+  auto k = tc_projection_kernel<T, true, false>;
+  if constexpr (kInt8)  // the sampler takes half-precision operands only
+    k = c.npad == 32 ? tc_projection_kernel<T, true, false> : tc_projection_kernel<T, false, false>;
+  else
+    k = c.npad == 32 ? (sample ? tc_projection_kernel<T, true, true> : tc_projection_kernel<T, true, false>)
+                     : (sample ? tc_projection_kernel<T, false, true> : tc_projection_kernel<T, false, false>);
   const size_t smem_bytes = L.total + 1024;
   if ((err = raise_smem_limit(reinterpret_cast<const void*>(k), smem_bytes, dev)) != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
@@ -797,15 +887,16 @@ cudaError_t launch_chunk(const BlockGemmParams& p, int dev, cudaStream_t stream)
 }
 
 template <typename T>
-cudaError_t launch_typed(const BlockGemmParams& p0, cudaStream_t stream) {
+cudaError_t launch_block_gemm_typed(const BlockGemmParams& p0, cudaStream_t stream) {
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   // TMA needs 16-byte aligned bases and row pitches; otherwise the row-sparse
   // kernel computes the same outputs (every legal row, -inf elsewhere).
-  const bool tma_ok = (p0.hidden_dim % 8 == 0) && ((reinterpret_cast<uintptr_t>(p0.weight) & 15) == 0) &&
-                      (p0.weight_stride % 8 == 0) && ((reinterpret_cast<uintptr_t>(p0.hidden) & 15) == 0) &&
-                      (p0.batch == 1 || p0.hidden_stride % 8 == 0);
+  constexpr int kPV = DTypeTraits<T>::kPerVec;
+  const bool tma_ok = (p0.hidden_dim % kPV == 0) && ((reinterpret_cast<uintptr_t>(p0.weight) & 15) == 0) &&
+                      (p0.weight_stride % kPV == 0) && ((reinterpret_cast<uintptr_t>(p0.hidden) & 15) == 0) &&
+                      (p0.batch == 1 || p0.hidden_stride % kPV == 0);
   if (!tma_ok) {
     RowSparseParams r{};
     r.hidden = p0.hidden;
@@ -836,16 +927,23 @@ cudaError_t launch_typed(const BlockGemmParams& p0, cudaStream_t stream) {
     r.inv_temp = p0.inv_temp;
     r.sample_keys = p0.sample_keys;
     r.stat_partials = p0.stat_partials;
-    return launch_row_sparse(r, std::is_same<T, __nv_bfloat16>::value ? 1 : 0, stream);
+    if constexpr (IsInt8Rows<T>::value) {
+      r.hidden_scales = p0.hidden_scales;
+      r.weight_scales = p0.weight_scales;
+      return launch_row_sparse_int8(r, Int8OutCode<T>::value, stream);
+    } else {
+      return launch_row_sparse(r, std::is_same<T, __nv_bfloat16>::value ? 1 : 0, stream);
+    }
   }
   // Batches above kMaxNpad run as consecutive chunks of requests.
   for (int b0 = 0; b0 < p0.batch; b0 += kMaxNpad) {
     BlockGemmParams p = p0;
     const int nb = std::min(kMaxNpad, p0.batch - b0);
     p.batch = nb;
-    p.hidden = static_cast<const uint16_t*>(p0.hidden) + (int64_t)b0 * p0.hidden_stride;
+    p.hidden = static_cast<const typename DTypeTraits<T>::Bits*>(p0.hidden) + (int64_t)b0 * p0.hidden_stride;
+    if (IsInt8Rows<T>::value) p.hidden_scales = p0.hidden_scales + b0;
     if (p0.mask) p.mask = p0.mask + (int64_t)b0 * p0.mask_stride;
-    if (p0.logits) p.logits = static_cast<uint16_t*>(p0.logits) + (int64_t)b0 * p0.logits_stride;
+    if (p0.logits) p.logits = static_cast<typename DTypeTraits<T>::OutBits*>(p0.logits) + (int64_t)b0 * p0.logits_stride;
     if (p0.top_value) p.top_value = p0.top_value + b0;
     if (p0.top_index) p.top_index = p0.top_index + b0;
     if (p0.top_key) p.top_key = p0.top_key + b0;
@@ -865,10 +963,4 @@ cudaError_t launch_typed(const BlockGemmParams& p0, cudaStream_t stream) {
 }
 
 }  // namespace
-
-cudaError_t launch_block_gemm(const BlockGemmParams& p, int dtype, cudaStream_t stream) {
-  if (dtype == 1) return launch_typed<__nv_bfloat16>(p, stream);
-  return launch_typed<__half>(p, stream);
-}
-
 }  // namespace gsp

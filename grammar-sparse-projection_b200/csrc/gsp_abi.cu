@@ -883,4 +883,188 @@ int32_t gsp_grouped_logits(const void* hidden, int64_t hidden_row_stride, const 
   return GSP_OK;
 }
 
+// ---- int8 head --------------------------------------------------------------
+namespace {
+
+constexpr int32_t kMaxInt8Hidden = 131071;  // 128 * 128 * 131071 < 2^31: the integer sums cannot overflow
+
+size_t int8_row_bytes(int32_t hidden_dim) { return ((size_t)hidden_dim + 15) / 16 * 16; }
+
+// The step's hidden states as int8 rows with scales: the caller's own, or
+// quantised into the scratch buffer ([batch] rows of int8_row_bytes, then
+// [batch] scales). Everything is checked before anything is queued.
+struct Int8Hidden {
+  const int8_t* values;
+  int64_t stride;
+  const float* scales;
+};
+
+int32_t validate_int8(const char* fn, const void* hidden, int64_t hidden_row_stride, int32_t hidden_dtype,
+                      const float* hidden_scales, const int8_t* weight, int64_t weight_row_stride,
+                      const float* weight_scales, const int32_t* bitmask, int64_t bitmask_row_stride, int32_t batch,
+                      int32_t vocab, int32_t hidden_dim, int32_t out_dtype, const void* logits,
+                      int64_t logits_row_stride, const void* scratch, size_t scratch_bytes) {
+  int32_t st = validate_projection(fn, hidden, hidden_row_stride, weight, weight_row_stride, bitmask,
+                                   bitmask_row_stride, batch, vocab, hidden_dim, out_dtype, logits,
+                                   logits_row_stride);
+  if (st != GSP_OK) return st;
+  if (!weight_scales) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: weight_scales is required", fn);
+  if (hidden_dim > kMaxInt8Hidden)
+    return fail(GSP_ERR_UNSUPPORTED, "%s: hidden_dim above %d could overflow the int32 sums", fn, kMaxInt8Hidden);
+  if (hidden_dtype == GSP_DTYPE_I8) {
+    if (!hidden_scales) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: int8 hidden states need hidden_scales", fn);
+    return GSP_OK;
+  }
+  if (hidden_dtype != GSP_DTYPE_F16 && hidden_dtype != GSP_DTYPE_BF16 && hidden_dtype != GSP_DTYPE_F32)
+    return fail(GSP_ERR_UNSUPPORTED, "%s: unknown hidden_dtype %d", fn, hidden_dtype);
+  if (!scratch || scratch_bytes < gsp_int8_scratch_bytes(batch, hidden_dim))
+    return fail(GSP_ERR_WORKSPACE, "%s: scratch has %zu bytes, needs %zu", fn, scratch ? scratch_bytes : (size_t)0,
+                gsp_int8_scratch_bytes(batch, hidden_dim));
+  if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0)
+    return fail(GSP_ERR_WORKSPACE, "%s: scratch must be 16-byte aligned", fn);
+  return GSP_OK;
+}
+
+int32_t int8_hidden(const char* fn, const void* hidden, int64_t hidden_row_stride, int32_t hidden_dtype,
+                    const float* hidden_scales, int32_t batch, int32_t hidden_dim, void* scratch, void* stream,
+                    Int8Hidden* out) {
+  if (hidden_dtype == GSP_DTYPE_I8) {
+    *out = Int8Hidden{static_cast<const int8_t*>(hidden), hidden_row_stride, hidden_scales};
+    return GSP_OK;
+  }
+  int8_t* values = static_cast<int8_t*>(scratch);
+  const int64_t stride = (int64_t)int8_row_bytes(hidden_dim);
+  float* scales = reinterpret_cast<float*>(values + stride * batch);
+  *out = Int8Hidden{values, stride, scales};
+  return cuda_status(launch_quantize_rows_int8(hidden, hidden_row_stride, batch, hidden_dim, hidden_dtype, values,
+                                               stride, scales, static_cast<cudaStream_t>(stream)),
+                     fn);
+}
+
+}  // namespace
+
+size_t gsp_int8_scratch_bytes(int32_t batch, int32_t hidden_dim) {
+  if (batch < 1 || hidden_dim < 1) return 0;
+  return align256((size_t)batch * (int8_row_bytes(hidden_dim) + sizeof(float)));
+}
+
+int32_t gsp_quantize_rows_int8(const void* src, int64_t src_row_stride, int64_t rows, int32_t cols, int32_t dtype,
+                               int8_t* values, int64_t values_row_stride, float* scales, void* stream) {
+  const char* fn = "gsp_quantize_rows_int8";
+  if (rows < 0 || cols < 1) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: rows must be >= 0 and cols positive", fn);
+  if (dtype != GSP_DTYPE_F16 && dtype != GSP_DTYPE_BF16 && dtype != GSP_DTYPE_F32)
+    return fail(GSP_ERR_UNSUPPORTED, "%s: dtype must be GSP_DTYPE_F16, GSP_DTYPE_BF16 or GSP_DTYPE_F32", fn);
+  if (rows == 0) return GSP_OK;
+  if (rows > INT32_MAX) return fail(GSP_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows", fn);
+  if (!src || !values || !scales) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: src, values and scales are required", fn);
+  if (rows > 1 && (src_row_stride < 0 || values_row_stride < cols))
+    return fail(GSP_ERR_INVALID_ARGUMENT, "%s: negative src_row_stride or values_row_stride < cols", fn);
+  return cuda_status(launch_quantize_rows_int8(src, rows > 1 ? src_row_stride : cols, rows, cols, dtype, values,
+                                               rows > 1 ? values_row_stride : cols, scales,
+                                               static_cast<cudaStream_t>(stream)),
+                     fn);
+}
+
+int32_t gsp_int8_logits(int32_t route, const void* hidden, int64_t hidden_row_stride, int32_t hidden_dtype,
+                        const float* hidden_scales, const int8_t* weight, int64_t weight_row_stride,
+                        const float* weight_scales, const int32_t* bitmask, int64_t bitmask_row_stride, int32_t batch,
+                        int32_t vocab, int32_t hidden_dim, int32_t out_dtype, int64_t vocab_offset, void* logits,
+                        int64_t logits_row_stride, float* top_value, int64_t* top_index, int64_t* top_key,
+                        void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes_, void* stream) {
+  const char* fn = "gsp_int8_logits";
+  if (route < GSP_ROUTE_ROW_SPARSE || route > GSP_ROUTE_DENSE_MASK)
+    return fail(GSP_ERR_INVALID_ARGUMENT, "%s: unknown route %d", fn, route);
+  int32_t st = validate_int8(fn, hidden, hidden_row_stride, hidden_dtype, hidden_scales, weight, weight_row_stride,
+                             weight_scales, bitmask, bitmask_row_stride, batch, vocab, hidden_dim, out_dtype, logits,
+                             logits_row_stride, scratch, scratch_bytes);
+  if (st != GSP_OK) return st;
+  const bool tensor_core = route != GSP_ROUTE_ROW_SPARSE;
+  const bool want_top = top_value || top_index || top_key;
+  st = check_workspace(fn, want_top || tensor_core, workspace, workspace_bytes_, batch, vocab);
+  if (st != GSP_OK) return st;
+  Int8Hidden h;
+  st = int8_hidden(fn, hidden, hidden_row_stride, hidden_dtype, hidden_scales, batch, hidden_dim, scratch, stream, &h);
+  if (st != GSP_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!tensor_core) {
+    RowSparseParams p = make_row_sparse(h.values, h.stride, weight, weight_row_stride, bitmask, bitmask_row_stride,
+                                        batch, vocab, hidden_dim, vocab_offset);
+    p.hidden_scales = h.scales;
+    p.weight_scales = weight_scales;
+    p.logits = logits;
+    p.logits_stride = batch > 1 ? logits_row_stride : vocab;
+    p.top_value = top_value;
+    p.top_index = top_index;
+    p.top_key = top_key;
+    if (workspace) attach_workspace(p, workspace);
+    return cuda_status(launch_row_sparse_int8(p, out_dtype, s), fn);
+  }
+  BlockGemmParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.hidden = h.values;
+  p.hidden_stride = batch > 1 ? h.stride : hidden_dim;
+  p.hidden_scales = h.scales;
+  p.weight = weight;
+  p.weight_stride = vocab > 1 ? weight_row_stride : hidden_dim;
+  p.weight_scales = weight_scales;
+  p.mask = reinterpret_cast<const uint32_t*>(bitmask);
+  p.mask_stride = batch > 1 ? bitmask_row_stride : 0;
+  p.batch = batch;
+  p.vocab = vocab;
+  p.hidden_dim = hidden_dim;
+  p.nw = (vocab + 31) / 32;
+  p.vocab_offset = vocab_offset;
+  p.logits = logits;
+  p.logits_stride = batch > 1 ? logits_row_stride : vocab;
+  p.top_value = top_value;
+  p.top_index = top_index;
+  p.top_key = top_key;
+  const Workspace w = carve_workspace(workspace, batch, vocab);
+  p.keys = w.keys;
+  p.ticket = w.ticket;
+  p.error = w.error;
+  p.tile_list = w.tile_list;
+  p.tile_counts = w.tile_counts;
+  p.dense = route == GSP_ROUTE_DENSE_MASK || bitmask == nullptr;
+  p.no_pdl = tl_no_pdl ? 1 : 0;
+  return cuda_status(launch_block_gemm_int8(p, out_dtype, s), fn);
+}
+
+int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t hidden_dtype,
+                         const float* hidden_scales, const int8_t* weight, int64_t weight_row_stride,
+                         const float* weight_scales, const int32_t* bitmask, int64_t bitmask_row_stride, int32_t batch,
+                         int32_t vocab, int32_t hidden_dim, int32_t out_dtype, int64_t vocab_offset,
+                         void* compact_logits, int64_t* compact_ids, int64_t capacity, int64_t* request_offsets,
+                         float* top_value, int64_t* top_index, int64_t* top_key, void* scratch, size_t scratch_bytes,
+                         void* workspace, size_t workspace_bytes_, void* stream) {
+  const char* fn = "gsp_int8_compact";
+  int32_t st = validate_int8(fn, hidden, hidden_row_stride, hidden_dtype, hidden_scales, weight, weight_row_stride,
+                             weight_scales, bitmask, bitmask_row_stride, batch, vocab, hidden_dim, out_dtype, nullptr,
+                             0, scratch, scratch_bytes);
+  if (st != GSP_OK) return st;
+  if (capacity < 0) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: negative capacity", fn);
+  if (capacity > 0 && (!compact_logits || !compact_ids))
+    return fail(GSP_ERR_INVALID_ARGUMENT, "%s: compact_logits and compact_ids are required", fn);
+  if (!request_offsets) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: request_offsets is required", fn);
+  const bool want_top = top_value || top_index || top_key;
+  st = check_workspace(fn, want_top, workspace, workspace_bytes_, batch, vocab);
+  if (st != GSP_OK) return st;
+  Int8Hidden h;
+  st = int8_hidden(fn, hidden, hidden_row_stride, hidden_dtype, hidden_scales, batch, hidden_dim, scratch, stream, &h);
+  if (st != GSP_OK) return st;
+  RowSparseParams p = make_row_sparse(h.values, h.stride, weight, weight_row_stride, bitmask, bitmask_row_stride,
+                                      batch, vocab, hidden_dim, vocab_offset);
+  p.hidden_scales = h.scales;
+  p.weight_scales = weight_scales;
+  p.compact = capacity > 0 ? compact_logits : nullptr;
+  p.compact_ids = compact_ids;
+  p.capacity = capacity;
+  p.offsets = request_offsets;
+  p.top_value = top_value;
+  p.top_index = top_index;
+  p.top_key = top_key;
+  if (workspace) attach_workspace(p, workspace);
+  return cuda_status(launch_row_sparse_int8(p, out_dtype, static_cast<cudaStream_t>(stream)), fn);
+}
+
 }  // extern "C"

@@ -23,10 +23,13 @@ constexpr unsigned FULL_MASK = 0xffffffffu;
 template <typename T>
 struct DTypeTraits;
 
-// Bits: the storage word of one element; kPerVec: elements per 16-byte vector.
+// Bits: the storage word of one operand element; kPerVec: operand elements per
+// 16-byte vector; OutBits: the storage word of one logit; Acc: accumulator.
 template <>
 struct DTypeTraits<__half> {
   using Bits = uint16_t;
+  using OutBits = Bits;
+  using Acc = float;
   static constexpr int kPerVec = 8;
   static constexpr uint16_t kNegInfBits = 0xFC00u;
   static __device__ __forceinline__ float2 pair_to_float2(uint32_t v) {
@@ -45,6 +48,8 @@ struct DTypeTraits<__half> {
 template <>
 struct DTypeTraits<__nv_bfloat16> {
   using Bits = uint16_t;
+  using OutBits = Bits;
+  using Acc = float;
   static constexpr int kPerVec = 8;
   static constexpr uint16_t kNegInfBits = 0xFF80u;
   static __device__ __forceinline__ float2 pair_to_float2(uint32_t v) {
@@ -65,10 +70,35 @@ struct DTypeTraits<__nv_bfloat16> {
 template <>
 struct DTypeTraits<float> {
   using Bits = uint32_t;
+  using OutBits = Bits;
+  using Acc = float;
   static constexpr int kPerVec = 4;
   static constexpr uint32_t kNegInfBits = 0xFF800000u;
   static __device__ __forceinline__ uint32_t round_bits(float f) { return __float_as_uint(f); }
   static __device__ __forceinline__ float bits_to_float(uint32_t u) { return __uint_as_float(u); }
+};
+
+// int8 operands with one fp32 scale per token and per vocabulary row, logits of
+// type Out. The dot product is an exact int32 sum (|q| <= 128, so it holds up to
+// hidden_dim 131,071); the logit is (float(sum) * token scale) * row scale, each
+// step rounded to fp32, then rounded once to Out.
+template <typename Out>
+struct Int8Rows {};
+
+template <typename T>
+struct IsInt8Rows : std::false_type {};
+template <typename Out>
+struct IsInt8Rows<Int8Rows<Out>> : std::true_type {};
+
+template <typename Out>
+struct DTypeTraits<Int8Rows<Out>> {
+  using Bits = int8_t;
+  using OutBits = typename DTypeTraits<Out>::OutBits;
+  using Acc = int;
+  static constexpr int kPerVec = 16;
+  static constexpr OutBits kNegInfBits = DTypeTraits<Out>::kNegInfBits;
+  static __device__ __forceinline__ OutBits round_bits(float f) { return DTypeTraits<Out>::round_bits(f); }
+  static __device__ __forceinline__ float bits_to_float(OutBits u) { return DTypeTraits<Out>::bits_to_float(u); }
 };
 
 // Order-preserving map float -> uint32 (total order on non-NaN values).
@@ -158,11 +188,18 @@ __device__ __forceinline__ float dot8(uint4 w, uint4 h, float acc) {
   return acc;
 }
 
-// fp32 dot of one 16-byte vector of weights with one of hidden states
-// (8 half-precision or 4 fp32 elements), accumulated into acc in element order.
+// Dot of one 16-byte vector of weights with one of hidden states (8
+// half-precision or 4 fp32 elements, accumulated into acc in element order; or
+// 16 int8 elements, four per integer dot-product instruction).
 template <typename T>
-__device__ __forceinline__ float dot_vec(uint4 w, uint4 h, float acc) {
-  if constexpr (std::is_same<T, float>::value) {
+__device__ __forceinline__ typename DTypeTraits<T>::Acc dot_vec(uint4 w, uint4 h, typename DTypeTraits<T>::Acc acc) {
+  if constexpr (IsInt8Rows<T>::value) {
+    acc = __dp4a((int)w.x, (int)h.x, acc);
+    acc = __dp4a((int)w.y, (int)h.y, acc);
+    acc = __dp4a((int)w.z, (int)h.z, acc);
+    acc = __dp4a((int)w.w, (int)h.w, acc);
+    return acc;
+  } else if constexpr (std::is_same<T, float>::value) {
     acc = fmaf(__uint_as_float(w.x), __uint_as_float(h.x), acc);
     acc = fmaf(__uint_as_float(w.y), __uint_as_float(h.y), acc);
     acc = fmaf(__uint_as_float(w.z), __uint_as_float(h.z), acc);
@@ -170,6 +207,26 @@ __device__ __forceinline__ float dot_vec(uint4 w, uint4 h, float acc) {
     return acc;
   } else {
     return dot8<T>(w, h, acc);
+  }
+}
+
+// Sums over the warp, in every lane (of two independent values: their shuffles
+// interleave).
+__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(FULL_MASK, v); }
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
+  return v;
+}
+__device__ __forceinline__ void warp_sum2(int& a, int& b) {
+  a = __reduce_add_sync(FULL_MASK, a);
+  b = __reduce_add_sync(FULL_MASK, b);
+}
+__device__ __forceinline__ void warp_sum2(float& a, float& b) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(FULL_MASK, a, o);
+    b += __shfl_xor_sync(FULL_MASK, b, o);
   }
 }
 

@@ -46,6 +46,9 @@ struct RowSparseParams {
   int hidden_dim;
   int nw;  // ceil(vocab / 32)
   int64_t vocab_offset;
+  // int8 operands: fp32 scale per request and per vocabulary row
+  const float* hidden_scales;
+  const float* weight_scales;
   // full logits [batch, vocab] (optional)
   void* logits;
   int64_t logits_stride;
@@ -97,6 +100,8 @@ struct BlockGemmParams {
   int hidden_dim;
   int nw;
   int64_t vocab_offset;
+  const float* hidden_scales;  // int8 operands: fp32 scale per request ...
+  const float* weight_scales;  // ... and per vocabulary row
   void* logits;
   int64_t logits_stride;
   float* top_value;
@@ -211,6 +216,13 @@ cudaError_t launch_merge_logsumexp(const float* lse, int parts, int batch, float
 cudaError_t launch_top1_from_keys(const int64_t* keys, int batch, float* top_value,
                                   int64_t* top_index, cudaStream_t stream);
 cudaError_t launch_block_gemm(const BlockGemmParams& p, int dtype, cudaStream_t stream);
+
+// ---- int8 operands (out_dtype: 0 fp16, 1 bf16, 2 fp32 logits) ---------------
+cudaError_t launch_row_sparse_int8(const RowSparseParams& p, int out_dtype, cudaStream_t stream);
+cudaError_t launch_block_gemm_int8(const BlockGemmParams& p, int out_dtype, cudaStream_t stream);
+// Rows of `src` (dtype 0 fp16, 1 bf16, 2 fp32) to int8 values and one scale each.
+cudaError_t launch_quantize_rows_int8(const void* src, int64_t src_stride, int64_t rows, int cols, int dtype,
+                                      int8_t* values, int64_t values_stride, float* scales, cudaStream_t stream);
 
 // ---- device-side route choice ----------------------------------------------
 // Route cost model (mirrors gsp_route_cost): each route is a fixed latency plus

@@ -43,6 +43,18 @@ __device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, uint64_t a_desc, uin
       : "memory");
 }
 
+// The same with kind::i8: signed 8-bit operands, exact int32 accumulation; 32
+// elements (32 bytes) of K per instruction.
+__device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrives once on `bar` when every tcgen05 operation this thread issued so far
 // has completed.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
@@ -60,10 +72,20 @@ __host__ __device__ constexpr uint32_t tc_idesc_f16(uint32_t n, bool bf16) {
          ((128u >> 4) << 24);             // M >> 4
 }
 
+// Instruction descriptor of kind::i8 with int32 accumulation, both operands
+// signed and K-major, M = 128 (N a multiple of 16).
+__host__ __device__ constexpr uint32_t tc_idesc_i8(uint32_t n) {
+  return (2u << 4) |         // D format: S32
+         (1u << 7) |         // A format: signed 8-bit
+         (1u << 10) |        // B format: signed 8-bit
+         ((n >> 3) << 17) |  // N >> 3
+         ((128u >> 4) << 24);  // M >> 4
+}
+
 // Shared-memory matrix descriptor of a K-major tile stored by TMA with the
 // 128-byte swizzle: rows of 128 bytes, 8-row groups 1024 bytes apart. The tile
-// must start on a 1024-byte boundary; advancing K by 16 elements (32 bytes)
-// within the swizzle row adds 2 to the descriptor.
+// must start on a 1024-byte boundary; advancing K by 32 bytes (16 half-precision
+// or 32 int8 elements) within the swizzle row adds 2 to the descriptor.
 __device__ __forceinline__ uint64_t tc_desc_sw128(const void* smem_tile) {
   const uint64_t addr = smem_u32(smem_tile);
   uint64_t d = (addr >> 4) & 0x3FFFull;     // start address

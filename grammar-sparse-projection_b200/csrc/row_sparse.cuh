@@ -44,6 +44,12 @@
 // workspace error word and skips its units) for the other CTAs' counts.
 //
 // In the staged and direct kernels no CTA ever waits on another.
+//
+// T is __half, __nv_bfloat16 or float (operands and logits of one type), or
+// Int8Rows<Out> (int8 operands with scales, logits of type Out). Each including
+// source instantiates launch_row_sparse_typed for its types.
+#pragma once
+
 #include "gsp_async.cuh"
 #include "gsp_common.cuh"
 #include "gsp_internal.h"
@@ -185,16 +191,37 @@ __device__ __forceinline__ void round_stats(const SampleSmem& ss, const uint32_t
   }
 }
 
+// The fp32 logit of unit (b, v): the accumulated dot product itself, or (int8
+// operands) the integer sum times the token's scale times the row's. The scales
+// are loaded with the unit's first row vectors, so their latency is not added
+// to the reduction's.
+template <typename T>
+struct UnitScale {
+  float token = 1.f, row = 1.f;
+  __device__ __forceinline__ void load(const RowSparseParams& p, int b, int v) {
+    if constexpr (IsInt8Rows<T>::value) {
+      token = __ldg(p.hidden_scales + b);
+      row = __ldg(p.weight_scales + v);
+    }
+  }
+  __device__ __forceinline__ float finish(typename DTypeTraits<T>::Acc acc) const {
+    if constexpr (IsInt8Rows<T>::value)
+      return __fmul_rn(__fmul_rn((float)acc, token), row);
+    else
+      return acc;
+  }
+};
+
 // ui: the unit's index in the round (its slot in the sampler's per-unit arrays).
 template <typename T, bool kSample>
 __device__ __forceinline__ void emit_unit(const RowSparseParams& p, int b, int v, uint64_t rank, float acc,
                                           bool want_top, RunningTop& top, unsigned long long* s_keys,
                                           RunningSample& rs, int ui) {
-  using Bits = typename DTypeTraits<T>::Bits;
-  const Bits bits = DTypeTraits<T>::round_bits(acc);
-  if (p.logits) static_cast<Bits*>(p.logits)[(int64_t)b * p.logits_stride + v] = bits;
+  using OutBits = typename DTypeTraits<T>::OutBits;
+  const OutBits bits = DTypeTraits<T>::round_bits(acc);
+  if (p.logits) static_cast<OutBits*>(p.logits)[(int64_t)b * p.logits_stride + v] = bits;
   if (p.compact && rank < (uint64_t)p.capacity) {
-    static_cast<Bits*>(p.compact)[rank] = bits;
+    static_cast<OutBits*>(p.compact)[rank] = bits;
     p.compact_ids[rank] = p.vocab_offset + v;
   }
   if (want_top)
@@ -391,7 +418,7 @@ __device__ __forceinline__ void fill_illegal_range(const RowSparseParams& p, I w
                                                    int nt) {
   const int V = p.vocab, nw = p.nw;
   const bool vec_ok = ((reinterpret_cast<uintptr_t>(p.logits) & 15) == 0) && (p.logits_stride % 8 == 0);
-  using Bits = typename DTypeTraits<T>::Bits;
+  using Bits = typename DTypeTraits<T>::OutBits;
   const Bits ninf = DTypeTraits<T>::kNegInfBits;
   for (I g = w_lo * 4 + me; g < w_hi * 4; g += nt) {
     const I f = g >> 2;
@@ -454,7 +481,10 @@ __device__ __forceinline__ void stream_rows(const RowSparseParams& p, const uint
     const uint4* hb = kHSmem ? reinterpret_cast<const uint4*>(static_cast<const Bits*>(s_h) + (size_t)(bb - b0) * H)
                              : reinterpret_cast<const uint4*>(static_cast<const Bits*>(p.hidden) +
                                                               (int64_t)bb * p.hidden_stride);
-    float acc_a = 0.f, acc_b = 0.f;
+    typename DTypeTraits<T>::Acc acc_a = 0, acc_b = 0;
+    UnitScale<T> sa, sb;
+    sa.load(p, ba, va);
+    sb.load(p, bb, vb);
     for (int base = 0; base < nvec; base += 32 * kUnroll) {
       uint4 ra[kUnroll], rb[kUnroll];
 #pragma unroll
@@ -472,13 +502,9 @@ __device__ __forceinline__ void stream_rows(const RowSparseParams& p, const uint
         }
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      acc_a += __shfl_xor_sync(FULL_MASK, acc_a, o);
-      acc_b += __shfl_xor_sync(FULL_MASK, acc_b, o);
-    }
-    if (lane == 0) emit_unit<T, kSample>(p, ba, va, rbase + (uint64_t)i, acc_a, want_top, top, s_keys, rs, i);
-    if (lane == 1 && has2) emit_unit<T, kSample>(p, bb, vb, rbase + (uint64_t)j, acc_b, want_top, top, s_keys, rs, j);
+    warp_sum2(acc_a, acc_b);
+    if (lane == 0) emit_unit<T, kSample>(p, ba, va, rbase + (uint64_t)i, sa.finish(acc_a), want_top, top, s_keys, rs, i);
+    if (lane == 1 && has2) emit_unit<T, kSample>(p, bb, vb, rbase + (uint64_t)j, sb.finish(acc_b), want_top, top, s_keys, rs, j);
   }
   if (lane < 2) {
     top.flush(s_keys);
@@ -501,12 +527,17 @@ __device__ __forceinline__ void stream_rows_scalar(const RowSparseParams& p, con
     using Bits = typename DTypeTraits<T>::Bits;
     const Bits* w = static_cast<const Bits*>(p.weight) + (int64_t)v * p.weight_stride;
     const Bits* h = static_cast<const Bits*>(p.hidden) + (int64_t)b * p.hidden_stride;
-    float acc = 0.f;
-    for (int k = lane; k < H; k += 32)
-      acc = fmaf(DTypeTraits<T>::bits_to_float(__ldg(w + k)), DTypeTraits<T>::bits_to_float(__ldg(h + k)), acc);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(FULL_MASK, acc, o);
-    if (lane == 0) emit_unit<T, kSample>(p, b, v, rbase + (uint64_t)i, acc, want_top, top, s_keys, rs, i);
+    typename DTypeTraits<T>::Acc acc = 0;
+    UnitScale<T> sc;
+    sc.load(p, b, v);
+    for (int k = lane; k < H; k += 32) {
+      if constexpr (IsInt8Rows<T>::value)
+        acc += (int)__ldg(w + k) * (int)__ldg(h + k);
+      else
+        acc = fmaf(DTypeTraits<T>::bits_to_float(__ldg(w + k)), DTypeTraits<T>::bits_to_float(__ldg(h + k)), acc);
+    }
+    acc = warp_sum(acc);
+    if (lane == 0) emit_unit<T, kSample>(p, b, v, rbase + (uint64_t)i, sc.finish(acc), want_top, top, s_keys, rs, i);
   }
   if (lane == 0) {
     top.flush(s_keys);
@@ -646,7 +677,10 @@ __device__ __forceinline__ void stream_rows_ranked(const RowSparseParams& p, uin
     const uint4* wb = reinterpret_cast<const uint4*>(static_cast<const Bits*>(p.weight) + (int64_t)vb * p.weight_stride);
     const uint4* ha = reinterpret_cast<const uint4*>(static_cast<const Bits*>(s_h) + (size_t)ba * H);
     const uint4* hb = reinterpret_cast<const uint4*>(static_cast<const Bits*>(s_h) + (size_t)bb * H);
-    float acc_a = 0.f, acc_b = 0.f;
+    typename DTypeTraits<T>::Acc acc_a = 0, acc_b = 0;
+    UnitScale<T> sa, sb;
+    sa.load(p, ba, va);
+    sb.load(p, bb, vb);
     for (int base = 0; base < nvec; base += 32 * kUnroll) {
       uint4 ra[kUnroll], rb[kUnroll];
 #pragma unroll
@@ -667,13 +701,9 @@ __device__ __forceinline__ void stream_rows_ranked(const RowSparseParams& p, uin
         }
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      acc_a += __shfl_xor_sync(FULL_MASK, acc_a, o);
-      acc_b += __shfl_xor_sync(FULL_MASK, acc_b, o);
-    }
-    if (lane == 0) emit_unit<T, false>(p, ba, va, rbase + (uint64_t)i, acc_a, want_top, top, s_keys, rs, 0);
-    if (lane == 1 && has2) emit_unit<T, false>(p, bb, vb, rbase + (uint64_t)j, acc_b, want_top, top, s_keys, rs, 0);
+    warp_sum2(acc_a, acc_b);
+    if (lane == 0) emit_unit<T, false>(p, ba, va, rbase + (uint64_t)i, sa.finish(acc_a), want_top, top, s_keys, rs, 0);
+    if (lane == 1 && has2) emit_unit<T, false>(p, bb, vb, rbase + (uint64_t)j, sb.finish(acc_b), want_top, top, s_keys, rs, 0);
     i = i_next;
   }
   if (lane < 2) top.flush(s_keys);
@@ -1335,7 +1365,7 @@ __global__ void __launch_bounds__(kThreads, 1) row_sparse_coop_kernel(const RowS
   // the count wait did not shorten the kernel.
   const int pollers = 32;
   const bool filled_early = p.logits != nullptr && max_slice <= kChunk &&
-                            (int64_t)B * p.vocab * (int64_t)sizeof(typename DTypeTraits<T>::Bits) >
+                            (int64_t)B * p.vocab * (int64_t)sizeof(typename DTypeTraits<T>::OutBits) >
                                 (int64_t)kEarlyFillBytes * G;
   if (filled_early && my_hi > my_lo)
     fill_illegal<T>(p, my_lo, my_hi, [&](int64_t f, int, int) { return s_words[f - my_lo]; }, pollers,
@@ -1496,7 +1526,7 @@ __global__ void __launch_bounds__(kThreads, 1) row_sparse_coop_kernel(const RowS
 // launch
 // ===========================================================================
 template <typename T, bool kSample>
-cudaError_t launch_typed(const RowSparseParams& p, cudaStream_t stream) {
+cudaError_t launch_row_sparse_typed(const RowSparseParams& p, cudaStream_t stream) {
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
@@ -1559,15 +1589,4 @@ cudaError_t launch_typed(const RowSparseParams& p, cudaStream_t stream) {
 }
 
 }  // namespace
-
-cudaError_t launch_row_sparse(const RowSparseParams& p, int dtype, cudaStream_t stream) {
-  const bool sample = p.sample_index != nullptr;
-  if (dtype == 2) {
-    if (sample) return cudaErrorNotSupported;  // the sampler takes half-precision inputs only
-    return launch_typed<float, false>(p, stream);
-  }
-  if (dtype == 1) return sample ? launch_typed<__nv_bfloat16, true>(p, stream) : launch_typed<__nv_bfloat16, false>(p, stream);
-  return sample ? launch_typed<__half, true>(p, stream) : launch_typed<__half, false>(p, stream);
-}
-
 }  // namespace gsp

@@ -1,0 +1,17 @@
+// Row-sparse projection with int8 operands and scales per token and per
+// vocabulary row (kernels and their description in row_sparse.cuh).
+//
+// Against fp16 operands a legal row is half the bytes, and its dot product four
+// products per instruction; one integer warp reduction replaces five shuffles.
+#include "row_sparse.cuh"
+
+namespace gsp {
+
+// out_dtype: 0 fp16, 1 bf16, 2 fp32 logits.
+cudaError_t launch_row_sparse_int8(const RowSparseParams& p, int out_dtype, cudaStream_t stream) {
+  if (out_dtype == 2) return launch_row_sparse_typed<Int8Rows<float>, false>(p, stream);
+  if (out_dtype == 1) return launch_row_sparse_typed<Int8Rows<__nv_bfloat16>, false>(p, stream);
+  return launch_row_sparse_typed<Int8Rows<__half>, false>(p, stream);
+}
+
+}  // namespace gsp

@@ -96,6 +96,12 @@ SIGNATURES = {
     "gsp_grouped_scratch_bytes": ([_i32, _i32, _i32, _i32], _sz),
     "gsp_grouped_logits": ([_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp,
                             ctypes.POINTER(RouteCost), ctypes.POINTER(_i32), _vp, _sz, _vp, _sz, _vp], _i32),
+    "gsp_quantize_rows_int8": ([_vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp, _vp], _i32),
+    "gsp_int8_scratch_bytes": ([_i32, _i32], _sz),
+    "gsp_int8_logits": ([_i32, _vp, _i64, _i32, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i64,
+                         _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp], _i32),
+    "gsp_int8_compact": ([_vp, _i64, _i32, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i64,
+                          _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp], _i32),
 }
 
 ROUTE_CODES = {"row-sparse": 0, "block-sparse": 1, "dense-mask": 2}
@@ -625,6 +631,89 @@ def grouped(hidden, weight, mask, logits=None, top_value=None, top_index=None, c
         _ptr(scratch), scratch.numel(), _ptr(ws), ws.numel(), _stream(hidden.device))
     _check(status, "gsp_grouped_logits")
     return list(hdr)
+
+
+# ---------------------------------------------------------------------------
+# int8 head. These wrappers take the tensors' device as the current one (a
+# guard where it is not), and under stream capture a workspace of the graph's
+# own: a captured memory fill zeroes it at every replay, so graphs share none.
+# ---------------------------------------------------------------------------
+DTYPE_I8 = 3
+
+
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+def on_device(device: torch.device):
+    """Context in which `device` is the current CUDA device."""
+    return _NO_GUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _call_workspace(device: torch.device, batch: int, vocab: int) -> torch.Tensor:
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(int(load().gsp_workspace_bytes(batch, vocab)), dtype=torch.uint8, device=device)
+    return workspace(device, batch, vocab)
+
+
+def quantize_rows_int8(x, values, scales) -> None:
+    """gsp_quantize_rows_int8: x [N, H] -> values int8 [N, H], scales float32 [N]."""
+    _require_cuda(x, values, scales)
+    with on_device(x.device):
+        status = load().gsp_quantize_rows_int8(_ptr(x), x.stride(0), x.shape[0], x.shape[1], dtype_code(x.dtype),
+                                               _ptr(values), values.stride(0), _ptr(scales), _stream(x.device))
+    if status:
+        _check(status, "gsp_quantize_rows_int8")
+
+
+def _int8_operands(hidden, hidden_scales, weight, weight_scales, mask):
+    """Leading arguments shared by gsp_int8_logits and gsp_int8_compact, and the scratch tensor (None for int8
+    hidden states)."""
+    scratch = None
+    if hidden_scales is None:
+        batch, hdim = hidden.shape
+        scratch = torch.empty(int(load().gsp_int8_scratch_bytes(batch, hdim)), dtype=torch.uint8, device=hidden.device)
+    return (_ptr(hidden), hidden.stride(0), DTYPE_I8 if hidden_scales is not None else dtype_code(hidden.dtype),
+            _ptr(hidden_scales), _ptr(weight), weight.stride(0), _ptr(weight_scales), _ptr(mask),
+            0 if mask is None else mask.stride(0), hidden.shape[0], weight.shape[0], weight.shape[1]), scratch
+
+
+def int8_logits(route: str, hidden, hidden_scales, weight, weight_scales, mask, out_dtype, logits=None,
+                top_value=None, top_index=None, top_key=None, vocab_offset: int = 0) -> None:
+    """gsp_int8_logits; hidden_scales None: `hidden` is floating point and quantised by the call."""
+    _require_cuda(hidden, hidden_scales, weight, weight_scales, mask, logits)
+    with on_device(hidden.device):
+        args, scratch = _int8_operands(hidden, hidden_scales, weight, weight_scales, mask)
+        ws = _call_workspace(hidden.device, hidden.shape[0], weight.shape[0])
+        status = load().gsp_int8_logits(
+            ROUTE_CODES[route], *args, dtype_code(out_dtype), vocab_offset, _ptr(logits),
+            0 if logits is None else logits.stride(0), _ptr(top_value), _ptr(top_index), _ptr(top_key),
+            _ptr(scratch), 0 if scratch is None else scratch.numel(), _ptr(ws), ws.numel(), _stream(hidden.device))
+    if status:
+        _check(status, "gsp_int8_logits")
+
+
+def int8_compact(hidden, hidden_scales, weight, weight_scales, mask, out_dtype, compact_logits, compact_ids, offsets,
+                 top_value=None, top_index=None, top_key=None, vocab_offset: int = 0) -> None:
+    """gsp_int8_compact."""
+    _require_cuda(hidden, hidden_scales, weight, weight_scales, mask, compact_logits, compact_ids, offsets)
+    with on_device(hidden.device):
+        args, scratch = _int8_operands(hidden, hidden_scales, weight, weight_scales, mask)
+        ws = _call_workspace(hidden.device, hidden.shape[0], weight.shape[0])
+        status = load().gsp_int8_compact(
+            *args, dtype_code(out_dtype), vocab_offset, _ptr(compact_logits), _ptr(compact_ids),
+            0 if compact_logits is None else compact_logits.numel(), _ptr(offsets), _ptr(top_value),
+            _ptr(top_index), _ptr(top_key), _ptr(scratch), 0 if scratch is None else scratch.numel(), _ptr(ws),
+            ws.numel(), _stream(hidden.device))
+    if status:
+        _check(status, "gsp_int8_compact")
 
 
 def copy_bytes(dst: torch.Tensor, src: torch.Tensor, nbytes: int | None = None) -> None:

@@ -65,6 +65,7 @@ extern "C" {
 #define GSP_DTYPE_F16 0
 #define GSP_DTYPE_BF16 1
 #define GSP_DTYPE_F32 2
+#define GSP_DTYPE_I8 3 /* hidden_dtype of the gsp_int8_* entries only */
 
 /* Rows of one vocabulary tile for the block and dense GEMM paths and for the
  * active-tile statistics. */
@@ -494,6 +495,52 @@ int32_t gsp_grouped_logits(const void* hidden, int64_t hidden_row_stride, const 
                            int64_t logits_row_stride, float* top_value, int64_t* top_index,
                            const gsp_route_cost* cost, int32_t* plan_header, void* scratch, size_t scratch_bytes,
                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- int8 head ---------------------------------------------------------------
+ * The projection on an int8 weight with one fp32 scale per vocabulary row
+ * (channel) and int8 hidden states with one scale per request (token): half
+ * the bytes of a half-precision head. No counterpart in the reference (its
+ * heads are fp16 / bf16 / fp32).
+ *
+ * gsp_quantize_rows_int8: rows of `src` (fp16, bf16 or fp32; row stride in
+ * elements, 0 allowed) to int8 values and one scale each:
+ *   scale = max |x| / 127 (fp32 division), value = x / scale (fp32 division)
+ *   rounded to the nearest integer, ties to even.
+ * A row of zeros has scale 0; a row holding an infinity or NaN has scale NaN
+ * and values 0. Every gsp_int8_* call quantises fp hidden states this way.
+ */
+int32_t gsp_quantize_rows_int8(const void* src, int64_t src_row_stride, int64_t rows, int32_t cols, int32_t dtype,
+                               int8_t* values, int64_t values_row_stride, float* scales, void* stream);
+
+/* Masked logits and fused greedy top-1 on any route (GSP_ROUTE_*):
+ *   logit[b, v] = (float(sum_h q[b, h] w[v, h]) * hidden_scale[b]) * weight_scale[v]
+ * with an exact int32 sum, each product rounded to fp32, then rounded once to
+ * out_dtype (GSP_DTYPE_F16 / _BF16 / _F32); every route gives the same bits.
+ * hidden_dtype GSP_DTYPE_I8: `hidden` is int8 with hidden_scales [batch], and
+ * scratch may be NULL. Otherwise `hidden` is fp16 / bf16 / fp32 and the call
+ * first quantises it into scratch (gsp_int8_scratch_bytes, 16-byte aligned,
+ * contents not preserved, one per concurrent call). hidden_dim <= 131,071
+ * (int32 sums). The other arguments, the workspace and the outputs are those
+ * of gsp_row_sparse_logits / gsp_block_gemm_logits / gsp_dense_masked_logits;
+ * the tensor-core routes want 16-byte aligned rows (hidden_dim a multiple of
+ * 16) and run the row-sparse kernel otherwise. */
+size_t gsp_int8_scratch_bytes(int32_t batch, int32_t hidden_dim);
+int32_t gsp_int8_logits(int32_t route, const void* hidden, int64_t hidden_row_stride, int32_t hidden_dtype,
+                        const float* hidden_scales, const int8_t* weight, int64_t weight_row_stride,
+                        const float* weight_scales, const int32_t* bitmask, int64_t bitmask_row_stride, int32_t batch,
+                        int32_t vocab, int32_t hidden_dim, int32_t out_dtype, int64_t vocab_offset, void* logits,
+                        int64_t logits_row_stride, float* top_value, int64_t* top_index, int64_t* top_key,
+                        void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Compact legal logits of the int8 head: gsp_row_sparse_compact's outputs with
+ * gsp_int8_logits' operands. */
+int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t hidden_dtype,
+                         const float* hidden_scales, const int8_t* weight, int64_t weight_row_stride,
+                         const float* weight_scales, const int32_t* bitmask, int64_t bitmask_row_stride, int32_t batch,
+                         int32_t vocab, int32_t hidden_dim, int32_t out_dtype, int64_t vocab_offset,
+                         void* compact_logits, int64_t* compact_ids, int64_t capacity, int64_t* request_offsets,
+                         float* top_value, int64_t* top_index, int64_t* top_key, void* scratch, size_t scratch_bytes,
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1067,4 +1067,79 @@ int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t 
   return cuda_status(launch_row_sparse_int8(p, out_dtype, static_cast<cudaStream_t>(stream)), fn);
 }
 
+// ---- sampling from logits -----------------------------------------------------
+static int32_t filtered_sample(const char* fn, FilteredSampleParams& p, int32_t dtype, int32_t batch, int64_t max_len,
+                               float temperature, const float* temperatures, int32_t top_k, const int32_t* top_ks,
+                               float top_p, const float* top_ps, float min_p, const float* min_ps,
+                               const float* uniforms, int64_t* token_ids, float* logprobs, int32_t* kept,
+                               void* stream) {
+  if (!uniforms || !token_ids)
+    return fail(GSP_ERR_INVALID_ARGUMENT, "%s: uniforms and token_ids are required", fn);
+  if (batch < 1 || batch > (1 << 26)) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: batch must be in 1..2^26", fn);
+  if (dtype != GSP_DTYPE_F16 && dtype != GSP_DTYPE_BF16 && dtype != GSP_DTYPE_F32)
+    return fail(GSP_ERR_UNSUPPORTED, "%s: dtype must be GSP_DTYPE_F16, GSP_DTYPE_BF16 or GSP_DTYPE_F32", fn);
+  if (!temperatures && !(temperature >= 0.f && temperature < INFINITY))
+    return fail(GSP_ERR_INVALID_ARGUMENT, "%s: temperature must be finite and not negative", fn);
+  if (!top_ps && std::isnan(top_p)) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: top_p is NaN", fn);
+  if (!min_ps && std::isnan(min_p)) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: min_p is NaN", fn);
+  p.temperature = temperature;
+  p.temperatures = temperatures;
+  p.top_k = top_k;
+  p.top_ks = top_ks;
+  p.top_p = top_p;
+  p.top_ps = top_ps;
+  p.min_p = min_p;
+  p.min_ps = min_ps;
+  p.uniforms = uniforms;
+  p.token_ids = token_ids;
+  p.logprobs = logprobs;
+  p.kept = kept;
+  return cuda_status(launch_filtered_sample(p, dtype, batch, max_len, static_cast<cudaStream_t>(stream)), fn);
+}
+
+int32_t gsp_sample_logits(const void* logits, int64_t logits_row_stride, int32_t dtype, const int32_t* bitmask,
+                          int64_t bitmask_row_stride, int32_t batch, int32_t vocab, int64_t vocab_offset,
+                          float temperature, const float* temperatures, int32_t top_k, const int32_t* top_ks,
+                          float top_p, const float* top_ps, float min_p, const float* min_ps, const float* uniforms,
+                          int64_t* token_ids, float* logprobs, int32_t* kept, void* stream) {
+  const char* fn = "gsp_sample_logits";
+  if (!logits) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: logits is required", fn);
+  if (vocab < 1) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: vocab must be positive", fn);
+  const int64_t nw = ((int64_t)vocab + 31) / 32;
+  if (logits_row_stride < 0) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: negative logits_row_stride", fn);
+  if (bitmask && (bitmask_row_stride < 0 || (batch > 1 && bitmask_row_stride != 0 && bitmask_row_stride < nw)))
+    return fail(GSP_ERR_INVALID_ARGUMENT, "%s: bitmask_row_stride must be 0 or >= ceil(vocab/32)", fn);
+  FilteredSampleParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.logits = logits;
+  p.row_stride = batch > 1 ? logits_row_stride : 0;
+  p.mask = reinterpret_cast<const uint32_t*>(bitmask);
+  p.mask_stride = batch > 1 ? bitmask_row_stride : 0;
+  p.vocab = vocab;
+  p.vocab_offset = vocab_offset;
+  return filtered_sample(fn, p, dtype, batch, vocab, temperature, temperatures, top_k, top_ks, top_p, top_ps, min_p,
+                         min_ps, uniforms, token_ids, logprobs, kept, stream);
+}
+
+int32_t gsp_sample_compact(const void* compact_logits, const int64_t* compact_ids, const int64_t* request_offsets,
+                           int64_t capacity, int32_t max_len, int32_t dtype, int32_t batch, float temperature,
+                           const float* temperatures, int32_t top_k, const int32_t* top_ks, float top_p,
+                           const float* top_ps, float min_p, const float* min_ps, const float* uniforms,
+                           int64_t* token_ids, float* logprobs, int32_t* kept, void* stream) {
+  const char* fn = "gsp_sample_compact";
+  if (capacity < 0 || max_len < 0)
+    return fail(GSP_ERR_INVALID_ARGUMENT, "%s: capacity and max_len must not be negative", fn);
+  if (!request_offsets) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: request_offsets is required", fn);
+  if (capacity > 0 && (!compact_logits || !compact_ids))
+    return fail(GSP_ERR_INVALID_ARGUMENT, "%s: compact_logits and compact_ids are required", fn);
+  FilteredSampleParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.logits = compact_logits;
+  p.ids = compact_ids;
+  p.offsets = request_offsets;
+  p.capacity = capacity;
+  return filtered_sample(fn, p, dtype, batch, max_len, temperature, temperatures, top_k, top_ks, top_p, top_ps, min_p,
+                         min_ps, uniforms, token_ids, logprobs, kept, stream);
+}
+
 }  // extern "C"

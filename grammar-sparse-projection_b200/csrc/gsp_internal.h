@@ -224,6 +224,35 @@ cudaError_t launch_block_gemm_int8(const BlockGemmParams& p, int out_dtype, cuda
 cudaError_t launch_quantize_rows_int8(const void* src, int64_t src_stride, int64_t rows, int cols, int dtype,
                                       int8_t* values, int64_t values_stride, float* scales, cudaStream_t stream);
 
+// ---- sampling with temperature, top-k, min-p and top-p (filtered_sample.cu) --
+struct FilteredSampleParams {
+  const void* logits;
+  int64_t row_stride;
+  const uint32_t* mask;
+  int64_t mask_stride;
+  int64_t vocab;            // row length (packed rows: ignored)
+  const int64_t* offsets;   // packed rows: [batch + 1], else nullptr
+  const int64_t* ids;       // packed rows: token id of each position
+  int64_t capacity;         // packed rows: positions that exist
+  int64_t vocab_offset;
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const float* temperatures;  // per-request values, or nullptr: the scalar above
+  const int32_t* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  const float* uniforms;
+  int64_t* token_ids;
+  float* logprobs;
+  int32_t* kept;
+  int resident;  // keys a CTA holds in shared memory
+};
+
+// max_len: tokens of the longest row (packed rows: an expectation that picks the
+// launch shape; longer rows are right all the same).
+cudaError_t launch_filtered_sample(const FilteredSampleParams& p, int dtype, int batch, int64_t max_len,
+                                   cudaStream_t stream);
+
 // ---- device-side route choice ----------------------------------------------
 // Route cost model (mirrors gsp_route_cost): each route is a fixed latency plus
 // its bytes at the rate measured for its kernel on B200.

@@ -51,6 +51,9 @@ class RouteCost(ctypes.Structure):
 _PROJECTION_ARGS = [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _i64,
                     _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp]
 
+_f32 = ctypes.c_float
+_FILTER_ARGS = [_f32, _vp, _i32, _vp, _f32, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp]
+
 SIGNATURES = {
     "gsp_abi_version": ([], _i32),
     "gsp_status_string": ([_i32], ctypes.c_char_p),
@@ -102,6 +105,8 @@ SIGNATURES = {
                          _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp], _i32),
     "gsp_int8_compact": ([_vp, _i64, _i32, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i64,
                           _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp], _i32),
+    "gsp_sample_logits": ([_vp, _i64, _i32, _vp, _i64, _i32, _i32, _i64] + _FILTER_ARGS, _i32),
+    "gsp_sample_compact": ([_vp, _vp, _vp, _i64, _i32, _i32, _i32] + _FILTER_ARGS, _i32),
 }
 
 ROUTE_CODES = {"row-sparse": 0, "block-sparse": 1, "dense-mask": 2}
@@ -714,6 +719,37 @@ def int8_compact(hidden, hidden_scales, weight, weight_scales, mask, out_dtype, 
             ws.numel(), _stream(hidden.device))
     if status:
         _check(status, "gsp_int8_compact")
+
+
+def _filter_args(settings, uniforms, token_ids, logprobs, kept):
+    """(temperature, top_k, top_p, min_p), each a number or a tensor, as scalar / array argument pairs."""
+    args = []
+    for v in settings:
+        args += [0, v.data_ptr()] if isinstance(v, torch.Tensor) else [v, None]
+    return (*args, uniforms.data_ptr(), token_ids.data_ptr(), logprobs.data_ptr(), kept.data_ptr())
+
+
+def sample_logits(logits, mask, settings, uniforms, token_ids, logprobs, kept, vocab_offset: int = 0) -> None:
+    """gsp_sample_logits; logits [B, V] (row stride free), mask [B, words] or None."""
+    _require_cuda(logits, mask, uniforms, token_ids)
+    with on_device(logits.device):
+        status = load().gsp_sample_logits(
+            logits.data_ptr(), logits.stride(0), DTYPE_CODES[logits.dtype], None if mask is None else mask.data_ptr(),
+            0 if mask is None else mask.stride(0), logits.shape[0], logits.shape[1], vocab_offset,
+            *_filter_args(settings, uniforms, token_ids, logprobs, kept), _stream(logits.device))
+    if status:
+        _check(status, "gsp_sample_logits")
+
+
+def sample_compact(logits, ids, offsets, max_len: int, settings, uniforms, token_ids, logprobs, kept) -> None:
+    """gsp_sample_compact; logits [N] and ids [N] packed by offsets [B + 1]."""
+    _require_cuda(logits, ids, offsets, uniforms, token_ids)
+    with on_device(logits.device):
+        status = load().gsp_sample_compact(
+            logits.data_ptr(), ids.data_ptr(), offsets.data_ptr(), logits.numel(), max_len, DTYPE_CODES[logits.dtype],
+            uniforms.numel(), *_filter_args(settings, uniforms, token_ids, logprobs, kept), _stream(logits.device))
+    if status:
+        _check(status, "gsp_sample_compact")
 
 
 def copy_bytes(dst: torch.Tensor, src: torch.Tensor, nbytes: int | None = None) -> None:

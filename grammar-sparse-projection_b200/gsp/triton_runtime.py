@@ -42,6 +42,9 @@ __all__ = [
     "grammar_logits_with_top1",
     "grammar_sample",
     "SampleResult",
+    "sample_logits",
+    "sample_compact_logits",
+    "FilteredSample",
     "bitmask_compact_logits",
     "mask_stats",
     "choose_route",
@@ -534,6 +537,121 @@ def grammar_sample(hidden: torch.Tensor, weight: torch.Tensor, bitmask_gpu: torc
                               sample_logsumexp=lse, logits=logits, top_value=top_value, top_index=top_index,
                               route=route)
     return SampleResult(token_ids, lse, top_value, top_index, logits)
+
+
+class FilteredSample(NamedTuple):
+    token_ids: torch.Tensor  # int64 [B]: drawn token per request
+    logprobs: torch.Tensor   # float32 [B]: its log-probability among the kept tokens
+    kept: torch.Tensor       # int32 [B]: tokens that the filters left
+
+
+_SETTINGS = (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32),
+             ("min_p", torch.float32))
+
+
+def _sample_settings(values, uniforms, device):
+    """Checked (temperature, top_k, top_p, min_p): numbers, or one device value per request."""
+    if uniforms.device != device or uniforms.dtype != torch.float32 or uniforms.ndim != 1 or not uniforms.is_contiguous():
+        raise ValueError("uniforms must be a contiguous float32 tensor [B] on the logits' device")
+    batch = uniforms.shape[0]
+    for v, (name, dtype) in zip(values, _SETTINGS):
+        if isinstance(v, torch.Tensor):
+            if v.device != device or v.dtype != dtype or v.shape != (batch,) or not v.is_contiguous():
+                raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor with one value per request")
+        elif v != v:
+            raise ValueError(f"{name} is NaN")
+    t, k = values[0], values[1]
+    if not isinstance(t, torch.Tensor) and not 0.0 <= t < float("inf"):
+        raise ValueError("temperature must be finite and not negative")
+    if not isinstance(k, torch.Tensor):
+        if int(k) != k:
+            raise ValueError("top_k must be a whole number")
+        values = (t, max(0, min(int(k), 2 ** 31 - 1)), values[2], values[3])
+    return values
+
+
+def _sample_outputs(batch, device):
+    return FilteredSample(torch.empty(batch, dtype=torch.int64, device=device),
+                          torch.empty(batch, dtype=torch.float32, device=device),
+                          torch.empty(batch, dtype=torch.int32, device=device))
+
+
+def sample_logits(logits: torch.Tensor, *, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  bitmask_gpu: torch.Tensor | None = None) -> FilteredSample:
+    """One token per request by temperature, top-k, min-p and top-p, from given
+    uniform numbers (float32 [B] in [0, 1), e.g. torch.rand).
+
+    logits [B, V] (or [V]) float16 / bfloat16 / float32: what any route of the
+    head writes (-inf on illegal tokens), or any logits with their bitmask;
+    NaN and -inf are never drawn. In the order "falling logit, ties by rising
+    id", with w = exp((x - max) / temperature): keep the first top_k (0: all),
+    of these w >= min_p, of these the shortest prefix with at least top_p of
+    the weight, and draw the first token whose running weight passes
+    uniforms[b] times the kept weight. Each setting is a number or a tensor
+    with one value per request (float32; top_k int32). Temperature 0 is greedy
+    (largest logit, lowest id). The sums are exact, so equal calls give equal
+    tokens, log-probabilities and counts. A request without a legal token
+    reports token 0, log-probability -inf, kept 0 (grammar_sample's token 0);
+    one with an invalid tensor setting or uniform token -1, NaN, 0. The rows
+    may have any stride; shapes of the results are [B] always. grammar_sample
+    draws inside the projection instead, from softmax(logits / T) unfiltered.
+    """
+    if logits.device.type != "cuda":
+        raise ValueError("logits must be a CUDA tensor")
+    rows = logits.reshape(1, -1) if logits.ndim == 1 else logits
+    if rows.ndim != 2 or rows.shape[0] < 1 or rows.shape[1] < 1:
+        raise ValueError("logits must have shape [V] or [B, V]")
+    if rows.shape[1] > 1 and rows.stride(1) != 1:
+        raise ValueError("logits must be contiguous along the vocabulary")
+    _native.dtype_code(rows.dtype)
+    dev = rows.device
+    if uniforms.shape != rows.shape[:1]:
+        raise ValueError("uniforms must hold one number per request")
+    settings = _sample_settings((temperature, top_k, top_p, min_p), uniforms, dev)
+    mask = bitmask_gpu
+    if mask is not None:
+        if mask.device != dev or mask.dtype != torch.int32:
+            raise ValueError("bitmask_gpu must be CUDA int32")
+        if mask.ndim == 1:
+            mask = mask.reshape(1, -1)
+        if mask.ndim != 2 or mask.shape[0] != rows.shape[0] or mask.shape[1] < (rows.shape[1] + 31) // 32:
+            raise ValueError("bitmask shape does not match logits")
+        if not mask.is_contiguous():
+            raise ValueError("bitmask must be contiguous")
+    out = _sample_outputs(rows.shape[0], dev)
+    _native.sample_logits(rows, mask, settings, uniforms, *out)
+    return out
+
+
+def sample_compact_logits(token_ids: torch.Tensor, logits: torch.Tensor, offsets: torch.Tensor, *,
+                          uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                          max_len: int | None = None) -> FilteredSample:
+    """sample_logits on packed legal rows: (token_ids int64 [N], logits [N],
+    offsets int64 [B+1]) as bitmask_compact_logits and int8_compact_logits
+    return them; the drawn ids come from token_ids. max_len, the longest row
+    expected (default: N), only picks the launch shape. Positions past the
+    end of the arrays are not read, whatever the offsets say."""
+    if logits.device.type != "cuda":
+        raise ValueError("logits must be a CUDA tensor")
+    if logits.ndim != 1 or token_ids.shape != logits.shape:
+        raise ValueError("token_ids and logits must have shape [N]")
+    if token_ids.dtype != torch.int64 or offsets.dtype != torch.int64:
+        raise ValueError("token_ids and offsets must be int64")
+    if token_ids.device != logits.device or offsets.device != logits.device:
+        raise ValueError("token_ids, logits and offsets must be on one device")
+    if not (token_ids.is_contiguous() and logits.is_contiguous() and offsets.is_contiguous()):
+        raise ValueError("token_ids, logits and offsets must be contiguous")
+    if offsets.ndim != 1 or offsets.shape[0] < 2 or uniforms.shape[0] != offsets.shape[0] - 1:
+        raise ValueError("offsets must have shape [B + 1], uniforms [B]")
+    _native.dtype_code(logits.dtype)
+    settings = _sample_settings((temperature, top_k, top_p, min_p), uniforms, logits.device)
+    if max_len is None:
+        max_len = logits.numel()
+    elif max_len < 0:
+        raise ValueError("max_len must not be negative")
+    out = _sample_outputs(uniforms.shape[0], logits.device)
+    _native.sample_compact(logits, token_ids, offsets, min(max_len, 2 ** 31 - 1), settings, uniforms, *out)
+    return out
 
 
 def bitmask_compact_logits(hidden: torch.Tensor, weight: torch.Tensor, bitmask_gpu: torch.Tensor,

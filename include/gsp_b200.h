@@ -542,6 +542,42 @@ int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t 
                          float* top_value, int64_t* top_index, int64_t* top_key, void* scratch, size_t scratch_bytes,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- sampling from logits ------------------------------------------------------
+ * One token per request from logits that a route of the head wrote (-inf on
+ * illegal tokens), or from any logits with the packed bitmask (NULL: none), by
+ * temperature, top-k, min-p and top-p from a given uniform number:
+ *   legal tokens (bit set, not NaN, not -inf) in the order "falling logit, ties
+ *   by rising id"; w = exp((x - max) / T);
+ *   keep the first top_k (<= 0: all), of these w >= min_p (<= 0: all), of these
+ *   the shortest prefix with sum >= top_p * sum (>= 1: all; at least one token);
+ *   draw the first kept token with w_1 + ... + w_i > uniforms[b] * sum.
+ * Outputs: token_ids [batch], logprobs [batch] (optional: log-probability among
+ * the kept tokens), kept [batch] (optional: how many were kept). Sums are exact
+ * integers (weights in units below 2^-44 for rows up to 2^18 tokens), so equal
+ * calls give equal bits. Temperature 0 is greedy: the largest logit, lowest id,
+ * log-probability 0, one token kept. A request without a legal token reports
+ * token 0, log-probability -inf, kept 0. Settings: the scalar, or (array not
+ * NULL) one device value per request; a request whose array values are not
+ * valid (negative, infinite or NaN temperature, NaN top_p or min_p, uniform
+ * outside [0, 1)) reports token -1, log-probability NaN, kept 0. No workspace.
+ * gsp_sample_logits: rows of `vocab` logits (row stride 0 shares one row); ids
+ * are vocab_offset + position. gsp_sample_compact: rows packed as
+ * gsp_row_sparse_compact / gsp_int8_compact write them, request b at positions
+ * [request_offsets[b], request_offsets[b+1]) below `capacity`; max_len is the
+ * longest row expected and only picks the launch shape. No counterpart in the
+ * reference, which takes logits.argmax(-1)
+ * (benchmarks/qwen35_adaptive_paired.py:94). */
+int32_t gsp_sample_logits(const void* logits, int64_t logits_row_stride, int32_t dtype, const int32_t* bitmask,
+                          int64_t bitmask_row_stride, int32_t batch, int32_t vocab, int64_t vocab_offset,
+                          float temperature, const float* temperatures, int32_t top_k, const int32_t* top_ks,
+                          float top_p, const float* top_ps, float min_p, const float* min_ps, const float* uniforms,
+                          int64_t* token_ids, float* logprobs, int32_t* kept, void* stream);
+int32_t gsp_sample_compact(const void* compact_logits, const int64_t* compact_ids, const int64_t* request_offsets,
+                           int64_t capacity, int32_t max_len, int32_t dtype, int32_t batch, float temperature,
+                           const float* temperatures, int32_t top_k, const int32_t* top_ks, float top_p,
+                           const float* top_ps, float min_p, const float* min_ps, const float* uniforms,
+                           int64_t* token_ids, float* logprobs, int32_t* kept, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

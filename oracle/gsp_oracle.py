@@ -363,6 +363,35 @@ def sample_reference(hidden, weight, mask, dtype: torch.dtype, temperature: floa
     return out
 
 
+def filtered_sample_reference(row, uniform: float, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                              min_p: float = 0.0):
+    """Temperature, top-k, min-p, top-p and one draw on one row of logits, in
+    float64: (position or 0, log-probability among the kept, number kept).
+    NaN and -inf are not drawn; order: falling logit, ties by rising position.
+    The settings are the fp32 values a kernel receives."""
+    x = np.asarray(row, dtype=np.float64)
+    at = np.flatnonzero(x > -np.inf)  # NaN compares false
+    if at.size == 0:
+        return 0, -np.inf, 0
+    at = at[np.argsort(-x[at], kind="stable")]
+    x = x[at]
+    t, p, m = (float(np.float32(v)) for v in (temperature, top_p, min_p))
+    if t == 0.0:
+        return int(at[0]), 0.0, 1
+    with np.errstate(invalid="ignore"):
+        score = np.where(x == x[0], 0.0, (x - x[0]) / t)
+    if top_k > 0:
+        score = score[:top_k]
+    w = np.exp(score)
+    w = w[w >= m]
+    upto = np.cumsum(w)
+    if p < 1.0:
+        w = w[:max(1, int(np.count_nonzero(upto - w < p * upto[-1])))]
+        upto = np.cumsum(w)
+    i = min(int(np.count_nonzero(upto <= float(np.float32(uniform)) * upto[-1])), w.size - 1)
+    return int(at[i]), float(score[i] - np.log(upto[-1])), int(w.size)
+
+
 def cpu_row_sparse_step(hidden: np.ndarray, weight: np.ndarray, mask: np.ndarray, vocab: int) -> tuple[np.ndarray, np.ndarray]:
     """One CPU step of the reference's row-sparse semantics for the timed CPU
     baseline: decode the bitmask, gather legal rows (gsp/runtime.py:50-51),

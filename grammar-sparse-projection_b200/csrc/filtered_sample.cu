@@ -18,20 +18,22 @@
 // answers bit for bit. The unit is below 2^-44 for rows up to 2^18 tokens.
 //
 // One cluster of CTAs per row; the row is read from global memory once and held
-// in the CTAs' shared memory (-inf where not legal). A search counts or weighs
-// the tokens in 1024 bins of shared memory, the CTAs read one another's bins
-// over distributed shared memory after one cluster barrier, and each picks the
-// bin at which the running sum passes the target.
+// in the CTAs' shared memory (-inf where the mask says not legal). A search
+// counts or weighs the tokens in 512 bins of shared memory, the CTAs read one
+// another's bins over distributed shared memory after one cluster barrier, and
+// each picks the bin at which the running sum passes the target.
 //   * The first bins are chosen by value, so that few tokens share one:
-//     sixteenths of an octave of the weight, or (top-k) 128ths of an octave of
-//     the distance to the maximum. They do not depend on the target, so top-p
-//     and the draw use the same weighing.
-//   * The picked bin's tokens are then listed (key and position, every CTA
-//     writing its own to all), and the rest of the search is each CTA's own,
-//     without cluster barriers: the range of keys narrows 1024-fold per pass. A
-//     list that does not fit leaves the search in the whole row.
-//   * After top-k or min-p the kept tokens themselves are listed if they fit,
-//     and only they are weighed.
+//     sixteenths of an octave of the weight (quarters below 2^-24), or (top-k)
+//     64ths of an octave of the distance to the maximum. They do not depend on
+//     the target, so top-p and the draw use the same weighing.
+//   * The tokens of the picked bins (for top-p: of the border's bin and of those
+//     the draw can fall into) are then listed, key and position, in the first
+//     CTA's shared memory; the other CTAs are done and leave, and the rest of the
+//     search needs no cluster barrier: the range of keys narrows 512-fold per
+//     pass over the list. Where a list does not fit, the search goes on in the
+//     whole row, 512-fold per pass all the same.
+//   * Rows with few legal tokens (a grammar's) are listed whole at once, and
+//     after top-k or min-p the kept tokens are.
 //
 // Bound: for long kept sets one 64-bit exponential per weighed token (11
 // double-precision operations, about 35 in all) and one shared-memory atomic;
@@ -52,16 +54,16 @@ namespace cg = cooperative_groups;
 
 constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
-constexpr int kBinBits = 10;
+constexpr int kBinBits = 9;
 constexpr int kBins = 1 << kBinBits;
 constexpr int kMaxCluster = 16;
 constexpr int kMaxShift = 50;
 constexpr int kExpBits = 8;
 constexpr int kExpTable = 1 << kExpBits;
-constexpr int kOctaveBits = 4;   // weighing bins per octave: 2^kOctaveBits
-constexpr int kListTotal = 2048; // tokens a cluster lists, an equal part for each CTA
-static_assert(kBins == 2 * kSampleThreads, "two bins per thread");
-static_assert(((kMaxShift + 1) << kOctaveBits) < kBins, "every weight has a bin");
+constexpr int kListBits = 12;
+constexpr int kListTotal = 1 << kListBits;  // tokens a cluster lists
+static_assert(kBins == kSampleThreads, "one bin per thread");
+static_assert(kMaxCluster <= kSampleWarps, "a warp for each part of the list");
 
 // Order-preserving keys: larger logit, larger key (-0 and +0 alike); 0 for NaN
 // and -inf, which are never drawn.
@@ -107,10 +109,10 @@ struct SampleKey<float> {
 struct SampleSmemHeader {
   uint32_t lo[kBins];                      // bins being filled: low and high halves of 64-bit sums
   uint32_t hi[kBins];
-  ulonglong2 tot[kBins / 2];               // this CTA's bins, read by the cluster
-  unsigned long long list[kListTotal];     // (key, position in the row); part r holds rank r's tokens
+  unsigned long long tot[kBins];           // this CTA's bins, read by the cluster
+  unsigned long long list[kListTotal];     // (key, position in the row), in parts (rank 0's is used)
   unsigned long long scan[kSampleWarps];
-  unsigned long long pick[4];              // picked bin, sum before it, its own sum, sum of all bins
+  unsigned long long pick[2][4];           // picked bin, sum before it, its own sum; [.][3] of 0: sum of all bins
   unsigned long long word[2][kMaxCluster]; // one value per CTA (all-gather)
   double exp2_table[kExpTable];            // 2^(j / kExpTable)
   uint32_t warp[2][kSampleWarps];
@@ -134,6 +136,56 @@ __device__ __forceinline__ float load_value(const Row<T>& r, int64_t i) {
   const float f = DTypeTraits<T>::bits_to_float(__ldg(r.x + i));
   return f == f ? f : -INFINITY;
 }
+
+// ---- comparisons of the values in one 32-bit word (two 16-bit ones, or one) ----
+// All ones in the half (word) of a value that is above, or at least, `x`, a
+// value of the type. NaN is neither.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_above(uint32_t w, float x) {
+  if constexpr (std::is_same<T, __half>::value)
+    return __hgt2_mask(*reinterpret_cast<const __half2*>(&w), __float2half2_rn(x));
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return __hgt2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w), __float2bfloat162_rn(x));
+  else
+    return __uint_as_float(w) > x ? 0xffffffffu : 0u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pair_at_least(uint32_t w, float x) {
+  if constexpr (std::is_same<T, __half>::value)
+    return __hge2_mask(*reinterpret_cast<const __half2*>(&w), __float2half2_rn(x));
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w), __float2bfloat162_rn(x));
+  else
+    return __uint_as_float(w) >= x ? 0xffffffffu : 0u;
+}
+// Counts of such masks add up in both halves of a word, over a vector's words.
+template <typename T>
+__device__ __forceinline__ uint32_t pair_count(uint32_t mask) {
+  return sizeof(typename DTypeTraits<T>::Bits) == 4 ? mask & 1u : mask & 0x00010001u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pair_total(uint32_t count) {
+  return sizeof(typename DTypeTraits<T>::Bits) == 4 ? count : (count & 0xffffu) + (count >> 16);
+}
+// Running maximum of pairs; NaN never wins.
+template <typename T>
+struct PairMax {
+  float a = -INFINITY;
+  __device__ __forceinline__ void add(uint32_t w) { a = fmaxf(a, __uint_as_float(w)); }
+  __device__ __forceinline__ float value() const { return a; }
+};
+template <>
+struct PairMax<__half> {
+  __half2 a = __float2half2_rn(-INFINITY);
+  __device__ __forceinline__ void add(uint32_t w) { a = __hmax2(a, *reinterpret_cast<const __half2*>(&w)); }
+  __device__ __forceinline__ float value() const { return fmaxf(__low2float(a), __high2float(a)); }
+};
+template <>
+struct PairMax<__nv_bfloat16> {
+  __nv_bfloat162 a = __float2bfloat162_rn(-INFINITY);
+  __device__ __forceinline__ void add(uint32_t w) { a = __hmax2(a, *reinterpret_cast<const __nv_bfloat162*>(&w)); }
+  __device__ __forceinline__ float value() const { return fmaxf(__low2float(a), __high2float(a)); }
+};
 
 // One CTA's part of the row: positions [lo, lo + len), the first `resident`
 // of them in shared memory at index `phase` on (so that 16-byte loads of the
@@ -159,50 +211,80 @@ struct Slice {
       return DTypeTraits<T>::bits_to_float((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
   }
 
+  // Value at a position of the CTA's part.
+  __device__ __forceinline__ float at(int64_t pos) const {
+    const int64_t i = pos - lo;
+    return i < resident ? DTypeTraits<T>::bits_to_float(held[phase + i]) : load_value(row, pos);
+  }
+
   // Fills the resident part; returns the thread's largest value and its number
-  // of legal tokens over the whole part.
+  // of legal tokens over the whole part. Whole vectors four at a time, the
+  // loads ahead of their use; NaN stays (every comparison with it is false).
   __device__ __forceinline__ float load(uint32_t& legal_count) {
-    float top = -INFINITY;
+    constexpr int kAhead = 4;
+    const int nv = vectors(), whole0 = phase > 0 ? 1 : 0, whole1 = (phase + resident) / kVec;
+    PairMax<T> most;
     legal_count = 0u;
-    const int nv = vectors();
-#pragma unroll 2
-    for (int v = threadIdx.x; v < nv; v += kSampleThreads) {
-      const int64_t i0 = lo + (int64_t)v * kVec - phase;
-      float f[kVec];
-      if (v * kVec >= phase && v * kVec + kVec <= phase + resident) {
-        const uint4 q = ld_stream_v4(row.x + i0);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        uint32_t legal = 0xffffffffu;
+    for (int v0 = whole0 + threadIdx.x; v0 < whole1; v0 += kAhead * kSampleThreads) {
+      uint4 q[kAhead];
+      uint32_t legal[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int v = v0 + k * kSampleThreads;
+        q[k] = make_uint4(0u, 0u, 0u, 0u);
+        legal[k] = 0u;
+        if (v < whole1) {
+          const int64_t i0 = lo + (int64_t)v * kVec - phase;
+          q[k] = ld_stream_v4(row.x + i0);
+          legal[k] = 0xffffffffu;
+          if (row.mask) {
+            const int64_t w0 = i0 >> 5;
+            const int sh = (int)(i0 & 31);
+            const uint32_t a = __ldg(row.mask + w0);
+            const uint32_t b = sh + kVec > 32 ? __ldg(row.mask + w0 + 1) : 0u;
+            legal[k] = __funnelshift_r(a, b, sh);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int v = v0 + k * kSampleThreads;
+        if (v >= whole1) break;
+        uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
         if (row.mask) {
-          const int64_t w0 = i0 >> 5;
-          const int s = (int)(i0 & 31);
-          const uint32_t a = __ldg(row.mask + w0);
-          const uint32_t b = s + kVec > 32 ? __ldg(row.mask + w0 + 1) : 0u;
-          legal = __funnelshift_r(a, b, s);
-        }
+          constexpr uint32_t kIllegal = DTypeTraits<T>::kNegInfBits;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          f[j] = unpack(w, j);
-          if (!((legal >> j) & 1u) || f[j] != f[j]) f[j] = -INFINITY;
+          for (int j = 0; j < kVec; ++j) {
+            const bool ok = (legal[k] >> j) & 1u;
+            if constexpr (sizeof(Bits) == 4)
+              w[j] = ok ? w[j] : kIllegal;
+            else if (j & 1)
+              w[j >> 1] = ok ? w[j >> 1] : (w[j >> 1] & 0xffffu) | (kIllegal << 16);
+            else
+              w[j >> 1] = ok ? w[j >> 1] : (w[j >> 1] & 0xffff0000u) | kIllegal;
+          }
         }
-      } else {
+        uint32_t c = 0u;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          const int at = v * kVec + j;
-          f[j] = (at >= phase && at < phase + resident) ? load_value(row, i0 + j) : -INFINITY;
+        for (int j = 0; j < 4; ++j) {
+          most.add(w[j]);
+          c += pair_count<T>(pair_above<T>(w[j], -INFINITY));
         }
+        legal_count += pair_total<T>(c);
+        reinterpret_cast<uint4*>(held)[v] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      uint32_t out[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        top = fmaxf(top, f[j]);
-        legal_count += f[j] > -INFINITY ? 1u : 0u;
-        if constexpr (sizeof(Bits) == 4)
-          out[j] = __float_as_uint(f[j]);
-        else
-          out[j >> 1] |= (uint32_t)DTypeTraits<T>::round_bits(f[j]) << (16 * (j & 1));
-      }
-      reinterpret_cast<uint4*>(held)[v] = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+    float top = most.value();
+    // the first and last vectors where they are not whole
+    for (int i = threadIdx.x; i < 2 * kVec; i += kSampleThreads) {
+      const int v = i < kVec ? 0 : nv - 1;
+      if (v < 0 || (v >= whole0 && v < whole1) || (i >= kVec && nv == 1)) continue;
+      const int slot = v * kVec + i % kVec;
+      const bool mine = slot >= phase && slot < phase + resident;
+      const float f = mine ? load_value(row, lo + slot - phase) : -INFINITY;
+      held[slot] = DTypeTraits<T>::round_bits(f);
+      top = fmaxf(top, f);
+      legal_count += f > -INFINITY ? 1u : 0u;
     }
     for (int64_t i = resident + threadIdx.x; i < len; i += kSampleThreads) {
       const float f = load_value(row, lo + i);
@@ -212,33 +294,91 @@ struct Slice {
     return top;
   }
 
-  // fn(value, position in the row) for every position of the CTA's part (-inf: not legal)
+  // fn(words, position of the first value) for every vector of the CTA's part
+  // (16 bytes of values; -inf or NaN: not legal, or not of the part)
+  template <typename Fn>
+  __device__ __forceinline__ void each_vector(Fn fn) const {
+    const int nv = vectors();
+    const int total = nv + (int)((len - resident + kVec - 1) / kVec);
+    for (int v = threadIdx.x; v < total; v += kSampleThreads) {
+      uint32_t w[4];
+      int64_t pos = lo - phase + (int64_t)v * kVec;
+      if (v < nv) {
+        const uint4 q = reinterpret_cast<const uint4*>(held)[v];
+        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+      } else {
+        pos = lo + resident + (int64_t)(v - nv) * kVec;
+        const uint4 q = gather_vector(row, pos, lo + len);
+        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+      }
+      fn(w, (uint32_t)pos);
+    }
+  }
+  // A vector of the part that is not resident (by value: nothing of the caller's goes through memory).
+  static __device__ __noinline__ uint4 gather_vector(Row<T> row, int64_t pos, int64_t end) {
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const uint32_t bits = DTypeTraits<T>::round_bits(pos + j < end ? load_value(row, pos + j) : -INFINITY);
+      if constexpr (sizeof(Bits) == 4) w[j] = bits;
+      else w[j >> 1] |= bits << (16 * (j & 1));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // fn(value) one by one
   template <typename Fn>
   __device__ __forceinline__ void each(Fn fn) const {
-    const int nv = vectors();
-    for (int v = threadIdx.x; v < nv; v += kSampleThreads) {
-      const uint4 q = reinterpret_cast<const uint4*>(held)[v];
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    each_vector([&](const uint32_t (&w)[4], uint32_t pos) {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) fn(unpack(w, j), (uint32_t)(lo - phase + v * kVec + j));
-    }
-    for (int64_t i = resident + threadIdx.x; i < len; i += kSampleThreads)
-      fn(load_value(row, lo + i), (uint32_t)(lo + i));
+      for (int j = 0; j < kVec; ++j) fn(unpack(w, j), pos + j);
+    });
+  }
+  // fn(value, position) for the values in [from, to] or [from2, to2], which are
+  // few; returns how many are above `to`. (Pairs are compared at once; a mask
+  // per vector, then its set bits.)
+  template <typename Fn>
+  __device__ __forceinline__ uint32_t each_between(float from, float to, float from2, float to2, Fn fn) const {
+    uint32_t above = 0u;
+    each_vector([&](const uint32_t (&w)[4], uint32_t pos) {
+      uint32_t in[4], c = 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t over = pair_above<T>(w[j], to);
+        c += pair_count<T>(over);
+        in[j] = (pair_at_least<T>(w[j], from) & ~over) | (pair_at_least<T>(w[j], from2) & ~pair_above<T>(w[j], to2));
+      }
+      above += pair_total<T>(c);
+      if ((in[0] | in[1] | in[2] | in[3]) == 0u) return;
+      uint32_t m = 0u;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        if constexpr (sizeof(Bits) == 4) m |= in[j] & (1u << j);
+        else m |= ((in[j >> 1] >> (16 * (j & 1))) & 1u) << j;
+      }
+      while (m) {
+        const uint32_t i = pos + (uint32_t)(__ffs(m) - 1);
+        m &= m - 1u;
+        fn(at(i), i);
+      }
+    });
+    return above;
   }
 };
 
-// The cluster's listed tokens, all of them in every CTA.
+// The listed tokens: one part per CTA of the cluster (or, listed whole, a
+// single part), whose tokens are spread over a share of the warps.
 template <typename T>
 struct List {
   const SampleSmemHeader* s;
-  int part_bits;  // log2 of the entries in one CTA's part
+  int parts_bits;  // log2 of the number of parts
   template <typename Fn>
   __device__ __forceinline__ void each(Fn fn) const {
-#pragma unroll
-    for (int i = threadIdx.x; i < kListTotal; i += kSampleThreads) {
-      if ((uint32_t)(i & ((1 << part_bits) - 1)) >= s->list_count[i >> part_bits]) continue;
-      const unsigned long long e = s->list[i];
-      fn(SampleKey<T>::value((uint32_t)(e >> 32)), (uint32_t)e);
+    const int warp = threadIdx.x >> 5, part = warp & ((1 << parts_bits) - 1);
+    const int step = kSampleThreads >> parts_bits, n = (int)s->list_count[part];
+    const unsigned long long* e = s->list + ((size_t)part << (kListBits - parts_bits));
+    for (int i = (warp >> parts_bits) * 32 + (threadIdx.x & 31); i < n; i += step) {
+      const unsigned long long x = e[i];
+      fn(SampleKey<T>::value((uint32_t)(x >> 32)), (uint32_t)x);
     }
   }
 };
@@ -255,30 +395,34 @@ __device__ __forceinline__ double widen(float f) {
 // multiple of 1/256 is q / 256, and 2^y = 2^(q / 256) * 2^(y - q / 256): a table
 // entry, an exponent, and the Taylor polynomial of 2^r = exp(r ln 2) to degree
 // 3 on |r| <= 1/512 (the next term is below 1.4e-13 and nearly the same for all).
+constexpr int kFineBins = 24 * 16;
+static_assert(kFineBins + 4 * (kMaxShift + 1 - 24) < kBins, "every weight has a bin");
+static_assert(kExpTable == 256, "bins are cut from multiples of 1/256");
+
 struct Weigher {
   int shift;
   double vmax, per_octave;  // the largest value; log2(e) / T
   const double* table;
 
-  __device__ __forceinline__ double log_weight(float v, int* q, double* r) const {
+  __device__ __forceinline__ void log_weight(float v, int* q, double* r) const {
     constexpr double kMagic = 26388279066624.0;  // 1.5 * 2^44: its last place is 1/256
     const double y = fma(widen(v) - vmax, per_octave, (double)shift);
     const double t = y + kMagic;
     *q = __double2loint(t);
     *r = y - (t - kMagic);
-    return y;
   }
-  // Weighing bin: 2^kOctaveBits per octave below the maximum (only for y >= -1).
-  __device__ __forceinline__ int bin(int q) const { return (shift * kExpTable - q) >> (kExpBits - kOctaveBits); }
-  __device__ __forceinline__ int bin_of(float v) const {
-    int q;
-    double r;
-    return log_weight(v, &q, &r) >= -1.0 ? bin(q) : kBins;
+  // Weighing bin: sixteenths of an octave down to 2^-24 of
+  // the maximum, quarters below.
+  __device__ __forceinline__ int bin(int q) const {
+    const int t = shift * kExpTable - q;
+    return min(t >> 4, (t >> 6) + kFineBins - kFineBins / 4);
   }
+  // Values below this weigh nothing (they would round to 0).
+  __device__ __forceinline__ double cut() const { return vmax - (double)(shift + 1) / per_octave; }
+  // The weight of a value of at least cut(), and its q.
   __device__ __forceinline__ unsigned long long weigh(float v, int* q) const {
     double r;
-    const double y = log_weight(v, q, &r);
-    if (!(y >= -1.0)) return 0ull;  // rounds to nothing
+    log_weight(v, q, &r);
     double p = fma(r, 5.5504108664821580e-02, 2.4022650695910072e-01);  // ln2^3 / 6, ln2^2 / 2
     p = fma(p, r, 6.9314718055994531e-01);                             // ln2
     const double m = table[*q & (kExpTable - 1)];
@@ -297,9 +441,9 @@ struct Weigher {
   // Values that bin j may hold: [lo, hi], 0.02 of a multiple of 1/256 wider than
   // the bin on both sides (rounding moves a border by less).
   __device__ __forceinline__ void bin_range(int j, double* lo, double* hi) const {
-    constexpr double kWidth = kExpTable >> kOctaveBits;
-    *hi = vmax + (-kWidth * j + 0.52) / kExpTable / per_octave;
-    *lo = vmax + (-kWidth * (j + 1) + 0.48) / kExpTable / per_octave;
+    const auto first = [](int k) { return k < kFineBins ? 16.0 * k : 64.0 * (k - kFineBins) + 16.0 * kFineBins; };
+    *hi = vmax + (0.52 - first(j)) / kExpTable / per_octave;
+    *lo = vmax + (0.48 - first(j + 1)) / kExpTable / per_octave;
   }
 };
 
@@ -322,8 +466,7 @@ struct Team {
   SampleSmemHeader* s;  // (this CTA's)
   cg::cluster_group cluster;
   int rank, size, size_bits;
-  int buf;          // which half of `word` the next all-gather uses
-  bool list_in_use; // a list may still be read by other CTAs
+  int buf;  // which half of `word` the next all-gather uses
 
   // All-gather of one value per CTA (the same in all its threads): the returned
   // array holds rank r's at index r until the all-gather after the next.
@@ -364,11 +507,10 @@ __device__ __forceinline__ unsigned long long cluster_sum(Team& team, uint32_t c
 
 // ---- bins ----------------------------------------------------------------------
 __device__ __forceinline__ void clear_bins(SampleSmemHeader* s) {
-  // lo and hi together are one array of 2 * kBins words
-  reinterpret_cast<uint4*>(s->lo)[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+  s->lo[threadIdx.x] = 0u;
+  s->hi[threadIdx.x] = 0u;
   __syncthreads();
 }
-static_assert(2 * kBins == 4 * kSampleThreads, "one 16-byte store per thread clears the bins");
 
 // 64-bit sum in two 32-bit words: the old low word tells the carry.
 __device__ __forceinline__ void add_to_bin(SampleSmemHeader* s, uint32_t bin, unsigned long long m) {
@@ -379,60 +521,49 @@ __device__ __forceinline__ void add_to_bin(SampleSmemHeader* s, uint32_t bin, un
   if (m_hi) atomicAdd(&s->hi[bin], m_hi);
 }
 
-// Sums of a thread's two bins and the running sum before them.
+// Sum of a thread's bin and the running sum before it.
 struct BinSums {
-  unsigned long long before, a, b;
-  // Whether one of the two is where the running sum passes the target; if so
-  // publishes it.
-  __device__ __forceinline__ void pick(SampleSmemHeader* s, unsigned long long target) const {
-    if (before <= target && target < before + a + b) {
-      const bool second = target >= before + a;
-      s->pick[0] = 2 * threadIdx.x + (second ? 1 : 0);
-      s->pick[1] = second ? before + a : before;
-      s->pick[2] = second ? b : a;
+  unsigned long long before, own;
+  // If the bin is where the running sum passes the target, publishes it in
+  // s->pick[slot] (read after the next barrier).
+  __device__ __forceinline__ void pick(SampleSmemHeader* s, int slot, unsigned long long target) const {
+    if (before <= target && target < before + own) {
+      s->pick[slot][0] = threadIdx.x;
+      s->pick[slot][1] = before;
+      s->pick[slot][2] = own;
     }
-    __syncthreads();
   }
 };
 
 // Closes a filling pass: the bins' sums over the cluster, or (local) this
-// CTA's. s->pick[3] holds the sum of all bins after the next barrier.
-__device__ __forceinline__ BinSums sum_bins(Team& team, bool local) {
+// CTA's; *total: the sum of all bins.
+__device__ __forceinline__ BinSums sum_bins(Team& team, bool local, unsigned long long* total) {
   SampleSmemHeader* s = team.s;
   const int tid = threadIdx.x;
   __syncthreads();
-  const uint2 lo = reinterpret_cast<const uint2*>(s->lo)[tid], hi = reinterpret_cast<const uint2*>(s->hi)[tid];
   BinSums v;
-  v.a = lo.x + ((unsigned long long)hi.x << 32);
-  v.b = lo.y + ((unsigned long long)hi.y << 32);
-  if (!local && team.size > 1) {
-    s->tot[tid] = make_ulonglong2(v.a, v.b);
+  v.own = s->lo[tid] + ((unsigned long long)s->hi[tid] << 32);
+  if (!local) {
+    s->tot[tid] = v.own;
     team.cluster.sync();
-    v.a = v.b = 0ull;
-    for (int r0 = 0; r0 < team.size; r0 += 4) {  // independent loads, four in flight
-      ulonglong2 x[4];
+    v.own = 0ull;
+    for (int r0 = 0; r0 < team.size; r0 += 8) {  // independent loads, eight in flight
+      unsigned long long x[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        x[k] = r0 + k < team.size ? team.cluster.map_shared_rank(s->tot, r0 + k)[tid] : make_ulonglong2(0ull, 0ull);
+      for (int k = 0; k < 8; ++k)
+        x[k] = r0 + k < team.size ? team.cluster.map_shared_rank(s->tot, r0 + k)[tid] : 0ull;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v.a += x[k].x;
-        v.b += x[k].y;
-      }
+      for (int k = 0; k < 8; ++k) v.own += x[k];
     }
   }
-  const unsigned long long incl = warp_scan_u64(v.a + v.b);
+  const unsigned long long incl = warp_scan_u64(v.own);
   if ((tid & 31) == 31) s->scan[tid >> 5] = incl;
   __syncthreads();
-  v.before = incl - (v.a + v.b);
-  unsigned long long total = 0ull;
-#pragma unroll
-  for (int w = 0; w < kSampleWarps; ++w) {
-    const unsigned long long x = s->scan[w];
-    if (w < (tid >> 5)) v.before += x;
-    total += x;
-  }
-  if (tid == 0) s->pick[3] = total;
+  // every warp scans the warps' totals
+  const unsigned long long w = warp_scan_u64((tid & 31) < kSampleWarps ? s->scan[tid & (kSampleWarps - 1)] : 0ull);
+  const unsigned long long before_warp = __shfl_sync(FULL_MASK, w, max((tid >> 5) - 1, 0));
+  *total = __shfl_sync(FULL_MASK, w, 31);
+  v.before = incl - v.own + (tid >= 32 ? before_warp : 0ull);
   return v;
 }
 
@@ -442,34 +573,38 @@ struct Found {
   unsigned long long above, own;
 };
 
-// Goes on with a search inside keys [klo, khi] of `tokens` (those that `member`
-// accepts): the first key, from khi down, at which the running sum of
-// measure(value) passes `target`, which it does (the caller knows the sum).
-// local: every CTA holds all the tokens.
-template <typename T, typename Tokens, typename Measure, typename Member>
+// Goes on with a search inside keys [klo, khi] of `tokens` (those that
+// take(value, &measure) accepts): the first key, from khi down, at which the
+// running sum of the measure passes `target`, which it does (the caller knows
+// the sum). local: every CTA holds all the tokens.
+template <typename T, typename Tokens, typename Take>
 __device__ __forceinline__ Found search(Team& team, bool local, const Tokens& tokens, uint32_t klo, uint32_t khi,
-                                        Measure measure, Member member, unsigned long long target) {
+                                        Take take, unsigned long long target) {
   SampleSmemHeader* s = team.s;
   Found f{khi, 0ull, 0ull};
-  for (;;) {
+  for (int slot = 0;; slot ^= 1) {
     const int width = 32 - __clz(khi - klo);  // bits of the range (0: a single key)
     const int sh = width > kBinBits ? width - kBinBits : 0;
     clear_bins(s);
     tokens.each([&](float v, uint32_t) {
       const uint32_t key = SampleKey<T>::from_value(v);
-      if (key >= klo && key <= khi && member(v)) add_to_bin(s, (khi - key) >> sh, measure(v));
+      unsigned long long m;
+      if (key >= klo && key <= khi && take(v, &m)) add_to_bin(s, (khi - key) >> sh, m);
     });
-    const BinSums sums = sum_bins(team, local);
-    sums.pick(s, target);
-    const uint32_t bin = (uint32_t)s->pick[0] & (kBins - 1);
-    f.above += s->pick[1];
-    f.own = s->pick[2];
-    target -= s->pick[1];
+    unsigned long long total;
+    sum_bins(team, local, &total).pick(s, slot, target);
+    if (local) __syncthreads();
+    else team.cluster.sync();  // (and the CTAs have read one another's bins)
+    const uint32_t bin = (uint32_t)s->pick[slot][0] & (kBins - 1);
+    f.above += s->pick[slot][1];
+    f.own = s->pick[slot][2];
+    target -= s->pick[slot][1];
     khi -= bin << sh;
     f.key = khi;
-    if (!local) team.cluster.sync();  // the CTAs have read one another's bins
-    else __syncthreads();             // the pick has been read
-    if (sh == 0) return f;
+    if (sh == 0) {
+      __syncthreads();  // the pick has been read
+      return f;
+    }
     const uint32_t span = (1u << sh) - 1u;
     klo = khi - klo > span ? khi - span : klo;
   }
@@ -477,26 +612,28 @@ __device__ __forceinline__ Found search(Team& team, bool local, const Tokens& to
 
 // ---- listing ---------------------------------------------------------------------
 __device__ __forceinline__ void open_list(Team& team) {
-  if (team.list_in_use) team.cluster.sync();  // nobody reads the last list any more
-  team.list_in_use = true;
   __syncthreads();
   if (threadIdx.x == 0) team.s->listed = 0u;
   __syncthreads();
 }
 
-// Offers a token to the list: every CTA of the cluster gets it.
-__device__ __forceinline__ void list_token(const Team& team, uint32_t key, uint32_t at) {
-  const uint32_t i = atomicAdd(&team.s->listed, 1u);
-  const uint32_t part = kListTotal >> team.size_bits;
-  if (i >= part) return;
-  const unsigned long long e = ((unsigned long long)key << 32) | at;
-  for (int r = 0; r < team.size; ++r) team.cluster.map_shared_rank(team.s->list, r)[team.rank * part + i] = e;
+// Writes an entry of the first CTA's list.
+__device__ __forceinline__ void put_in_list(const Team& team, uint32_t i, uint32_t key, uint32_t at) {
+  team.cluster.map_shared_rank(team.s->list, 0)[i] = ((unsigned long long)key << 32) | at;
 }
 
-// After a listing pass: whether every CTA's part fits, and the cluster's sum of `count`.
+// Offers a token to the CTA's part of the list.
+__device__ __forceinline__ void list_token(const Team& team, uint32_t key, uint32_t at) {
+  const uint32_t i = atomicAdd(&team.s->listed, 1u), part_bits = (uint32_t)(kListBits - team.size_bits);
+  if (i < (1u << part_bits)) put_in_list(team, ((uint32_t)team.rank << part_bits) + i, key, at);
+}
+
+// After a listing pass: whether every CTA's part fits (then the first CTA has
+// them all and goes on alone), and the cluster's sum of `count`. A list that
+// does not fit is not read, so the next may be written at once.
 __device__ __forceinline__ bool close_list(Team& team, uint32_t count, unsigned long long* sum) {
   SampleSmemHeader* s = team.s;
-  const uint32_t part = kListTotal >> team.size_bits;
+  const uint32_t part = 1u << (kListBits - team.size_bits);
   count = block_sum(count, s);
   const uint32_t mine = min(s->listed, part + 1u);
   const unsigned long long* all = team.gather(((unsigned long long)mine << 32) | count);
@@ -512,11 +649,11 @@ __device__ __forceinline__ bool close_list(Team& team, uint32_t count, unsigned 
   return fits;
 }
 
-// Bin of the top-k search: 128ths of an octave of the distance to the maximum,
+// Bin of the top-k search: 64ths of an octave of the distance to the maximum,
 // from 1/4 to 64; nearer and farther tokens share the first and last.
-constexpr uint32_t kDistanceBase = 0x3e800000u >> 16;
+constexpr uint32_t kDistanceShift = 17, kDistanceBase = 0x3e800000u >> kDistanceShift;
 __device__ __forceinline__ uint32_t distance_bin(float vmax, float v) {
-  return min((__float_as_uint(vmax - v + 0.25f) >> 16) - kDistanceBase, (uint32_t)kBins - 1u);
+  return min((__float_as_uint(vmax - v + 0.25f) >> kDistanceShift) - kDistanceBase, (uint32_t)kBins - 1u);
 }
 
 template <typename T>
@@ -525,12 +662,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   using Bits = typename DTypeTraits<T>::Bits;
   extern __shared__ __align__(128) unsigned char smem[];
   SampleSmemHeader* s = reinterpret_cast<SampleSmemHeader*>(smem);
-  Team team{s, cg::this_cluster(), 0, 0, 0, 0, false};
+  Team team{s, cg::this_cluster(), 0, 0, 0, 0};
   team.rank = (int)team.cluster.block_rank();
   team.size = (int)team.cluster.num_blocks();
   team.size_bits = 31 - __clz(team.size);
   const int b = blockIdx.x / team.size, tid = threadIdx.x;
-  const bool leader = team.rank == 0 && tid == 0;
 
   // ---- the row and its settings ---------------------------------------------
   Slice<T> slice;
@@ -549,16 +685,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   const float top_p = p.top_ps ? p.top_ps[b] : p.top_p;
   const float min_p = p.min_ps ? p.min_ps[b] : p.min_p;
   const float u = p.uniforms[b];
-  const bool valid = temperature >= 0.f && temperature < INFINITY && top_p == top_p && min_p == min_p && u >= 0.f &&
-                     u < 1.f;
-  if (!valid) {
-    if (leader) {
-      p.token_ids[b] = -1;
-      if (p.logprobs) p.logprobs[b] = __int_as_float(0x7fc00000);
-      if (p.kept) p.kept[b] = 0;
-    }
-    return;  // the whole cluster returns
-  }
   // every CTA of the cluster runs before its shared memory is written to
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const int64_t n = slice.row.n;
@@ -573,6 +699,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   uint32_t legal = 0u;
   float vmax = slice.load(legal);
   if (tid < kExpTable) s->exp2_table[tid] = exp2((double)tid / kExpTable);
+  if (tid == 0) s->listed = 0u;
   {
     const uint32_t key = __reduce_max_sync(FULL_MASK, K::from_value(vmax));
     legal = __reduce_add_sync(FULL_MASK, legal);
@@ -586,29 +713,35 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   legal = __reduce_add_sync(FULL_MASK, (tid & 31) < kSampleWarps ? s->warp[1][tid & (kSampleWarps - 1)] : 0u);
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   unsigned long long kept = 0ull;  // tokens left so far
+  uint32_t list_base = 0u;         // legal tokens of the CTAs before this one
   {
     const unsigned long long* all = team.gather(((unsigned long long)legal << 32) | kmax);
     for (int r = 0; r < team.size; ++r) {
-      kmax = max(kmax, (uint32_t)all[r]);
-      kept += all[r] >> 32;
+      const unsigned long long x = all[r];
+      kmax = max(kmax, (uint32_t)x);
+      kept += x >> 32;
+      if (r < team.rank) list_base += (uint32_t)(x >> 32);
     }
   }
-  if (kmax == 0u) {  // nothing is legal
-    if (leader) {
-      p.token_ids[b] = 0;
-      if (p.logprobs) p.logprobs[b] = -INFINITY;
+  const bool valid = temperature >= 0.f && temperature < INFINITY && top_p == top_p && min_p == min_p && u >= 0.f &&
+                     u < 1.f;
+  if (!valid || kmax == 0u) {  // not to be drawn, or nothing is legal
+    if (team.rank == 0 && tid == 0) {
+      p.token_ids[b] = valid ? 0 : -1;
+      if (p.logprobs) p.logprobs[b] = valid ? -INFINITY : __int_as_float(0x7fc00000);
       if (p.kept) p.kept[b] = 0;
     }
     return;
   }
   vmax = K::value(kmax);
+  const float vmin = K::value(K::kNegInf + 1u);  // the lowest legal value
   const bool infinite = !(vmax < INFINITY);
-  const List<T> list{s, 31 - __clz(kListTotal) - team.size_bits};
+  List<T> list{s, team.size_bits};
 
   float draw_value = vmax;
   unsigned long long ordinal = 0ull;  // among the tokens of draw_value, by rising position
   float logprob = 0.f;
-  bool listed = false;  // the list holds every token of draw_value
+  bool solo = false;  // the list holds all that is still needed: this CTA goes on alone
   if (temperature > 0.f && !infinite) {
     Weigher weigh;
     weigh.shift = min(kMaxShift, 62 - (64 - __clzll((unsigned long long)n)));
@@ -616,34 +749,59 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
     weigh.per_octave = 1.4426950408889634 / (double)temperature;
     weigh.table = s->exp2_table;
     // ---- the kept set: values above `border`, and `ties` tokens at it --------------
-    float border = -INFINITY;             // (none: every legal token)
+    float border = vmin;
     unsigned long long ties = ~0ull, excess = 0ull;  // excess: tokens at the border beyond `ties`
-    bool in_list = false;                 // the list holds every token >= border
-    const auto all_of = [](float) { return true; };
+    bool in_list = false;                            // the list holds every kept token
+    const auto one = [](float, unsigned long long* m) {
+      *m = 1ull;
+      return true;
+    };
+    if (kept <= kListTotal) {
+      // few legal tokens: all of them, each CTA's behind the others'
+      slice.each_between(vmin, vmax, vmin, vmax, [&](float v, uint32_t at) {
+        put_in_list(team, list_base + atomicAdd(&s->listed, 1u), K::from_value(v), at);
+      });
+      if (tid < kMaxCluster) s->list_count[tid] = tid == 0 ? (uint32_t)kept : 0u;
+      list.parts_bits = 0;
+      team.cluster.sync();
+      if (team.rank != 0) return;
+      in_list = solo = true;
+    }
     if (top_k > 0 && (unsigned long long)top_k < kept) {
-      const auto one = [](float) { return 1ull; };
-      clear_bins(s);
-      slice.each([&](float v, uint32_t) {
-        if (v > -INFINITY) atomicAdd(&s->lo[distance_bin(vmax, v)], 1u);
-      });
       const unsigned long long target = (unsigned long long)top_k - 1ull;
-      sum_bins(team, false).pick(s, target);
-      // every token down to the picked bin: its lower border, a little wider
-      const int j = (int)s->pick[0] & (kBins - 1);
-      float low = -INFINITY;
-      if (j < kBins - 1) {
-        const float edge = __uint_as_float((uint32_t)(j + 1 + kDistanceBase) << 16) - 0.25f;
-        low = K::value_at_least((double)vmax - (double)edge * 1.00001 - 1e-6 * fabs((double)vmax));
+      uint32_t klo = 1u;
+      if (in_list) {  // the lowest listed key bounds the range
+        uint32_t low = kmax;
+        list.each([&](float v, uint32_t) { low = min(low, K::from_value(v)); });
+        low = __reduce_min_sync(FULL_MASK, low);
+        if ((tid & 31) == 0) s->warp[0][tid >> 5] = low;
+        __syncthreads();
+        klo = __reduce_min_sync(FULL_MASK, s->warp[0][tid & (kSampleWarps - 1)]);
+      } else {
+        clear_bins(s);
+        slice.each([&](float v, uint32_t) {
+          if (v > -INFINITY) atomicAdd(&s->lo[distance_bin(vmax, v)], 1u);
+        });
+        unsigned long long total;
+        sum_bins(team, false, &total).pick(s, 0, target);
+        __syncthreads();
+        // every token down to the picked bin: its lower border, a little wider
+        const int j = (int)s->pick[0][0] & (kBins - 1);
+        float low = vmin;
+        if (j < kBins - 1) {
+          const float edge = __uint_as_float((uint32_t)(j + 1 + kDistanceBase) << kDistanceShift) - 0.25f;
+          low = fmaxf(vmin, K::value_at_least((double)vmax - (double)edge * 1.00001 - 1e-6 * fabs((double)vmax)));
+        }
+        open_list(team);
+        slice.each_between(low, vmax, low, vmax,
+                           [&](float v, uint32_t at) { list_token(team, K::from_value(v), at); });
+        unsigned long long unused;
+        in_list = solo = close_list(team, 0u, &unused);
+        if (solo && team.rank != 0) return;
+        if (in_list) klo = K::from_value(low);
       }
-      open_list(team);
-      slice.each([&](float v, uint32_t at) {
-        if (v >= low && v > -INFINITY) list_token(team, K::from_value(v), at);
-      });
-      unsigned long long unused;
-      in_list = close_list(team, 0u, &unused);
-      const uint32_t klo = max(K::from_value(low), 1u);
-      const Found f = in_list ? search<T>(team, true, list, klo, kmax, one, all_of, target)
-                              : search<T>(team, false, slice, 1u, kmax, one, all_of, target);
+      const Found f = in_list ? search<T>(team, true, list, klo, kmax, one, target)
+                              : search<T>(team, false, slice, klo, kmax, one, target);
       border = K::value(f.key);
       ties = (unsigned long long)top_k - f.above;
       excess = f.own - ties;
@@ -662,88 +820,105 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
           kept = block_sum(count, s);
         } else {
           open_list(team);
-          slice.each([&](float v, uint32_t at) {
-            if (v >= border && v > -INFINITY) {
-              ++count;
-              list_token(team, K::from_value(v), at);
-            }
+          slice.each_between(border, vmax, border, vmax, [&](float v, uint32_t at) {
+            ++count;
+            list_token(team, K::from_value(v), at);
           });
-          in_list = close_list(team, count, &kept);
+          in_list = solo = close_list(team, count, &kept);
+          if (solo && team.rank != 0) return;
         }
       }
     }
     // ---- weigh what is left, by bins ---------------------------------------------
     clear_bins(s);
+    const float lowest = fmaxf(border, fminf(vmax, K::value_at_least(weigh.cut())));
     const auto into_bin = [&](float v, uint32_t) {
-      if (!(v >= border)) return;
       int q;
       const unsigned long long w = weigh.weigh(v, &q);
-      if (w) add_to_bin(s, (uint32_t)weigh.bin(q), w);
+      if (v >= lowest) add_to_bin(s, (uint32_t)weigh.bin(q), w);
     };
     if (in_list) list.each(into_bin);
     else slice.each(into_bin);
-    const BinSums bins = sum_bins(team, in_list);
-    __syncthreads();
-    unsigned long long sum = s->pick[3];
-    if (excess) sum -= excess * weigh(border);
-    // The bin at which the running sum passes `target`, and the search inside
-    // it; *n_above: tokens in the bins above it (where the list holds the bin alone).
-    const auto find = [&](unsigned long long target, unsigned long long* n_above) {
-      bins.pick(s, target);
-      const int j = (int)s->pick[0];
-      const unsigned long long before = s->pick[1];
-      double lo, hi;
-      weigh.bin_range(j, &lo, &hi);
-      const float flo = fmaxf(border, K::value_at_least(lo)), fhi = fminf(vmax, K::value_at_least(hi));
-      const uint32_t khi = K::from_value(fhi), klo = min(max(K::from_value(flo), 1u), khi);
-      const auto in_bin = [&](float v) { return weigh.bin_of(v) == j; };
-      Found f;
-      if (in_list) {
-        listed = true;
-        __syncthreads();  // the pick has been read
-        f = search<T>(team, true, list, klo, khi, weigh, in_bin, target - before);
-      } else {
-        open_list(team);
-        uint32_t count = 0u;
-        slice.each([&](float v, uint32_t at) {
-          if (v > fhi) {
-            ++count;
-          } else if (v >= flo && v > -INFINITY) {
-            const int mine = weigh.bin_of(v);
-            if (mine == j) list_token(team, K::from_value(v), at);
-            else count += mine < j ? 1u : 0u;
-          }
-        });
-        listed = close_list(team, count, n_above);
-        f = listed ? search<T>(team, true, list, klo, khi, weigh, all_of, target - before)
-                   : search<T>(team, false, slice, klo, khi, weigh, in_bin, target - before);
-      }
+    unsigned long long sum;
+    const BinSums bins = sum_bins(team, in_list, &sum);
+    if (excess && border >= lowest) sum -= excess * weigh(border);
+    // Values of a bin, as [*from, *to], a little wider than it.
+    const auto bin_values = [&](int first, int last, float* from, float* to) {
+      double lo, hi, unused;
+      weigh.bin_range(first, &unused, &hi);
+      weigh.bin_range(last, &lo, &unused);
+      *from = fmaxf(lowest, K::value_at_least(lo));
+      *to = fmaxf(*from, fminf(vmax, K::value_at_least(hi)));
+    };
+    // The search for `target` inside bin j (its sum before the bin, its values).
+    const auto within = [&](int j, float from, float to, unsigned long long before, unsigned long long target) {
+      const auto in_bin = [&](float v, unsigned long long* m) {
+        int q;
+        *m = weigh.weigh(v, &q);
+        return weigh.bin(q) == j;
+      };
+      const uint32_t klo = K::from_value(from), khi = K::from_value(to);
+      Found f = solo ? search<T>(team, true, list, klo, khi, in_bin, target - before)
+                     : search<T>(team, false, slice, klo, khi, in_bin, target - before);
       f.above += before;
       return f;
     };
+    const unsigned long long p_target = top_p < 1.f ? prefix_target(top_p, sum) : 0ull;
+    int p_bin = 0;
+    unsigned long long p_before = 0ull, most = sum;  // most: the kept weight, at most
+    float p_from = 0.f, p_to = 0.f;
     if (top_p < 1.f) {
-      const unsigned long long target = prefix_target(top_p, sum);
-      unsigned long long n_above = 0ull;
-      const Found f = find(target, &n_above);
+      bins.pick(s, 0, p_target);
+      __syncthreads();
+      p_bin = (int)s->pick[0][0];
+      p_before = s->pick[0][1];
+      most = min(sum, p_before + s->pick[0][2]);
+      bin_values(p_bin, p_bin, &p_from, &p_to);
+      __syncthreads();  // the pick has been read
+    }
+    const unsigned long long u64 = fraction64(u);
+    unsigned long long n_above = 0ull;
+    if (!in_list) {
+      // list the border's bin and the bins the draw can fall into
+      float from, to;
+      bins.pick(s, 0, __umul64hi(u64, top_p < 1.f ? p_before + 1ull : sum));
+      bins.pick(s, 1, __umul64hi(u64, most));
+      __syncthreads();
+      bin_values((int)s->pick[0][0], (int)s->pick[1][0], &from, &to);
+      if (!(top_p < 1.f)) p_from = from, p_to = to;
+      open_list(team);
+      const uint32_t above = slice.each_between(
+          p_from, p_to, from, to, [&](float v, uint32_t at) { list_token(team, K::from_value(v), at); });
+      solo = close_list(team, above, &n_above);
+      if (solo && team.rank != 0) return;
+    }
+    if (top_p < 1.f) {
+      const Found f = within(p_bin, p_from, p_to, p_before, p_target);
       const float value = K::value(f.key);
       const unsigned long long w = weigh(value);
-      ties = (target - f.above) / w + 1ull;
+      ties = (p_target - f.above) / w + 1ull;
       sum = f.above + ties * w;
-      // how many that keeps: those above the bin, and above the value within it
+      // how many that keeps (of a list of bins: those above the border's bin have been counted)
       uint32_t count = 0u;
-      const auto above_value = [&](float v, uint32_t) { count += v > value ? 1u : 0u; };
-      if (listed) {
-        list.each(above_value);
-        kept = ties + block_sum(count, s) + (in_list ? 0ull : n_above);
+      if (solo) {
+        const float top = in_list ? vmax : p_to;
+        list.each([&](float v, uint32_t) { count += v > value && v <= top ? 1u : 0u; });
+        kept = ties + block_sum(count, s) + n_above;
       } else {
-        slice.each(above_value);
+        slice.each([&](float v, uint32_t) { count += v > value ? 1u : 0u; });
         kept = ties + cluster_sum(team, count);
       }
     }
     // ---- the draw ------------------------------------------------------------------
-    const unsigned long long target = __umul64hi(fraction64(u), sum);
-    unsigned long long unused;
-    const Found f = find(target, &unused);
+    const unsigned long long target = __umul64hi(u64, sum);
+    bins.pick(s, 0, target);
+    __syncthreads();
+    const int j = (int)s->pick[0][0];
+    const unsigned long long before = s->pick[0][1];
+    __syncthreads();  // the pick has been read
+    float from, to;
+    bin_values(j, j, &from, &to);
+    const Found f = within(j, from, to, before, target);
     draw_value = K::value(f.key);
     ordinal = (target - f.above) / weigh(draw_value);
     logprob = (float)(((double)draw_value - (double)vmax) / (double)temperature -
@@ -769,19 +944,33 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
     if (p.logprobs) p.logprobs[b] = logprob;
     if (p.kept) p.kept[b] = (int32_t)kept;
   };
-  if (listed) {  // every CTA holds all of them: the first one answers
-    if (team.rank != 0) return;
-    // the positions of draw_value's tokens, into the bins' space; each counts those before it
-    uint32_t* ties_at = s->lo;
-    static_assert(kListTotal <= 2 * kBins, "the listed positions fit the bins' space");
+  if (solo) {
+    // the positions of draw_value's tokens, into the table's space; each counts those before it
+    uint32_t* ties_at = reinterpret_cast<uint32_t*>(s->exp2_table);
+    constexpr uint32_t kTiesCap = sizeof(s->exp2_table) / sizeof(uint32_t);
     __syncthreads();
     if (tid == 0) s->listed = 0u;
     __syncthreads();
     list.each([&](float v, uint32_t at) {
-      if (v == draw_value) ties_at[atomicAdd(&s->listed, 1u)] = at;
+      if (v != draw_value) return;
+      const uint32_t i = atomicAdd(&s->listed, 1u);
+      if (i < kTiesCap) ties_at[i] = at;
     });
     __syncthreads();
     const uint32_t m = s->listed;
+    if (m > kTiesCap) {  // very many ties: each counts those before it in the list itself
+      list.each([&](float v, uint32_t at) {
+        if (v != draw_value) return;
+        uint32_t lower = 0u;
+        for (int r = 0; r < (1 << list.parts_bits); ++r)
+          for (uint32_t k = 0; k < s->list_count[r]; ++k) {
+            const unsigned long long e = s->list[((uint32_t)r << (kListBits - list.parts_bits)) + k];
+            lower += ((uint32_t)(e >> 32) == K::from_value(draw_value) && (uint32_t)e < at) ? 1u : 0u;
+          }
+        if (lower == ordinal) put(at);
+      });
+      return;
+    }
     for (uint32_t i = tid; i < m; i += kSampleThreads) {
       const uint32_t at = ties_at[i];
       uint32_t lower = 0u;

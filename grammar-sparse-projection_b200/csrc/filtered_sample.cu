@@ -23,8 +23,7 @@
 // another's bins over distributed shared memory after one cluster barrier, and
 // each picks the bin at which the running sum passes the target.
 //   * The first bins are chosen by value, so that few tokens share one:
-//     sixteenths of an octave of the weight (quarters below 2^-24), or (top-k)
-//     64ths of an octave of the distance to the maximum. They do not depend on
+//     sixteenths of an octave of the weight, or (top-k) 64ths of an octave of the distance to the maximum. They do not depend on
 //     the target, so top-p and the draw use the same weighing.
 //   * The tokens of the picked bins (for top-p: of the border's bin and of those
 //     the draw can fall into) are then listed, key and position, in the first
@@ -58,11 +57,12 @@ constexpr int kBinBits = 9;
 constexpr int kBins = 1 << kBinBits;
 constexpr int kMaxCluster = 16;
 constexpr int kMaxShift = 50;
-constexpr int kExpBits = 8;
-constexpr int kExpTable = 1 << kExpBits;
+constexpr int kExpTable = 16;
+constexpr int kTiesCap = 512;    // tokens of one value whose positions are set side by side
 constexpr int kListBits = 12;
 constexpr int kListTotal = 1 << kListBits;  // tokens a cluster lists
 static_assert(kBins == kSampleThreads, "one bin per thread");
+static_assert(32 * 16 <= kBins, "32 octaves of weights in sixteenths");
 static_assert(kMaxCluster <= kSampleWarps, "a warp for each part of the list");
 
 // Order-preserving keys: larger logit, larger key (-0 and +0 alike); 0 for NaN
@@ -107,14 +107,16 @@ struct SampleKey<float> {
 };
 
 struct SampleSmemHeader {
-  uint32_t lo[kBins];                      // bins being filled: low and high halves of 64-bit sums
-  uint32_t hi[kBins];
+  uint32_t lo[kBins + 32];                 // bins being filled: low and high halves of 64-bit sums (and a
+  uint32_t hi[kBins + 32];                 // place for each lane's values that have none)
   unsigned long long tot[kBins];           // this CTA's bins, read by the cluster
   unsigned long long list[kListTotal];     // (key, position in the row), in parts (rank 0's is used)
   unsigned long long scan[kSampleWarps];
   unsigned long long pick[2][4];           // picked bin, sum before it, its own sum; [.][3] of 0: sum of all bins
   unsigned long long word[2][kMaxCluster]; // one value per CTA (all-gather)
-  double exp2_table[kExpTable];            // 2^(j / kExpTable)
+  double exp2_table[kExpTable];            // Weigher's
+  double log2_table[kExpTable];            // log2(1 + j / 16)
+  uint32_t ties_at[kTiesCap];              // positions of the drawn value's tokens
   uint32_t warp[2][kSampleWarps];
   uint32_t list_count[kMaxCluster];        // tokens in each part of the list
   uint32_t listed;                         // tokens this CTA has offered to the list
@@ -187,10 +189,10 @@ struct PairMax<__nv_bfloat16> {
   __device__ __forceinline__ float value() const { return fmaxf(__low2float(a), __high2float(a)); }
 };
 
-// One CTA's part of the row: positions [lo, lo + len), the first `resident`
-// of them in shared memory at index `phase` on (so that 16-byte loads of the
-// row and stores to shared memory are both aligned), the rest read from global
-// memory in every pass.
+// One CTA's part of the row: positions [lo, lo + len), as 16-byte vectors
+// aligned in global memory (position lo has place `phase` in the first). The
+// first `held_vectors` are kept in shared memory by load(), the others are read
+// from global memory (mostly L2) in every pass.
 template <typename T>
 struct Slice {
   using Bits = typename DTypeTraits<T>::Bits;
@@ -198,9 +200,18 @@ struct Slice {
   Row<T> row;
   Bits* held;
   int64_t lo, len;
-  int phase, resident;
+  int phase;
+  int vectors, held_vectors;
 
-  __device__ __forceinline__ int vectors() const { return (phase + resident + kVec - 1) / kVec; }
+  __device__ __forceinline__ void set(const Row<T>& r, int64_t lo_, int64_t len_, unsigned char* smem, int room) {
+    row = r;
+    lo = lo_;
+    len = len_;
+    held = reinterpret_cast<Bits*>(smem);
+    phase = (int)((reinterpret_cast<uintptr_t>(row.x + lo) & 15) / sizeof(Bits));
+    vectors = (int)((phase + len + kVec - 1) / kVec);
+    held_vectors = min(vectors, room);
+  }
 
   static __device__ __forceinline__ float unpack(const uint32_t (&w)[4], int j) {
     if constexpr (sizeof(Bits) == 4)
@@ -211,21 +222,65 @@ struct Slice {
       return DTypeTraits<T>::bits_to_float((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
   }
 
-  // Value at a position of the CTA's part.
+  // Value at a position of the part.
   __device__ __forceinline__ float at(int64_t pos) const {
-    const int64_t i = pos - lo;
-    return i < resident ? DTypeTraits<T>::bits_to_float(held[phase + i]) : load_value(row, pos);
+    const int64_t slot = pos - lo + phase;
+    return slot < (int64_t)held_vectors * kVec ? DTypeTraits<T>::bits_to_float(held[slot]) : load_value(row, pos);
   }
 
-  // Fills the resident part; returns the thread's largest value and its number
-  // of legal tokens over the whole part. Whole vectors four at a time, the
-  // loads ahead of their use; NaN stays (every comparison with it is false).
+  // A vector at the part's ends, of which only some places are its own (by
+  // value: nothing of the caller's goes through memory).
+  static __device__ __noinline__ uint4 end_vector(Row<T> row, int64_t pos, int64_t begin, int64_t end) {
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const bool mine = pos + j >= begin && pos + j < end;
+      const uint32_t bits = DTypeTraits<T>::round_bits(mine ? load_value(row, pos + j) : -INFINITY);
+      if constexpr (sizeof(Bits) == 4) w[j] = bits;
+      else w[j >> 1] |= bits << (16 * (j & 1));
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+
+  // Vector v from global memory (in two steps, so that several can be under
+  // way): its words, then -inf where the mask says not legal. NaN stays (every
+  // comparison with it is false).
+  __device__ __forceinline__ uint4 fetch(int v, uint32_t* legal) const {
+    const int64_t pos = lo - phase + (int64_t)v * kVec;
+    *legal = 0xffffffffu;
+    if (pos < lo || pos + kVec > lo + len) return end_vector(row, pos, lo, lo + len);
+    if (row.mask) {
+      const int64_t w0 = pos >> 5;
+      const int sh = (int)(pos & 31);
+      const uint32_t a = __ldg(row.mask + w0);
+      const uint32_t b = sh + kVec > 32 ? __ldg(row.mask + w0 + 1) : 0u;
+      *legal = __funnelshift_r(a, b, sh);
+    }
+    return ld_stream_v4(row.x + pos);
+  }
+  __device__ __forceinline__ void settle(const uint4& q, uint32_t legal, uint32_t (&w)[4]) const {
+    w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+    if (row.mask == nullptr) return;
+    constexpr uint32_t kIllegal = DTypeTraits<T>::kNegInfBits;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const bool ok = (legal >> j) & 1u;
+      if constexpr (sizeof(Bits) == 4)
+        w[j] = ok ? w[j] : kIllegal;
+      else if (j & 1)
+        w[j >> 1] = ok ? w[j >> 1] : (w[j >> 1] & 0xffffu) | (kIllegal << 16);
+      else
+        w[j >> 1] = ok ? w[j >> 1] : (w[j >> 1] & 0xffff0000u) | kIllegal;
+    }
+  }
+
+  // Reads the whole part, keeping the held vectors; returns the thread's
+  // largest value and its number of legal tokens. Four loads under way.
   __device__ __forceinline__ float load(uint32_t& legal_count) {
     constexpr int kAhead = 4;
-    const int nv = vectors(), whole0 = phase > 0 ? 1 : 0, whole1 = (phase + resident) / kVec;
     PairMax<T> most;
     legal_count = 0u;
-    for (int v0 = whole0 + threadIdx.x; v0 < whole1; v0 += kAhead * kSampleThreads) {
+    for (int v0 = threadIdx.x; v0 < vectors; v0 += kAhead * kSampleThreads) {
       uint4 q[kAhead];
       uint32_t legal[kAhead];
 #pragma unroll
@@ -233,37 +288,14 @@ struct Slice {
         const int v = v0 + k * kSampleThreads;
         q[k] = make_uint4(0u, 0u, 0u, 0u);
         legal[k] = 0u;
-        if (v < whole1) {
-          const int64_t i0 = lo + (int64_t)v * kVec - phase;
-          q[k] = ld_stream_v4(row.x + i0);
-          legal[k] = 0xffffffffu;
-          if (row.mask) {
-            const int64_t w0 = i0 >> 5;
-            const int sh = (int)(i0 & 31);
-            const uint32_t a = __ldg(row.mask + w0);
-            const uint32_t b = sh + kVec > 32 ? __ldg(row.mask + w0 + 1) : 0u;
-            legal[k] = __funnelshift_r(a, b, sh);
-          }
-        }
+        if (v < vectors) q[k] = fetch(v, &legal[k]);
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int v = v0 + k * kSampleThreads;
-        if (v >= whole1) break;
-        uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
-        if (row.mask) {
-          constexpr uint32_t kIllegal = DTypeTraits<T>::kNegInfBits;
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) {
-            const bool ok = (legal[k] >> j) & 1u;
-            if constexpr (sizeof(Bits) == 4)
-              w[j] = ok ? w[j] : kIllegal;
-            else if (j & 1)
-              w[j >> 1] = ok ? w[j >> 1] : (w[j >> 1] & 0xffffu) | (kIllegal << 16);
-            else
-              w[j >> 1] = ok ? w[j >> 1] : (w[j >> 1] & 0xffff0000u) | kIllegal;
-          }
-        }
+        if (v >= vectors) break;
+        uint32_t w[4];
+        settle(q[k], legal[k], w);
         uint32_t c = 0u;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -271,59 +303,33 @@ struct Slice {
           c += pair_count<T>(pair_above<T>(w[j], -INFINITY));
         }
         legal_count += pair_total<T>(c);
-        reinterpret_cast<uint4*>(held)[v] = make_uint4(w[0], w[1], w[2], w[3]);
+        if (v < held_vectors) reinterpret_cast<uint4*>(held)[v] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    float top = most.value();
-    // the first and last vectors where they are not whole
-    for (int i = threadIdx.x; i < 2 * kVec; i += kSampleThreads) {
-      const int v = i < kVec ? 0 : nv - 1;
-      if (v < 0 || (v >= whole0 && v < whole1) || (i >= kVec && nv == 1)) continue;
-      const int slot = v * kVec + i % kVec;
-      const bool mine = slot >= phase && slot < phase + resident;
-      const float f = mine ? load_value(row, lo + slot - phase) : -INFINITY;
-      held[slot] = DTypeTraits<T>::round_bits(f);
-      top = fmaxf(top, f);
-      legal_count += f > -INFINITY ? 1u : 0u;
-    }
-    for (int64_t i = resident + threadIdx.x; i < len; i += kSampleThreads) {
-      const float f = load_value(row, lo + i);
-      top = fmaxf(top, f);
-      legal_count += f > -INFINITY ? 1u : 0u;
-    }
-    return top;
+    return most.value();
   }
 
-  // fn(words, position of the first value) for every vector of the CTA's part
-  // (16 bytes of values; -inf or NaN: not legal, or not of the part)
+  // fn(words, position of the first value) for every vector of the part (-inf
+  // or NaN: not legal, or not of the part); the next one is under way meanwhile.
   template <typename Fn>
   __device__ __forceinline__ void each_vector(Fn fn) const {
-    const int nv = vectors();
-    const int total = nv + (int)((len - resident + kVec - 1) / kVec);
-    for (int v = threadIdx.x; v < total; v += kSampleThreads) {
-      uint32_t w[4];
-      int64_t pos = lo - phase + (int64_t)v * kVec;
-      if (v < nv) {
-        const uint4 q = reinterpret_cast<const uint4*>(held)[v];
-        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
-      } else {
-        pos = lo + resident + (int64_t)(v - nv) * kVec;
-        const uint4 q = gather_vector(row, pos, lo + len);
-        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+    uint4 next = make_uint4(0u, 0u, 0u, 0u);
+    uint32_t next_legal = 0u;
+    const auto get = [&](int v) {
+      if (v < held_vectors) {
+        next = reinterpret_cast<const uint4*>(held)[v];
+        next_legal = 0xffffffffu;
+      } else if (v < vectors) {
+        next = fetch(v, &next_legal);
       }
-      fn(w, (uint32_t)pos);
+    };
+    get(threadIdx.x);
+    for (int v = threadIdx.x; v < vectors; v += kSampleThreads) {
+      uint32_t w[4];
+      settle(next, next_legal, w);
+      get(v + kSampleThreads);
+      fn(w, (uint32_t)(lo - phase + (int64_t)v * kVec));
     }
-  }
-  // A vector of the part that is not resident (by value: nothing of the caller's goes through memory).
-  static __device__ __noinline__ uint4 gather_vector(Row<T> row, int64_t pos, int64_t end) {
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const uint32_t bits = DTypeTraits<T>::round_bits(pos + j < end ? load_value(row, pos + j) : -INFINITY);
-      if constexpr (sizeof(Bits) == 4) w[j] = bits;
-      else w[j >> 1] |= bits << (16 * (j & 1));
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
   }
   // fn(value) one by one
   template <typename Fn>
@@ -331,6 +337,19 @@ struct Slice {
     each_vector([&](const uint32_t (&w)[4], uint32_t pos) {
 #pragma unroll
       for (int j = 0; j < kVec; ++j) fn(unpack(w, j), pos + j);
+    });
+  }
+  // fn(four values) for all of them
+  template <typename Fn>
+  __device__ __forceinline__ void each_four(Fn fn) const {
+    each_vector([&](const uint32_t (&w)[4], uint32_t) {
+#pragma unroll
+      for (int h = 0; h < kVec / 4; ++h) {
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = unpack(w, 4 * h + j);
+        fn(f);
+      }
     });
   }
   // fn(value, position) for the values in [from, to] or [from2, to2], which are
@@ -383,67 +402,70 @@ struct List {
   }
 };
 
-// A finite float as a double by integer operations (the conversion unit is
-// slower); zero and subnormals become some value below 2^-126, which moves no
-// weight.
+// A finite value of type T as a double by integer operations (the conversion
+// unit is slower); zero and subnormals become some value below 2^-126, which
+// moves no weight. 16-bit types end in the high word.
+template <typename T>
 __device__ __forceinline__ double widen(float f) {
   const uint32_t u = __float_as_uint(f);
-  return __hiloint2double((int)((((uint32_t)((int)u >> 3)) & 0x8fffffffu) + (896u << 20)), (int)(u << 29));
+  return __hiloint2double((int)((((uint32_t)((int)u >> 3)) & 0x8fffffffu) + (896u << 20)),
+                          sizeof(typename DTypeTraits<T>::Bits) == 2 ? 0 : (int)(u << 29));
 }
 
 // Weight of a value in units of 2^-shift: with y = shift + log2 w, the nearest
-// multiple of 1/256 is q / 256, and 2^y = 2^(q / 256) * 2^(y - q / 256): a table
-// entry, an exponent, and the Taylor polynomial of 2^r = exp(r ln 2) to degree
-// 3 on |r| <= 1/512 (the next term is below 1.4e-13 and nearly the same for all).
-constexpr int kFineBins = 24 * 16;
-static_assert(kFineBins + 4 * (kMaxShift + 1 - 24) < kBins, "every weight has a bin");
-static_assert(kExpTable == 256, "bins are cut from multiples of 1/256");
-
+// multiple of 1/16 is q / 16, and 2^y = 2^(q / 16) * 2^(y - q / 16): a table
+// entry with its exponent, and the Taylor polynomial of 2^r = exp(r ln 2) to
+// degree 5 on |r| <= 1/32 (the next term is below 1.5e-13 and nearly the same
+// for all). Sixteen entries take each of the 32 banks once: whatever entries a
+// warp's lanes want, there is no bank conflict (with 256 entries and degree 3
+// the loads met 5 to a bank, and shared memory was what bound the pass).
+template <typename T>
 struct Weigher {
   int shift;
-  double vmax, per_octave;  // the largest value; log2(e) / T
-  const double* table;
+  double vmax, per_octave, octave;  // the largest value; log2(e) / T and its inverse
+  const double* table;              // 2^(j / 16), j << 16 taken off the high word
 
-  __device__ __forceinline__ void log_weight(float v, int* q, double* r) const {
-    constexpr double kMagic = 26388279066624.0;  // 1.5 * 2^44: its last place is 1/256
-    const double y = fma(widen(v) - vmax, per_octave, (double)shift);
+  // The weight of a value of at least cut(), as a double before its rounding.
+  __device__ __forceinline__ double unrounded(float v) const {
+    constexpr double kMagic = 422212465065984.0;  // 1.5 * 2^48: its last place is 1/16
+    const double y = fma(widen<T>(v) - vmax, per_octave, (double)shift);
     const double t = y + kMagic;
-    *q = __double2loint(t);
-    *r = y - (t - kMagic);
+    const double r = y - (t - kMagic);
+    const int q = __double2loint(t);
+    double p = fma(r, 1.3333558146428443e-03, 9.6181291076284772e-03);  // ln2^5 / 120, ln2^4 / 24
+    p = fma(p, r, 5.5504108664821580e-02);                              // ln2^3 / 6
+    p = fma(p, r, 2.4022650695910072e-01);                              // ln2^2 / 2
+    p = fma(p, r, 6.9314718055994531e-01);                              // ln2
+    const double e = table[q & (kExpTable - 1)];
+    const double m = __hiloint2double(__double2hiint(e) + (q << 16), __double2loint(e));
+    return fma(p * r, m, m);
   }
-  // Weighing bin: sixteenths of an octave down to 2^-24 of
-  // the maximum, quarters below.
-  __device__ __forceinline__ int bin(int q) const {
-    const int t = shift * kExpTable - q;
-    return min(t >> 4, (t >> 6) + kFineBins - kFineBins / 4);
-  }
-  // Values below this weigh nothing (they would round to 0).
-  __device__ __forceinline__ double cut() const { return vmax - (double)(shift + 1) / per_octave; }
-  // The weight of a value of at least cut(), and its q.
-  __device__ __forceinline__ unsigned long long weigh(float v, int* q) const {
-    double r;
-    log_weight(v, q, &r);
-    double p = fma(r, 5.5504108664821580e-02, 2.4022650695910072e-01);  // ln2^3 / 6, ln2^2 / 2
-    p = fma(p, r, 6.9314718055994531e-01);                             // ln2
-    const double m = table[*q & (kExpTable - 1)];
-    p = fma(p * r, m, m);
-    const double w =
-        __hiloint2double(__double2hiint(p) + ((*q & ~(kExpTable - 1)) << (20 - kExpBits)), __double2loint(p));
+  static __device__ __forceinline__ unsigned long long round(double w) {
     // adding 2^52 rounds to an integer, held in the low mantissa bits
     const double rounded = w + 4503599627370496.0;
     return ((unsigned long long)(uint32_t)(__double2hiint(rounded) - 0x43300000) << 32) |
            (uint32_t)__double2loint(rounded);
   }
-  __device__ __forceinline__ unsigned long long operator()(float v) const {
-    int q;
-    return weigh(v, &q);
+  // Weighing bin: sixteenths of the weight's octaves, read off its exponent and
+  // leading mantissa bits; all below 2^-32 of the maximum share the last.
+  __device__ __forceinline__ int bin(double w) const {
+    return min(((1023 + shift) << 4) - (__double2hiint(w) >> 16), kBins - 1);
   }
-  // Values that bin j may hold: [lo, hi], 0.02 of a multiple of 1/256 wider than
-  // the bin on both sides (rounding moves a border by less).
-  __device__ __forceinline__ void bin_range(int j, double* lo, double* hi) const {
-    const auto first = [](int k) { return k < kFineBins ? 16.0 * k : 64.0 * (k - kFineBins) + 16.0 * kFineBins; };
-    *hi = vmax + (0.52 - first(j)) / kExpTable / per_octave;
-    *lo = vmax + (0.48 - first(j + 1)) / kExpTable / per_octave;
+  // Values below this weigh nothing (they would round to 0).
+  __device__ __forceinline__ double cut() const { return vmax - (double)(shift + 1) * octave; }
+  __device__ __forceinline__ unsigned long long operator()(float v) const { return round(unrounded(v)); }
+  // Values that the bins first..last may hold: [*lo, *hi], wider by 2^-20 octave
+  // on both sides (rounding moves a border by far less).
+  __device__ __forceinline__ void bin_values(int first, int last, const double* log2_table, double* lo,
+                                             double* hi) const {
+    const auto border = [&](int k) {  // log2 of the least weight of bin k, below the maximum
+      // (in doubles: with an integer shift here, nvcc 12.9 lost the shift where
+      // first == last)
+      const double e = -0.0625 * k, whole = floor(e);
+      return whole + log2_table[(int)((e - whole) * 16.0)];
+    };
+    *hi = vmax + (border(first - 1) + 9.5367431640625e-07) * octave;
+    *lo = last == kBins - 1 ? cut() : vmax + (border(last) - 9.5367431640625e-07) * octave;
   }
 };
 
@@ -519,6 +541,20 @@ __device__ __forceinline__ void add_to_bin(SampleSmemHeader* s, uint32_t bin, un
   const uint32_t old = atomicAdd(&s->lo[bin], m_lo);
   m_hi += (old + m_lo < old) ? 1u : 0u;
   if (m_hi) atomicAdd(&s->hi[bin], m_hi);
+}
+
+// Four at a time: the additions of the low words are under way together before
+// the first carry is waited for. Bins from kBins on take anything.
+__device__ __forceinline__ void add_to_bins(SampleSmemHeader* s, const uint32_t (&bin)[4],
+                                            const unsigned long long (&m)[4]) {
+  uint32_t old[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) old[k] = atomicAdd(&s->lo[bin[k]], (uint32_t)m[k]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t hi = (uint32_t)(m[k] >> 32) + (old[k] + (uint32_t)m[k] < old[k] ? 1u : 0u);
+    if (hi) atomicAdd(&s->hi[bin[k]], hi);
+  }
 }
 
 // Sum of a thread's bin and the running sum before it.
@@ -669,16 +705,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   const int b = blockIdx.x / team.size, tid = threadIdx.x;
 
   // ---- the row and its settings ---------------------------------------------
-  Slice<T> slice;
+  Row<T> row;
   int64_t start = 0;
   if (p.offsets) {
     // positions outside the packed arrays are not read, whatever the offsets say
     start = min(max(p.offsets[b], (int64_t)0), p.capacity);
     const int64_t end = min(max(p.offsets[b + 1], start), p.capacity);
-    slice.row = Row<T>{static_cast<const Bits*>(p.logits) + start, nullptr, end - start};
+    row = Row<T>{static_cast<const Bits*>(p.logits) + start, nullptr, end - start};
   } else {
-    slice.row = Row<T>{static_cast<const Bits*>(p.logits) + (int64_t)b * p.row_stride,
-                       p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.vocab};
+    row = Row<T>{static_cast<const Bits*>(p.logits) + (int64_t)b * p.row_stride,
+                 p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.vocab};
   }
   const float temperature = p.temperatures ? p.temperatures[b] : p.temperature;
   const int64_t top_k = p.top_ks ? p.top_ks[b] : p.top_k;
@@ -687,18 +723,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   const float u = p.uniforms[b];
   // every CTA of the cluster runs before its shared memory is written to
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  const int64_t n = slice.row.n;
+  Slice<T> slice;
+  const int64_t n = row.n;
   const int64_t part = ((n + team.size - 1) / team.size + 31) / 32 * 32;
-  slice.lo = min(part * team.rank, n);
-  slice.len = min(part, n - slice.lo);
-  slice.held = reinterpret_cast<Bits*>(smem + kHeaderBytes);
-  slice.phase = (int)((reinterpret_cast<uintptr_t>(slice.row.x + slice.lo) & 15) / sizeof(Bits));
-  slice.resident = (int)min(slice.len, (int64_t)p.resident);
+  const int64_t lo = min(part * team.rank, n);
+  slice.set(row, lo, min(part, n - lo), smem + kHeaderBytes, p.held_vectors);
 
   // ---- the row into shared memory, largest value, number of legal tokens ----------
   uint32_t legal = 0u;
   float vmax = slice.load(legal);
-  if (tid < kExpTable) s->exp2_table[tid] = exp2((double)tid / kExpTable);
+  if (tid < kExpTable) {
+    const double e = exp2((double)tid / kExpTable);
+    s->exp2_table[tid] = __hiloint2double(__double2hiint(e) - (tid << 16), __double2loint(e));
+    s->log2_table[tid] = log2(1.0 + tid / 16.0);
+  }
   if (tid == 0) s->listed = 0u;
   {
     const uint32_t key = __reduce_max_sync(FULL_MASK, K::from_value(vmax));
@@ -743,10 +781,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   float logprob = 0.f;
   bool solo = false;  // the list holds all that is still needed: this CTA goes on alone
   if (temperature > 0.f && !infinite) {
-    Weigher weigh;
+    Weigher<T> weigh;
     weigh.shift = min(kMaxShift, 62 - (64 - __clzll((unsigned long long)n)));
-    weigh.vmax = widen(vmax);
+    weigh.vmax = widen<T>(vmax);
     weigh.per_octave = 1.4426950408889634 / (double)temperature;
+    weigh.octave = 0.6931471805599453 * (double)temperature;
     weigh.table = s->exp2_table;
     // ---- the kept set: values above `border`, and `ties` tokens at it --------------
     float border = vmin;
@@ -763,6 +802,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
       });
       if (tid < kMaxCluster) s->list_count[tid] = tid == 0 ? (uint32_t)kept : 0u;
       list.parts_bits = 0;
+      __syncthreads();
       team.cluster.sync();
       if (team.rank != 0) return;
       in_list = solo = true;
@@ -833,29 +873,40 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
     clear_bins(s);
     const float lowest = fmaxf(border, fminf(vmax, K::value_at_least(weigh.cut())));
     const auto into_bin = [&](float v, uint32_t) {
-      int q;
-      const unsigned long long w = weigh.weigh(v, &q);
-      if (v >= lowest) add_to_bin(s, (uint32_t)weigh.bin(q), w);
+      const double w = weigh.unrounded(v);
+      if (v >= lowest) add_to_bin(s, (uint32_t)weigh.bin(w), weigh.round(w));
     };
-    if (in_list) list.each(into_bin);
-    else slice.each(into_bin);
+    if (in_list) {
+      list.each(into_bin);
+    } else {
+      slice.each_four([&](const float (&f)[4]) {
+        uint32_t bin[4];
+        unsigned long long m[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const double w = weigh.unrounded(f[k]);
+          m[k] = weigh.round(w);
+          bin[k] = f[k] >= lowest ? (uint32_t)weigh.bin(w) : (uint32_t)kBins + (tid & 31);
+        }
+        add_to_bins(s, bin, m);
+      });
+    }
     unsigned long long sum;
     const BinSums bins = sum_bins(team, in_list, &sum);
     if (excess && border >= lowest) sum -= excess * weigh(border);
     // Values of a bin, as [*from, *to], a little wider than it.
     const auto bin_values = [&](int first, int last, float* from, float* to) {
-      double lo, hi, unused;
-      weigh.bin_range(first, &unused, &hi);
-      weigh.bin_range(last, &lo, &unused);
+      double lo, hi;
+      weigh.bin_values(first, last, s->log2_table, &lo, &hi);
       *from = fmaxf(lowest, K::value_at_least(lo));
       *to = fmaxf(*from, fminf(vmax, K::value_at_least(hi)));
     };
     // The search for `target` inside bin j (its sum before the bin, its values).
     const auto within = [&](int j, float from, float to, unsigned long long before, unsigned long long target) {
       const auto in_bin = [&](float v, unsigned long long* m) {
-        int q;
-        *m = weigh.weigh(v, &q);
-        return weigh.bin(q) == j;
+        const double w = weigh.unrounded(v);
+        *m = weigh.round(w);
+        return weigh.bin(w) == j;
       };
       const uint32_t klo = K::from_value(from), khi = K::from_value(to);
       Found f = solo ? search<T>(team, true, list, klo, khi, in_bin, target - before)
@@ -945,9 +996,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
     if (p.kept) p.kept[b] = (int32_t)kept;
   };
   if (solo) {
-    // the positions of draw_value's tokens, into the table's space; each counts those before it
-    uint32_t* ties_at = reinterpret_cast<uint32_t*>(s->exp2_table);
-    constexpr uint32_t kTiesCap = sizeof(s->exp2_table) / sizeof(uint32_t);
+    // the positions of draw_value's tokens; each counts those before it
+    uint32_t* ties_at = s->ties_at;
     __syncthreads();
     if (tid == 0) s->listed = 0u;
     __syncthreads();
@@ -989,9 +1039,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   // blocks of kSampleThreads positions in order
   for (int64_t i0 = 0; i0 < slice.len; i0 += kSampleThreads) {
     const int64_t i = i0 + tid;
-    float v = -INFINITY;
-    if (i < slice.resident) v = DTypeTraits<T>::bits_to_float(slice.held[slice.phase + i]);
-    else if (i < slice.len) v = load_value(slice.row, slice.lo + i);
+    const float v = i < slice.len ? slice.at(slice.lo + i) : -INFINITY;
     const bool hit = v == draw_value;
     const unsigned hits = __ballot_sync(FULL_MASK, hit);
     __syncthreads();
@@ -1015,21 +1063,20 @@ cudaError_t launch_typed(FilteredSampleParams p, int batch, int64_t max_len, cud
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  using Key = typename DTypeTraits<T>::Bits;
+  // CTAs per row (a power of two, up to 16): enough that shared memory holds the
+  // whole row beside a second CTA on each SM, and more while the batch leaves SMs
+  // idle and a CTA has over 4,096 tokens. What is not held is read again from L2.
   constexpr size_t kSmemMax = 227 * 1024;
-  // CTAs per row: one for short rows; for long ones enough that a CTA's part
-  // leaves room for a second CTA on the SM (their barriers overlap), and more
-  // while the batch leaves SMs idle.
-  const size_t room = (kSmemMax - kHeaderBytes - 64) / sizeof(Key) / 32 * 32;
-  constexpr size_t kShare = (kSmemMax / 2 - 1024 - kHeaderBytes - 64) / sizeof(Key);
+  constexpr int64_t kShare = (int64_t)(kSmemMax / 2 - 1024 - kHeaderBytes - 16) / (int64_t)sizeof(typename DTypeTraits<T>::Bits);
   int size = 1;
-  while (size < kMaxCluster &&
-         ((int64_t)(size < 8 ? kShare : room) * size < max_len ||
-          (max_len > (int64_t)4096 * size && (int64_t)batch * size * 2 <= 2 * num_sms(dev))))
+  while (size < kMaxCluster && ((size < 8 && kShare * size < max_len) ||
+                                (max_len > (int64_t)4096 * size && (int64_t)batch * size <= (int64_t)num_sms(dev))))
     size *= 2;
+  const size_t room = ((int64_t)batch * size <= num_sms(dev) ? kSmemMax : kSmemMax / 2 - 1024) - kHeaderBytes;
   const int64_t part = ((max_len + size - 1) / size + 31) / 32 * 32;
-  p.resident = (int)std::min<int64_t>((int64_t)room, std::max<int64_t>(part, 32));
-  const size_t smem = kHeaderBytes + ((size_t)p.resident + 16) * sizeof(Key);
+  const int64_t part_vectors = (part * (int64_t)sizeof(typename DTypeTraits<T>::Bits) + 15) / 16 + 1;
+  p.held_vectors = (int)std::min<int64_t>((int64_t)(room / 16), part_vectors);
+  const size_t smem = kHeaderBytes + (size_t)p.held_vectors * 16;
   auto k = filtered_sample_kernel<T>;
   if ((err = raise_smem_limit(reinterpret_cast<const void*>(k), smem, dev)) != cudaSuccess) return err;
   static std::atomic<uint64_t> wide_ok[2];  // devices on which clusters of 16 have been allowed

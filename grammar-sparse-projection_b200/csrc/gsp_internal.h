@@ -245,7 +245,7 @@ struct FilteredSampleParams {
   int64_t* token_ids;
   float* logprobs;
   int32_t* kept;
-  int resident;  // keys a CTA holds in shared memory
+  int held_vectors;  // 16-byte vectors a CTA keeps in shared memory (set by the launcher)
 };
 
 // max_len: tokens of the longest row (packed rows: an expectation that picks the

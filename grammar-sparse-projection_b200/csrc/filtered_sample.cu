@@ -1057,6 +1057,440 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   }
 }
 
+// ===========================================================================
+// rows of 16-bit logits, one CTA per row: every value is counted
+// ===========================================================================
+// A row of fp16 or bf16 logits has few distinct values (some thousand), so one
+// shared-memory addition per token, whatever its weight, is all that the row's
+// pass costs: count[m] holds, for the magnitude m (the value's bits without the
+// sign), how many tokens have it (low half) and how many of those are negative
+// (high half). The exponentials are then taken once per distinct value, and
+// every search (top-k, top-p, the draw) is one over the counts. The row is read
+// a second time, from L2, to find the drawn value's positions.
+//
+// A magnitude of more than 65,535 tokens overflows its half; the sum of the
+// counts then differs from the number of tokens (every overflow makes it
+// smaller), and the counts of a chunk are taken from the row each time they are
+// needed, in 32 bits (several passes: right, but slow).
+//
+// Order: chunks of 1024 magnitudes, positive ones from the largest magnitude
+// down, then negative ones up; within a chunk thread t has the t-th value.
+constexpr int kCountThreads = 1024;
+constexpr int kCountWarps = kCountThreads / 32;
+constexpr int kMagnitudes = 1 << 15;
+constexpr int kChunks = 2 * kMagnitudes / kCountThreads;
+static_assert(kChunks == 64 && kCountWarps == 32, "a warp scans the chunks and the warps");
+
+struct CountSmem {
+  uint32_t count[kMagnitudes];
+  uint32_t lo[kChunks], hi[kChunks];  // weights of the chunks, in 64 bits
+  uint32_t tokens[kChunks];           // tokens of the chunks
+  unsigned long long scan[kCountWarps];
+  unsigned long long pick[4];
+  double exp2_table[kExpTable];
+  uint32_t warp[2][kCountWarps];
+};
+
+// Magnitude and sign of chunk o's place t.
+struct Place {
+  uint32_t m;
+  bool negative;
+};
+__device__ __forceinline__ Place place_of(int o, int t) {
+  return o < kChunks / 2 ? Place{(uint32_t)((kChunks / 2 - 1 - o) * kCountThreads + (kCountThreads - 1 - t)), false}
+                         : Place{(uint32_t)((o - kChunks / 2) * kCountThreads + t), true};
+}
+__device__ __forceinline__ int chunk_of(uint32_t m, bool negative) {
+  const int j = (int)(m / kCountThreads);
+  return negative ? kChunks / 2 + j : kChunks / 2 - 1 - j;
+}
+
+template <typename T>
+struct Counted {
+  static constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  CountSmem* s;
+  const Slice<T>* row;
+  bool overflow;
+
+  // fn(16-bit pattern) for every token whose pattern is not -inf (NaN included)
+  template <typename Fn>
+  __device__ __forceinline__ void each_pattern(Fn fn) const {
+    constexpr int kAhead = 4;
+    for (int v0 = threadIdx.x; v0 < row->vectors; v0 += kAhead * kCountThreads) {
+      uint4 q[kAhead];
+      uint32_t legal[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int v = v0 + k * kCountThreads;
+        q[k] = make_uint4(0u, 0u, 0u, 0u);
+        legal[k] = 0u;
+        if (v < row->vectors) q[k] = row->fetch(v, &legal[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (v0 + k * kCountThreads >= row->vectors) break;
+        uint32_t w[4];
+        row->settle(q[k], legal[k], w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          fn(w[j] & 0xffffu);
+          fn(w[j] >> 16);
+        }
+      }
+    }
+  }
+
+  // Fills the counts; returns the thread's number of tokens counted.
+  __device__ __forceinline__ uint32_t count_all() const {
+    uint32_t counted = 0u;
+    each_pattern([&](uint32_t b) {
+      if (b == (0x8000u | kInf)) return;
+      ++counted;
+      atomicAdd(&s->count[b & 0x7fffu], ((b & 0x8000u) << 1) | 1u);
+    });
+    return counted;
+  }
+
+  // Before chunk o's counts are asked for (all threads): after an overflow they
+  // are counted from the row.
+  __device__ __forceinline__ void prepare(int o) const {
+    if (!overflow) return;
+    __syncthreads();
+    s->count[threadIdx.x] = 0u;
+    __syncthreads();
+    each_pattern([&](uint32_t b) {
+      const uint32_t m = b & 0x7fffu;
+      const bool negative = (b & 0x8000u) != 0u && m != 0u;
+      if (m > kInf || (negative && m == kInf) || chunk_of(m, negative) != o) return;
+      atomicAdd(&s->count[negative ? m % kCountThreads : kCountThreads - 1u - m % kCountThreads], 1u);
+    });
+    __syncthreads();
+  }
+  // Tokens of chunk o's place threadIdx.x.
+  __device__ __forceinline__ uint32_t tokens(int o) const {
+    if (overflow) return s->count[threadIdx.x];
+    const Place at = place_of(o, threadIdx.x);
+    if (at.m > kInf) return 0u;
+    const uint32_t c = s->count[at.m];
+    if (at.m == 0u) return at.negative ? 0u : c & 0xffffu;  // -0 is 0
+    return at.negative ? c >> 16 : (c & 0xffffu) - (c >> 16);
+  }
+  static __device__ __forceinline__ float value(int o, int t) {
+    const Place at = place_of(o, t);
+    return DTypeTraits<T>::bits_to_float((uint16_t)(at.m | (at.negative ? 0x8000u : 0u)));
+  }
+};
+
+__device__ __forceinline__ uint32_t count_block_sum(uint32_t a, CountSmem* s) {
+  a = __reduce_add_sync(FULL_MASK, a);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s->warp[0][threadIdx.x >> 5] = a;
+  __syncthreads();
+  return __reduce_add_sync(FULL_MASK, s->warp[0][threadIdx.x & 31]);
+}
+
+// The chunk (of two per lane: a, b) at which the running sum passes the target:
+// its number, and the sum before it. All warps compute the same.
+__device__ __forceinline__ int pick_chunk(unsigned long long a, unsigned long long b, unsigned long long target,
+                                          unsigned long long* before) {
+  const unsigned long long incl = warp_scan_u64(a + b), excl = incl - (a + b);
+  const bool here = excl <= target && target < incl, second = target >= excl + a;
+  const unsigned m = __ballot_sync(FULL_MASK, here);
+  const int lane = m ? __ffs(m) - 1 : 31;
+  *before = __shfl_sync(FULL_MASK, second ? excl + a : excl, lane);
+  return __shfl_sync(FULL_MASK, 2 * (int)(threadIdx.x & 31) + (second ? 1 : 0), lane);
+}
+
+// The place at which the running sum over the block's `own` passes the target
+// (which it does); pick: {place, sum before it, its own}.
+__device__ __forceinline__ void pick_place(CountSmem* s, unsigned long long own, unsigned long long target) {
+  const int tid = threadIdx.x;
+  const unsigned long long incl_w = warp_scan_u64(own);
+  __syncthreads();  // the last pick has been read
+  if ((tid & 31) == 31) s->scan[tid >> 5] = incl_w;
+  __syncthreads();
+  const unsigned long long w = warp_scan_u64(s->scan[tid & 31]);
+  const unsigned long long warp_before = __shfl_sync(FULL_MASK, w, max((tid >> 5) - 1, 0));
+  const unsigned long long incl = incl_w + (tid >= 32 ? warp_before : 0ull), excl = incl - own;
+  if (excl <= target && target < incl) {
+    s->pick[0] = tid;
+    s->pick[1] = excl;
+    s->pick[2] = own;
+  }
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kCountThreads, 1) counted_sample_kernel(const FilteredSampleParams p) {
+  using K = SampleKey<T>;
+  using Bits = typename DTypeTraits<T>::Bits;
+  extern __shared__ __align__(128) unsigned char smem[];
+  CountSmem* s = reinterpret_cast<CountSmem*>(smem);
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+
+  // ---- the row and its settings ---------------------------------------------
+  Row<T> row;
+  int64_t start = 0;
+  if (p.offsets) {
+    // positions outside the packed arrays are not read, whatever the offsets say
+    start = min(max(p.offsets[b], (int64_t)0), p.capacity);
+    const int64_t end = min(max(p.offsets[b + 1], start), p.capacity);
+    row = Row<T>{static_cast<const Bits*>(p.logits) + start, nullptr, end - start};
+  } else {
+    row = Row<T>{static_cast<const Bits*>(p.logits) + (int64_t)b * p.row_stride,
+                 p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.vocab};
+  }
+  const float temperature = p.temperatures ? p.temperatures[b] : p.temperature;
+  const int64_t top_k = p.top_ks ? p.top_ks[b] : p.top_k;
+  const float top_p = p.top_ps ? p.top_ps[b] : p.top_p;
+  const float min_p = p.min_ps ? p.min_ps[b] : p.min_p;
+  const float u = p.uniforms[b];
+  const int64_t n = row.n;
+  Slice<T> slice;
+  slice.set(row, 0, n, nullptr, 0);
+
+  // ---- count ------------------------------------------------------------------
+#pragma unroll
+  for (int i = 0; i < kMagnitudes / 4 / kCountThreads; ++i)
+    reinterpret_cast<uint4*>(s->count)[i * kCountThreads + tid] = make_uint4(0u, 0u, 0u, 0u);
+  if (tid < kChunks) s->lo[tid] = s->hi[tid] = s->tokens[tid] = 0u;
+  if (tid < kExpTable) {
+    const double e = exp2((double)tid / kExpTable);
+    s->exp2_table[tid] = __hiloint2double(__double2hiint(e) - (tid << 16), __double2loint(e));
+  }
+  __syncthreads();
+  Counted<T> c{s, &slice, false};
+  const uint32_t counted = count_block_sum(c.count_all(), s);
+  // tokens of each chunk; all magnitudes' low halves must add up to what was counted
+  uint32_t low = 0u;
+  for (int j = 0; j < kMagnitudes / kCountThreads; ++j) {
+    const uint32_t m = (uint32_t)(j * kCountThreads + tid), x = s->count[m];
+    low += x & 0xffffu;
+    if (__ballot_sync(FULL_MASK, x != 0u) == 0u) continue;
+    const uint32_t negative = m == 0u || m >= Counted<T>::kInf ? 0u : x >> 16;
+    const uint32_t positive = m > Counted<T>::kInf ? 0u : (x & 0xffffu) - (m == 0u ? 0u : x >> 16);
+    const uint32_t a = __reduce_add_sync(FULL_MASK, positive), d = __reduce_add_sync(FULL_MASK, negative);
+    if (lane == 0 && a) atomicAdd(&s->tokens[chunk_of(m, false)], a);
+    if (lane == 0 && d) atomicAdd(&s->tokens[chunk_of(m, true)], d);
+  }
+  c.overflow = count_block_sum(low, s) != counted;
+  if (c.overflow) {
+    __syncthreads();
+    if (tid < kChunks) s->tokens[tid] = 0u;
+    __syncthreads();
+    c.each_pattern([&](uint32_t x) {
+      const uint32_t m = x & 0x7fffu;
+      const bool negative = (x & 0x8000u) != 0u && m != 0u;
+      if (m <= Counted<T>::kInf && !(negative && m == Counted<T>::kInf))
+        atomicAdd(&s->tokens[chunk_of(m, negative)], 1u);
+    });
+    __syncthreads();
+  }
+  // two chunks per lane, in every warp
+  const uint32_t t0 = s->tokens[2 * lane], t1 = s->tokens[2 * lane + 1];
+  unsigned long long kept = __reduce_add_sync(FULL_MASK, t0 + t1);  // tokens left so far
+  const unsigned long long filled =
+      (unsigned long long)__ballot_sync(FULL_MASK, t0 != 0u) | ((unsigned long long)__ballot_sync(FULL_MASK, t1 != 0u) << 32);
+  const auto is_filled = [&](int o) { return ((filled >> ((o & 1) * 32 + (o >> 1))) & 1ull) != 0ull; };
+  const bool valid = temperature >= 0.f && temperature < INFINITY && top_p == top_p && min_p == min_p && u >= 0.f &&
+                     u < 1.f;
+  if (!valid || kept == 0ull) {  // not to be drawn, or nothing is legal
+    if (tid == 0) {
+      p.token_ids[b] = valid ? 0 : -1;
+      if (p.logprobs) p.logprobs[b] = valid ? -INFINITY : __int_as_float(0x7fc00000);
+      if (p.kept) p.kept[b] = 0;
+    }
+    return;
+  }
+
+  // The value at which the running number of tokens passes a target.
+  struct Border {
+    float value;
+    unsigned long long above, own;  // tokens above it, and of it
+  };
+  const auto by_tokens = [&](unsigned long long target) {
+    unsigned long long before;
+    const int o = pick_chunk(t0, t1, target, &before);
+    c.prepare(o);
+    pick_place(s, c.tokens(o), target - before);
+    return Border{Counted<T>::value(o, (int)s->pick[0]), before + s->pick[1], s->pick[2]};
+  };
+  const float vmax = by_tokens(0ull).value;
+  const bool infinite = !(vmax < INFINITY);
+  float draw_value = vmax;
+  unsigned long long ordinal = 0ull;  // among the tokens of draw_value, by rising position
+  float logprob = 0.f;
+  if (temperature > 0.f && !infinite) {
+    Weigher<T> weigh;
+    weigh.shift = min(kMaxShift, 62 - (64 - __clzll((unsigned long long)n)));
+    weigh.vmax = widen<T>(vmax);
+    weigh.per_octave = 1.4426950408889634 / (double)temperature;
+    weigh.octave = 0.6931471805599453 * (double)temperature;
+    weigh.table = s->exp2_table;
+    // ---- the kept set: values above `border`, and `ties` tokens at it ----------------
+    float border = -INFINITY;
+    unsigned long long ties = ~0ull, excess = 0ull;
+    if (top_k > 0 && (unsigned long long)top_k < kept) {
+      const Border f = by_tokens((unsigned long long)top_k - 1ull);
+      border = f.value;
+      ties = (unsigned long long)top_k - f.above;
+      excess = f.own - ties;
+      kept = (unsigned long long)top_k;
+    }
+    const float lowest_weighed = fminf(vmax, K::value_at_least(weigh.cut()));
+    bool below = false;  // min-p moved the border
+    if (min_p > 0.f) {
+      const float low_value =
+          min_p >= 1.f ? vmax : fminf(vmax, K::value_at_least((double)vmax + (double)temperature * log((double)min_p)));
+      if (low_value > border) {
+        border = low_value;
+        ties = ~0ull;
+        excess = 0ull;
+        below = true;
+      }
+    }
+    // ---- weigh the chunks' values -------------------------------------------------------
+    const float lowest = fmaxf(border, lowest_weighed);
+    const auto weight_here = [&](int o) {
+      const uint32_t x = c.tokens(o);
+      const float v = Counted<T>::value(o, tid);
+      return x != 0u && v >= lowest ? (unsigned long long)x * weigh(v) : 0ull;
+    };
+    uint32_t n_kept = 0u;
+    for (int o = 0; o < kChunks; ++o) {
+      if (!is_filled(o)) continue;
+      c.prepare(o);
+      const unsigned long long w = weight_here(o);
+      if (below) n_kept += Counted<T>::value(o, tid) >= border ? c.tokens(o) : 0u;
+      if (__ballot_sync(FULL_MASK, w != 0ull) == 0u) continue;
+      const unsigned long long sum_w = warp_scan_u64(w);
+      if (lane == 31) {
+        const uint32_t old = atomicAdd(&s->lo[o], (uint32_t)sum_w);
+        const uint32_t hi = (uint32_t)(sum_w >> 32) + (old + (uint32_t)sum_w < old ? 1u : 0u);
+        if (hi) atomicAdd(&s->hi[o], hi);
+      }
+    }
+    if (below) kept = count_block_sum(n_kept, s);
+    __syncthreads();
+    const unsigned long long w0 = s->lo[2 * lane] + ((unsigned long long)s->hi[2 * lane] << 32);
+    const unsigned long long w1 = s->lo[2 * lane + 1] + ((unsigned long long)s->hi[2 * lane + 1] << 32);
+    unsigned long long sum = __shfl_sync(FULL_MASK, warp_scan_u64(w0 + w1), 31);
+    if (excess && border >= lowest) sum -= excess * weigh(border);
+    // The value at which the running weight passes a target, its chunk and place.
+    const auto by_weight = [&](unsigned long long target, int* o, int* place) {
+      unsigned long long before;
+      *o = pick_chunk(w0, w1, target, &before);
+      c.prepare(*o);
+      pick_place(s, weight_here(*o), target - before);
+      *place = (int)s->pick[0];
+      return Border{Counted<T>::value(*o, *place), before + s->pick[1], s->pick[2]};
+    };
+    if (top_p < 1.f) {
+      const unsigned long long target = prefix_target(top_p, sum);
+      int o, place;
+      const Border f = by_weight(target, &o, &place);
+      const unsigned long long w = weigh(f.value);
+      ties = (target - f.above) / w + 1ull;
+      sum = f.above + ties * w;
+      // the tokens above it: of the chunks before, and of its chunk's places before
+      const uint32_t upto = (2 * lane < o ? t0 : 0u) + (2 * lane + 1 < o ? t1 : 0u);
+      kept = ties + __reduce_add_sync(FULL_MASK, upto) + count_block_sum(tid < place ? c.tokens(o) : 0u, s);
+    }
+    // ---- the draw ------------------------------------------------------------------------
+    const unsigned long long target = __umul64hi(fraction64(u), sum);
+    int o, place;
+    const Border f = by_weight(target, &o, &place);
+    draw_value = f.value;
+    ordinal = (target - f.above) / weigh(draw_value);
+    logprob = (float)(((double)draw_value - (double)vmax) / (double)temperature -
+                      log((double)sum / (double)(1ull << weigh.shift)));
+  } else if (temperature > 0.f) {
+    // a maximum of +inf: its tokens weigh 1 each, every other nothing
+    unsigned long long m = by_tokens(0ull).own;
+    if (top_k > 0) kept = min(kept, (unsigned long long)top_k);
+    m = min(m, kept);
+    if (min_p > 0.f) kept = m;
+    if (top_p < 1.f) kept = m = prefix_target(top_p, m) + 1ull;
+    ordinal = __umul64hi(fraction64(u), m);
+    logprob = (float)-log((double)m);
+  } else {
+    kept = 1ull;
+  }
+
+  // ---- the drawn token: the ordinal-th of draw_value, by rising position ----------------
+  // Each warp has a run of vectors; the warp whose run holds it is found from the
+  // runs' counts, and goes over its run again in order.
+  const int run = (slice.vectors + kCountWarps - 1) / kCountWarps;
+  const int v_lo = min((tid >> 5) * run, slice.vectors), v_hi = min(v_lo + run, slice.vectors);
+  constexpr int kVec = Slice<T>::kVec;
+  // the vector's places that hold the value, as bits
+  const auto hits = [&](const uint4& q, uint32_t legal) {
+    uint32_t w[4], m = 0u;
+    slice.settle(q, legal, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t same = pair_at_least<T>(w[j], draw_value) & ~pair_above<T>(w[j], draw_value);
+      m |= ((same & 1u) | ((same >> 15) & 2u)) << (2 * j);
+    }
+    return m;
+  };
+  uint32_t here = 0u;
+  for (int v0 = v_lo + lane; v0 < v_hi; v0 += 4 * 32) {
+    uint4 q[4];
+    uint32_t legal[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      legal[k] = 0u;
+      q[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (v0 + 32 * k < v_hi) q[k] = slice.fetch(v0 + 32 * k, &legal[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (v0 + 32 * k < v_hi) here += __popc(hits(q[k], legal[k]));
+  }
+  here = __reduce_add_sync(FULL_MASK, here);
+  __syncthreads();
+  if (lane == 0) s->warp[0][tid >> 5] = here;
+  __syncthreads();
+  const uint32_t mine = s->warp[0][lane];
+  const uint32_t upto = (uint32_t)warp_scan_u64(mine) - mine;  // hits of the runs before run `lane`
+  const uint32_t before = __shfl_sync(FULL_MASK, upto, tid >> 5);
+  if (ordinal < before || ordinal >= (unsigned long long)before + here) return;
+  uint32_t left = (uint32_t)ordinal - before;
+  for (int v0 = v_lo; v0 < v_hi; v0 += 32) {
+    const int v = v0 + lane;
+    uint32_t legal, m = 0u;
+    if (v < v_hi) {
+      const uint4 q = slice.fetch(v, &legal);
+      m = hits(q, legal);
+    }
+    const uint32_t k = __popc(m), incl = (uint32_t)warp_scan_u64(k), total = __shfl_sync(FULL_MASK, incl, 31);
+    if (left >= total) {
+      left -= total;
+      continue;
+    }
+    if (incl - k <= left && left < incl) {
+      for (uint32_t i = incl - k; i < left; ++i) m &= m - 1u;
+      const int64_t at = slice.lo - slice.phase + (int64_t)v * kVec + (__ffs(m) - 1);
+      p.token_ids[b] = p.ids ? p.ids[start + at] : p.vocab_offset + at;
+      if (p.logprobs) p.logprobs[b] = logprob;
+      if (p.kept) p.kept[b] = (int32_t)kept;
+    }
+    break;
+  }
+}
+
+template <typename T>
+cudaError_t launch_counted(const FilteredSampleParams& p, int batch, cudaStream_t stream) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  auto k = counted_sample_kernel<T>;
+  if ((err = raise_smem_limit(reinterpret_cast<const void*>(k), sizeof(CountSmem), dev)) != cudaSuccess) return err;
+  k<<<batch, kCountThreads, sizeof(CountSmem), stream>>>(p);
+  return cudaGetLastError();
+}
+
 // Launch: one cluster per row.
 template <typename T>
 cudaError_t launch_typed(FilteredSampleParams p, int batch, int64_t max_len, cudaStream_t stream) {
@@ -1103,9 +1537,15 @@ cudaError_t launch_typed(FilteredSampleParams p, int batch, int64_t max_len, cud
 
 }  // namespace
 
+// 16-bit rows are counted by one CTA each, unless they are few and long.
+constexpr int64_t kCountedAlone = 65536;
+constexpr int kCountedBatch = 16;
+
 cudaError_t launch_filtered_sample(const FilteredSampleParams& p, int dtype, int batch, int64_t max_len,
                                    cudaStream_t stream) {
   if (dtype == 2) return launch_typed<float>(p, batch, max_len, stream);
+  if (max_len <= kCountedAlone || batch >= kCountedBatch)
+    return dtype == 1 ? launch_counted<__nv_bfloat16>(p, batch, stream) : launch_counted<__half>(p, batch, stream);
   if (dtype == 1) return launch_typed<__nv_bfloat16>(p, batch, max_len, stream);
   return launch_typed<__half>(p, batch, max_len, stream);
 }

@@ -83,10 +83,12 @@ def test_matches_oracle(cuda_device, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(6, 20011), (3, 140001), (17, 140001)])
 @pytest.mark.parametrize("form", ["equal", "two", "coarse"])
-def test_ties_go_to_the_lowest_id(cuda_device, form, dtype):
-    """Every logit equal, two values, a few values: borders fall inside ties."""
-    batch, vocab = 6, 20011
+def test_ties_go_to_the_lowest_id(cuda_device, form, shape, dtype):
+    """Every logit equal, two values, a few values: borders fall inside ties.
+    (Over 65,535 tokens of one value, in few rows and in many.)"""
+    batch, vocab = shape
     g = torch.Generator(device="cpu").manual_seed(3)
     if form == "equal":
         x = torch.full((batch, vocab), -1.5)
@@ -95,7 +97,7 @@ def test_ties_go_to_the_lowest_id(cuda_device, form, dtype):
     else:
         x = (torch.randn(batch, vocab, generator=g) * 2).round() / 2
     x = x.to(dtype).to(cuda_device)
-    u = torch.tensor([0.0, 1 - 2.0 ** -24, 0.5, 0.25, 0.123, 0.987], device=cuda_device)
+    u = torch.tensor([0.0, 1 - 2.0 ** -24, 0.5, 0.25, 0.123, 0.987] * 3, device=cuda_device)[:batch].contiguous()
     for settings in SETTINGS + [dict(top_k=7001, top_p=0.3), dict(top_k=100, min_p=1.0), dict(top_k=9000, min_p=0.9)]:
         _check(tr.sample_logits(x, uniforms=u, **settings), x, u, settings)
 

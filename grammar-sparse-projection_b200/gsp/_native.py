@@ -7,6 +7,7 @@ tensor is not on a CUDA device, calls raise instead of computing elsewhere.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -655,52 +656,80 @@ class _NoGuard:
 
 
 _NO_GUARD = _NoGuard()
+# (torch.cuda.current_stream builds a Stream object for every call; the handle alone is 30 times quicker to get)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def on_device(device: torch.device):
-    """Context in which `device` is the current CUDA device."""
-    return _NO_GUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def on_device(index: int):
+    """Context in which CUDA device `index` is the current one."""
+    return _NO_GUARD if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
-def _call_workspace(device: torch.device, batch: int, vocab: int) -> torch.Tensor:
+def raw_stream(index: int) -> int:
+    """Handle of the current stream of CUDA device `index`."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(batch: int, vocab: int) -> int:
+    return int(load().gsp_workspace_bytes(batch, vocab))
+
+
+@functools.lru_cache(maxsize=1024)
+def _int8_scratch_bytes(batch: int, hidden_dim: int) -> int:
+    return int(load().gsp_int8_scratch_bytes(batch, hidden_dim))
+
+
+def _call_workspace(device: torch.device, stream: int, batch: int, vocab: int) -> torch.Tensor:
+    need = _workspace_bytes(batch, vocab)
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(int(load().gsp_workspace_bytes(batch, vocab)), dtype=torch.uint8, device=device)
-    return workspace(device, batch, vocab)
+        return torch.zeros(need, dtype=torch.uint8, device=device)
+    ws = _workspaces.get((device.index, stream))  # (dict reads and writes are atomic; workspace() takes the lock)
+    return ws if ws is not None and ws.numel() >= need else workspace(device, batch, vocab)
+
+
+def _address(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
 
 
 def quantize_rows_int8(x, values, scales) -> None:
     """gsp_quantize_rows_int8: x [N, H] -> values int8 [N, H], scales float32 [N]."""
-    _require_cuda(x, values, scales)
-    with on_device(x.device):
-        status = load().gsp_quantize_rows_int8(_ptr(x), x.stride(0), x.shape[0], x.shape[1], dtype_code(x.dtype),
-                                               _ptr(values), values.stride(0), _ptr(scales), _stream(x.device))
+    index = x.get_device()
+    with on_device(index):
+        status = load().gsp_quantize_rows_int8(x.data_ptr(), x.stride(0), x.shape[0], x.shape[1],
+                                               DTYPE_CODES[x.dtype], values.data_ptr(), values.stride(0),
+                                               scales.data_ptr(), raw_stream(index))
     if status:
         _check(status, "gsp_quantize_rows_int8")
 
 
-def _int8_operands(hidden, hidden_scales, weight, weight_scales, mask):
-    """Leading arguments shared by gsp_int8_logits and gsp_int8_compact, and the scratch tensor (None for int8
-    hidden states)."""
-    scratch = None
+def _int8_call(hidden, hidden_scales, weight, weight_scales, mask):
+    """Arguments shared by gsp_int8_logits and gsp_int8_compact: the operands, and (scratch, workspace, stream)."""
+    device, index = hidden.device, hidden.get_device()
+    batch, hidden_dim = hidden.shape
+    vocab = weight.shape[0]
+    stream = raw_stream(index)
+    ws = _call_workspace(device, stream, batch, vocab)
     if hidden_scales is None:
-        batch, hdim = hidden.shape
-        scratch = torch.empty(int(load().gsp_int8_scratch_bytes(batch, hdim)), dtype=torch.uint8, device=hidden.device)
-    return (_ptr(hidden), hidden.stride(0), DTYPE_I8 if hidden_scales is not None else dtype_code(hidden.dtype),
-            _ptr(hidden_scales), _ptr(weight), weight.stride(0), _ptr(weight_scales), _ptr(mask),
-            0 if mask is None else mask.stride(0), hidden.shape[0], weight.shape[0], weight.shape[1]), scratch
+        code, scratch = DTYPE_CODES[hidden.dtype], torch.empty(_int8_scratch_bytes(batch, hidden_dim),
+                                                               dtype=torch.uint8, device=device)
+        tail = (scratch.data_ptr(), scratch.numel(), ws.data_ptr(), ws.numel(), stream)
+    else:
+        code, scratch, tail = DTYPE_I8, None, (None, 0, ws.data_ptr(), ws.numel(), stream)
+    args = (hidden.data_ptr(), hidden.stride(0), code, _address(hidden_scales), weight.data_ptr(), weight.stride(0),
+            weight_scales.data_ptr(), _address(mask), 0 if mask is None else mask.stride(0), batch, vocab, hidden_dim)
+    return args, tail, (scratch, ws)
 
 
 def int8_logits(route: str, hidden, hidden_scales, weight, weight_scales, mask, out_dtype, logits=None,
                 top_value=None, top_index=None, top_key=None, vocab_offset: int = 0) -> None:
     """gsp_int8_logits; hidden_scales None: `hidden` is floating point and quantised by the call."""
-    _require_cuda(hidden, hidden_scales, weight, weight_scales, mask, logits)
-    with on_device(hidden.device):
-        args, scratch = _int8_operands(hidden, hidden_scales, weight, weight_scales, mask)
-        ws = _call_workspace(hidden.device, hidden.shape[0], weight.shape[0])
+    with on_device(hidden.get_device()):
+        args, tail, keep = _int8_call(hidden, hidden_scales, weight, weight_scales, mask)
         status = load().gsp_int8_logits(
-            ROUTE_CODES[route], *args, dtype_code(out_dtype), vocab_offset, _ptr(logits),
-            0 if logits is None else logits.stride(0), _ptr(top_value), _ptr(top_index), _ptr(top_key),
-            _ptr(scratch), 0 if scratch is None else scratch.numel(), _ptr(ws), ws.numel(), _stream(hidden.device))
+            ROUTE_CODES[route], *args, DTYPE_CODES[out_dtype], vocab_offset, _address(logits),
+            0 if logits is None else logits.stride(0), _address(top_value), _address(top_index), _address(top_key),
+            *tail)
     if status:
         _check(status, "gsp_int8_logits")
 
@@ -708,15 +737,12 @@ def int8_logits(route: str, hidden, hidden_scales, weight, weight_scales, mask, 
 def int8_compact(hidden, hidden_scales, weight, weight_scales, mask, out_dtype, compact_logits, compact_ids, offsets,
                  top_value=None, top_index=None, top_key=None, vocab_offset: int = 0) -> None:
     """gsp_int8_compact."""
-    _require_cuda(hidden, hidden_scales, weight, weight_scales, mask, compact_logits, compact_ids, offsets)
-    with on_device(hidden.device):
-        args, scratch = _int8_operands(hidden, hidden_scales, weight, weight_scales, mask)
-        ws = _call_workspace(hidden.device, hidden.shape[0], weight.shape[0])
+    with on_device(hidden.get_device()):
+        args, tail, keep = _int8_call(hidden, hidden_scales, weight, weight_scales, mask)
         status = load().gsp_int8_compact(
-            *args, dtype_code(out_dtype), vocab_offset, _ptr(compact_logits), _ptr(compact_ids),
-            0 if compact_logits is None else compact_logits.numel(), _ptr(offsets), _ptr(top_value),
-            _ptr(top_index), _ptr(top_key), _ptr(scratch), 0 if scratch is None else scratch.numel(), _ptr(ws),
-            ws.numel(), _stream(hidden.device))
+            *args, DTYPE_CODES[out_dtype], vocab_offset, _address(compact_logits), compact_ids.data_ptr(),
+            0 if compact_logits is None else compact_logits.numel(), offsets.data_ptr(), _address(top_value),
+            _address(top_index), _address(top_key), *tail)
     if status:
         _check(status, "gsp_int8_compact")
 
@@ -725,29 +751,32 @@ def _filter_args(settings, uniforms, token_ids, logprobs, kept):
     """(temperature, top_k, top_p, min_p), each a number or a tensor, as scalar / array argument pairs."""
     args = []
     for v in settings:
-        args += [0, v.data_ptr()] if isinstance(v, torch.Tensor) else [v, None]
+        if isinstance(v, torch.Tensor):
+            args += (0, v.data_ptr())
+        else:
+            args += (v, None)
     return (*args, uniforms.data_ptr(), token_ids.data_ptr(), logprobs.data_ptr(), kept.data_ptr())
 
 
 def sample_logits(logits, mask, settings, uniforms, token_ids, logprobs, kept, vocab_offset: int = 0) -> None:
     """gsp_sample_logits; logits [B, V] (row stride free), mask [B, words] or None."""
-    _require_cuda(logits, mask, uniforms, token_ids)
-    with on_device(logits.device):
+    index = logits.get_device()
+    with on_device(index):
         status = load().gsp_sample_logits(
-            logits.data_ptr(), logits.stride(0), DTYPE_CODES[logits.dtype], None if mask is None else mask.data_ptr(),
+            logits.data_ptr(), logits.stride(0), DTYPE_CODES[logits.dtype], _address(mask),
             0 if mask is None else mask.stride(0), logits.shape[0], logits.shape[1], vocab_offset,
-            *_filter_args(settings, uniforms, token_ids, logprobs, kept), _stream(logits.device))
+            *_filter_args(settings, uniforms, token_ids, logprobs, kept), raw_stream(index))
     if status:
         _check(status, "gsp_sample_logits")
 
 
 def sample_compact(logits, ids, offsets, max_len: int, settings, uniforms, token_ids, logprobs, kept) -> None:
     """gsp_sample_compact; logits [N] and ids [N] packed by offsets [B + 1]."""
-    _require_cuda(logits, ids, offsets, uniforms, token_ids)
-    with on_device(logits.device):
+    index = logits.get_device()
+    with on_device(index):
         status = load().gsp_sample_compact(
             logits.data_ptr(), ids.data_ptr(), offsets.data_ptr(), logits.numel(), max_len, DTYPE_CODES[logits.dtype],
-            uniforms.numel(), *_filter_args(settings, uniforms, token_ids, logprobs, kept), _stream(logits.device))
+            uniforms.numel(), *_filter_args(settings, uniforms, token_ids, logprobs, kept), raw_stream(index))
     if status:
         _check(status, "gsp_sample_compact")
 

@@ -45,16 +45,17 @@ def quantize_rows_int8(x: torch.Tensor, *, out: QuantizedRows | None = None) -> 
     NaN and values 0, so logits computed from it are NaN. x may have any row
     stride; `out` reuses tensors (for a CUDA graph, or a preallocated head).
     """
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
-    if x.ndim != 2 or x.shape[1] < 1:
+    if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError("x must have shape [N, H]")
     if x.shape[1] > 1 and x.stride(1) != 1:
         raise ValueError("x must be contiguous along its rows")
     _native.dtype_code(x.dtype)
     if out is None:
-        out = QuantizedRows(torch.empty(x.shape, dtype=torch.int8, device=x.device),
-                            torch.empty(x.shape[0], dtype=torch.float32, device=x.device))
+        device = x.device
+        out = QuantizedRows(torch.empty(x.shape, dtype=torch.int8, device=device),
+                            torch.empty(x.shape[0], dtype=torch.float32, device=device))
     else:
         _check_rows(out, "out")
         if out.values.shape != x.shape or out.values.device != x.device:
@@ -66,11 +67,11 @@ def quantize_rows_int8(x: torch.Tensor, *, out: QuantizedRows | None = None) -> 
 
 def _check_rows(rows, what: str) -> None:
     values, scales = rows
-    if values.device.type != "cuda" or scales.device != values.device:
+    if not values.is_cuda or scales.get_device() != values.get_device():
         raise ValueError(f"{what} must hold CUDA tensors on one device")
     if values.dtype != torch.int8 or scales.dtype != torch.float32:
         raise ValueError(f"{what} must hold int8 values and float32 scales")
-    if values.ndim != 2 or scales.ndim != 1 or scales.shape[0] != values.shape[0]:
+    if values.dim() != 2 or scales.shape != values.shape[:1]:
         raise ValueError(f"{what} must hold values [N, H] and scales [N]")
     if not values.is_contiguous() or not scales.is_contiguous():
         raise ValueError(f"{what} must be contiguous")
@@ -80,15 +81,17 @@ def _inputs(hidden, weight, bitmask_gpu, out_dtype):
     """Checked operands: (hidden values [B, H], token scales or None, mask [B, words] or None, logits dtype)."""
     _check_rows(weight, "weight")
     if isinstance(hidden, torch.Tensor):
-        if hidden.device.type != "cuda":
+        if not hidden.is_cuda:
             raise ValueError("hidden and weight must be CUDA tensors")
-        values, scales = (hidden.reshape(1, -1) if hidden.ndim == 1 else hidden), None
-        if values.ndim != 2:
+        values, scales = (hidden.reshape(1, -1) if hidden.dim() == 1 else hidden), None
+        if values.dim() != 2:
             raise ValueError("hidden must have shape [D] or [B, D]")
         if not values.is_contiguous():
             raise ValueError("hidden and weight must be contiguous")
-        _native.dtype_code(values.dtype)
-        dtype = values.dtype if out_dtype is None else out_dtype
+        dtype = values.dtype
+        _native.dtype_code(dtype)
+        if out_dtype is not None:
+            dtype = out_dtype
     else:
         _check_rows(hidden, "hidden")
         values, scales = hidden
@@ -96,22 +99,23 @@ def _inputs(hidden, weight, bitmask_gpu, out_dtype):
             raise ValueError("int8 hidden states need out_dtype")
         dtype = out_dtype
     _native.dtype_code(dtype)
-    if values.device != weight.values.device:
+    if values.get_device() != weight.values.get_device():
         raise ValueError("hidden and weight must be on one device")
     vocab, hidden_dim = weight.values.shape
-    if values.shape[0] < 1 or vocab < 1:
+    batch, width = values.shape
+    if batch < 1 or vocab < 1:
         raise ValueError("hidden and weight must have at least one row")
-    if values.shape[1] != hidden_dim:
+    if width != hidden_dim:
         raise ValueError("hidden dimension mismatch")
     if hidden_dim > MAX_HIDDEN:
         raise ValueError(f"hidden dimensions above {MAX_HIDDEN} could overflow the integer sums")
     mask = bitmask_gpu
     if mask is not None:
-        if mask.device != values.device or mask.dtype != torch.int32:
+        if mask.get_device() != values.get_device() or mask.dtype != torch.int32:
             raise ValueError("bitmask_gpu must be CUDA int32")
-        if mask.ndim == 1:
+        if mask.dim() == 1:
             mask = mask.reshape(1, -1)
-        if mask.ndim != 2 or mask.shape[0] != values.shape[0] or mask.shape[1] < (vocab + 31) // 32:
+        if mask.dim() != 2 or mask.shape[0] != batch or mask.shape[1] < (vocab + 31) // 32:
             raise ValueError("bitmask shape does not match hidden batch/vocabulary")
         if not mask.is_contiguous():
             raise ValueError("bitmask must be contiguous")

@@ -551,12 +551,11 @@ _SETTINGS = (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", t
 
 def _sample_settings(values, uniforms, device):
     """Checked (temperature, top_k, top_p, min_p): numbers, or one device value per request."""
-    if uniforms.device != device or uniforms.dtype != torch.float32 or uniforms.ndim != 1 or not uniforms.is_contiguous():
+    if uniforms.device != device or uniforms.dtype != torch.float32 or uniforms.dim() != 1 or not uniforms.is_contiguous():
         raise ValueError("uniforms must be a contiguous float32 tensor [B] on the logits' device")
-    batch = uniforms.shape[0]
     for v, (name, dtype) in zip(values, _SETTINGS):
         if isinstance(v, torch.Tensor):
-            if v.device != device or v.dtype != dtype or v.shape != (batch,) or not v.is_contiguous():
+            if v.device != device or v.dtype != dtype or v.shape != uniforms.shape or not v.is_contiguous():
                 raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor with one value per request")
         elif v != v:
             raise ValueError(f"{name} is NaN")
@@ -596,29 +595,30 @@ def sample_logits(logits: torch.Tensor, *, uniforms: torch.Tensor, temperature=1
     may have any stride; shapes of the results are [B] always. grammar_sample
     draws inside the projection instead, from softmax(logits / T) unfiltered.
     """
-    if logits.device.type != "cuda":
+    if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
-    rows = logits.reshape(1, -1) if logits.ndim == 1 else logits
-    if rows.ndim != 2 or rows.shape[0] < 1 or rows.shape[1] < 1:
+    rows = logits.reshape(1, -1) if logits.dim() == 1 else logits
+    if rows.dim() != 2 or rows.shape[0] < 1 or rows.shape[1] < 1:
         raise ValueError("logits must have shape [V] or [B, V]")
-    if rows.shape[1] > 1 and rows.stride(1) != 1:
+    batch, vocab = rows.shape
+    if vocab > 1 and rows.stride(1) != 1:
         raise ValueError("logits must be contiguous along the vocabulary")
     _native.dtype_code(rows.dtype)
     dev = rows.device
-    if uniforms.shape != rows.shape[:1]:
+    if uniforms.shape != (batch,):
         raise ValueError("uniforms must hold one number per request")
     settings = _sample_settings((temperature, top_k, top_p, min_p), uniforms, dev)
     mask = bitmask_gpu
     if mask is not None:
         if mask.device != dev or mask.dtype != torch.int32:
             raise ValueError("bitmask_gpu must be CUDA int32")
-        if mask.ndim == 1:
+        if mask.dim() == 1:
             mask = mask.reshape(1, -1)
-        if mask.ndim != 2 or mask.shape[0] != rows.shape[0] or mask.shape[1] < (rows.shape[1] + 31) // 32:
+        if mask.dim() != 2 or mask.shape[0] != batch or mask.shape[1] < (vocab + 31) // 32:
             raise ValueError("bitmask shape does not match logits")
         if not mask.is_contiguous():
             raise ValueError("bitmask must be contiguous")
-    out = _sample_outputs(rows.shape[0], dev)
+    out = _sample_outputs(batch, dev)
     _native.sample_logits(rows, mask, settings, uniforms, *out)
     return out
 
@@ -631,9 +631,9 @@ def sample_compact_logits(token_ids: torch.Tensor, logits: torch.Tensor, offsets
     return them; the drawn ids come from token_ids. max_len, the longest row
     expected (default: N), only picks the launch shape. Positions past the
     end of the arrays are not read, whatever the offsets say."""
-    if logits.device.type != "cuda":
+    if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
-    if logits.ndim != 1 or token_ids.shape != logits.shape:
+    if logits.dim() != 1 or token_ids.shape != logits.shape:
         raise ValueError("token_ids and logits must have shape [N]")
     if token_ids.dtype != torch.int64 or offsets.dtype != torch.int64:
         raise ValueError("token_ids and offsets must be int64")

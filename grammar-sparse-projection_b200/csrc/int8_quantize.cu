@@ -8,16 +8,20 @@
 // has scale NaN and values 0, so that everything computed from it is NaN.
 //
 // One pass over memory: a group of 1 to 8 warps holds one row in registers
-// (chunks of 16 elements, up to kChunks per thread), takes the maximum, then
-// writes 16 bytes per chunk. Rows longer than a group's registers are read
+// (16-byte vectors, up to kHeld per thread, neighbouring lanes holding
+// neighbouring vectors), takes the maximum, then writes a vector's 8 (fp32: 4)
+// bytes. Rows longer than a group's registers are read
 // twice, the second time mostly from L2. Bound: HBM bytes (2 or 4 read, 1
 // written per element) for a whole weight, latency for a step's few rows, where
 // the group is widened until every SM-resident thread holds little.
 //
-// The division: a quotient's rounding differs from that of x * (1 / scale) only
-// where the product lies within its error (three roundings, 3 * 2^-24
-// relative, at most 127.5 * 2^-22 absolute) of a half; only those elements
-// divide.
+// The division: x * (1 / scale) is within 3 * 2^-24 relative of the quotient
+// (at most 2.3e-5 absolute), so their roundings to an integer differ only where
+// the product lies that near a half; a vector that has such an element divides.
+// Rounding by adding 1.5 * 2^23 leaves the integer in the low byte, ready to be
+// packed: an element costs about six instructions (with a float-to-integer
+// conversion, two clamps and a branch each, a weight of 248,320 x 2,048 fp16
+// took 490 us).
 #include <algorithm>
 
 #include "gsp_common.cuh"
@@ -28,13 +32,7 @@ namespace {
 
 constexpr int kQuantThreads = 256;
 constexpr int kQuantWarps = kQuantThreads / 32;
-constexpr int kChunk = 16;   // elements: one 16-byte store
-constexpr int kChunks = 4;   // chunks a thread holds
-
-template <typename T>
-struct ChunkWords {
-  static constexpr int value = kChunk * (int)sizeof(T) / 4;
-};
+constexpr int kHeld = 8;     // vectors a thread holds
 
 // |x| as ordered fp32 bits: the maximum of the bits is the maximum of the
 // magnitudes, infinities and NaN above every finite value.
@@ -56,7 +54,8 @@ __device__ __forceinline__ float magnitude(uint32_t running) {
 
 struct RowScale {
   float scale, inverse;
-  bool zero;  // nothing but zeros, or not finite: every value is 0
+  bool zero;    // nothing but zeros, or not finite: every value is 0
+  bool divide;  // the inverse is not finite (a denormal scale)
 };
 
 __device__ __forceinline__ RowScale row_scale(float amax) {
@@ -65,16 +64,14 @@ __device__ __forceinline__ RowScale row_scale(float amax) {
   r.scale = finite ? __fdiv_rn(amax, 127.f) : __int_as_float(0x7fc00000);
   r.zero = !finite || !(r.scale > 0.f);
   r.inverse = r.zero ? 0.f : __fdiv_rn(1.f, r.scale);
+  r.divide = !(r.inverse < INFINITY);
   return r;
 }
 
-__device__ __forceinline__ int quantize(float x, const RowScale& r) {
-  if (r.zero) return 0;
-  const float t = x * r.inverse;
-  float q = rintf(t);
-  // a denormal scale has an infinite inverse: its quotients divide too
-  if (!(fabsf(t - q) < 0.4999f)) q = rintf(__fdiv_rn(x, r.scale));
-  return (int)fminf(fmaxf(q, -127.f), 127.f);
+// The definition itself (the scale is positive); a denormal scale may be so
+// coarse that its quotients pass 127.
+__device__ __forceinline__ int quantize_by_division(float x, float scale) {
+  return (int)fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -127.f), 127.f);
 }
 
 template <typename T>
@@ -85,29 +82,58 @@ __device__ __forceinline__ float element(const uint32_t* words, int i) {
     return DTypeTraits<T>::bits_to_float((uint16_t)(words[i >> 1] >> (16 * (i & 1))));
 }
 
+// A vector's values, 8 (fp32: 4) bytes.
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T* src, uint32_t (&w)[ChunkWords<T>::value]) {
-  const uint4* p = reinterpret_cast<const uint4*>(src);
+struct Packed {
+  static constexpr int kWords = DTypeTraits<T>::kPerVec / 4;
+  uint32_t w[kWords];
+};
+
+template <typename T>
+__device__ __forceinline__ Packed<T> quantize_vector(const uint4& v, const RowScale& r) {
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, ties to even
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  Packed<T> out;
+  float farthest = 0.f;  // from the integer
 #pragma unroll
-  for (int v = 0; v < ChunkWords<T>::value / 4; ++v) {
-    const uint4 x = ld_stream_v4(p + v);
-    w[4 * v] = x.x;
-    w[4 * v + 1] = x.y;
-    w[4 * v + 2] = x.z;
-    w[4 * v + 3] = x.w;
+  for (int k = 0; k < Packed<T>::kWords; ++k) {
+    uint32_t q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = element<T>(w, 4 * k + j);
+      const float t = fmaf(x, r.inverse, kMagic);
+      farthest = fmaxf(farthest, fabsf(fmaf(x, r.inverse, kMagic - t)));
+      q[j] = __float_as_uint(t);
+    }
+    out.w[k] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
   }
+  if (r.divide || farthest > 0.4999f) {
+#pragma unroll
+    for (int k = 0; k < Packed<T>::kWords; ++k) {
+      out.w[k] = 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        out.w[k] |= ((uint32_t)quantize_by_division(element<T>(w, 4 * k + j), r.scale) & 0xffu) << (8 * j);
+    }
+  }
+  if (r.zero) {
+#pragma unroll
+    for (int k = 0; k < Packed<T>::kWords; ++k) out.w[k] = 0u;
+  }
+  return out;
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 quantize_chunk(const uint32_t (&w)[ChunkWords<T>::value], const RowScale& r) {
-  uint32_t out[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    out[k] = 0u;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) out[k] |= ((uint32_t)quantize(element<T>(w, 4 * k + j), r) & 0xffu) << (8 * j);
-  }
-  return make_uint4(out[0], out[1], out[2], out[3]);
+__device__ __forceinline__ void store_packed(int8_t* row, int i, const Packed<T>& v) {
+  if constexpr (Packed<T>::kWords == 2)
+    reinterpret_cast<uint2*>(row)[i] = make_uint2(v.w[0], v.w[1]);
+  else
+    reinterpret_cast<uint32_t*>(row)[i] = v.w[0];
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t vector_max(uint32_t running, const uint4& v) {
+  return word_max<T>(word_max<T>(word_max<T>(word_max<T>(running, v.x), v.y), v.z), v.w);
 }
 
 // Maximum over the row's group of `gw` warps (uniform over the CTA).
@@ -123,7 +149,7 @@ __device__ __forceinline__ float group_max(uint32_t running, int gw, float* s_ma
   return __uint_as_float(m);
 }
 
-// kVec: rows and outputs aligned to 16 bytes and whole chunks long.
+// kVec: rows and outputs aligned to 16 bytes, rows whole vectors long.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads)
     quantize_rows_kernel(const T* __restrict__ src, int64_t src_stride, int64_t rows, int cols, int8_t* values,
@@ -139,35 +165,26 @@ __global__ void __launch_bounds__(kQuantThreads)
   int8_t* out = values + (live ? row : 0) * values_stride;
   uint32_t running = 0u;
   if constexpr (kVec) {
-    const int n = live ? cols / kChunk : 0;
-    uint32_t w[kChunks][ChunkWords<T>::value];
+    const int n = live ? cols / DTypeTraits<T>::kPerVec : 0;
+    const void* base = x;
+    uint4 v[kHeld];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < kHeld; ++c) {
       const int i = t + c * nt;
-      if (i < n) {
-        load_chunk(x + (int64_t)i * kChunk, w[c]);
-#pragma unroll
-        for (int k = 0; k < ChunkWords<T>::value; ++k) running = word_max<T>(running, w[c][k]);
-      }
+      v[c] = i < n ? ld_stream_v4(static_cast<const uint4*>(base) + i) : make_uint4(0u, 0u, 0u, 0u);
+      running = vector_max<T>(running, v[c]);
     }
-    for (int i = t + kChunks * nt; i < n; i += nt) {
-      uint32_t y[ChunkWords<T>::value];
-      load_chunk(x + (int64_t)i * kChunk, y);
-#pragma unroll
-      for (int k = 0; k < ChunkWords<T>::value; ++k) running = word_max<T>(running, y[k]);
-    }
+    for (int i = t + kHeld * nt; i < n; i += nt)
+      running = vector_max<T>(running, ld_stream_v4(static_cast<const uint4*>(base) + i));
     const RowScale r = row_scale(group_max<T>(running, gw, s_max));
     if (live && t == 0) scales[row] = r.scale;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < kHeld; ++c) {
       const int i = t + c * nt;
-      if (i < n) reinterpret_cast<uint4*>(out)[i] = quantize_chunk<T>(w[c], r);
+      if (i < n) store_packed<T>(out, i, quantize_vector<T>(v[c], r));
     }
-    for (int i = t + kChunks * nt; i < n; i += nt) {
-      uint32_t y[ChunkWords<T>::value];
-      load_chunk(x + (int64_t)i * kChunk, y);
-      reinterpret_cast<uint4*>(out)[i] = quantize_chunk<T>(y, r);
-    }
+    for (int i = t + kHeld * nt; i < n; i += nt)
+      store_packed<T>(out, i, quantize_vector<T>(ld_stream_v4(static_cast<const uint4*>(base) + i), r));
   } else {
     using Bits = typename DTypeTraits<T>::Bits;
     const Bits* xb = reinterpret_cast<const Bits*>(x);
@@ -175,7 +192,8 @@ __global__ void __launch_bounds__(kQuantThreads)
     for (int i = t; i < n; i += nt) running = word_max<T>(running, (uint32_t)__ldg(xb + i));
     const RowScale r = row_scale(group_max<T>(running, gw, s_max));
     if (live && t == 0) scales[row] = r.scale;
-    for (int i = t; i < n; i += nt) out[i] = (int8_t)quantize(DTypeTraits<T>::bits_to_float(__ldg(xb + i)), r);
+    for (int i = t; i < n; i += nt)
+      out[i] = r.zero ? (int8_t)0 : (int8_t)quantize_by_division(DTypeTraits<T>::bits_to_float(__ldg(xb + i)), r.scale);
   }
 }
 
@@ -185,15 +203,15 @@ cudaError_t launch_typed(const void* src, int64_t src_stride, int64_t rows, int 
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  const bool vec = cols % kChunk == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0 &&
+  const bool vec = cols % DTypeTraits<T>::kPerVec == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0 &&
                    (reinterpret_cast<uintptr_t>(values) & 15) == 0 &&
-                   (rows == 1 || ((src_stride * (int64_t)sizeof(T)) % 16 == 0 && values_stride % 16 == 0));
+                   (rows == 1 || ((src_stride * (int64_t)sizeof(T)) % 16 == 0 && values_stride % 8 == 0));
   // Warps per row: enough to hold the row in registers; with few rows, more,
-  // until the grid fills the SMs or a thread is left with one chunk (or one
+  // until the grid fills the SMs or a thread is left with one vector (or one
   // element of the unaligned path).
-  const int64_t units = vec ? cols / kChunk : cols;
+  const int64_t units = vec ? cols / DTypeTraits<T>::kPerVec : cols;
   int gw = 1;
-  while (gw < kQuantWarps && ((vec && units > (int64_t)32 * gw * kChunks) ||
+  while (gw < kQuantWarps && ((vec && units > (int64_t)32 * gw * kHeld) ||
                               (units > 32 * gw && rows * gw < (int64_t)num_sms(dev) * kQuantWarps)))
     gw *= 2;
   const int64_t per_block = kQuantWarps / gw;

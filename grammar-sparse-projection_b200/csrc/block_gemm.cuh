@@ -131,6 +131,14 @@ __device__ __forceinline__ int list_slot(const GemmConfig& c, const int* s_pref,
   return lo * kBuilderTiles + (pos - s_pref[lo]);
 }
 
+// int8 kernels load only the 32-row groups of a tile that hold a legal token
+// (the other rows of the accumulator come out of whatever the stage held before
+// and are masked): list entries carry the groups' four flags above the tile id.
+constexpr int kGroupRows = 32;
+constexpr int kEntryBits = 24;
+constexpr int32_t kEntryTile = (1 << kEntryBits) - 1;
+constexpr uint32_t kGroupBytes = kGroupRows * kTileKBytes;
+
 // Tile id of compacted position `pos`, the CTA's i-th tile.
 __device__ __forceinline__ int tile_at(const BlockGemmParams& p, const GemmConfig& c, const int* s_pref,
                                        const int* s_mine, int pos, int i) {
@@ -328,24 +336,46 @@ __device__ __forceinline__ WarpKey<T> epilogue_unit(uint32_t taddr, uint32_t wor
       if constexpr (kSample) sample_column<T>(su, jj, legal, bits);
     }
   }
-  // transpose-reduce: lane l ends with the maximum over the 32 rows of
-  // column l % kCols
+  if constexpr (IsInt8Rows<T>::value) {
+    // one integer warp reduction per column (a 16-bit logit's key in one; an
+    // fp32 logit's value, then the lowest row that holds it); lane l keeps
+    // column l % kCols. (A third of the transpose-reduce's instructions.)
+    Key mine = Key(0);
 #pragma unroll
-  for (int h = kCols / 2; h >= 1; h >>= 1) {
-    const bool upper = (lane & h) != 0;
-#pragma unroll
-    for (int j = 0; j < h; ++j) {
-      const Key send = upper ? key[j] : key[j + h];
-      const Key keep = upper ? key[j + h] : key[j];
-      const Key recv = shfl_xor_key(send, h);
-      key[j] = keep > recv ? keep : recv;
+    for (int jj = 0; jj < kCols; ++jj) {
+      Key best;
+      if constexpr (sizeof(Key) == 4) {
+        best = __reduce_max_sync(FULL_MASK, (uint32_t)key[jj]);
+      } else {
+        const uint32_t o = (uint32_t)(key[jj] >> 32);  // 0: not legal
+        const uint32_t top = __reduce_max_sync(FULL_MASK, o);
+        const unsigned at = __ballot_sync(FULL_MASK, o == top);
+        best = top == 0u ? Key(0) : ((unsigned long long)top << 32) | (0xffffffffu - (uint32_t)(__ffs(at) - 1));
+      }
+      if ((lane & (kCols - 1)) == jj) mine = best;
     }
+    return mine;
   }
-  if constexpr (kCols == 16) {
-    const Key other = shfl_xor_key(key[0], 16);
-    key[0] = key[0] > other ? key[0] : other;
+  if constexpr (!IsInt8Rows<T>::value) {
+    // transpose-reduce: lane l ends with the maximum over the 32 rows of
+    // column l % kCols
+#pragma unroll
+    for (int h = kCols / 2; h >= 1; h >>= 1) {
+      const bool upper = (lane & h) != 0;
+#pragma unroll
+      for (int j = 0; j < h; ++j) {
+        const Key send = upper ? key[j] : key[j + h];
+        const Key keep = upper ? key[j + h] : key[j];
+        const Key recv = shfl_xor_key(send, h);
+        key[j] = keep > recv ? keep : recv;
+      }
+    }
+    if constexpr (kCols == 16) {
+      const Key other = shfl_xor_key(key[0], 16);
+      key[0] = key[0] > other ? key[0] : other;
+    }
+    return key[0];
   }
-  return key[0];
 }
 
 // kNarrow: the batch pads to 32 columns (one 16-column unit per epilogue warp).
@@ -353,7 +383,8 @@ __device__ __forceinline__ WarpKey<T> epilogue_unit(uint32_t taddr, uint32_t wor
 template <typename T, bool kNarrow, bool kSample>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     tc_projection_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_h,
-                         const BlockGemmParams p, const GemmConfig c) {
+                         const __grid_constant__ CUtensorMap tmap_group, const BlockGemmParams p,
+                         const GemmConfig c) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   // 128-byte-swizzled TMA tiles need 1024-byte alignment; the launch reserves
   // 1 KB of slack for this round-up.
@@ -490,19 +521,36 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   if (warp == 0) {
     // ---- TMA producer -------------------------------------------------------
     if (lane == 0) {
-      uint32_t g = 0;
+      // (stage and parity are counted up: the division that gave them from g was
+      // a good part of the thread's time per stage)
+      uint32_t g = 0, parity = 1;  // a fresh `empty` barrier lets parity 1 pass
+      int s = 0;
       for (int pos = cta, i = 0; pos < total && !*abort_flag; pos += G, ++i) {
-        const int tile = tile_at(p, c, s_pref, s_mine, pos, i);
+        int tile = tile_at(p, c, s_pref, s_mine, pos, i), groups = 15;
+        if (kInt8 && !p.dense) {
+          groups = tile >> kEntryBits;
+          tile &= kEntryTile;
+        }
+        const uint32_t w_bytes = (uint32_t)__popc(groups) * kGroupBytes;
         for (int kb = 0; kb < c.kblocks; ++kb, ++g) {
-          const int s = (int)(g % (uint32_t)c.stages);
-          const uint32_t use = g / (uint32_t)c.stages;
-          if (use > 0 && !mbar_wait(empty + s, (use - 1) & 1u, abort_flag)) {
+          if (!mbar_wait(empty + s, parity, abort_flag)) {
             *abort_flag = 1;
             break;
           }
-          mbar_arrive_expect_tx(full + s, kABytes + (uint32_t)(c.npad * kTileKBytes));
-          tma_load_2d(s_a + (size_t)s * kABytes, &tmap_w, kb * kTileK, tile * kTileRows, full + s);
+          mbar_arrive_expect_tx(full + s, w_bytes + (uint32_t)(c.npad * kTileKBytes));
+          if (!kInt8 || groups == 15) {
+            tma_load_2d(s_a + (size_t)s * kABytes, &tmap_w, kb * kTileK, tile * kTileRows, full + s);
+          } else {
+            for (int gr = 0; gr < 4; ++gr)
+              if ((groups >> gr) & 1)
+                tma_load_2d(s_a + (size_t)s * kABytes + gr * kGroupBytes, &tmap_group, kb * kTileK,
+                            tile * kTileRows + gr * kGroupRows, full + s);
+          }
           tma_load_2d(s_b + (size_t)s * c.npad * kTileKBytes, &tmap_h, kb * kTileK, 0, full + s);
+          if (++s == c.stages) {
+            s = 0;
+            parity ^= 1u;
+          }
         }
       }
       // Let every issued copy land before the CTA can exit: the stage ring is
@@ -517,9 +565,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   } else if (warp == 1) {
     // ---- MMA issuer ---------------------------------------------------------
     if (lane == 0) {
-      uint32_t g = 0;
-      int last_stage = -1;
-      uint32_t last_use = 0;
+      int s = 0, last_stage = -1;
+      uint32_t parity = 0, last_parity = 0;
+      const uint64_t a_desc = tc_desc_sw128(s_a), b_desc = tc_desc_sw128(s_b);  // stage 0; addresses count 16 bytes
+      const uint32_t b_step = (uint32_t)(c.npad * kTileKBytes) >> 4;
       int i = 0;
       for (int pos = cta; pos < total && !*abort_flag; pos += G, ++i) {
         const int acc = i & ((1 << c.acc_shift) - 1);
@@ -531,17 +580,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         tc_fence_after_sync();
         const uint32_t d = tmem_base + (uint32_t)(acc * c.npad);
         bool ok = true;
-        for (int kb = 0; kb < c.kblocks; ++kb, ++g) {
-          const int s = (int)(g % (uint32_t)c.stages);
-          const uint32_t use = g / (uint32_t)c.stages;
-          if (!mbar_wait(full + s, use & 1u, abort_flag)) {
+        for (int kb = 0; kb < c.kblocks; ++kb) {
+          if (!mbar_wait(full + s, parity, abort_flag)) {
             *abort_flag = 1;
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint64_t ad = tc_desc_sw128(s_a + (size_t)s * kABytes);
-          const uint64_t bd = tc_desc_sw128(s_b + (size_t)s * c.npad * kTileKBytes);
+          const uint64_t ad = a_desc + (uint64_t)((uint32_t)s * (kABytes >> 4));
+          const uint64_t bd = b_desc + (uint64_t)((uint32_t)s * b_step);
 #pragma unroll
           for (int k = 0; k < kTileKBytes / 32; ++k) {
             if constexpr (kInt8)
@@ -551,14 +598,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
           tc_commit(empty + s);  // stage s is free once these MMAs complete
           last_stage = s;
-          last_use = use;
+          last_parity = parity;
+          if (++s == c.stages) {
+            s = 0;
+            parity ^= 1u;
+          }
         }
         if (!ok) break;
         tc_commit(tfull + acc);  // accumulator `acc` is complete
       }
       // all tensor-core work of this CTA has finished once the last stage
       // commit has arrived
-      if (last_stage >= 0) mbar_wait(empty + last_stage, last_use & 1u, nullptr);
+      if (last_stage >= 0) mbar_wait(empty + last_stage, last_parity, nullptr);
     }
   } else {
     // ---- epilogue: warps 2..9; warp w reads TMEM lane quadrant w % 4 -------
@@ -578,7 +629,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     for (int pos = cta; pos < total; pos += G, ++i) {
       const int acc = i & ((1 << c.acc_shift) - 1);
       const uint32_t ause = (uint32_t)(i >> c.acc_shift);
-      const int tile = tile_at(p, c, s_pref, s_mine, pos, i);
+      int tile = tile_at(p, c, s_pref, s_mine, pos, i);
+      if (kInt8 && !p.dense) tile &= kEntryTile;
       const int row0 = tile * kTileRows + q * 32;
       const int word_idx = tile * 4 + q;  // mask word holding this warp's 32 rows
       // mask words first: their loads overlap the wait for the accumulator
@@ -732,14 +784,22 @@ __global__ void __launch_bounds__(kBuilderThreads) tile_builder_kernel(const Blo
     const int groups = kBuilderThreads / kBuilderTiles;
     const int t = t0 + lt;
     uint32_t any = 0u;
+    uint32_t word[4] = {0u, 0u, 0u, 0u};  // int8: the tile's words one by one
     if (t < ntiles && t * 4 + 4 <= nw && (reinterpret_cast<uintptr_t>(p.mask) & 15) == 0 && p.mask_stride % 4 == 0) {
       // the tile's 4 words as one 16-byte load per request: a warp reads 512
       // contiguous bytes per request
 #pragma unroll 4
       for (int b = grp; b < B; b += groups) {
         const uint4 q = __ldg(reinterpret_cast<const uint4*>(p.mask + (int64_t)b * p.mask_stride + t * 4));
-        any |= tail_clip(q.x, t * 4, V) | tail_clip(q.y, t * 4 + 1, V) | tail_clip(q.z, t * 4 + 2, V) |
-               tail_clip(q.w, t * 4 + 3, V);
+        if constexpr (IsInt8Rows<T>::value) {
+          word[0] |= tail_clip(q.x, t * 4, V);
+          word[1] |= tail_clip(q.y, t * 4 + 1, V);
+          word[2] |= tail_clip(q.z, t * 4 + 2, V);
+          word[3] |= tail_clip(q.w, t * 4 + 3, V);
+        } else {
+          any |= tail_clip(q.x, t * 4, V) | tail_clip(q.y, t * 4 + 1, V) | tail_clip(q.z, t * 4 + 2, V) |
+                 tail_clip(q.w, t * 4 + 3, V);
+        }
       }
     } else if (t < ntiles) {
 #pragma unroll 4
@@ -748,11 +808,19 @@ __global__ void __launch_bounds__(kBuilderThreads) tile_builder_kernel(const Blo
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int w = t * 4 + j;
-          if (w < nw) any |= tail_clip(__ldg(row + w), w, V);
+          if (w >= nw) continue;
+          const uint32_t x = tail_clip(__ldg(row + w), w, V);
+          if constexpr (IsInt8Rows<T>::value) word[j] |= x;
+          else any |= x;
         }
       }
     }
-    if (any) atomicOr(&s_act[lt], 1u);
+    if constexpr (IsInt8Rows<T>::value) {
+      const uint32_t groups = (word[0] ? 1u : 0u) | (word[1] ? 2u : 0u) | (word[2] ? 4u : 0u) | (word[3] ? 8u : 0u);
+      if (groups) atomicOr(&s_act[lt], groups);
+    } else {
+      if (any) atomicOr(&s_act[lt], 1u);
+    }
   }
   __syncthreads();
   if (tid < 32) {
@@ -761,7 +829,8 @@ __global__ void __launch_bounds__(kBuilderThreads) tile_builder_kernel(const Blo
     const bool act = valid && s_act[tid] != 0u;
     const unsigned am = __ballot_sync(FULL_MASK, act);
     const unsigned below = (1u << tid) - 1u;
-    if (act) p.tile_list[t0 + __popc(am & below)] = t;
+    const int32_t flags = IsInt8Rows<T>::value && act ? (int32_t)(s_act[tid] << kEntryBits) : 0;
+    if (act) p.tile_list[t0 + __popc(am & below)] = t | flags;
     if (tid == 0) p.tile_counts[blockIdx.x] = __popc(am);
   }
 }
@@ -853,7 +922,10 @@ cudaError_t launch_chunk(const BlockGemmParams& p, int dev, cudaStream_t stream)
   // the whole list fits the A stages and each CTA's share fits s_mine
   c.stage_list = (size_t)c.ntiles * 4 <= (size_t)c.stages * kABytes && (c.ntiles + G - 1) / G <= kMaxMine;
 
-  CUtensorMap tw, th;
+  CUtensorMap tw, th, tg = {};
+  if (kInt8 && !p.dense &&
+      !make_map<T>(&tg, p.weight, (uint64_t)p.vocab, (uint64_t)p.hidden_dim, (uint64_t)p.weight_stride, kGroupRows))
+    return cudaErrorInvalidValue;
   if (!make_map<T>(&tw, p.weight, (uint64_t)p.vocab, (uint64_t)p.hidden_dim, (uint64_t)p.weight_stride, kTileRows) ||
       !make_map<T>(&th, p.hidden, (uint64_t)p.batch, (uint64_t)p.hidden_dim, (uint64_t)p.hidden_stride,
                    (uint32_t)c.npad))
@@ -883,7 +955,7 @@ cudaError_t launch_chunk(const BlockGemmParams& p, int dev, cudaStream_t stream)
   attr[0].val.programmaticStreamSerializationAllowed = (p.dense || p.no_pdl) ? 0 : 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, tw, th, p, c);
+  return cudaLaunchKernelEx(&cfg, k, tw, th, tg, p, c);
 }
 
 template <typename T>

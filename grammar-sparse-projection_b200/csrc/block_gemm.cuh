@@ -84,6 +84,7 @@ struct GemmConfig {
   int nbuild;    // builder blocks (block mode)
   int acc_shift; // log2 of the accumulator count
   int stage_list; // block mode: the set-up copies the tile list into shared memory
+  int split;     // int8: 1: each tile has two accumulators that take turns, added up by the epilogue
   uint32_t tmem_cols;
   uint32_t idesc;
 };
@@ -307,13 +308,23 @@ template <typename T, int kCols, bool kSample>
 __device__ __forceinline__ WarpKey<T> epilogue_unit(uint32_t taddr, uint32_t word_l, int b0, int B, bool row_ok,
                                                     bool store, typename DTypeTraits<T>::OutBits* out, int64_t stride,
                                                     int lane, const UnitSampler& su, const float* s_hscale,
-                                                    float row_scale) {
+                                                    float row_scale, uint32_t second) {
   using OutBits = typename DTypeTraits<T>::OutBits;
   using Key = WarpKey<T>;
   uint32_t v[kCols];
   if constexpr (kCols == 32) tmem_ld32(taddr, v);
   else tmem_ld16(taddr, v);
   tmem_ld_wait();
+  if constexpr (IsInt8Rows<T>::value) {
+    if (second != 0u) {  // the tile's other accumulator, so many columns on
+      uint32_t v2[kCols];
+      if constexpr (kCols == 32) tmem_ld32(taddr + second, v2);
+      else tmem_ld16(taddr + second, v2);
+      tmem_ld_wait();
+#pragma unroll
+      for (int jj = 0; jj < kCols; ++jj) v[jj] += v2[jj];
+    }
+  }
   const OutBits ninf = DTypeTraits<T>::kNegInfBits;
   const uint32_t lanebit = row_ok ? (1u << lane) : 0u;
   Key key[kCols];
@@ -578,7 +589,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           break;
         }
         tc_fence_after_sync();
-        const uint32_t d = tmem_base + (uint32_t)(acc * c.npad);
+        const uint32_t d = tmem_base + (uint32_t)((acc * c.npad) << c.split);
         bool ok = true;
         for (int kb = 0; kb < c.kblocks; ++kb) {
           if (!mbar_wait(full + s, parity, abort_flag)) {
@@ -592,7 +603,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
           for (int k = 0; k < kTileKBytes / 32; ++k) {
             if constexpr (kInt8)
-              tc_mma_i8(d, ad + 2ull * k, bd + 2ull * k, c.idesc, (kb | k) != 0);
+              tc_mma_i8(d + (uint32_t)((k & c.split) * c.npad), ad + 2ull * k, bd + 2ull * k, c.idesc,
+                        (kb | (k >> c.split)) != 0);
             else
               tc_mma_f16(d, ad + 2ull * k, bd + 2ull * k, c.idesc, (kb | k) != 0);
           }
@@ -656,7 +668,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int row = row0 + lane;
       const bool row_ok = row < V;
       const bool store = row_ok && p.logits != nullptr;
-      const uint32_t tcol = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * c.npad);
+      const uint32_t tcol = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)((acc * c.npad) << c.split);
+      const uint32_t second = c.split ? (uint32_t)c.npad : 0u;
       typename DTypeTraits<T>::OutBits* out = static_cast<typename DTypeTraits<T>::OutBits*>(p.logits) + row;
       if constexpr (narrow) {
         const int b0 = 16 * half;
@@ -665,7 +678,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           su = UnitSampler{p.seeds + b0, s_skeys + b0, s_stats + b0, p.offset, p.inv_temp, p.vocab_offset + row};
         const WarpKey<T> k = epilogue_unit<T, 16, kSample>(tcol + (uint32_t)b0, words[0], b0, B, row_ok, store,
                                                            out + (int64_t)b0 * p.logits_stride, p.logits_stride, lane,
-                                                           su, s_hscale + b0, row_scale);
+                                                           su, s_hscale + b0, row_scale, second);
         running[0] = merge_warp_key<T>(running[0], k, p.vocab_offset + row0);
       } else {
 #pragma unroll
@@ -677,7 +690,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
               su = UnitSampler{p.seeds + b0, s_skeys + b0, s_stats + b0, p.offset, p.inv_temp, p.vocab_offset + row};
             const WarpKey<T> k = epilogue_unit<T, 32, kSample>(tcol + (uint32_t)b0, words[u], b0, B, row_ok, store,
                                                                out + (int64_t)b0 * p.logits_stride, p.logits_stride,
-                                                               lane, su, s_hscale + b0, row_scale);
+                                                               lane, su, s_hscale + b0, row_scale, second);
             running[u] = merge_warp_key<T>(running[u], k, p.vocab_offset + row0);
           }
         }
@@ -907,8 +920,11 @@ cudaError_t launch_chunk(const BlockGemmParams& p, int dev, cudaStream_t stream)
   // 4 accumulators let the MMA run up to 3 tiles ahead of the epilogue; TMEM
   // holds 512 fp32 columns per SM
   c.acc_shift = c.npad <= 128 ? 2 : 1;
+  // int8 with up to 64 columns: consecutive MMAs go to two accumulators in turn
+  // (the sums are exact integers, so their order does not matter)
+  c.split = kInt8 && c.npad <= 64 ? 1 : 0;
   uint32_t cols = 32;
-  while (cols < ((uint32_t)c.npad << c.acc_shift)) cols <<= 1;
+  while (cols < ((uint32_t)c.npad << (c.acc_shift + c.split))) cols <<= 1;
   c.tmem_cols = cols;
   c.idesc = kInt8 ? tc_idesc_i8((uint32_t)c.npad)
                   : tc_idesc_f16((uint32_t)c.npad, std::is_same<T, __nv_bfloat16>::value);

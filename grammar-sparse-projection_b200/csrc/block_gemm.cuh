@@ -67,11 +67,17 @@ namespace {
 
 constexpr int kTileRows = 128;
 constexpr int kTileKBytes = 128;  // K bytes per stage: one swizzle row (64 half-precision, 128 int8 elements)
-constexpr int kEpilogueWarps = 8;  // two per TMEM lane quadrant
-constexpr int kGemmThreads = 32 * (2 + kEpilogueWarps);
+// Epilogue warps: two per TMEM lane quadrant, or four for int8 operands (whose
+// tiles arrive twice as fast; their units are 16 columns wide, which keeps a
+// thread within the registers that 18 warps leave).
+template <typename T>
+struct Epilogue {
+  static constexpr int kWarps = IsInt8Rows<T>::value ? 16 : 8;
+  static constexpr int kThreads = 32 * (2 + kWarps);
+};
 constexpr int kMaxNpad = 256;
 constexpr int kMaxAcc = 4;          // TMEM accumulators (4 when npad <= 128, else 2)
-constexpr int kMaxUnits = kMaxNpad / 64;  // 32-column units per epilogue warp
+constexpr int kMaxUnits = kMaxNpad / 64;  // units per epilogue warp
 constexpr int kMaxStages = 8;
 constexpr int kMaxMine = 64;  // tiles per CTA that the set-up can list in shared memory
 constexpr uint32_t kABytes = kTileRows * kTileKBytes;  // 16 KB
@@ -148,9 +154,9 @@ __device__ __forceinline__ int tile_at(const BlockGemmParams& p, const GemmConfi
 }
 
 // -inf over every request's outputs in the inactive 128-row tiles
-// t = cta + G * (ew + kEpilogueWarps j) (block mode): a tile is inactive when
+// t = cta + G * (ew + warps * j) (block mode): a tile is inactive when
 // no request has a legal token in it, the same test the builder applies. Run
-// by the epilogue warps (ew = 0..kEpilogueWarps-1) before their first
+// by the epilogue warps (ew = 0, 1, ...) before their first
 // accumulator arrives.
 template <typename T>
 __device__ __forceinline__ void fill_inactive_tiles(const BlockGemmParams& p, int ntiles, int cta, int G, int ew,
@@ -161,7 +167,7 @@ __device__ __forceinline__ void fill_inactive_tiles(const BlockGemmParams& p, in
   const OutBits ninf = DTypeTraits<T>::kNegInfBits;
   const uint32_t x = sizeof(OutBits) == 2 ? (uint32_t)ninf | ((uint32_t)ninf << 16) : (uint32_t)ninf;
   const bool vec_ok = ((reinterpret_cast<uintptr_t>(p.logits) & 15) == 0) && (p.logits_stride % kOutVec == 0);
-  for (int t = cta + ew * G; t < ntiles; t += kEpilogueWarps * G) {
+  for (int t = cta + ew * G; t < ntiles; t += Epilogue<T>::kWarps * G) {
     uint32_t any = 0u;
     for (int b = lane; b < B; b += 32) {
       const uint32_t* row = p.mask + (int64_t)b * p.mask_stride;
@@ -215,34 +221,6 @@ __device__ __forceinline__ unsigned long long merge_unit_key(unsigned long long 
   return key > running ? key : running;
 }
 
-// Warp-local keys by logit width: 32 bits for 16-bit logits (above), 64 bits
-// (order-preserving fp32 bits, then 0xffffffff - lane) for fp32 logits.
-template <typename T>
-using WarpKey = std::conditional_t<sizeof(typename DTypeTraits<T>::OutBits) == 2, uint32_t, unsigned long long>;
-
-template <typename T>
-__device__ __forceinline__ WarpKey<T> warp_key(typename DTypeTraits<T>::OutBits bits, int lane) {
-  if constexpr (sizeof(bits) == 2)
-    return warp_key16(bits, 0xffffu - (uint32_t)lane);
-  else
-    return top1_key(__uint_as_float(bits), (uint64_t)lane);
-}
-
-template <typename T>
-__device__ __forceinline__ unsigned long long merge_warp_key(unsigned long long running, WarpKey<T> k,
-                                                             int64_t row_base) {
-  if constexpr (sizeof(WarpKey<T>) == 4) {
-    return merge_unit_key<T>(running, k, row_base);
-  } else {
-    if (k == 0ull) return running;
-    const unsigned long long key = top1_key(key_value(k), (uint64_t)(row_base + key_index(k)));
-    return key > running ? key : running;
-  }
-}
-
-__device__ __forceinline__ uint32_t shfl_xor_key(uint32_t k, int m) { return __shfl_xor_sync(FULL_MASK, k, m); }
-__device__ __forceinline__ unsigned long long shfl_xor_key(unsigned long long k, int m) { return shfl_xor_u64(k, m); }
-
 // Sampler state of one epilogue unit (kSample kernels): its requests' seeds and
 // the CTA's per-request accumulators in shared memory, all offset to the
 // unit's first column, and the global token id of this lane's row.
@@ -287,115 +265,122 @@ __device__ __forceinline__ void sample_column(const UnitSampler& su, int jj, boo
   }
 }
 
-// One accumulator column's logit: the fp32 sum, or (int8 operands) the exact
-// integer sum times the request's scale times the vocabulary row's.
-template <typename T>
-__device__ __forceinline__ float column_logit(uint32_t acc, const float* s_hscale, int jj, float row_scale) {
-  if constexpr (IsInt8Rows<T>::value)
-    return __fmul_rn(__fmul_rn((float)(int)acc, s_hscale[jj]), row_scale);
-  else
-    return __uint_as_float(acc);
-}
-
 // One epilogue unit: kCols accumulator columns (requests b0 .. b0 + kCols - 1)
 // of this warp's 32 TMEM lanes (one vocabulary row per thread). Rounds to the
 // logits dtype, applies the mask bit (word_l: this lane's mask word for
 // request b0 + lane % kCols), stores the row's logits (-inf where illegal) and
 // returns in lane l < kCols the warp_key maximum over the 32 rows for
 // request b0 + l. With kSample, also feeds every column to sample_column.
-// s_hscale (the unit's requests) and row_scale: int8 operands only.
 template <typename T, int kCols, bool kSample>
-__device__ __forceinline__ WarpKey<T> epilogue_unit(uint32_t taddr, uint32_t word_l, int b0, int B, bool row_ok,
-                                                    bool store, typename DTypeTraits<T>::OutBits* out, int64_t stride,
-                                                    int lane, const UnitSampler& su, const float* s_hscale,
-                                                    float row_scale, uint32_t second) {
-  using OutBits = typename DTypeTraits<T>::OutBits;
-  using Key = WarpKey<T>;
+__device__ __forceinline__ uint32_t epilogue_unit(uint32_t taddr, uint32_t word_l, int b0, int B, bool row_ok,
+                                                  bool store, uint16_t* out, int64_t stride, int lane,
+                                                  const UnitSampler& su) {
   uint32_t v[kCols];
   if constexpr (kCols == 32) tmem_ld32(taddr, v);
   else tmem_ld16(taddr, v);
   tmem_ld_wait();
-  if constexpr (IsInt8Rows<T>::value) {
-    if (second != 0u) {  // the tile's other accumulator, so many columns on
-      uint32_t v2[kCols];
-      if constexpr (kCols == 32) tmem_ld32(taddr + second, v2);
-      else tmem_ld16(taddr + second, v2);
-      tmem_ld_wait();
-#pragma unroll
-      for (int jj = 0; jj < kCols; ++jj) v[jj] += v2[jj];
-    }
-  }
-  const OutBits ninf = DTypeTraits<T>::kNegInfBits;
+  const uint16_t ninf = DTypeTraits<T>::kNegInfBits;
   const uint32_t lanebit = row_ok ? (1u << lane) : 0u;
-  Key key[kCols];
+  const uint32_t low = 0xffffu - (uint32_t)lane;
+  uint32_t key[kCols];
   if (b0 + kCols <= B) {
 #pragma unroll
     for (int jj = 0; jj < kCols; ++jj) {
       const bool legal = (__shfl_sync(FULL_MASK, word_l, jj) & lanebit) != 0u;
-      const OutBits bits = legal ? DTypeTraits<T>::round_bits(column_logit<T>(v[jj], s_hscale, jj, row_scale)) : ninf;
+      const uint16_t bits = legal ? DTypeTraits<T>::round_bits(__uint_as_float(v[jj])) : ninf;
       if (store) out[jj * stride] = bits;
-      key[jj] = legal ? warp_key<T>(bits, lane) : Key(0);
+      key[jj] = legal ? warp_key16(bits, low) : 0u;
       if constexpr (kSample) sample_column<T>(su, jj, legal, bits);
     }
   } else {
 #pragma unroll
     for (int jj = 0; jj < kCols; ++jj) {
       const bool legal = (__shfl_sync(FULL_MASK, word_l, jj) & lanebit) != 0u;  // word is 0 past B
-      const OutBits bits = legal ? DTypeTraits<T>::round_bits(column_logit<T>(v[jj], s_hscale, jj, row_scale)) : ninf;
+      const uint16_t bits = legal ? DTypeTraits<T>::round_bits(__uint_as_float(v[jj])) : ninf;
       if (store && b0 + jj < B) out[jj * stride] = bits;
-      key[jj] = legal ? warp_key<T>(bits, lane) : Key(0);
+      key[jj] = legal ? warp_key16(bits, low) : 0u;
       if constexpr (kSample) sample_column<T>(su, jj, legal, bits);
     }
   }
-  if constexpr (IsInt8Rows<T>::value) {
-    // one integer warp reduction per column (a 16-bit logit's key in one; an
-    // fp32 logit's value, then the lowest row that holds it); lane l keeps
-    // column l % kCols. (A third of the transpose-reduce's instructions.)
-    Key mine = Key(0);
+  // transpose-reduce: lane l ends with the maximum over the 32 rows of
+  // column l % kCols
 #pragma unroll
-    for (int jj = 0; jj < kCols; ++jj) {
-      Key best;
-      if constexpr (sizeof(Key) == 4) {
-        best = __reduce_max_sync(FULL_MASK, (uint32_t)key[jj]);
-      } else {
-        const uint32_t o = (uint32_t)(key[jj] >> 32);  // 0: not legal
-        const uint32_t top = __reduce_max_sync(FULL_MASK, o);
-        const unsigned at = __ballot_sync(FULL_MASK, o == top);
-        best = top == 0u ? Key(0) : ((unsigned long long)top << 32) | (0xffffffffu - (uint32_t)(__ffs(at) - 1));
-      }
+  for (int h = kCols / 2; h >= 1; h >>= 1) {
+    const bool upper = (lane & h) != 0;
+#pragma unroll
+    for (int j = 0; j < h; ++j) {
+      const uint32_t send = upper ? key[j] : key[j + h];
+      const uint32_t keep = upper ? key[j + h] : key[j];
+      const uint32_t recv = __shfl_xor_sync(FULL_MASK, send, h);
+      key[j] = keep > recv ? keep : recv;
+    }
+  }
+  if constexpr (kCols == 16) {
+    const uint32_t other = __shfl_xor_sync(FULL_MASK, key[0], 16);
+    key[0] = key[0] > other ? key[0] : other;
+  }
+  return key[0];
+}
+
+// The same for int8 operands, 16 columns: the exact integer sum (of two
+// accumulators, the other `second` columns on, unless that is 0) times the
+// request's scale times the row's. One integer warp reduction per column finds
+// the top-1 (a third of the transpose-reduce's instructions): of the key for
+// 16-bit logits, of the value for fp32 ones, whose lowest row a ballot tells.
+// Returns in lane l < 16 request b0 + l's top1_key (0: no legal token).
+template <typename T>
+__device__ __forceinline__ unsigned long long epilogue_unit_int8(
+    uint32_t taddr, uint32_t second, uint32_t word_l, int b0, int B, bool row_ok, bool store,
+    typename DTypeTraits<T>::OutBits* out, int64_t stride, int lane, const float* s_hscale, float row_scale,
+    int64_t row_base) {
+  using OutBits = typename DTypeTraits<T>::OutBits;
+  constexpr int kCols = 16;
+  uint32_t v[kCols];
+  tmem_ld16(taddr, v);
+  if (second != 0u) {
+    uint32_t v2[kCols];
+    tmem_ld16(taddr + second, v2);
+    tmem_ld_wait();
+#pragma unroll
+    for (int jj = 0; jj < kCols; ++jj) v[jj] += v2[jj];
+  } else {
+    tmem_ld_wait();
+  }
+  const OutBits ninf = DTypeTraits<T>::kNegInfBits;
+  const uint32_t lanebit = row_ok ? (1u << lane) : 0u;
+  const uint32_t low = 0xffffu - (uint32_t)lane;
+  uint32_t mine = 0u, mine_at = 0u;
+#pragma unroll
+  for (int jj = 0; jj < kCols; ++jj) {
+    const bool legal = (__shfl_sync(FULL_MASK, word_l, jj) & lanebit) != 0u;  // word is 0 past B
+    const float y = __fmul_rn(__fmul_rn((float)(int)v[jj], s_hscale[jj]), row_scale);
+    const OutBits bits = legal ? DTypeTraits<T>::round_bits(y) : ninf;
+    if (store && b0 + jj < B) out[jj * stride] = bits;
+    if constexpr (sizeof(OutBits) == 2) {
+      const uint32_t best = __reduce_max_sync(FULL_MASK, legal ? warp_key16(bits, low) : 0u);
       if ((lane & (kCols - 1)) == jj) mine = best;
-    }
-    return mine;
-  }
-  if constexpr (!IsInt8Rows<T>::value) {
-    // transpose-reduce: lane l ends with the maximum over the 32 rows of
-    // column l % kCols
-#pragma unroll
-    for (int h = kCols / 2; h >= 1; h >>= 1) {
-      const bool upper = (lane & h) != 0;
-#pragma unroll
-      for (int j = 0; j < h; ++j) {
-        const Key send = upper ? key[j] : key[j + h];
-        const Key keep = upper ? key[j + h] : key[j];
-        const Key recv = shfl_xor_key(send, h);
-        key[j] = keep > recv ? keep : recv;
+    } else {
+      const uint32_t o = legal ? ordered_bits(y) : 0u;
+      const uint32_t best = __reduce_max_sync(FULL_MASK, o);
+      const unsigned at = __ballot_sync(FULL_MASK, o == best);
+      if ((lane & (kCols - 1)) == jj) {
+        mine = best;
+        mine_at = (uint32_t)(__ffs(at) - 1);
       }
     }
-    if constexpr (kCols == 16) {
-      const Key other = shfl_xor_key(key[0], 16);
-      key[0] = key[0] > other ? key[0] : other;
-    }
-    return key[0];
   }
+  if constexpr (sizeof(OutBits) == 2) return merge_unit_key<T>(0ull, mine, row_base);
+  return mine == 0u ? 0ull : top1_key(from_ordered_bits(mine), (uint64_t)(row_base + mine_at));
 }
 
 // kNarrow: the batch pads to 32 columns (one 16-column unit per epilogue warp).
 // kSample: the fused sampler (p.sample_index != nullptr) runs in the epilogue.
 template <typename T, bool kNarrow, bool kSample>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(Epilogue<T>::kThreads, 1)
     tc_projection_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_h,
                          const __grid_constant__ CUtensorMap tmap_group, const BlockGemmParams p,
                          const GemmConfig c) {
+  constexpr int kEpilogueWarps = Epilogue<T>::kWarps, kGemmThreads = Epilogue<T>::kThreads;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   // 128-byte-swizzled TMA tiles need 1024-byte alignment; the launch reserves
   // 1 KB of slack for this round-up.
@@ -627,16 +612,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     // ---- epilogue: warps 2..9; warp w reads TMEM lane quadrant w % 4 -------
     // The quadrant's two warps split the accumulator's columns: 16 each when
     // the batch pads to 32, else alternating 32-column units.
+    // (int8: the quadrant's four warps alternate 16-column units.)
     const int ew = warp - 2;
     const int q = warp & 3;
     const int half = ew >> 2;
     constexpr bool narrow = kNarrow;
-    const int nunits = narrow ? 1 : (c.npad / 32 - half + 1) / 2;
+    const int nunits = kInt8 ? (c.npad / 16 - half + 3) / 4 : narrow ? 1 : (c.npad / 32 - half + 1) / 2;
+    const auto first_col = [&](int u) { return kInt8 ? 16 * (half + 4 * u) : unit_col(narrow, half, u); };
     if (!p.dense && p.logits) fill_inactive_tiles<T>(p, c.ntiles, cta, G, ew, lane);
     unsigned long long running[kMaxUnits];  // lane l: best key of the unit's request l
 #pragma unroll
     for (int u = 0; u < kMaxUnits; ++u) running[u] = 0ull;
-    const int ulane = narrow ? (lane & 15) : lane;  // request column a lane's mask word serves
+    const int ulane = narrow || kInt8 ? (lane & 15) : lane;  // request column a lane's mask word serves
     int i = 0;
     for (int pos = cta; pos < total; pos += G, ++i) {
       const int acc = i & ((1 << c.acc_shift) - 1);
@@ -650,7 +637,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
       for (int u = 0; u < kMaxUnits; ++u) {
         words[u] = 0u;
-        const int b = unit_col(narrow, half, u) + ulane;
+        const int b = first_col(u) + ulane;
         if (u < nunits && b < B) {
           if (!p.mask) words[u] = 0xffffffffu;
           else if (word_idx < p.nw) words[u] = __ldg(p.mask + (int64_t)b * p.mask_stride + word_idx);
@@ -671,15 +658,29 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const uint32_t tcol = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)((acc * c.npad) << c.split);
       const uint32_t second = c.split ? (uint32_t)c.npad : 0u;
       typename DTypeTraits<T>::OutBits* out = static_cast<typename DTypeTraits<T>::OutBits*>(p.logits) + row;
-      if constexpr (narrow) {
+      if constexpr (kInt8) {
+        // one copy of the unit's code: unrolled four times it pushed the copy and
+        // MMA threads' loops out of the instruction cache (4.1 -> 7.4 us a tile)
+#pragma unroll 1
+        for (int u = 0; u < nunits; ++u) {
+          const int b0 = first_col(u);
+          const uint32_t word = u == 0 ? words[0] : u == 1 ? words[1] : u == 2 ? words[2] : words[3];
+          const unsigned long long k =
+              epilogue_unit_int8<T>(tcol + (uint32_t)b0, second, word, b0, B, row_ok, store,
+                                    out + (int64_t)b0 * p.logits_stride, p.logits_stride, lane, s_hscale + b0,
+                                    row_scale, p.vocab_offset + row0);
+#pragma unroll
+          for (int r = 0; r < kMaxUnits; ++r)
+            if (r == u) running[r] = k > running[r] ? k : running[r];
+        }
+      } else if constexpr (narrow) {
         const int b0 = 16 * half;
         UnitSampler su{};
         if constexpr (kSample)
           su = UnitSampler{p.seeds + b0, s_skeys + b0, s_stats + b0, p.offset, p.inv_temp, p.vocab_offset + row};
-        const WarpKey<T> k = epilogue_unit<T, 16, kSample>(tcol + (uint32_t)b0, words[0], b0, B, row_ok, store,
-                                                           out + (int64_t)b0 * p.logits_stride, p.logits_stride, lane,
-                                                           su, s_hscale + b0, row_scale, second);
-        running[0] = merge_warp_key<T>(running[0], k, p.vocab_offset + row0);
+        const uint32_t k = epilogue_unit<T, 16, kSample>(tcol + (uint32_t)b0, words[0], b0, B, row_ok, store,
+                                                 out + (int64_t)b0 * p.logits_stride, p.logits_stride, lane, su);
+        running[0] = merge_unit_key<T>(running[0], k, p.vocab_offset + row0);
       } else {
 #pragma unroll
         for (int u = 0; u < kMaxUnits; ++u) {
@@ -688,10 +689,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             UnitSampler su{};
             if constexpr (kSample)
               su = UnitSampler{p.seeds + b0, s_skeys + b0, s_stats + b0, p.offset, p.inv_temp, p.vocab_offset + row};
-            const WarpKey<T> k = epilogue_unit<T, 32, kSample>(tcol + (uint32_t)b0, words[u], b0, B, row_ok, store,
-                                                               out + (int64_t)b0 * p.logits_stride, p.logits_stride,
-                                                               lane, su, s_hscale + b0, row_scale, second);
-            running[u] = merge_warp_key<T>(running[u], k, p.vocab_offset + row0);
+            const uint32_t k = epilogue_unit<T, 32, kSample>(tcol + (uint32_t)b0, words[u], b0, B, row_ok, store,
+                                                     out + (int64_t)b0 * p.logits_stride, p.logits_stride, lane, su);
+            running[u] = merge_unit_key<T>(running[u], k, p.vocab_offset + row0);
           }
         }
       }
@@ -702,8 +702,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (want_top) {
 #pragma unroll
       for (int u = 0; u < kMaxUnits; ++u) {
-        const int b = unit_col(narrow, half, u) + lane;
-        if (u < nunits && lane < (narrow ? 16 : 32) && b < B && running[u] != 0ull) atomicMax(&s_keys[b], running[u]);
+        const int b = first_col(u) + lane;
+        if (u < nunits && lane < (narrow || kInt8 ? 16 : 32) && b < B && running[u] != 0ull) atomicMax(&s_keys[b], running[u]);
       }
     }
   }
@@ -953,17 +953,15 @@ cudaError_t launch_chunk(const BlockGemmParams& p, int dev, cudaStream_t stream)
     if ((err = cudaGetLastError()) != cudaSuccess) return err;
   }
   const bool sample = p.sample_index != nullptr;
-  auto k = tc_projection_kernel<T, true, false>;
-  if constexpr (kInt8)  // the sampler takes half-precision operands only
-    k = c.npad == 32 ? tc_projection_kernel<T, true, false> : tc_projection_kernel<T, false, false>;
-  else
+  auto k = tc_projection_kernel<T, false, false>;
+  if constexpr (!kInt8)  // (int8 units are 16 columns wide at any batch; its kernels do not sample)
     k = c.npad == 32 ? (sample ? tc_projection_kernel<T, true, true> : tc_projection_kernel<T, true, false>)
                      : (sample ? tc_projection_kernel<T, false, true> : tc_projection_kernel<T, false, false>);
   const size_t smem_bytes = L.total + 1024;
   if ((err = raise_smem_limit(reinterpret_cast<const void*>(k), smem_bytes, dev)) != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(G);
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(Epilogue<T>::kThreads);
   cfg.dynamicSmemBytes = smem_bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

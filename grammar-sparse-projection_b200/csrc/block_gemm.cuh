@@ -624,27 +624,42 @@ __global__ void __launch_bounds__(Epilogue<T>::kThreads, 1)
 #pragma unroll
     for (int u = 0; u < kMaxUnits; ++u) running[u] = 0ull;
     const int ulane = narrow || kInt8 ? (lane & 15) : lane;  // request column a lane's mask word serves
+    // A tile's mask words and (int8) row scales are loaded while the tile before
+    // it is worked on: when the epilogue is what bounds the kernel, nothing else
+    // would hide their latency.
+    uint32_t next_words[kMaxUnits];
+    float next_scale = 0.f;
+    int next_tile = 0;
+    const auto load_next = [&](int pos, int k) {
+      if (pos >= total) return;
+      next_tile = tile_at(p, c, s_pref, s_mine, pos, k);
+      if (kInt8 && !p.dense) next_tile &= kEntryTile;
+      const int word_idx = next_tile * 4 + q;  // mask word holding this warp's 32 rows
+#pragma unroll
+      for (int u = 0; u < kMaxUnits; ++u) {
+        next_words[u] = 0u;
+        const int b = first_col(u) + ulane;
+        if (u < nunits && b < B) {
+          if (!p.mask) next_words[u] = 0xffffffffu;
+          else if (word_idx < p.nw) next_words[u] = __ldg(p.mask + (int64_t)b * p.mask_stride + word_idx);
+        }
+      }
+      if constexpr (kInt8) {
+        const int r = next_tile * kTileRows + q * 32 + lane;
+        next_scale = r < V ? __ldg(p.weight_scales + r) : 0.f;
+      }
+    };
+    load_next(cta, 0);
     int i = 0;
     for (int pos = cta; pos < total; pos += G, ++i) {
       const int acc = i & ((1 << c.acc_shift) - 1);
       const uint32_t ause = (uint32_t)(i >> c.acc_shift);
-      int tile = tile_at(p, c, s_pref, s_mine, pos, i);
-      if (kInt8 && !p.dense) tile &= kEntryTile;
-      const int row0 = tile * kTileRows + q * 32;
-      const int word_idx = tile * 4 + q;  // mask word holding this warp's 32 rows
-      // mask words first: their loads overlap the wait for the accumulator
+      const int row0 = next_tile * kTileRows + q * 32;
       uint32_t words[kMaxUnits];
 #pragma unroll
-      for (int u = 0; u < kMaxUnits; ++u) {
-        words[u] = 0u;
-        const int b = first_col(u) + ulane;
-        if (u < nunits && b < B) {
-          if (!p.mask) words[u] = 0xffffffffu;
-          else if (word_idx < p.nw) words[u] = __ldg(p.mask + (int64_t)b * p.mask_stride + word_idx);
-        }
-      }
-      float row_scale = 0.f;
-      if constexpr (kInt8) row_scale = row0 + lane < V ? __ldg(p.weight_scales + row0 + lane) : 0.f;
+      for (int u = 0; u < kMaxUnits; ++u) words[u] = next_words[u];
+      const float row_scale = next_scale;
+      load_next(pos + G, i + 1);
       const bool ok = mbar_wait(tfull + acc, ause & 1u, abort_flag);
       __syncwarp();
       if (!ok) {

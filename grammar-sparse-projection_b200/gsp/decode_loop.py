@@ -12,8 +12,12 @@ Per step, as the reference does it:
   5. the head projects it (adaptive_grammar_logits with the reference's
      signature, or the dense route, or the fused greedy top-1, or the
      CUDA-graphed head with its device-side route choice);
-  6. the next token is taken (teacher-forced target or greedy argmax) and
-     given to the matcher (accept_token), which must accept it.
+  6. the next token is taken (teacher-forced target, greedy argmax, or a draw
+     by temperature, top-k, top-p and min-p) and given to the matcher
+     (accept_token), which must accept it.
+
+Beyond the reference's heads, head="int8" projects with the weight quantised
+to int8 once (gsp.int8_head) on the route the reference rule picks.
 
 The reference drives Qwen3.5-2B from Hugging Face. Any model works here: the
 loop needs only `step(tokens) -> hidden [B, H]` and the LM-head weight
@@ -30,6 +34,7 @@ import time
 
 import torch
 
+from . import int8_head
 from . import triton_runtime as tr
 from .graphed import GraphedGrammarHead
 
@@ -128,7 +133,7 @@ class StepRecord:
     head_us: float
 
 
-HEAD_MODES = ("adaptive", "dense", "fused-top1", "graphed")
+HEAD_MODES = ("adaptive", "dense", "fused-top1", "graphed", "int8")
 
 
 class GrammarDecodeLoop:
@@ -146,6 +151,7 @@ class GrammarDecodeLoop:
         self.head, self.policy = head, policy
         self.compiler = xgr.GrammarCompiler(vocab.tokenizer_info())
         self._graphed = None
+        self.weight_int8 = int8_head.quantize_rows_int8(weight) if head == "int8" else None
 
     def new_matchers(self, schemas) -> list:
         import xgrammar as xgr
@@ -163,6 +169,10 @@ class GrammarDecodeLoop:
         if self.head == "dense":
             logits = tr.dense_masked_logits(hidden, self.weight, mask_gpu)
             return logits, logits.argmax(-1), "dense-mask"
+        if self.head == "int8":
+            route = tr._reference_route(hidden.shape[0], fractions, 0.80)
+            logits, _, top_index = int8_head.int8_grammar_logits(hidden, self.weight_int8, mask_gpu, route=route)
+            return logits, top_index, route
         if self.head == "fused-top1":
             route = tr._reference_route(hidden.shape[0], fractions, 0.80)
             logits, _, top_index = tr.grammar_logits_with_top1(hidden, self.weight, mask_gpu, route=route)
@@ -172,13 +182,19 @@ class GrammarDecodeLoop:
         logits = logits.reshape(hidden.shape[0], -1)
         return logits, logits.argmax(-1), route
 
-    def run(self, schemas, *, targets: list[list[int]] | None = None, max_steps: int = 64, on_step=None):
+    def run(self, schemas, *, targets: list[list[int]] | None = None, max_steps: int = 64, on_step=None,
+            sampling: dict | None = None, generator: torch.Generator | None = None):
         """Decodes one request per schema. With `targets` (token ids per
         request) the loop is teacher-forced, as the reference's is; without,
-        it takes the greedy token. Finished requests (matcher terminated) keep
+        it takes the greedy token, or with `sampling` (settings of
+        triton_runtime.sample_logits: temperature, top_k, top_p, min_p) a draw
+        from the masked logits, its uniform numbers from `generator` (a CUDA
+        generator; one per request and step). Finished requests (matcher terminated) keep
         an all-legal mask and are not advanced. on_step(step, hidden, mask_cpu,
         logits, tokens, route) is called before the tokens are accepted.
         Returns (token ids per request, list of StepRecord)."""
+        if sampling is not None and targets is not None:
+            raise ValueError("a teacher-forced run takes its targets: no sampling")
         batch = len(schemas)
         matchers = self.new_matchers(schemas)
         vocab = self.weight.shape[0]
@@ -207,6 +223,9 @@ class GrammarDecodeLoop:
             hidden = self.model.step(prev)
             t0 = time.perf_counter()
             logits, greedy, route = self._project(hidden, mask_cpu, mask_gpu, fractions)
+            if sampling is not None:
+                uniforms = torch.rand(batch, device=self.weight.device, generator=generator)
+                drawn = tr.sample_logits(logits, uniforms=uniforms, **sampling).token_ids.tolist()
             greedy = greedy.tolist()
             head_us = (time.perf_counter() - t0) * 1e6
             tokens = []
@@ -214,7 +233,7 @@ class GrammarDecodeLoop:
                 if targets is not None:
                     tokens.append(targets[b][step] if step < len(targets[b]) else self.vocab.stop_id)
                 else:
-                    tokens.append(int(greedy[b]))
+                    tokens.append(int(greedy[b] if sampling is None else drawn[b]))
             if on_step is not None:
                 on_step(step, hidden, mask_cpu, logits, greedy, route)
             for b, m in enumerate(matchers):

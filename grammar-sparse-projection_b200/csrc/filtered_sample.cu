@@ -65,6 +65,18 @@ static_assert(kBins == kSampleThreads, "one bin per thread");
 static_assert(32 * 16 <= kBins, "32 octaves of weights in sixteenths");
 static_assert(kMaxCluster <= kSampleWarps, "a warp for each part of the list");
 
+// 2^(j / 16) and log2(1 + j / 16).
+__constant__ double kExp2[kExpTable] = {
+    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
+    1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
+    1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
+    1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+__constant__ double kLog2[kExpTable] = {
+    0.0, 0.0874628412503394, 0.16992500144231237, 0.2479275134435855,
+    0.32192809488736235, 0.3923174227787603, 0.45943161863729726, 0.5235619560570128,
+    0.5849625007211562, 0.6438561897747247, 0.7004397181410922, 0.7548875021634686,
+    0.8073549220576041, 0.8579809951275721, 0.9068905956085185, 0.9541963103868752};
+
 // Order-preserving keys: larger logit, larger key (-0 and +0 alike); 0 for NaN
 // and -inf, which are never drawn.
 template <typename T>
@@ -115,7 +127,6 @@ struct SampleSmemHeader {
   unsigned long long pick[2][4];           // picked bin, sum before it, its own sum; [.][3] of 0: sum of all bins
   unsigned long long word[2][kMaxCluster]; // one value per CTA (all-gather)
   double exp2_table[kExpTable];            // Weigher's
-  double log2_table[kExpTable];            // log2(1 + j / 16)
   uint32_t ties_at[kTiesCap];              // positions of the drawn value's tokens
   uint32_t warp[2][kSampleWarps];
   uint32_t list_count[kMaxCluster];        // tokens in each part of the list
@@ -128,8 +139,22 @@ template <typename T>
 struct Row {
   const typename DTypeTraits<T>::Bits* x;  // the row's first logit
   const uint32_t* mask;                    // its mask words, or nullptr
-  int64_t n;                               // tokens
+  int n;                                   // tokens
 };
+
+// Request b's row; *start: its first position in the packed arrays. Positions
+// outside those are not read, whatever the offsets say, nor more than 2^30 of them.
+template <typename T>
+__device__ __forceinline__ Row<T> row_of(const FilteredSampleParams& p, int b, int64_t* start) {
+  const auto* x = static_cast<const typename DTypeTraits<T>::Bits*>(p.logits);
+  *start = 0;
+  if (p.offsets) {
+    *start = min(max(p.offsets[b], (int64_t)0), p.capacity);
+    const int64_t end = min(max(p.offsets[b + 1], *start), p.capacity);
+    return Row<T>{x + *start, nullptr, (int)min(end - *start, (int64_t)1 << 30)};
+  }
+  return Row<T>{x + (int64_t)b * p.row_stride, p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.vocab};
+}
 
 // Value at position i, read from global memory; -inf where not legal or NaN.
 template <typename T>
@@ -198,18 +223,24 @@ struct Slice {
   using Bits = typename DTypeTraits<T>::Bits;
   static constexpr int kVec = 16 / (int)sizeof(Bits);
   Row<T> row;
-  Bits* held;
-  int64_t lo, len;
-  int phase;
+  const uint4* base;     // vector 0
+  uint4* held;
+  int first;             // position of vector 0's first value (up to `phase` before the part)
+  int lo, len;
   int vectors, held_vectors;
+  int whole0, whole1;    // vectors [whole0, whole1) are the part's own throughout
 
-  __device__ __forceinline__ void set(const Row<T>& r, int64_t lo_, int64_t len_, unsigned char* smem, int room) {
+  __device__ __forceinline__ void set(const Row<T>& r, int lo_, int len_, unsigned char* smem, int room) {
     row = r;
     lo = lo_;
     len = len_;
-    held = reinterpret_cast<Bits*>(smem);
-    phase = (int)((reinterpret_cast<uintptr_t>(row.x + lo) & 15) / sizeof(Bits));
-    vectors = (int)((phase + len + kVec - 1) / kVec);
+    held = reinterpret_cast<uint4*>(smem);
+    const int phase = (int)((reinterpret_cast<uintptr_t>(row.x + lo) & 15) / sizeof(Bits));
+    base = reinterpret_cast<const uint4*>(row.x + lo - phase);
+    first = lo - phase;
+    vectors = (phase + len + kVec - 1) / kVec;
+    whole0 = phase > 0 ? 1 : 0;
+    whole1 = (phase + len) / kVec;
     held_vectors = min(vectors, room);
   }
 
@@ -223,14 +254,15 @@ struct Slice {
   }
 
   // Value at a position of the part.
-  __device__ __forceinline__ float at(int64_t pos) const {
-    const int64_t slot = pos - lo + phase;
-    return slot < (int64_t)held_vectors * kVec ? DTypeTraits<T>::bits_to_float(held[slot]) : load_value(row, pos);
+  __device__ __forceinline__ float at(uint32_t pos) const {
+    const int slot = (int)pos - first;
+    return slot / kVec < held_vectors ? DTypeTraits<T>::bits_to_float(reinterpret_cast<const Bits*>(held)[slot])
+                                      : load_value(row, pos);
   }
 
   // A vector at the part's ends, of which only some places are its own (by
   // value: nothing of the caller's goes through memory).
-  static __device__ __noinline__ uint4 end_vector(Row<T> row, int64_t pos, int64_t begin, int64_t end) {
+  static __device__ __noinline__ uint4 end_vector(Row<T> row, int pos, int begin, int end) {
     uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
@@ -246,17 +278,15 @@ struct Slice {
   // way): its words, then -inf where the mask says not legal. NaN stays (every
   // comparison with it is false).
   __device__ __forceinline__ uint4 fetch(int v, uint32_t* legal) const {
-    const int64_t pos = lo - phase + (int64_t)v * kVec;
     *legal = 0xffffffffu;
-    if (pos < lo || pos + kVec > lo + len) return end_vector(row, pos, lo, lo + len);
+    if (v < whole0 || v >= whole1) return end_vector(row, first + v * kVec, lo, lo + len);
     if (row.mask) {
-      const int64_t w0 = pos >> 5;
-      const int sh = (int)(pos & 31);
+      const int pos = first + v * kVec, w0 = pos >> 5, sh = pos & 31;
       const uint32_t a = __ldg(row.mask + w0);
       const uint32_t b = sh + kVec > 32 ? __ldg(row.mask + w0 + 1) : 0u;
       *legal = __funnelshift_r(a, b, sh);
     }
-    return ld_stream_v4(row.x + pos);
+    return ld_stream_v4(base + v);
   }
   __device__ __forceinline__ void settle(const uint4& q, uint32_t legal, uint32_t (&w)[4]) const {
     w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
@@ -303,32 +333,35 @@ struct Slice {
           c += pair_count<T>(pair_above<T>(w[j], -INFINITY));
         }
         legal_count += pair_total<T>(c);
-        if (v < held_vectors) reinterpret_cast<uint4*>(held)[v] = make_uint4(w[0], w[1], w[2], w[3]);
+        if (v < held_vectors) held[v] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
     return most.value();
   }
 
   // fn(words, position of the first value) for every vector of the part (-inf
-  // or NaN: not legal, or not of the part); the next one is under way meanwhile.
+  // or NaN: not legal, or not of the part); the next two are under way meanwhile.
   template <typename Fn>
   __device__ __forceinline__ void each_vector(Fn fn) const {
-    uint4 next = make_uint4(0u, 0u, 0u, 0u);
-    uint32_t next_legal = 0u;
+    uint4 q0 = make_uint4(0u, 0u, 0u, 0u), q1 = q0;
+    uint32_t legal0 = 0u, legal1 = 0u;
     const auto get = [&](int v) {
       if (v < held_vectors) {
-        next = reinterpret_cast<const uint4*>(held)[v];
-        next_legal = 0xffffffffu;
+        q1 = held[v];
+        legal1 = 0xffffffffu;
       } else if (v < vectors) {
-        next = fetch(v, &next_legal);
+        q1 = fetch(v, &legal1);
       }
     };
     get(threadIdx.x);
+    q0 = q1, legal0 = legal1;
+    get(threadIdx.x + kSampleThreads);
     for (int v = threadIdx.x; v < vectors; v += kSampleThreads) {
       uint32_t w[4];
-      settle(next, next_legal, w);
-      get(v + kSampleThreads);
-      fn(w, (uint32_t)(lo - phase + (int64_t)v * kVec));
+      settle(q0, legal0, w);
+      q0 = q1, legal0 = legal1;
+      get(v + 2 * kSampleThreads);
+      fn(w, (uint32_t)(first + v * kVec));
     }
   }
   // fn(value) one by one
@@ -456,13 +489,12 @@ struct Weigher {
   __device__ __forceinline__ unsigned long long operator()(float v) const { return round(unrounded(v)); }
   // Values that the bins first..last may hold: [*lo, *hi], wider by 2^-20 octave
   // on both sides (rounding moves a border by far less).
-  __device__ __forceinline__ void bin_values(int first, int last, const double* log2_table, double* lo,
-                                             double* hi) const {
+  __device__ __forceinline__ void bin_values(int first, int last, double* lo, double* hi) const {
     const auto border = [&](int k) {  // log2 of the least weight of bin k, below the maximum
       // (in doubles: with an integer shift here, nvcc 12.9 lost the shift where
       // first == last)
       const double e = -0.0625 * k, whole = floor(e);
-      return whole + log2_table[(int)((e - whole) * 16.0)];
+      return whole + kLog2[(int)((e - whole) * 16.0)];
     };
     *hi = vmax + (border(first - 1) + 9.5367431640625e-07) * octave;
     *lo = last == kBins - 1 ? cut() : vmax + (border(last) - 9.5367431640625e-07) * octave;
@@ -487,7 +519,7 @@ __device__ __forceinline__ unsigned long long prefix_target(float x, unsigned lo
 struct Team {
   SampleSmemHeader* s;  // (this CTA's)
   cg::cluster_group cluster;
-  int rank, size, size_bits;
+  int rank, size, size_bits;  // size_bits: log2 of the size, rounded up
   int buf;  // which half of `word` the next all-gather uses
 
   // All-gather of one value per CTA (the same in all its threads): the returned
@@ -679,7 +711,8 @@ __device__ __forceinline__ bool close_list(Team& team, uint32_t count, unsigned 
     total += (uint32_t)all[r];
     fits &= (uint32_t)(all[r] >> 32) <= part;
   }
-  if ((int)threadIdx.x < team.size) s->list_count[threadIdx.x] = (uint32_t)(all[threadIdx.x] >> 32);
+  if (threadIdx.x < kMaxCluster)
+    s->list_count[threadIdx.x] = (int)threadIdx.x < team.size ? (uint32_t)(all[threadIdx.x] >> 32) : 0u;
   __syncthreads();
   *sum = total;
   return fits;
@@ -701,21 +734,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   Team team{s, cg::this_cluster(), 0, 0, 0, 0};
   team.rank = (int)team.cluster.block_rank();
   team.size = (int)team.cluster.num_blocks();
-  team.size_bits = 31 - __clz(team.size);
+  team.size_bits = team.size > 1 ? 32 - __clz(team.size - 1) : 0;
   const int b = blockIdx.x / team.size, tid = threadIdx.x;
 
   // ---- the row and its settings ---------------------------------------------
-  Row<T> row;
-  int64_t start = 0;
-  if (p.offsets) {
-    // positions outside the packed arrays are not read, whatever the offsets say
-    start = min(max(p.offsets[b], (int64_t)0), p.capacity);
-    const int64_t end = min(max(p.offsets[b + 1], start), p.capacity);
-    row = Row<T>{static_cast<const Bits*>(p.logits) + start, nullptr, end - start};
-  } else {
-    row = Row<T>{static_cast<const Bits*>(p.logits) + (int64_t)b * p.row_stride,
-                 p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.vocab};
-  }
+  int64_t start;
+  const Row<T> row = row_of<T>(p, b, &start);
   const float temperature = p.temperatures ? p.temperatures[b] : p.temperature;
   const int64_t top_k = p.top_ks ? p.top_ks[b] : p.top_k;
   const float top_p = p.top_ps ? p.top_ps[b] : p.top_p;
@@ -724,18 +748,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   // every CTA of the cluster runs before its shared memory is written to
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   Slice<T> slice;
-  const int64_t n = row.n;
-  const int64_t part = ((n + team.size - 1) / team.size + 31) / 32 * 32;
-  const int64_t lo = min(part * team.rank, n);
-  slice.set(row, lo, min(part, n - lo), smem + kHeaderBytes, p.held_vectors);
+  const int n = row.n;
+  const int64_t part = (((int64_t)n + team.size - 1) / team.size + 31) / 32 * 32;
+  const int lo = (int)min(part * team.rank, (int64_t)n);
+  slice.set(row, lo, (int)min(part, (int64_t)(n - lo)), smem + kHeaderBytes, p.held_vectors);
 
   // ---- the row into shared memory, largest value, number of legal tokens ----------
   uint32_t legal = 0u;
   float vmax = slice.load(legal);
   if (tid < kExpTable) {
-    const double e = exp2((double)tid / kExpTable);
+    const double e = kExp2[tid];
     s->exp2_table[tid] = __hiloint2double(__double2hiint(e) - (tid << 16), __double2loint(e));
-    s->log2_table[tid] = log2(1.0 + tid / 16.0);
   }
   if (tid == 0) s->listed = 0u;
   {
@@ -897,7 +920,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
     // Values of a bin, as [*from, *to], a little wider than it.
     const auto bin_values = [&](int first, int last, float* from, float* to) {
       double lo, hi;
-      weigh.bin_values(first, last, s->log2_table, &lo, &hi);
+      weigh.bin_values(first, last, &lo, &hi);
       *from = fmaxf(lowest, K::value_at_least(lo));
       *to = fmaxf(*from, fminf(vmax, K::value_at_least(hi)));
     };
@@ -1037,9 +1060,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   for (int r = 0; r < team.rank; ++r) ordinal -= all[r];  // wraps for CTAs behind the owner
   if (ordinal >= here) return;
   // blocks of kSampleThreads positions in order
-  for (int64_t i0 = 0; i0 < slice.len; i0 += kSampleThreads) {
-    const int64_t i = i0 + tid;
-    const float v = i < slice.len ? slice.at(slice.lo + i) : -INFINITY;
+  for (int i0 = 0; i0 < slice.len; i0 += kSampleThreads) {
+    const int i = i0 + tid;
+    const float v = i < slice.len ? slice.at((uint32_t)(slice.lo + i)) : -INFINITY;
     const bool hit = v == draw_value;
     const unsigned hits = __ballot_sync(FULL_MASK, hit);
     __syncthreads();
@@ -1229,23 +1252,14 @@ __global__ void __launch_bounds__(kCountThreads, 1) counted_sample_kernel(const 
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
 
   // ---- the row and its settings ---------------------------------------------
-  Row<T> row;
-  int64_t start = 0;
-  if (p.offsets) {
-    // positions outside the packed arrays are not read, whatever the offsets say
-    start = min(max(p.offsets[b], (int64_t)0), p.capacity);
-    const int64_t end = min(max(p.offsets[b + 1], start), p.capacity);
-    row = Row<T>{static_cast<const Bits*>(p.logits) + start, nullptr, end - start};
-  } else {
-    row = Row<T>{static_cast<const Bits*>(p.logits) + (int64_t)b * p.row_stride,
-                 p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.vocab};
-  }
+  int64_t start;
+  const Row<T> row = row_of<T>(p, b, &start);
   const float temperature = p.temperatures ? p.temperatures[b] : p.temperature;
   const int64_t top_k = p.top_ks ? p.top_ks[b] : p.top_k;
   const float top_p = p.top_ps ? p.top_ps[b] : p.top_p;
   const float min_p = p.min_ps ? p.min_ps[b] : p.min_p;
   const float u = p.uniforms[b];
-  const int64_t n = row.n;
+  const int n = row.n;
   Slice<T> slice;
   slice.set(row, 0, n, nullptr, 0);
 
@@ -1255,24 +1269,27 @@ __global__ void __launch_bounds__(kCountThreads, 1) counted_sample_kernel(const 
     reinterpret_cast<uint4*>(s->count)[i * kCountThreads + tid] = make_uint4(0u, 0u, 0u, 0u);
   if (tid < kChunks) s->lo[tid] = s->hi[tid] = s->tokens[tid] = 0u;
   if (tid < kExpTable) {
-    const double e = exp2((double)tid / kExpTable);
+    const double e = kExp2[tid];
     s->exp2_table[tid] = __hiloint2double(__double2hiint(e) - (tid << 16), __double2loint(e));
   }
   __syncthreads();
   Counted<T> c{s, &slice, false};
   const uint32_t counted = count_block_sum(c.count_all(), s);
   // tokens of each chunk; all magnitudes' low halves must add up to what was counted
-  uint32_t low = 0u;
+  uint32_t low = 0u, top = 0u;  // top: the largest key met
   for (int j = 0; j < kMagnitudes / kCountThreads; ++j) {
     const uint32_t m = (uint32_t)(j * kCountThreads + tid), x = s->count[m];
     low += x & 0xffffu;
     if (__ballot_sync(FULL_MASK, x != 0u) == 0u) continue;
     const uint32_t negative = m == 0u || m >= Counted<T>::kInf ? 0u : x >> 16;
     const uint32_t positive = m > Counted<T>::kInf ? 0u : (x & 0xffffu) - (m == 0u ? 0u : x >> 16);
+    top = max(top, positive ? 0x8000u + m : negative ? 0x8000u - m : 0u);
     const uint32_t a = __reduce_add_sync(FULL_MASK, positive), d = __reduce_add_sync(FULL_MASK, negative);
     if (lane == 0 && a) atomicAdd(&s->tokens[chunk_of(m, false)], a);
     if (lane == 0 && d) atomicAdd(&s->tokens[chunk_of(m, true)], d);
   }
+  top = __reduce_max_sync(FULL_MASK, top);
+  if (lane == 0) s->warp[1][tid >> 5] = top;
   c.overflow = count_block_sum(low, s) != counted;
   if (c.overflow) {
     __syncthreads();
@@ -1315,7 +1332,7 @@ __global__ void __launch_bounds__(kCountThreads, 1) counted_sample_kernel(const 
     pick_place(s, c.tokens(o), target - before);
     return Border{Counted<T>::value(o, (int)s->pick[0]), before + s->pick[1], s->pick[2]};
   };
-  const float vmax = by_tokens(0ull).value;
+  const float vmax = c.overflow ? by_tokens(0ull).value : K::value(__reduce_max_sync(FULL_MASK, s->warp[1][lane]));
   const bool infinite = !(vmax < INFINITY);
   float draw_value = vmax;
   unsigned long long ordinal = 0ull;  // among the tokens of draw_value, by rising position
@@ -1357,23 +1374,49 @@ __global__ void __launch_bounds__(kCountThreads, 1) counted_sample_kernel(const 
       return x != 0u && v >= lowest ? (unsigned long long)x * weigh(v) : 0ull;
     };
     uint32_t n_kept = 0u;
-    for (int o = 0; o < kChunks; ++o) {
-      if (!is_filled(o)) continue;
-      c.prepare(o);
-      const uint32_t x = c.tokens(o);
-      if (__ballot_sync(FULL_MASK, x != 0u) == 0u) continue;
-      const float v = Counted<T>::value(o, tid);
+    const auto add_chunk = [&](int o, uint32_t x, float v, unsigned long long w) {
       if (below) n_kept += v >= border ? x : 0u;
-      const unsigned long long w = x != 0u && v >= lowest ? (unsigned long long)x * weigh(v) : 0ull;
       // (w < 2^62: three parts whose sums over the warp fit 32 bits)
       const unsigned long long sum_w =
           (unsigned long long)__reduce_add_sync(FULL_MASK, (uint32_t)w & 0x7ffffffu) +
           ((unsigned long long)__reduce_add_sync(FULL_MASK, (uint32_t)(w >> 27) & 0x7ffffffu) << 27) +
           ((unsigned long long)__reduce_add_sync(FULL_MASK, (uint32_t)(w >> 54)) << 54);
-      if (lane == 31) {
+      if (lane == 31 && sum_w) {
         const uint32_t old = atomicAdd(&s->lo[o], (uint32_t)sum_w);
         const uint32_t hi = (uint32_t)(sum_w >> 32) + (old + (uint32_t)sum_w < old ? 1u : 0u);
         if (hi) atomicAdd(&s->hi[o], hi);
+      }
+    };
+    if (c.overflow) {
+      for (int o = 0; o < kChunks; ++o) {
+        if (!is_filled(o)) continue;
+        c.prepare(o);
+        const uint32_t x = c.tokens(o);
+        const float v = Counted<T>::value(o, tid);
+        add_chunk(o, x, v, x != 0u && v >= lowest ? (unsigned long long)x * weigh(v) : 0ull);
+      }
+    } else {
+      // every warp by itself, over the chunks in which its places have tokens;
+      // two at a time, so that their chains of arithmetic run side by side
+      uint32_t busy_lo = 0u, busy_hi = 0u;  // those chunks, a bit each
+      for (int o = 0; o < kChunks; ++o) {
+        if (!is_filled(o)) continue;
+        if (__ballot_sync(FULL_MASK, c.tokens(o) != 0u) == 0u) continue;
+        if (o < 32) busy_lo |= 1u << o;
+        else busy_hi |= 1u << (o - 32);
+      }
+      unsigned long long busy = ((unsigned long long)busy_hi << 32) | busy_lo;
+      while (busy) {
+        const int o0 = __ffsll((long long)busy) - 1;
+        busy &= busy - 1ull;
+        const int o1 = busy ? __ffsll((long long)busy) - 1 : o0;
+        const bool two = busy != 0ull;
+        busy &= busy - 1ull;  // (0 stays 0)
+        const uint32_t x0 = c.tokens(o0), x1 = c.tokens(o1);
+        const float v0 = Counted<T>::value(o0, tid), v1 = Counted<T>::value(o1, tid);
+        const unsigned long long e0 = weigh(v0), e1 = weigh(v1);
+        add_chunk(o0, x0, v0, x0 != 0u && v0 >= lowest ? (unsigned long long)x0 * e0 : 0ull);
+        if (two) add_chunk(o1, x1, v1, x1 != 0u && v1 >= lowest ? (unsigned long long)x1 * e1 : 0ull);
       }
     }
     if (below) kept = count_block_sum(n_kept, s);
@@ -1486,7 +1529,7 @@ __global__ void __launch_bounds__(kCountThreads, 1) counted_sample_kernel(const 
       }
       if (incl - k <= left && left < incl) {
         for (uint32_t i = incl - k; i < left; ++i) m &= m - 1u;
-        const int64_t at = slice.lo - slice.phase + (int64_t)v * kVec + (__ffs(m) - 1);
+        const int64_t at = slice.first + v * kVec + (__ffs(m) - 1);
         p.token_ids[b] = p.ids ? p.ids[start + at] : p.vocab_offset + at;
         if (p.logprobs) p.logprobs[b] = logprob;
         if (p.kept) p.kept[b] = (int32_t)kept;
@@ -1514,15 +1557,13 @@ cudaError_t launch_typed(FilteredSampleParams p, int batch, int64_t max_len, cud
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  // CTAs per row (a power of two, up to 16): enough that shared memory holds the
-  // whole row beside a second CTA on each SM, and more while the batch leaves SMs
-  // idle and a CTA has over 4,096 tokens. What is not held is read again from L2.
+  // CTAs per row: as many as the batch leaves two per SM for, up to 8 (16 for
+  // one row alone), while each has over 4,096 tokens. What shared memory does not
+  // hold beside a second CTA on the SM is read again from L2.
   constexpr size_t kSmemMax = 227 * 1024;
-  constexpr int64_t kShare = (int64_t)(kSmemMax / 2 - 1024 - kHeaderBytes - 16) / (int64_t)sizeof(typename DTypeTraits<T>::Bits);
-  int size = 1;
-  while (size < kMaxCluster && ((size < 8 && kShare * size < max_len) ||
-                                (max_len > (int64_t)4096 * size && (int64_t)batch * size <= (int64_t)num_sms(dev))))
-    size *= 2;
+  const int64_t spare = 2 * (int64_t)num_sms(dev) / batch;
+  int64_t size64 = std::min<int64_t>(std::max<int64_t>(1, (max_len + 4095) / 4096), std::max<int64_t>(1, spare));
+  const int size = size64 >= 16 ? 16 : (int)std::min<int64_t>(size64, 8);
   const size_t room = ((int64_t)batch * size <= num_sms(dev) ? kSmemMax : kSmemMax / 2 - 1024) - kHeaderBytes;
   const int64_t part = ((max_len + size - 1) / size + 31) / 32 * 32;
   const int64_t part_vectors = (part * (int64_t)sizeof(typename DTypeTraits<T>::Bits) + 15) / 16 + 1;

@@ -1105,6 +1105,7 @@ int32_t gsp_sample_logits(const void* logits, int64_t logits_row_stride, int32_t
   const char* fn = "gsp_sample_logits";
   if (!logits) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: logits is required", fn);
   if (vocab < 1) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: vocab must be positive", fn);
+  if (vocab > (1 << 30)) return fail(GSP_ERR_UNSUPPORTED, "%s: vocab above 2^30", fn);
   const int64_t nw = ((int64_t)vocab + 31) / 32;
   if (logits_row_stride < 0) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: negative logits_row_stride", fn);
   if (bitmask && (bitmask_row_stride < 0 || (batch > 1 && bitmask_row_stride != 0 && bitmask_row_stride < nw)))

@@ -230,7 +230,7 @@ struct FilteredSampleParams {
   int64_t row_stride;
   const uint32_t* mask;
   int64_t mask_stride;
-  int64_t vocab;            // row length (packed rows: ignored)
+  int vocab;                // row length (packed rows: ignored)
   const int64_t* offsets;   // packed rows: [batch + 1], else nullptr
   const int64_t* ids;       // packed rows: token id of each position
   int64_t capacity;         // packed rows: positions that exist

@@ -44,6 +44,7 @@ def test_sample_logits_refusals():
         assert _sample(**kw) == _native.GSP_ERR_INVALID_ARGUMENT, kw
         assert word in lib.gsp_last_error(), (kw, lib.gsp_last_error())
     assert _sample(d=7) == _native.GSP_ERR_UNSUPPORTED
+    assert _sample(vocab=(1 << 30) + 1, s=1 << 31) == _native.GSP_ERR_UNSUPPORTED and b"2^30" in lib.gsp_last_error()
 
 
 def test_sample_compact_refusals():

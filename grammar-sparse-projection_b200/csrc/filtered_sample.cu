@@ -1135,7 +1135,8 @@ struct Counted {
   const Slice<T>* row;
   bool overflow;
 
-  // fn(16-bit pattern) for every token whose pattern is not -inf (NaN included)
+  // fn(16-bit pattern) for every token that the mask allows and whose pattern is
+  // not -inf (NaN included)
   template <typename Fn>
   __device__ __forceinline__ void each_pattern(Fn fn) const {
     constexpr int kAhead = 4;
@@ -1152,12 +1153,11 @@ struct Counted {
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         if (v0 + k * kCountThreads >= row->vectors) break;
-        uint32_t w[4];
-        row->settle(q[k], legal[k], w);
+        const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          fn(w[j] & 0xffffu);
-          fn(w[j] >> 16);
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t b = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu;
+          if (b != (0x8000u | kInf) && (legal[k] & (1u << j))) fn(b);
         }
       }
     }
@@ -1167,7 +1167,6 @@ struct Counted {
   __device__ __forceinline__ uint32_t count_all() const {
     uint32_t counted = 0u;
     each_pattern([&](uint32_t b) {
-      if (b == (0x8000u | kInf)) return;
       ++counted;
       atomicAdd(&s->count[b & 0x7fffu], ((b & 0x8000u) << 1) | 1u);
     });
@@ -1473,14 +1472,14 @@ __global__ void __launch_bounds__(kCountThreads, 1) counted_sample_kernel(const 
   constexpr int kVec = Slice<T>::kVec;
   // the vector's places that hold the value, as bits
   const auto hits = [&](const uint4& q, uint32_t legal) {
-    uint32_t w[4], m = 0u;
-    slice.settle(q, legal, w);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    uint32_t m = 0u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t same = pair_at_least<T>(w[j], draw_value) & ~pair_above<T>(w[j], draw_value);
       m |= ((same & 1u) | ((same >> 15) & 2u)) << (2 * j);
     }
-    return m;
+    return m & legal;
   };
   const int quarter = max((slice.vectors + 3) / 4, 8 * kCountThreads / kVec);
   uint32_t passed = 0u;  // its tokens in the quarters before

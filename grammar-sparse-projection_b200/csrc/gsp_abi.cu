@@ -956,6 +956,7 @@ int32_t gsp_quantize_rows_int8(const void* src, int64_t src_row_stride, int64_t 
     return fail(GSP_ERR_UNSUPPORTED, "%s: dtype must be GSP_DTYPE_F16, GSP_DTYPE_BF16 or GSP_DTYPE_F32", fn);
   if (rows == 0) return GSP_OK;
   if (rows > INT32_MAX) return fail(GSP_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows", fn);
+  if (cols > (1 << 30)) return fail(GSP_ERR_UNSUPPORTED, "%s: more than 2^30 columns", fn);
   if (!src || !values || !scales) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: src, values and scales are required", fn);
   if (rows > 1 && (src_row_stride < 0 || values_row_stride < cols))
     return fail(GSP_ERR_INVALID_ARGUMENT, "%s: negative src_row_stride or values_row_stride < cols", fn);

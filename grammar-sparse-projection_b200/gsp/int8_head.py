@@ -51,6 +51,8 @@ def quantize_rows_int8(x: torch.Tensor, *, out: QuantizedRows | None = None) -> 
         raise ValueError("x must have shape [N, H]")
     if x.shape[1] > 1 and x.stride(1) != 1:
         raise ValueError("x must be contiguous along its rows")
+    if x.shape[0] >= 2 ** 31 or x.shape[1] > 2 ** 30:  # (the C entries take 32-bit sizes)
+        raise ValueError("x may hold up to 2^31 - 1 rows of 2^30 columns")
     _native.dtype_code(x.dtype)
     if out is None:
         device = x.device
@@ -105,6 +107,8 @@ def _inputs(hidden, weight, bitmask_gpu, out_dtype):
     batch, width = values.shape
     if batch < 1 or vocab < 1:
         raise ValueError("hidden and weight must have at least one row")
+    if batch >= 2 ** 31 or vocab >= 2 ** 31:  # (the C entries take 32-bit sizes)
+        raise ValueError("hidden and weight may hold up to 2^31 - 1 rows")
     if width != hidden_dim:
         raise ValueError("hidden dimension mismatch")
     if hidden_dim > MAX_HIDDEN:

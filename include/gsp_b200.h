@@ -503,7 +503,7 @@ int32_t gsp_grouped_logits(const void* hidden, int64_t hidden_row_stride, const 
  * heads are fp16 / bf16 / fp32).
  *
  * gsp_quantize_rows_int8: rows of `src` (fp16, bf16 or fp32; row stride in
- * elements, 0 allowed) to int8 values and one scale each:
+ * elements, 0 allowed; up to 2^30 columns) to int8 values and one scale each:
  *   scale = max |x| / 127 (fp32 division), value = x / scale (fp32 division)
  *   rounded to the nearest integer, ties to even.
  * A row of zeros has scale 0; a row holding an infinity or NaN has scale NaN
@@ -553,15 +553,15 @@ int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t 
  *   draw the first kept token with w_1 + ... + w_i > uniforms[b] * sum.
  * Outputs: token_ids [batch], logprobs [batch] (optional: log-probability among
  * the kept tokens), kept [batch] (optional: how many were kept). Sums are exact
- * integers (weights in units below 2^-44 for rows up to 2^18 tokens), so equal
+ * integers (weights in units of 2^-43 or less for rows up to 2^18 tokens), so equal
  * calls give equal bits. Temperature 0 is greedy: the largest logit, lowest id,
  * log-probability 0, one token kept. A request without a legal token reports
  * token 0, log-probability -inf, kept 0. Settings: the scalar, or (array not
  * NULL) one device value per request; a request whose array values are not
  * valid (negative, infinite or NaN temperature, NaN top_p or min_p, uniform
  * outside [0, 1)) reports token -1, log-probability NaN, kept 0. No workspace.
- * gsp_sample_logits: rows of `vocab` logits (row stride 0 shares one row); ids
- * are vocab_offset + position. gsp_sample_compact: rows packed as
+ * gsp_sample_logits: rows of `vocab` logits, at most 2^30 (row stride 0 shares
+ * one row); ids are vocab_offset + position. gsp_sample_compact: rows packed as
  * gsp_row_sparse_compact / gsp_int8_compact write them, request b at positions
  * [request_offsets[b], request_offsets[b+1]) below `capacity`; max_len is the
  * longest row expected and only picks the launch shape. No counterpart in the

@@ -276,3 +276,25 @@ def test_streams_and_graphs(cuda_device, route):
     torch.cuda.synchronize()
     for o, w in zip(outs, want):
         assert all(torch.equal(a, b) for a, b in zip(o, w))
+
+
+@pytest.mark.parametrize("route", tr.ROUTES)
+@pytest.mark.parametrize("hidden", [31, 256])
+def test_operands_at_odd_addresses(cuda_device, route, hidden):
+    """Contiguous operands that begin in the middle of an allocation: bytes 3 and 5 off a 16-byte boundary."""
+    vocab, batch = 517, 3
+    dev = cuda_device
+    w, q = _int8_weight(41, vocab, hidden, dev), I.quantize_rows_int8(_rows(42, batch, hidden, torch.float16, dev))
+    values = torch.empty(vocab * hidden + 3, dtype=torch.int8, device=dev)[3:].view(vocab, hidden).copy_(w.values)
+    states = torch.empty(batch * hidden + 5, dtype=torch.int8, device=dev)[5:].view(batch, hidden).copy_(q.values)
+    mask = torch.from_numpy(O.make_batch_mask(np.random.default_rng(43), batch, vocab, [60, 0, 500])).to(dev)
+    legal = _legal(mask, vocab)
+    for weight, h in ((I.QuantizedRows(values, w.scales), q), (w, I.QuantizedRows(states, q.scales))):
+        got = I.int8_grammar_logits(h, weight, mask, route=route, out_dtype=torch.float16)
+        _check(h, weight, mask, torch.float16, got, legal)
+
+
+def test_sizes_past_32_bits_are_refused(cuda_device):
+    x = torch.empty(1, 2 ** 32 + 32, dtype=torch.float16, device=cuda_device)  # (32 columns, cut to 32 bits)
+    with pytest.raises(ValueError, match="2\\^30 columns"):
+        I.quantize_rows_int8(x)

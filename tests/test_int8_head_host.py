@@ -59,6 +59,7 @@ def test_int8_compact_and_quantize_refusals():
     assert q(None, 8, 4, 8, 0, FAKE, 8, FAKE, None) == _native.GSP_ERR_INVALID_ARGUMENT
     assert q(FAKE, 8, 4, 8, 0, FAKE, 4, FAKE, None) == _native.GSP_ERR_INVALID_ARGUMENT
     assert q(FAKE, 8, 1 << 31, 8, 0, FAKE, 8, FAKE, None) == _native.GSP_ERR_UNSUPPORTED
+    assert q(FAKE, 8, 1, (1 << 30) + 1, 0, FAKE, 8, FAKE, None) == _native.GSP_ERR_UNSUPPORTED
     assert q(None, 8, 0, 8, 0, None, 8, None, None) == _native.GSP_OK  # no rows: nothing to do
     assert lib.gsp_int8_scratch_bytes(0, 8) == 0 and lib.gsp_int8_scratch_bytes(3, 100) >= 3 * (112 + 4)
 

@@ -12,19 +12,21 @@
 // are the search for the first position where a running sum (of ones or of
 // weights) passes a target.
 //
-// The weights are 64-bit integers in units of 2^-shift (shift = 62 -
-// ceil(log2 n), at most 52): their sums are exact, so no order of additions
-// and no split over threads or CTAs changes a token, and equal calls give equal
-// answers bit for bit. The unit is below 2^-44 for rows up to 2^18 tokens.
+// The weights are 64-bit integers in units of 2^-shift (shift = 62 - the bit
+// length of n, at most 50): their sums are exact, so no order of additions and
+// no split over threads or CTAs changes a token, and equal calls give equal
+// answers bit for bit. The unit is at most 2^-43 for rows up to 2^18 tokens.
 //
-// One cluster of CTAs per row; the row is read from global memory once and held
+// Two kernels; long 16-bit rows in batches take the one that counts values (its
+// description below). In the other, one cluster of CTAs per row; the row is read from global memory once and held
 // in the CTAs' shared memory (-inf where the mask says not legal). A search
 // counts or weighs the tokens in 512 bins of shared memory, the CTAs read one
 // another's bins over distributed shared memory after one cluster barrier, and
 // each picks the bin at which the running sum passes the target.
 //   * The first bins are chosen by value, so that few tokens share one:
-//     sixteenths of an octave of the weight, or (top-k) 64ths of an octave of the distance to the maximum. They do not depend on
-//     the target, so top-p and the draw use the same weighing.
+//     sixteenths of an octave of the weight, or (top-k) 64ths of an octave of
+//     the distance to the maximum. They do not depend on the target, so top-p
+//     and the draw use the same weighing.
 //   * The tokens of the picked bins (for top-p: of the border's bin and of those
 //     the draw can fall into) are then listed, key and position, in the first
 //     CTA's shared memory; the other CTAs are done and leave, and the rest of the

@@ -563,7 +563,7 @@ def _sample_settings(values, uniforms, device):
     if not isinstance(t, torch.Tensor) and not 0.0 <= t < float("inf"):
         raise ValueError("temperature must be finite and not negative")
     if not isinstance(k, torch.Tensor):
-        if int(k) != k:
+        if not abs(k) < float("inf") or int(k) != k:
             raise ValueError("top_k must be a whole number")
         values = (t, max(0, min(int(k), 2 ** 31 - 1)), values[2], values[3])
     return values
@@ -601,6 +601,8 @@ def sample_logits(logits: torch.Tensor, *, uniforms: torch.Tensor, temperature=1
     if rows.dim() != 2 or rows.shape[0] < 1 or rows.shape[1] < 1:
         raise ValueError("logits must have shape [V] or [B, V]")
     batch, vocab = rows.shape
+    if batch > 2 ** 26 or vocab > 2 ** 30:  # (the C entries take 32-bit sizes)
+        raise ValueError("logits may hold up to 2^26 rows of 2^30 tokens")
     if vocab > 1 and rows.stride(1) != 1:
         raise ValueError("logits must be contiguous along the vocabulary")
     _native.dtype_code(rows.dtype)
@@ -629,7 +631,7 @@ def sample_compact_logits(token_ids: torch.Tensor, logits: torch.Tensor, offsets
     """sample_logits on packed legal rows: (token_ids int64 [N], logits [N],
     offsets int64 [B+1]) as bitmask_compact_logits and int8_compact_logits
     return them; the drawn ids come from token_ids. max_len, the longest row
-    expected (default: N), only picks the launch shape. Positions past the
+    expected (default: twice the mean), only picks the launch shape. Positions past the
     end of the arrays are not read, whatever the offsets say."""
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
@@ -641,12 +643,12 @@ def sample_compact_logits(token_ids: torch.Tensor, logits: torch.Tensor, offsets
         raise ValueError("token_ids, logits and offsets must be on one device")
     if not (token_ids.is_contiguous() and logits.is_contiguous() and offsets.is_contiguous()):
         raise ValueError("token_ids, logits and offsets must be contiguous")
-    if offsets.ndim != 1 or offsets.shape[0] < 2 or uniforms.shape[0] != offsets.shape[0] - 1:
+    if offsets.ndim != 1 or offsets.shape[0] < 2 or uniforms.shape != (offsets.shape[0] - 1,):
         raise ValueError("offsets must have shape [B + 1], uniforms [B]")
     _native.dtype_code(logits.dtype)
     settings = _sample_settings((temperature, top_k, top_p, min_p), uniforms, logits.device)
     if max_len is None:
-        max_len = logits.numel()
+        max_len = min(logits.numel(), 2 * logits.numel() // uniforms.shape[0])
     elif max_len < 0:
         raise ValueError("max_len must not be negative")
     out = _sample_outputs(uniforms.shape[0], logits.device)

@@ -69,6 +69,7 @@ def test_python_refuses_cpu_tensors():
 @pytest.mark.parametrize("values, word", [
     ((float("nan"), 0, 1.0, 0.0), "temperature"), ((-1.0, 0, 1.0, 0.0), "temperature"),
     ((float("inf"), 0, 1.0, 0.0), "temperature"), ((1.0, 2.5, 1.0, 0.0), "top_k"),
+    ((1.0, float("inf"), 1.0, 0.0), "top_k"),
     ((1.0, 0, float("nan"), 0.0), "top_p"), ((1.0, 0, 1.0, float("nan")), "min_p"),
     ((torch.ones(3), 0, 1.0, 0.0), "temperature"), ((1.0, torch.ones(2), 1.0, 0.0), "top_k"),
     ((1.0, 0, torch.ones(4)[::2], 0.0), "top_p"),

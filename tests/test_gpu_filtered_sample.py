@@ -269,3 +269,35 @@ def test_repeatable_on_streams_and_in_graphs(cuda_device):
     g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out, want2))
+
+
+def test_refusals_of_device_tensors(cuda_device):
+    dev = cuda_device
+    ids, x = torch.arange(8, device=dev), torch.zeros(8, device=dev)
+    offsets = torch.tensor([0, 8], device=dev)
+    for u in (torch.zeros((), device=dev), torch.zeros(2, device=dev), torch.zeros(1, 1, device=dev)):
+        with pytest.raises(ValueError, match="uniforms"):
+            tr.sample_compact_logits(ids, x, offsets, uniforms=u)
+        with pytest.raises(ValueError, match="uniforms"):
+            tr.sample_logits(x, uniforms=u)
+    long = torch.empty(1, 2 ** 32 + 32, dtype=torch.float16, device=dev)  # (32 tokens, cut to 32 bits)
+    with pytest.raises(ValueError, match="2\\^30 tokens"):
+        tr.sample_logits(long, uniforms=torch.zeros(1, device=dev))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_packed_rows_of_very_different_lengths(cuda_device, dtype):
+    """The launch shape follows the mean length: rows far longer and shorter than it, and any stated length, agree."""
+    dev = cuda_device
+    lengths = [1, 90000, 0, 3, 700, 20]
+    x = _logits(23, 1, sum(lengths), dtype, dev)[0]
+    ids = torch.arange(x.numel(), device=dev)
+    offsets = torch.tensor([0, *np.cumsum(lengths)], device=dev)
+    u = _uniforms(24, len(lengths), dev)
+    got = tr.sample_compact_logits(ids, x, offsets, uniforms=u, top_p=0.9)
+    at = offsets.tolist()
+    rows = [x[at[i]:at[i + 1]] for i in range(len(lengths))]
+    _check(got, rows, u, dict(top_p=0.9), ids=[ids[at[i]:at[i + 1]] for i in range(len(lengths))])
+    for max_len in (0, 1, 5000, 2 ** 40):
+        again = tr.sample_compact_logits(ids, x, offsets, uniforms=u, top_p=0.9, max_len=max_len)
+        assert all(torch.equal(a, b) for a, b in zip(again, got))

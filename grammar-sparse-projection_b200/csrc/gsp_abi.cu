@@ -890,13 +890,16 @@ constexpr int32_t kMaxInt8Hidden = 131071;  // 128 * 128 * 131071 < 2^31: the in
 
 size_t int8_row_bytes(int32_t hidden_dim) { return ((size_t)hidden_dim + 15) / 16 * 16; }
 
-// The step's hidden states as int8 rows with scales: the caller's own, or
-// quantised into the scratch buffer ([batch] rows of int8_row_bytes, then
-// [batch] scales). Everything is checked before anything is queued.
+// The step's hidden states as int8 rows with scales: the caller's own, or raw
+// rows still to be quantised into the scratch buffer ([batch] rows of
+// int8_row_bytes, then [batch] scales). Everything is checked before anything
+// is queued.
 struct Int8Hidden {
   const int8_t* values;
   int64_t stride;
   const float* scales;
+  const void* raw;  // nullptr: the values are there
+  int64_t raw_stride;
 };
 
 int32_t validate_int8(const char* fn, const void* hidden, int64_t hidden_row_stride, int32_t hidden_dtype,
@@ -925,20 +928,13 @@ int32_t validate_int8(const char* fn, const void* hidden, int64_t hidden_row_str
   return GSP_OK;
 }
 
-int32_t int8_hidden(const char* fn, const void* hidden, int64_t hidden_row_stride, int32_t hidden_dtype,
-                    const float* hidden_scales, int32_t batch, int32_t hidden_dim, void* scratch, void* stream,
-                    Int8Hidden* out) {
-  if (hidden_dtype == GSP_DTYPE_I8) {
-    *out = Int8Hidden{static_cast<const int8_t*>(hidden), hidden_row_stride, hidden_scales};
-    return GSP_OK;
-  }
+Int8Hidden int8_hidden(const void* hidden, int64_t hidden_row_stride, int32_t hidden_dtype, const float* hidden_scales,
+                       int32_t batch, int32_t hidden_dim, void* scratch) {
+  if (hidden_dtype == GSP_DTYPE_I8)
+    return Int8Hidden{static_cast<const int8_t*>(hidden), hidden_row_stride, hidden_scales, nullptr, 0};
   int8_t* values = static_cast<int8_t*>(scratch);
   const int64_t stride = (int64_t)int8_row_bytes(hidden_dim);
-  float* scales = reinterpret_cast<float*>(values + stride * batch);
-  *out = Int8Hidden{values, stride, scales};
-  return cuda_status(launch_quantize_rows_int8(hidden, hidden_row_stride, batch, hidden_dim, hidden_dtype, values,
-                                               stride, scales, static_cast<cudaStream_t>(stream)),
-                     fn);
+  return Int8Hidden{values, stride, reinterpret_cast<float*>(values + stride * batch), hidden, hidden_row_stride};
 }
 
 }  // namespace
@@ -983,14 +979,15 @@ int32_t gsp_int8_logits(int32_t route, const void* hidden, int64_t hidden_row_st
   const bool want_top = top_value || top_index || top_key;
   st = check_workspace(fn, want_top || tensor_core, workspace, workspace_bytes_, batch, vocab);
   if (st != GSP_OK) return st;
-  Int8Hidden h;
-  st = int8_hidden(fn, hidden, hidden_row_stride, hidden_dtype, hidden_scales, batch, hidden_dim, scratch, stream, &h);
-  if (st != GSP_OK) return st;
+  const Int8Hidden h = int8_hidden(hidden, hidden_row_stride, hidden_dtype, hidden_scales, batch, hidden_dim, scratch);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (!tensor_core) {
     RowSparseParams p = make_row_sparse(h.values, h.stride, weight, weight_row_stride, bitmask, bitmask_row_stride,
                                         batch, vocab, hidden_dim, vocab_offset);
     p.hidden_scales = h.scales;
+    p.raw_hidden = h.raw;
+    p.raw_stride = h.raw_stride;
+    p.raw_dtype = hidden_dtype;
     p.weight_scales = weight_scales;
     p.logits = logits;
     p.logits_stride = batch > 1 ? logits_row_stride : vocab;
@@ -999,6 +996,12 @@ int32_t gsp_int8_logits(int32_t route, const void* hidden, int64_t hidden_row_st
     p.top_key = top_key;
     if (workspace) attach_workspace(p, workspace);
     return cuda_status(launch_row_sparse_int8(p, out_dtype, s), fn);
+  }
+  if (h.raw != nullptr) {
+    const cudaError_t err =
+        launch_quantize_rows_int8(h.raw, h.raw_stride, batch, hidden_dim, hidden_dtype,
+                                  const_cast<int8_t*>(h.values), h.stride, const_cast<float*>(h.scales), s);
+    if (err != cudaSuccess) return cuda_status(err, fn);
   }
   BlockGemmParams p;
   std::memset(&p, 0, sizeof(p));
@@ -1050,12 +1053,13 @@ int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t 
   const bool want_top = top_value || top_index || top_key;
   st = check_workspace(fn, want_top, workspace, workspace_bytes_, batch, vocab);
   if (st != GSP_OK) return st;
-  Int8Hidden h;
-  st = int8_hidden(fn, hidden, hidden_row_stride, hidden_dtype, hidden_scales, batch, hidden_dim, scratch, stream, &h);
-  if (st != GSP_OK) return st;
+  const Int8Hidden h = int8_hidden(hidden, hidden_row_stride, hidden_dtype, hidden_scales, batch, hidden_dim, scratch);
   RowSparseParams p = make_row_sparse(h.values, h.stride, weight, weight_row_stride, bitmask, bitmask_row_stride,
                                       batch, vocab, hidden_dim, vocab_offset);
   p.hidden_scales = h.scales;
+  p.raw_hidden = h.raw;
+  p.raw_stride = h.raw_stride;
+  p.raw_dtype = hidden_dtype;
   p.weight_scales = weight_scales;
   p.compact = capacity > 0 ? compact_logits : nullptr;
   p.compact_ids = compact_ids;

@@ -49,6 +49,12 @@ struct RowSparseParams {
   // int8 operands: fp32 scale per request and per vocabulary row
   const float* hidden_scales;
   const float* weight_scales;
+  // int8 operands, hidden states still to be quantised (raw_hidden not null):
+  // rows of raw_dtype (GSP_DTYPE_*); `hidden` and `hidden_scales` are then
+  // buffers for them (written unless the projection quantises for itself)
+  const void* raw_hidden;
+  int64_t raw_stride;
+  int raw_dtype;
   // full logits [batch, vocab] (optional)
   void* logits;
   int64_t logits_stride;

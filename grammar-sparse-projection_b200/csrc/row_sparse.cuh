@@ -55,6 +55,7 @@
 #include "gsp_internal.h"
 #include "gsp_peer.cuh"
 #include "gsp_sampler.cuh"
+#include "int8_quantize.cuh"
 
 namespace gsp {
 namespace {
@@ -198,9 +199,10 @@ __device__ __forceinline__ void round_stats(const SampleSmem& ss, const uint32_t
 template <typename T>
 struct UnitScale {
   float token = 1.f, row = 1.f;
-  __device__ __forceinline__ void load(const RowSparseParams& p, int b, int v) {
+  // s_tokens: the token scales in shared memory, or nullptr: p.hidden_scales
+  __device__ __forceinline__ void load(const RowSparseParams& p, int b, int v, const float* s_tokens = nullptr) {
     if constexpr (IsInt8Rows<T>::value) {
-      token = __ldg(p.hidden_scales + b);
+      token = s_tokens ? s_tokens[b] : __ldg(p.hidden_scales + b);
       row = __ldg(p.weight_scales + v);
     }
   }
@@ -654,8 +656,8 @@ template <typename T, int kWpt>
 __device__ __forceinline__ void stream_rows_ranked(const RowSparseParams& p, uint64_t rbase, int n, bool has_mask,
                                                    const uint32_t* s_wincl, const uint32_t* s_excl,
                                                    const uint32_t* s_words, const uint32_t* s_pre,
-                                                   uint32_t code_stride, const void* s_h, bool want_top,
-                                                   unsigned long long* s_keys) {
+                                                   uint32_t code_stride, const void* s_h, const float* s_tokens,
+                                                   bool want_top, unsigned long long* s_keys) {
   using Bits = typename DTypeTraits<T>::Bits;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int H = p.hidden_dim, nvec = H / DTypeTraits<T>::kPerVec;
@@ -679,8 +681,8 @@ __device__ __forceinline__ void stream_rows_ranked(const RowSparseParams& p, uin
     const uint4* hb = reinterpret_cast<const uint4*>(static_cast<const Bits*>(s_h) + (size_t)bb * H);
     typename DTypeTraits<T>::Acc acc_a = 0, acc_b = 0;
     UnitScale<T> sa, sb;
-    sa.load(p, ba, va);
-    sb.load(p, bb, vb);
+    sa.load(p, ba, va, s_tokens);
+    sb.load(p, bb, vb, s_tokens);
     for (int base = 0; base < nvec; base += 32 * kUnroll) {
       uint4 ra[kUnroll], rb[kUnroll];
 #pragma unroll
@@ -713,8 +715,17 @@ __device__ __forceinline__ void stream_rows_ranked(const RowSparseParams& p, uin
 // staged kernel
 // ===========================================================================
 struct StagedLayout {
-  size_t list, keys, warp, misc, excl, words, pre, hidden, total;
+  size_t list, keys, warp, misc, excl, words, pre, hidden, quant, total;
 };
+
+// int8: hidden states of up to this many requests and bytes are quantised by
+// the kernel. Device time, against a quantiser launched before it: 1 request of
+// 2,048 fp16 (V = 248,320, 1% legal) 8.7 against 9.9 us, 1 of 8,192 12.1 / 13.4,
+// 2 of 2,048 14.0 / 15.1, 4 of 2,048 (V = 50,257) 12.6 / 13.1, but 4 of 8,192
+// 17.1 / 17.1, 4 of 4,096 fp32 15.1 / 14.3; host time 19.4 / 22.4 us
+// a call.
+constexpr int kRawMaxBatch = 4;
+constexpr int64_t kRawMaxBytes = 32 * 1024;
 
 // `words` = number of mask words staged (kThreads * words per thread).
 __host__ __device__ inline StagedLayout staged_layout(int batch, int hidden_dim, int words, int elem_bytes) {
@@ -736,9 +747,60 @@ __host__ __device__ inline StagedLayout staged_layout(int batch, int hidden_dim,
   off = l.pre + 4 * (size_t)words;
   l.hidden = align_up(off, 16);
   off = l.hidden + (size_t)elem_bytes * batch * hidden_dim;
+  l.quant = align_up(off, 16);  // int8: token scales, and each warp's maximum per request
+  if (elem_bytes == 1) off = l.quant + 4 * (size_t)kRawMaxBatch * (1 + kWarps);
   l.total = align_up(off, 128);
   return l;
 }
+
+// ---- int8 operands: hidden states quantised by the staged kernel -------------
+// A step of few requests is bound by latency: every CTA rounds the few rows for
+// itself between the barriers of its mask scan, instead of waiting for a launch
+// of the quantiser.
+// The type of the rows is the logits'. Flat 16-byte vectors: request i / rvec.
+template <typename T>
+struct RawRows {
+  __device__ __forceinline__ RawRows(const RowSparseParams&) {}
+  __device__ __forceinline__ void fetch(int) {}
+  __device__ __forceinline__ void maxima(int, float*) const {}
+  __device__ __forceinline__ void store(int, const float*, float*, void*) const {}
+};
+template <typename Out>
+struct RawRows<Int8Rows<Out>> {
+  const RowSparseParams& p;
+  const int rvec;     // vectors per request
+  uint4 first;        // this thread's first
+  __device__ __forceinline__ explicit RawRows(const RowSparseParams& p_)
+      : p(p_), rvec(p_.hidden_dim / DTypeTraits<Out>::kPerVec), first(make_uint4(0u, 0u, 0u, 0u)) {}
+  __device__ __forceinline__ uint4 at(int b, int i) const {
+    const Out* row = static_cast<const Out*>(p.raw_hidden) + (int64_t)b * p.raw_stride;
+    return __ldg(reinterpret_cast<const uint4*>(row) + (i - b * rvec));
+  }
+  __device__ __forceinline__ void fetch(int tid) {
+    if (tid < p.batch * rvec) first = at(tid / rvec, tid);
+  }
+  // Largest magnitudes of the thread's vectors, per request and warp.
+  __device__ __forceinline__ void maxima(int tid, float* s_max) const {
+    int i = tid;
+    for (int b = 0; b < p.batch; ++b) {
+      uint32_t m = 0u;
+      for (; i < (b + 1) * rvec; i += kThreads) m = vector_max<Out>(m, i == tid ? first : at(b, i));
+      m = __reduce_max_sync(FULL_MASK, __float_as_uint(magnitude<Out>(m)));
+      if ((tid & 31) == 0) s_max[b * kWarps + (tid >> 5)] = __uint_as_float(m);
+    }
+  }
+  // Values and scales, once all warps' maxima are there.
+  __device__ __forceinline__ void store(int tid, const float* s_max, float* s_tokens, void* s_h) const {
+    int i = tid;
+    for (int b = 0; b < p.batch; ++b) {
+      const uint32_t m = __reduce_max_sync(FULL_MASK, __float_as_uint(s_max[b * kWarps + (tid & (kWarps - 1))]));
+      const RowScale r = row_scale(__uint_as_float(m));
+      if (tid == 0) s_tokens[b] = r.scale;
+      for (; i < (b + 1) * rvec; i += kThreads)
+        store_packed<Out>(static_cast<int8_t*>(s_h), i, quantize_vector<Out>(i == tid ? first : at(b, i), r));
+    }
+  }
+};
 
 
 // kV 16-byte mask vectors (4 * kV words) per thread: the whole flat
@@ -761,12 +823,15 @@ __global__ void __launch_bounds__(kThreads, 1) row_sparse_staged_kernel(const Ro
   uint32_t* s_pre = reinterpret_cast<uint32_t*>(smem + L.pre);
   uint32_t* s_excl = reinterpret_cast<uint32_t*>(smem + L.excl);
   Bits* s_h = reinterpret_cast<Bits*>(smem + L.hidden);
+  float* s_tokens = reinterpret_cast<float*>(smem + L.quant);
+  float* s_max = s_tokens + kRawMaxBatch;
 
   const int tid = threadIdx.x;
   const int G = gridDim.x, cta = blockIdx.x;
   const int B = p.batch, V = p.vocab, H = p.hidden_dim, nw = p.nw;
   const int nvec = H / DTypeTraits<T>::kPerVec;
   const bool has_mask = p.mask != nullptr;
+  const bool raw = IsInt8Rows<T>::value && p.raw_hidden != nullptr;
   const bool want_top = (p.top_value != nullptr) | (p.top_index != nullptr) | (p.top_key != nullptr);
   const int F = has_mask ? B * nw : 0;  // <= kThreads * kWpt (checked on the host)
   const int w_lo = (int)((int64_t)F * cta / G), w_hi = (int)((int64_t)F * (cta + 1) / G);
@@ -776,8 +841,10 @@ __global__ void __launch_bounds__(kThreads, 1) row_sparse_staged_kernel(const Ro
   // ---- 1. loads: this thread's mask words (registers), hidden states (smem).
   //         Every load of the phase is issued before any result is used, so
   //         the phase costs one round trip, not one per load. -----------------
-  const int hvec = B * nvec;
+  const int hvec = raw ? 0 : B * nvec;
   uint4 hx = make_uint4(0, 0, 0, 0);
+  RawRows<T> rows(p);
+  if (raw) rows.fetch(tid);
   if (tid < hvec) {
     const int b = tid / nvec, j = tid - b * nvec;
     hx = __ldg(reinterpret_cast<const uint4*>(static_cast<const Bits*>(p.hidden) + (int64_t)b * p.hidden_stride) + j);
@@ -834,6 +901,7 @@ __global__ void __launch_bounds__(kThreads, 1) row_sparse_staged_kernel(const Ro
     reinterpret_cast<uint4*>(s_h)[i] = __ldg(
         reinterpret_cast<const uint4*>(static_cast<const Bits*>(p.hidden) + (int64_t)b * p.hidden_stride) + j);
   }
+  if (raw) rows.maxima(tid, s_max);
   for (int b = tid; b < B; b += kThreads) s_keys[b] = 0ull;
   if constexpr (kSample) sample_smem_init(p, s_keys);
 
@@ -882,6 +950,7 @@ __global__ void __launch_bounds__(kThreads, 1) row_sparse_staged_kernel(const Ro
   }
   // ---- 3. scan of the warp totals --------------------------------------------
   __syncthreads();
+  if (raw) rows.store(tid, s_max, s_tokens, s_h);  // (read after the next barrier)
   if (tid < 32) {
     uint32_t x = tid < kWarps ? s_warp[tid] : 0u;
 #pragma unroll
@@ -928,7 +997,7 @@ __global__ void __launch_bounds__(kThreads, 1) row_sparse_staged_kernel(const Ro
   if constexpr (!kSample) {
     // greedy: the half-warps resolve each pair's units from the prefixes, no unit list
     stream_rows_ranked<T, kWpt>(p, lo, (int)(hi - lo), has_mask, s_warp, s_excl, s_words, s_pre, code_stride, s_h,
-                                want_top, s_keys);
+                                raw ? s_tokens : nullptr, want_top, s_keys);
   } else {
   for (uint64_t rbase = lo; rbase < hi; rbase += kListCap) {
     const uint64_t rend = min(hi, rbase + (uint64_t)kListCap);
@@ -1525,8 +1594,25 @@ __global__ void __launch_bounds__(kThreads, 1) row_sparse_coop_kernel(const RowS
 // ===========================================================================
 // launch
 // ===========================================================================
+// Whether the staged kernel quantises the raw hidden states: rows of the logits'
+// type, aligned vectors, few requests.
+template <typename Out>
+constexpr int kRawCode = std::is_same<Out, __half>::value ? 0 : std::is_same<Out, __nv_bfloat16>::value ? 1 : 2;
+template <typename T>
+struct RawFit;
+template <typename Out>
+struct RawFit<Int8Rows<Out>> {
+  static bool holds(const RowSparseParams& p) {
+    return p.raw_dtype == kRawCode<Out> && p.batch <= kRawMaxBatch &&
+           (int64_t)p.batch * p.hidden_dim * (int64_t)sizeof(Out) <= kRawMaxBytes &&
+           (reinterpret_cast<uintptr_t>(p.raw_hidden) & 15) == 0 &&
+           (p.batch == 1 || p.raw_stride % DTypeTraits<Out>::kPerVec == 0);
+  }
+};
+
 template <typename T, bool kSample>
-cudaError_t launch_row_sparse_typed(const RowSparseParams& p, cudaStream_t stream) {
+cudaError_t launch_row_sparse_typed(const RowSparseParams& p0, cudaStream_t stream) {
+  RowSparseParams p = p0;
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
@@ -1536,44 +1622,50 @@ cudaError_t launch_row_sparse_typed(const RowSparseParams& p, cudaStream_t strea
                    (p.weight_stride % kPV == 0) && ((reinterpret_cast<uintptr_t>(p.hidden) & 15) == 0) &&
                    (p.batch == 1 || p.hidden_stride % kPV == 0);
   const int64_t F64 = p.mask ? (int64_t)p.batch * p.nw : 0;
-  if (vec && F64 > kCoopMinWords && p.slice_counts != nullptr && p.published != nullptr && p.slice_ready != nullptr &&
-      F64 * 32 < (int64_t)1 << 32) {
-    const CoopLayout L = coop_layout(p.batch);
-    if (L.total <= kStagedSmemMax) {
-      auto k = row_sparse_coop_kernel<T, kSample>;
-      if ((err = raise_smem_limit(reinterpret_cast<const void*>(k), L.total, dev)) != cudaSuccess) return err;
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3((unsigned)min(grid, kMaxSlices));
-      cfg.blockDim = dim3(kThreads);
-      cfg.dynamicSmemBytes = L.total;
-      cfg.stream = stream;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeCooperative;
-      attr[0].val.cooperative = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      return cudaLaunchKernelEx(&cfg, k, p);
+  const CoopLayout coop = coop_layout(p.batch);
+  const bool use_coop = vec && F64 > kCoopMinWords && p.slice_counts != nullptr && p.published != nullptr &&
+                        p.slice_ready != nullptr && F64 * 32 < (int64_t)1 << 32 && coop.total <= kStagedSmemMax;
+  const int wpt = F64 <= kThreads * 16 ? 16 : 32;
+  const StagedLayout staged = staged_layout(p.batch, p.hidden_dim, kThreads * wpt, (int)sizeof(typename DTypeTraits<T>::Bits));
+  const bool use_staged = !use_coop && vec && staged.total <= kStagedSmemMax && F64 <= kThreads * 32;
+  if constexpr (IsInt8Rows<T>::value) {
+    if (p.raw_hidden != nullptr && !(use_staged && RawFit<T>::holds(p))) {
+      err = launch_quantize_rows_int8(p.raw_hidden, p.raw_stride, p.batch, p.hidden_dim, p.raw_dtype,
+                                      static_cast<int8_t*>(const_cast<void*>(p.hidden)), p.hidden_stride,
+                                      const_cast<float*>(p.hidden_scales), stream);
+      if (err != cudaSuccess) return err;
+      p.raw_hidden = nullptr;
     }
   }
-  if (vec) {
-    const int F = p.mask ? p.batch * p.nw : 0;
-    const int wpt = F <= kThreads * 16 ? 16 : 32;
-    const StagedLayout L = staged_layout(p.batch, p.hidden_dim, kThreads * wpt, (int)sizeof(typename DTypeTraits<T>::Bits));
-    if (L.total <= kStagedSmemMax && F <= kThreads * 32) {
-      auto k = wpt == 16 ? row_sparse_staged_kernel<T, 4, kSample> : row_sparse_staged_kernel<T, 8, kSample>;
-      if ((err = raise_smem_limit(reinterpret_cast<const void*>(k), L.total, dev)) != cudaSuccess) return err;
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3((unsigned)grid);
-      cfg.blockDim = dim3(kThreads);
-      cfg.dynamicSmemBytes = L.total;
-      cfg.stream = stream;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      attr[0].val.programmaticStreamSerializationAllowed = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      return cudaLaunchKernelEx(&cfg, k, p);
-    }
+  if (use_coop) {
+    auto k = row_sparse_coop_kernel<T, kSample>;
+    if ((err = raise_smem_limit(reinterpret_cast<const void*>(k), coop.total, dev)) != cudaSuccess) return err;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)min(grid, kMaxSlices));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = coop.total;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, p);
+  }
+  if (use_staged) {
+    auto k = wpt == 16 ? row_sparse_staged_kernel<T, 4, kSample> : row_sparse_staged_kernel<T, 8, kSample>;
+    if ((err = raise_smem_limit(reinterpret_cast<const void*>(k), staged.total, dev)) != cudaSuccess) return err;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = staged.total;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, p);
   }
   const DirectLayout L = direct_layout(p.batch);
   if (vec) {

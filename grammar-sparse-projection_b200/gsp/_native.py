@@ -164,6 +164,15 @@ def dtype_code(dtype: torch.dtype) -> int:
 # ---------------------------------------------------------------------------
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
 _ws_lock = threading.Lock()
+_thread = threading.local()
+
+
+def _thread_buffers() -> dict:
+    """The calling thread's (workspace, scratch) of its int8 calls, by (device index, stream)."""
+    held = getattr(_thread, "buffers", None)
+    if held is None:
+        held = _thread.buffers = {}
+    return held
 
 
 def workspace(device: torch.device, batch: int, vocab: int) -> torch.Tensor:
@@ -180,22 +189,26 @@ def workspace(device: torch.device, batch: int, vocab: int) -> torch.Tensor:
 
 
 def reset_workspace(device: torch.device) -> None:
-    """Re-zeroes the current stream's workspace (needed after a call whose
+    """Re-zeroes the current stream's workspaces (needed after a call whose
     kernel reported an error through workspace_error)."""
     dev_index = device.index if device.index is not None else torch.cuda.current_device()
-    ws = _workspaces.get((dev_index, torch.cuda.current_stream(device).cuda_stream))
-    if ws is not None:
-        ws.zero_()
+    key = (dev_index, torch.cuda.current_stream(device).cuda_stream)
+    for ws in (_workspaces.get(key), _thread_buffers().get(key, (None, None))[0]):
+        if ws is not None:
+            ws.zero_()
 
 
 def workspace_error(device: torch.device) -> int:
-    """Error word of the current stream's workspace: non-zero after a kernel
-    gave up a bounded wait (reads the device, so it synchronises)."""
+    """Error word of the current stream's workspace, or of the calling thread's
+    own for int8 calls: non-zero after a kernel gave up a bounded wait (reads
+    the device, so it synchronises)."""
     dev_index = device.index if device.index is not None else torch.cuda.current_device()
-    ws = _workspaces.get((dev_index, torch.cuda.current_stream(device).cuda_stream))
-    if ws is None:
-        return 0
-    return int(ws[4:8].view(torch.int32).item())
+    key = (dev_index, torch.cuda.current_stream(device).cuda_stream)
+    for ws in (_workspaces.get(key), _thread_buffers().get(key, (None, None))[0]):
+        word = 0 if ws is None else int(ws[4:8].view(torch.int32).item())
+        if word:
+            return word
+    return 0
 
 
 def _require_cuda(*tensors: torch.Tensor) -> None:
@@ -641,8 +654,8 @@ def grouped(hidden, weight, mask, logits=None, top_value=None, top_index=None, c
 
 # ---------------------------------------------------------------------------
 # int8 head. These wrappers take the tensors' device as the current one (a
-# guard where it is not), and under stream capture a workspace of the graph's
-# own: a captured memory fill zeroes it at every replay, so graphs share none.
+# guard where it is not), and under stream capture buffers of the graph's own:
+# a captured memory fill zeroes the workspace at every replay, so graphs share none.
 # ---------------------------------------------------------------------------
 DTYPE_I8 = 3
 
@@ -680,12 +693,21 @@ def _int8_scratch_bytes(batch: int, hidden_dim: int) -> int:
     return int(load().gsp_int8_scratch_bytes(batch, hidden_dim))
 
 
-def _call_workspace(device: torch.device, stream: int, batch: int, vocab: int) -> torch.Tensor:
+def _int8_buffers(device: torch.device, stream: int, batch: int, vocab: int, scratch_bytes: int):
+    """Zero-filled workspace and scratch of an int8 call. A call can be two
+    launches, so another thread's launch on the same stream must not come
+    between them with the same buffers: they are the calling thread's own."""
     need = _workspace_bytes(batch, vocab)
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(need, dtype=torch.uint8, device=device)
-    ws = _workspaces.get((device.index, stream))  # (dict reads and writes are atomic; workspace() takes the lock)
-    return ws if ws is not None and ws.numel() >= need else workspace(device, batch, vocab)
+        return (torch.zeros(need, dtype=torch.uint8, device=device),
+                torch.empty(scratch_bytes, dtype=torch.uint8, device=device))
+    held, key = _thread_buffers(), (device.index, stream)
+    buffers = held.get(key)
+    if buffers is None or buffers[0].numel() < need or buffers[1].numel() < scratch_bytes:
+        sizes = (64 * 1024, 64 * 1024) if buffers is None else tuple(2 * t.numel() for t in buffers)
+        buffers = held[key] = (torch.zeros(max(need, sizes[0]), dtype=torch.uint8, device=device),
+                               torch.empty(max(scratch_bytes, sizes[1]), dtype=torch.uint8, device=device))
+    return buffers
 
 
 def _address(t: torch.Tensor | None):
@@ -704,18 +726,18 @@ def quantize_rows_int8(x, values, scales) -> None:
 
 
 def _int8_call(hidden, hidden_scales, weight, weight_scales, mask):
-    """Arguments shared by gsp_int8_logits and gsp_int8_compact: the operands, and (scratch, workspace, stream)."""
+    """Arguments shared by gsp_int8_logits and gsp_int8_compact: the operands,
+    (scratch, workspace, stream), and the tensors to keep until the launch."""
     device, index = hidden.device, hidden.get_device()
     batch, hidden_dim = hidden.shape
     vocab = weight.shape[0]
     stream = raw_stream(index)
-    ws = _call_workspace(device, stream, batch, vocab)
     if hidden_scales is None:
-        code, scratch = DTYPE_CODES[hidden.dtype], torch.empty(_int8_scratch_bytes(batch, hidden_dim),
-                                                               dtype=torch.uint8, device=device)
-        tail = (scratch.data_ptr(), scratch.numel(), ws.data_ptr(), ws.numel(), stream)
+        code, scratch_bytes = DTYPE_CODES[hidden.dtype], _int8_scratch_bytes(batch, hidden_dim)
     else:
-        code, scratch, tail = DTYPE_I8, None, (None, 0, ws.data_ptr(), ws.numel(), stream)
+        code, scratch_bytes = DTYPE_I8, 0
+    ws, scratch = _int8_buffers(device, stream, batch, vocab, scratch_bytes)
+    tail = (scratch.data_ptr(), scratch.numel(), ws.data_ptr(), ws.numel(), stream)
     args = (hidden.data_ptr(), hidden.stride(0), code, _address(hidden_scales), weight.data_ptr(), weight.stride(0),
             weight_scales.data_ptr(), _address(mask), 0 if mask is None else mask.stride(0), batch, vocab, hidden_dim)
     return args, tail, (scratch, ws)

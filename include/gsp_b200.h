@@ -519,8 +519,9 @@ int32_t gsp_quantize_rows_int8(const void* src, int64_t src_row_stride, int64_t 
  * hidden_dtype GSP_DTYPE_I8: `hidden` is int8 with hidden_scales [batch], and
  * scratch may be NULL. Otherwise `hidden` is fp16 / bf16 / fp32 and the call
  * first quantises it into scratch (gsp_int8_scratch_bytes, 16-byte aligned,
- * contents not preserved, one per concurrent call). hidden_dim <= 131,071
- * (int32 sums). The other arguments, the workspace and the outputs are those
+ * contents not preserved, one per concurrent call; row-sparse calls of few
+ * requests quantise inside the projection, to the same bits). hidden_dim <=
+ * 131,071 (int32 sums). The other arguments, the workspace and the outputs are those
  * of gsp_row_sparse_logits / gsp_block_gemm_logits / gsp_dense_masked_logits;
  * the tensor-core routes want 16-byte aligned rows (hidden_dim a multiple of
  * 16) and run the row-sparse kernel otherwise. */

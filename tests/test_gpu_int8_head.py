@@ -12,6 +12,8 @@ Bounds, derived from the definition (gsp/int8_head.py):
 The product has one definition in fp32, so the routes agree bit for bit and
 equal the same expression evaluated by torch.
 """
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -298,3 +300,62 @@ def test_sizes_past_32_bits_are_refused(cuda_device):
     x = torch.empty(1, 2 ** 32 + 32, dtype=torch.float16, device=cuda_device)  # (32 columns, cut to 32 bits)
     with pytest.raises(ValueError, match="2\\^30 columns"):
         I.quantize_rows_int8(x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [(5000, 2048, 1), (5000, 4096, 4), (2000, 48, 2), (900, 16400, 1), (900, 1040, 3)])
+def test_hidden_states_of_few_requests(cuda_device, case, dtype):
+    """Quantised inside the projection (or, past its limits, before it): the
+    bits of the quantiser's values and scales, zeros and rows that are not
+    finite among them, contiguous rows at any 16-byte address and others."""
+    vocab, hidden, batch = case
+    dev = cuda_device
+    weight = _int8_weight(51, vocab, hidden, dev)
+    mask = torch.from_numpy(O.make_batch_mask(np.random.default_rng(52), batch, vocab, [vocab // 9] * batch)).to(dev)
+    legal = _legal(mask, vocab)
+    h = _rows(53, batch, hidden, dtype, dev)
+    h[batch - 1, hidden - 1] = -9.0  # the maximum in the last place
+    _check(h, weight, mask, dtype, I.int8_grammar_logits(h, weight, mask), legal)
+    space = torch.zeros(batch * hidden + 9, dtype=dtype, device=dev)
+    for shift in (8, 1):  # 16 bytes (fp32: 32), and an odd address
+        moved = space[shift:shift + batch * hidden].view(batch, hidden).copy_(h)
+        _check(moved, weight, mask, dtype, I.int8_grammar_logits(moved, weight, mask), legal)
+    ids, logits, offsets = I.int8_compact_logits(h, weight, mask)
+    full = I.int8_grammar_logits(h, weight, mask)[0]
+    assert torch.equal(logits, full[legal.to(dev)]) and offsets[-1].item() == int(legal.sum())
+    h[0] = 0.0
+    _check(h, weight, mask, dtype, I.int8_grammar_logits(h, weight, mask), legal)
+    h[batch - 1, 3] = float("inf")
+    out = I.int8_grammar_logits(h, weight, mask)[0]
+    assert out[batch - 1][legal[batch - 1].to(dev)].isnan().all() and out[~legal.to(dev)].isneginf().all()
+
+
+@pytest.mark.parametrize("route", tr.ROUTES)
+def test_threads_on_one_stream(cuda_device, route):
+    """Two threads' calls of two launches each, on the same stream: neither's
+    scratch nor tile list is the other's."""
+    dev = cuda_device
+    vocab, hidden, batch, rounds = 6000, 128, 7, 60
+    weight = _int8_weight(61, vocab, hidden, dev)
+    hs = [_rows(62 + i, batch, hidden, torch.float16, dev) for i in range(2)]
+    masks = [torch.from_numpy(O.make_batch_mask(np.random.default_rng(64 + i), batch, vocab, [9] * batch)).to(dev)
+             for i in range(2)]
+    want = [I.int8_grammar_logits(h, weight, m, route=route) for h, m in zip(hs, masks)]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        for _ in range(rounds):
+            got[i].append(I.int8_grammar_logits(hs[i], weight, masks[i], route=route))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == rounds
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+    assert _native.workspace_error(dev) == 0

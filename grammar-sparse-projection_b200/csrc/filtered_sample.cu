@@ -34,7 +34,8 @@
 //     pass over the list. Where a list does not fit, the search goes on in the
 //     whole row, 512-fold per pass all the same.
 //   * Rows with few legal tokens (a grammar's) are listed whole at once, and
-//     after top-k or min-p the kept tokens are.
+//     after top-k or min-p the kept tokens are; up to 256 tokens left are put in
+//     order by comparing each with all, and one running sum gives both borders.
 //
 // Bound: for long kept sets one 64-bit exponential per weighed token (11
 // double-precision operations, about 35 in all) and one shared-memory atomic;
@@ -61,11 +62,13 @@ constexpr int kMaxCluster = 16;
 constexpr int kMaxShift = 50;
 constexpr int kExpTable = 16;
 constexpr int kTiesCap = 512;    // tokens of one value whose positions are set side by side
+constexpr int kFew = 256;        // tokens left that are put in order at once
 constexpr int kListBits = 12;
 constexpr int kListTotal = 1 << kListBits;  // tokens a cluster lists
 static_assert(kBins == kSampleThreads, "one bin per thread");
 static_assert(32 * 16 <= kBins, "32 octaves of weights in sixteenths");
 static_assert(kMaxCluster <= kSampleWarps, "a warp for each part of the list");
+static_assert(2 * kFew <= kSampleThreads, "two threads per token of few");
 
 // 2^(j / 16) and log2(1 + j / 16).
 __constant__ double kExp2[kExpTable] = {
@@ -605,6 +608,20 @@ struct BinSums {
   }
 };
 
+// The block's inclusive running sum, and the sum of all.
+__device__ __forceinline__ unsigned long long block_scan_u64(unsigned long long v, SampleSmemHeader* s,
+                                                             unsigned long long* total) {
+  const int tid = threadIdx.x;
+  const unsigned long long incl = warp_scan_u64(v);
+  if ((tid & 31) == 31) s->scan[tid >> 5] = incl;
+  __syncthreads();
+  // every warp scans the warps' totals
+  const unsigned long long w = warp_scan_u64((tid & 31) < kSampleWarps ? s->scan[tid & (kSampleWarps - 1)] : 0ull);
+  const unsigned long long before_warp = __shfl_sync(FULL_MASK, w, max((tid >> 5) - 1, 0));
+  *total = __shfl_sync(FULL_MASK, w, 31);
+  return incl + (tid >= 32 ? before_warp : 0ull);
+}
+
 // Closes a filling pass: the bins' sums over the cluster, or (local) this
 // CTA's; *total: the sum of all bins.
 __device__ __forceinline__ BinSums sum_bins(Team& team, bool local, unsigned long long* total) {
@@ -626,14 +643,7 @@ __device__ __forceinline__ BinSums sum_bins(Team& team, bool local, unsigned lon
       for (int k = 0; k < 8; ++k) v.own += x[k];
     }
   }
-  const unsigned long long incl = warp_scan_u64(v.own);
-  if ((tid & 31) == 31) s->scan[tid >> 5] = incl;
-  __syncthreads();
-  // every warp scans the warps' totals
-  const unsigned long long w = warp_scan_u64((tid & 31) < kSampleWarps ? s->scan[tid & (kSampleWarps - 1)] : 0ull);
-  const unsigned long long before_warp = __shfl_sync(FULL_MASK, w, max((tid >> 5) - 1, 0));
-  *total = __shfl_sync(FULL_MASK, w, 31);
-  v.before = incl - v.own + (tid >= 32 ? before_warp : 0ull);
+  v.before = block_scan_u64(v.own, s, total) - v.own;
   return v;
 }
 
@@ -718,6 +728,48 @@ __device__ __forceinline__ bool close_list(Team& team, uint32_t count, unsigned 
   __syncthreads();
   *sum = total;
   return fits;
+}
+
+// Puts up to kFew of the first CTA's listed tokens, those that take(value) says,
+// in order. gather_few: how many it says (beyond kFew, they are not kept).
+template <typename T, typename Take>
+__device__ __forceinline__ int gather_few(SampleSmemHeader* s, const List<T>& list, Take take) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if (tid == 0) s->listed = 0u;
+  s->lo[tid] = 0u;
+  __syncthreads();
+  list.each([&](float v, uint32_t at) {
+    if (!take(v)) return;
+    const uint32_t i = atomicAdd(&s->listed, 1u);
+    if (i < (uint32_t)kFew) s->tot[i] = ((unsigned long long)SampleKey<T>::from_value(v) << 32) | (uint32_t)~at;
+  });
+  __syncthreads();
+  return (int)s->listed;
+}
+// The gathered token of rank threadIdx.x as (key, ~position), 0 past the last.
+// Each is compared with all others, by two threads with half of them each.
+__device__ __forceinline__ unsigned long long order_few(SampleSmemHeader* s, int count) {
+  const int tid = threadIdx.x;
+  const int i = tid & (kFew - 1), half = (count + 1) / 2;
+  const unsigned long long mine = i < count ? s->tot[i] : 0ull;
+  if (i < count) {
+    uint32_t before = 0u;
+    const int k0 = tid < kFew ? 0 : half, k1 = tid < kFew ? half : count;
+#pragma unroll 8
+    for (int k = k0; k < k1; ++k) before += s->tot[k] > mine ? 1u : 0u;
+    if (before) atomicAdd(&s->lo[i], before);
+  }
+  __syncthreads();
+  if (tid < count) s->tot[kFew + s->lo[tid]] = mine;
+  __syncthreads();
+  return tid < count ? s->tot[kFew + tid] : 0ull;
+}
+
+// Tokens in the list.
+__device__ __forceinline__ uint32_t listed_tokens(const SampleSmemHeader* s) {
+  const uint32_t lane = threadIdx.x & 31u;
+  return __reduce_add_sync(FULL_MASK, lane < (uint32_t)kMaxCluster ? s->list_count[lane] : 0u);
 }
 
 // Bin of the top-k search: 64ths of an octave of the distance to the maximum,
@@ -805,6 +857,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   unsigned long long ordinal = 0ull;  // among the tokens of draw_value, by rising position
   float logprob = 0.f;
   bool solo = false;  // the list holds all that is still needed: this CTA goes on alone
+  // the answer: the token at a position
+  const auto put = [&](int64_t at) {
+    p.token_ids[b] = p.ids ? p.ids[start + at] : p.vocab_offset + at;
+    if (p.logprobs) p.logprobs[b] = logprob;
+    if (p.kept) p.kept[b] = (int32_t)kept;
+  };
   if (temperature > 0.f && !infinite) {
     Weigher<T> weigh;
     weigh.shift = min(kMaxShift, 62 - (64 - __clzll((unsigned long long)n)));
@@ -816,6 +874,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
     float border = vmin;
     unsigned long long ties = ~0ull, excess = 0ull;  // excess: tokens at the border beyond `ties`
     bool in_list = false;                            // the list holds every kept token
+    const auto logprob_of = [&](const Weigher<T>& weigh, float v, unsigned long long sum) {
+      return (float)(((double)v - (double)vmax) / (double)temperature -
+                     log((double)sum / (double)(1ull << weigh.shift)));
+    };
     const auto one = [](float, unsigned long long* m) {
       *m = 1ull;
       return true;
@@ -894,9 +956,34 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
         }
       }
     }
+    const float lowest = fmaxf(border, fminf(vmax, K::value_at_least(weigh.cut())));
+    // ---- few are left (a top-k, a grammar's tokens): all in order, then running sums --
+    if (in_list && kept + excess <= kFew) {
+      const int left = gather_few<T>(s, list, [&](float v) { return v >= border; });  // kept + excess
+      const unsigned long long token = order_few(s, left);
+      const float v = K::value((uint32_t)(token >> 32));
+      const unsigned long long w = (unsigned long long)tid < kept && v >= lowest ? weigh(v) : 0ull;
+      unsigned long long sum;
+      const unsigned long long upto = block_scan_u64(w, s, &sum);
+      if (top_p < 1.f) {  // the last kept: the first whose running sum passes the target
+        const unsigned long long target = prefix_target(top_p, sum);
+        if (upto - w <= target && target < upto) {
+          s->pick[0][0] = (unsigned long long)tid + 1ull;
+          s->pick[0][1] = upto;
+        }
+        __syncthreads();
+        kept = s->pick[0][0];
+        sum = s->pick[0][1];
+      }
+      const unsigned long long target = __umul64hi(fraction64(u), sum);
+      if (upto - w <= target && target < upto) {
+        logprob = logprob_of(weigh, v, sum);
+        put((uint32_t)~(uint32_t)token);
+      }
+      return;
+    }
     // ---- weigh what is left, by bins ---------------------------------------------
     clear_bins(s);
-    const float lowest = fmaxf(border, fminf(vmax, K::value_at_least(weigh.cut())));
     const auto into_bin = [&](float v, uint32_t) {
       const double w = weigh.unrounded(v);
       if (v >= lowest) add_to_bin(s, (uint32_t)weigh.bin(w), weigh.round(w));
@@ -952,14 +1039,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
       bin_values(p_bin, p_bin, &p_from, &p_to);
       __syncthreads();  // the pick has been read
     }
-    const unsigned long long u64 = fraction64(u);
-    unsigned long long n_above = 0ull;
+    unsigned long long n_above = 0ull;  // tokens above p_to (list of bins)
+    // the bins that the draw can fall into, the sums before the first and of all
+    bins.pick(s, 0, __umul64hi(fraction64(u), top_p < 1.f ? p_before + 1ull : sum));
+    bins.pick(s, 1, __umul64hi(fraction64(u), most));
+    __syncthreads();
     if (!in_list) {
-      // list the border's bin and the bins the draw can fall into
+      // list the border's bin and the draw's
       float from, to;
-      bins.pick(s, 0, __umul64hi(u64, top_p < 1.f ? p_before + 1ull : sum));
-      bins.pick(s, 1, __umul64hi(u64, most));
-      __syncthreads();
       bin_values((int)s->pick[0][0], (int)s->pick[1][0], &from, &to);
       if (!(top_p < 1.f)) p_from = from, p_to = to;
       open_list(team);
@@ -967,6 +1054,47 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
           p_from, p_to, from, to, [&](float v, uint32_t at) { list_token(team, K::from_value(v), at); });
       solo = close_list(team, above, &n_above);
       if (solo && team.rank != 0) return;
+    }
+    // ---- few tokens in those bins: in order, and their running sums ------------------
+    // (a list of bins holds little else; of a list of all tokens they are a small part)
+    if (solo && (in_list || listed_tokens(s) <= (uint32_t)kFew)) {
+      const int j0 = (int)s->pick[0][0], j1 = (int)s->pick[1][0];
+      const float top = in_list ? vmax : p_to;
+      uint32_t others = 0u;  // tokens of bins before the border's that are not gathered (less those counted in n_above)
+      const int count = gather_few<T>(s, list, [&](float v) {
+        if (!(v >= lowest)) return false;
+        const int j = weigh.bin(weigh.unrounded(v));
+        const bool take = (j >= j0 && j <= j1) || (top_p < 1.f && j == p_bin);
+        if (top_p < 1.f && j < p_bin) others += (v <= top ? 1u : 0u) - (take ? 1u : 0u);
+        return take;
+      });
+      if (count <= kFew) {
+        others = block_sum(others, s);
+        const unsigned long long token = order_few(s, count);
+        const float v = K::value((uint32_t)(token >> 32));
+        const double unrounded = weigh.unrounded(v);
+        const int j = weigh.bin(unrounded);
+        const unsigned long long w = tid < count ? weigh.round(unrounded) : 0ull;
+        const unsigned long long j_before = s->pick[0][1], j_sum = s->pick[1][1] + s->pick[1][2] - j_before;
+        unsigned long long all;  // (its barrier: the picks have been read)
+        unsigned long long upto = block_scan_u64(w, s, &all);
+        upto = j <= j1 ? j_before + upto : p_before + (upto - j_sum);  // (the draw's bins come first)
+        if (top_p < 1.f) {
+          if (j == p_bin && upto - w <= p_target && p_target < upto) {
+            s->pick[0][0] = (unsigned long long)(tid + 1);
+            s->pick[0][1] = upto;
+          }
+          __syncthreads();
+          kept = n_above + (unsigned long long)(int32_t)others + s->pick[0][0];
+          sum = s->pick[0][1];
+        }
+        const unsigned long long target = __umul64hi(fraction64(u), sum);
+        if (j <= j1 && upto - w <= target && target < upto) {
+          logprob = logprob_of(weigh, v, sum);
+          put((uint32_t)~(uint32_t)token);
+        }
+        return;
+      }
     }
     if (top_p < 1.f) {
       const Found f = within(p_bin, p_from, p_to, p_before, p_target);
@@ -986,7 +1114,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
       }
     }
     // ---- the draw ------------------------------------------------------------------
-    const unsigned long long target = __umul64hi(u64, sum);
+    const unsigned long long target = __umul64hi(fraction64(u), sum);
     bins.pick(s, 0, target);
     __syncthreads();
     const int j = (int)s->pick[0][0];
@@ -997,8 +1125,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
     const Found f = within(j, from, to, before, target);
     draw_value = K::value(f.key);
     ordinal = (target - f.above) / weigh(draw_value);
-    logprob = (float)(((double)draw_value - (double)vmax) / (double)temperature -
-                      log((double)sum / (double)(1ull << weigh.shift)));
+    logprob = logprob_of(weigh, draw_value, sum);
   } else if (temperature > 0.f) {
     // a maximum of +inf: its tokens weigh 1 each, every other nothing
     uint32_t at_max = 0u;
@@ -1015,11 +1142,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   }
 
   // ---- the drawn token: the ordinal-th of draw_value, by rising position ----------------
-  const auto put = [&](int64_t at) {
-    p.token_ids[b] = p.ids ? p.ids[start + at] : p.vocab_offset + at;
-    if (p.logprobs) p.logprobs[b] = logprob;
-    if (p.kept) p.kept[b] = (int32_t)kept;
-  };
   if (solo) {
     // the positions of draw_value's tokens; each counts those before it
     uint32_t* ties_at = s->ties_at;

@@ -63,8 +63,7 @@ constexpr int kMaxShift = 50;
 constexpr int kExpTable = 16;
 constexpr int kTiesCap = 512;    // tokens of one value whose positions are set side by side
 constexpr int kFew = 256;        // tokens left that are put in order at once
-constexpr int kListBits = 12;
-constexpr int kListTotal = 1 << kListBits;  // tokens a cluster lists
+constexpr int kListTotal = 4096; // tokens a cluster lists
 static_assert(kBins == kSampleThreads, "one bin per thread");
 static_assert(32 * 16 <= kBins, "32 octaves of weights in sixteenths");
 static_assert(kMaxCluster <= kSampleWarps, "a warp for each part of the list");
@@ -423,17 +422,22 @@ struct Slice {
 };
 
 // The listed tokens: one part per CTA of the cluster (or, listed whole, a
-// single part), whose tokens are spread over a share of the warps.
+// single part), each with a share of the warps.
 template <typename T>
 struct List {
   const SampleSmemHeader* s;
-  int parts_bits;  // log2 of the number of parts
+  int room;        // tokens a part can hold
+  uint32_t share;  // this thread's part, its first token there and its step (a byte, two 12-bit fields)
+  __device__ __forceinline__ List(const SampleSmemHeader* s_, int parts) : s(s_), room(kListTotal / parts) {
+    const uint32_t warp = threadIdx.x >> 5, part = warp % parts;
+    const uint32_t step = (kSampleWarps - part + parts - 1u) / parts * 32u;
+    share = part | (warp / parts * 32u + (threadIdx.x & 31u)) << 8 | step << 20;
+  }
   template <typename Fn>
   __device__ __forceinline__ void each(Fn fn) const {
-    const int warp = threadIdx.x >> 5, part = warp & ((1 << parts_bits) - 1);
-    const int step = kSampleThreads >> parts_bits, n = (int)s->list_count[part];
-    const unsigned long long* e = s->list + ((size_t)part << (kListBits - parts_bits));
-    for (int i = (warp >> parts_bits) * 32 + (threadIdx.x & 31); i < n; i += step) {
+    const int part = (int)(share & 0xffu), step = (int)(share >> 20), n = (int)s->list_count[part];
+    const unsigned long long* e = s->list + part * room;
+    for (int i = (int)(share >> 8 & 0xfffu); i < n; i += step) {
       const unsigned long long x = e[i];
       fn(SampleKey<T>::value((uint32_t)(x >> 32)), (uint32_t)x);
     }
@@ -524,7 +528,8 @@ __device__ __forceinline__ unsigned long long prefix_target(float x, unsigned lo
 struct Team {
   SampleSmemHeader* s;  // (this CTA's)
   cg::cluster_group cluster;
-  int rank, size, size_bits;  // size_bits: log2 of the size, rounded up
+  int rank, size;
+  int room;  // tokens in a CTA's part of the list
   int buf;  // which half of `word` the next all-gather uses
 
   // All-gather of one value per CTA (the same in all its threads): the returned
@@ -704,8 +709,8 @@ __device__ __forceinline__ void put_in_list(const Team& team, uint32_t i, uint32
 
 // Offers a token to the CTA's part of the list.
 __device__ __forceinline__ void list_token(const Team& team, uint32_t key, uint32_t at) {
-  const uint32_t i = atomicAdd(&team.s->listed, 1u), part_bits = (uint32_t)(kListBits - team.size_bits);
-  if (i < (1u << part_bits)) put_in_list(team, ((uint32_t)team.rank << part_bits) + i, key, at);
+  const uint32_t i = atomicAdd(&team.s->listed, 1u);
+  if (i < (uint32_t)team.room) put_in_list(team, (uint32_t)(team.rank * team.room) + i, key, at);
 }
 
 // After a listing pass: whether every CTA's part fits (then the first CTA has
@@ -713,7 +718,7 @@ __device__ __forceinline__ void list_token(const Team& team, uint32_t key, uint3
 // does not fit is not read, so the next may be written at once.
 __device__ __forceinline__ bool close_list(Team& team, uint32_t count, unsigned long long* sum) {
   SampleSmemHeader* s = team.s;
-  const uint32_t part = 1u << (kListBits - team.size_bits);
+  const uint32_t part = (uint32_t)team.room;
   count = block_sum(count, s);
   const uint32_t mine = min(s->listed, part + 1u);
   const unsigned long long* all = team.gather(((unsigned long long)mine << 32) | count);
@@ -788,7 +793,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   Team team{s, cg::this_cluster(), 0, 0, 0, 0};
   team.rank = (int)team.cluster.block_rank();
   team.size = (int)team.cluster.num_blocks();
-  team.size_bits = team.size > 1 ? 32 - __clz(team.size - 1) : 0;
+  team.room = kListTotal / team.size;
   const int b = blockIdx.x / team.size, tid = threadIdx.x;
 
   // ---- the row and its settings ---------------------------------------------
@@ -851,7 +856,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   vmax = K::value(kmax);
   const float vmin = K::value(K::kNegInf + 1u);  // the lowest legal value
   const bool infinite = !(vmax < INFINITY);
-  List<T> list{s, team.size_bits};
+  List<T> list{s, team.size};
 
   float draw_value = vmax;
   unsigned long long ordinal = 0ull;  // among the tokens of draw_value, by rising position
@@ -888,7 +893,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
         put_in_list(team, list_base + atomicAdd(&s->listed, 1u), K::from_value(v), at);
       });
       if (tid < kMaxCluster) s->list_count[tid] = tid == 0 ? (uint32_t)kept : 0u;
-      list.parts_bits = 0;
+      list = List<T>(s, 1);
       __syncthreads();
       team.cluster.sync();
       if (team.rank != 0) return;
@@ -1159,9 +1164,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
       list.each([&](float v, uint32_t at) {
         if (v != draw_value) return;
         uint32_t lower = 0u;
-        for (int r = 0; r < (1 << list.parts_bits); ++r)
+        for (int r = 0; r < kMaxCluster; ++r)  // (parts that there are not have count 0)
           for (uint32_t k = 0; k < s->list_count[r]; ++k) {
-            const unsigned long long e = s->list[((uint32_t)r << (kListBits - list.parts_bits)) + k];
+            const unsigned long long e = s->list[(uint32_t)(r * list.room) + k];
             lower += ((uint32_t)(e >> 32) == K::from_value(draw_value) && (uint32_t)e < at) ? 1u : 0u;
           }
         if (lower == ordinal) put(at);
@@ -1674,33 +1679,95 @@ cudaError_t launch_counted(const FilteredSampleParams& p, int batch, cudaStream_
   return cudaGetLastError();
 }
 
-// Launch: one cluster per row.
+// ---- launch: one cluster per row ------------------------------------------------
+constexpr size_t kSmemFull = 227 * 1024, kSmemHalf = kSmemFull / 2 - 1024;  // a CTA alone on its SM, or two
+
+// How many clusters of `size` CTAs with that shared memory the device holds at a
+// time: a cluster lies within one GPC, and what a GPC has left over is lost (of
+// 148 SMs, 45 clusters of 3 CTAs alone on their SMs, 93 of half the shared memory).
+template <typename T>
+int resident_clusters(int dev, int size, bool full) {
+  static std::atomic<int> known[32][kMaxCluster + 1][2];  // plus one; 0: not asked yet
+  const bool keep = dev < 32;
+  if (keep) {
+    const int n = known[dev][size][full].load(std::memory_order_relaxed);
+    if (n > 0) return n - 1;
+  }
+  auto k = filtered_sample_kernel<T>;
+  const size_t smem = full ? kSmemFull : kSmemHalf;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)size);
+  cfg.blockDim = dim3(kSampleThreads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (raise_smem_limit(reinterpret_cast<const void*>(k), smem, dev) != cudaSuccess ||
+      (size > 8 && cudaFuncSetAttribute(reinterpret_cast<const void*>(k),
+                                        cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
+      cudaOccupancyMaxActiveClusters(&n, k, &cfg) != cudaSuccess) {
+    cudaGetLastError();  // (then that size is not taken)
+    n = 0;
+  }
+  if (keep) known[dev][size][full].store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
+// CTAs per row, and whether each has its SM's shared memory to itself. Every
+// row's cluster has to be resident at once (a second wave doubles the time); of
+// those sizes, the one that is done first by this count, in tokens: those of a
+// CTA (1.75 times as many where two share an SM), and for every CTA of the
+// cluster what the barriers cost, about 1,000 tokens' time, more past 8 CTAs.
+// Measured, no filter / top-k 50, us (normal logits): 48 x 262,144 fp32 in
+// clusters of 6 (a second wave) 80 / 47, of 5 65 / 35, of 4 75 / 39, of 3 on
+// half the shared memory 96 / 49; 40 x 50,257 bf16 of 7 26 / 22, of 3 21 / 14;
+// 16 x 262,144 fp32 of 16 45 / 31, of 6 38 / 22; 8 x 151,936 bf16 of 16 21 / 19,
+// of 8 24 / 14; 4 x 262,144 fp32 of 16 24 / 17, of 8 29 / 19.
+struct LaunchShape {
+  int size;
+  bool full;
+};
+template <typename T>
+LaunchShape launch_shape(int dev, int batch, int64_t max_len) {
+  const int sms = num_sms(dev);
+  LaunchShape best{1, false};
+  if (batch > sms) return best;
+  int64_t best_cost = INT64_MAX;
+  for (int size = 1; size <= kMaxCluster; size = size < 8 ? size + 1 : 2 * size) {
+    const int64_t ctas = (int64_t)batch * size, part = (max_len + size - 1) / size;
+    const int64_t barriers = 1000 * size + (size > 8 ? 4000 : 0);
+    for (const bool full : {true, false}) {
+      const int64_t cost = (full ? part : part + part * 3 / 4) + barriers;
+      if (ctas > (full ? 1 : 2) * (int64_t)sms || cost >= best_cost ||
+          resident_clusters<T>(dev, size, full) < batch)
+        continue;
+      best_cost = cost;
+      best = LaunchShape{size, full};
+    }
+  }
+  return best;
+}
+
 template <typename T>
 cudaError_t launch_typed(FilteredSampleParams p, int batch, int64_t max_len, cudaStream_t stream) {
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  // CTAs per row: as many as the batch leaves two per SM for, up to 8 (16 for
-  // one row alone), while each has over 4,096 tokens. What shared memory does not
-  // hold beside a second CTA on the SM is read again from L2.
-  constexpr size_t kSmemMax = 227 * 1024;
-  const int64_t spare = 2 * (int64_t)num_sms(dev) / batch;
-  int64_t size64 = std::min<int64_t>(std::max<int64_t>(1, (max_len + 4095) / 4096), std::max<int64_t>(1, spare));
-  const int size = size64 >= 16 ? 16 : (int)std::min<int64_t>(size64, 8);
-  const size_t room = ((int64_t)batch * size <= num_sms(dev) ? kSmemMax : kSmemMax / 2 - 1024) - kHeaderBytes;
+  const LaunchShape shape = launch_shape<T>(dev, batch, max_len);
+  const int size = shape.size;
+  // what shared memory does not hold is read again from L2
+  const size_t room = (shape.full ? kSmemFull : kSmemHalf) - kHeaderBytes;
   const int64_t part = ((max_len + size - 1) / size + 31) / 32 * 32;
   const int64_t part_vectors = (part * (int64_t)sizeof(typename DTypeTraits<T>::Bits) + 15) / 16 + 1;
   p.held_vectors = (int)std::min<int64_t>((int64_t)(room / 16), part_vectors);
   const size_t smem = kHeaderBytes + (size_t)p.held_vectors * 16;
   auto k = filtered_sample_kernel<T>;
   if ((err = raise_smem_limit(reinterpret_cast<const void*>(k), smem, dev)) != cudaSuccess) return err;
-  static std::atomic<uint64_t> wide_ok[2];  // devices on which clusters of 16 have been allowed
-  if (size > 8 && dev < 128 && !((wide_ok[dev >> 6].load() >> (dev & 63)) & 1u)) {
-    if ((err = cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeNonPortableClusterSizeAllowed,
-                                    1)) != cudaSuccess)
-      return err;
-    wide_ok[dev >> 6].fetch_or(1ull << (dev & 63));
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(batch * size));
   cfg.blockDim = dim3(kSampleThreads);

@@ -308,6 +308,16 @@ struct Slice {
     }
   }
 
+  // The places of vector v that hold a value, as bits.
+  __device__ __forceinline__ uint32_t places_of(int v, float x) const {
+    uint32_t legal = 0xffffffffu, w[4], m = 0u;
+    const uint4 q = v < held_vectors ? held[v] : fetch(v, &legal);
+    settle(q, legal, w);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) m |= unpack(w, j) == x ? 1u << j : 0u;
+    return m;
+  }
+
   // Reads the whole part, keeping the held vectors; returns the thread's
   // largest value and its number of legal tokens. Four loads under way.
   __device__ __forceinline__ float load(uint32_t& legal_count) {
@@ -1188,24 +1198,33 @@ __global__ void __launch_bounds__(kSampleThreads, 2) filtered_sample_kernel(cons
   const unsigned long long* all = team.gather(here);
   for (int r = 0; r < team.rank; ++r) ordinal -= all[r];  // wraps for CTAs behind the owner
   if (ordinal >= here) return;
-  // blocks of kSampleThreads positions in order
-  for (int i0 = 0; i0 < slice.len; i0 += kSampleThreads) {
-    const int i = i0 + tid;
-    const float v = i < slice.len ? slice.at((uint32_t)(slice.lo + i)) : -INFINITY;
-    const bool hit = v == draw_value;
-    const unsigned hits = __ballot_sync(FULL_MASK, hit);
-    __syncthreads();
-    if ((tid & 31) == 0) s->warp[0][tid >> 5] = __popc(hits);
-    __syncthreads();
-    unsigned long long before = 0ull, in_block = 0ull;
-    for (int w = 0; w < kSampleWarps; ++w) {
-      if (w < (tid >> 5)) before += s->warp[0][w];
-      in_block += s->warp[0][w];
+  // a vector per thread at a time, in order
+  constexpr int kVec = Slice<T>::kVec;
+  for (int v0 = 0; v0 < slice.vectors; v0 += kSampleThreads) {
+    const uint32_t hits = v0 + tid < slice.vectors ? slice.places_of(v0 + tid, draw_value) : 0u;
+    uint32_t incl = __popc(hits);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t t = __shfl_up_sync(FULL_MASK, incl, o);
+      if ((tid & 31) >= o) incl += t;
     }
-    before += __popc(hits & ((1u << (tid & 31)) - 1u));
-    if (hit && before == ordinal) put(slice.lo + i);
-    if (ordinal < in_block) break;
-    ordinal -= in_block;
+    __syncthreads();
+    if ((tid & 31) == 31) s->warp[0][tid >> 5] = incl;
+    __syncthreads();
+    const uint32_t of_warp = (tid & 31) < kSampleWarps ? s->warp[0][tid & (kSampleWarps - 1)] : 0u;
+    const uint32_t in_block = __reduce_add_sync(FULL_MASK, of_warp);
+    if (ordinal >= in_block) {
+      ordinal -= in_block;
+      continue;
+    }
+    const uint32_t last = incl + __reduce_add_sync(FULL_MASK, (tid & 31) < (tid >> 5) ? of_warp : 0u);
+    const uint32_t before = last - __popc(hits);
+    if (before <= ordinal && ordinal < last) {
+      uint32_t m = hits;
+      for (uint32_t i = before; i < (uint32_t)ordinal; ++i) m &= m - 1u;
+      put(slice.first + (v0 + tid) * kVec + (__ffs(m) - 1));
+    }
+    return;
   }
 }
 
@@ -1783,20 +1802,36 @@ cudaError_t launch_typed(FilteredSampleParams p, int batch, int64_t max_len, cud
   return cudaLaunchKernelEx(&cfg, k, p);
 }
 
+// Whether rows of 16-bit logits are better counted, one CTA per row, than
+// weighed by a cluster each. Counting costs a row some 18 us (fp16, which has
+// more distinct values: 36) and 1 us per 8,000 tokens, a row per SM at a time;
+// clusters some 13 us and 1 us per 312,500 tokens of the batch. A top-k or min-p
+// known to leave few tokens spares a cluster the weighing, and is left to it.
+// Measured, counted / clusters, no filter and top-k 50, us (normal logits): 128 x
+// 248,320 bf16 49 / 117 and 50 / 48, fp16 69 / 114 and 67 / 49; 64 x 151,936 bf16
+// 37 / 46 and 38 / 23, fp16 56 / 44 and 54 / 23; 64 x 65,536 bf16 27 / 27 and
+// 28 / 16; 256 x 32,768 bf16 43 / 37; 32 x 248,320 fp16 69 / 39. Greedy, 64 x
+// 151,936 bf16 28 / 15, 128 x 248,320 fp16 42 / 40. Settings per request are not
+// known here and count as no filter.
+bool counting_pays(const FilteredSampleParams& p, int dtype, int batch, int64_t max_len, int sms) {
+  const bool few = (p.top_ks == nullptr && p.top_k > 0 && p.top_k <= 1000) ||
+                   (p.min_ps == nullptr && p.min_p >= 0.02f) || (p.temperatures == nullptr && p.temperature == 0.f);
+  if (few) return false;
+  const int64_t waves = (batch + sms - 1) / sms;
+  const double counted = (double)waves * ((dtype == 1 ? 18.0 : 36.0) + (double)max_len / 8000.0);
+  const double clusters = 13.0 + (double)batch * (double)max_len / 312500.0;
+  return counted < clusters;
+}
+
 }  // namespace
 
 cudaError_t launch_filtered_sample(const FilteredSampleParams& p, int dtype, int batch, int64_t max_len,
                                    cudaStream_t stream) {
   if (dtype == 2) return launch_typed<float>(p, batch, max_len, stream);
-  // Long 16-bit rows of a batch that fills two SMs in five with one CTA per row
-  // are counted. Measured, counted against a cluster per row, top-p 0.9 of
-  // normal logits: 128 x 248,320 bf16 / fp16 62 / 79 against 213 / 158 us, 64 x
-  // 151,936 bf16 42 against 67; 32 x 248,320 fp16 74 against 49, 256 x 32,768
-  // bf16 46 against 44 (the counts cost a row of any length some 15 us).
   int dev = 0;
   const cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  if (max_len >= 65536 && (int64_t)batch * 5 >= (int64_t)num_sms(dev) * 2)
+  if (counting_pays(p, dtype, batch, max_len, num_sms(dev)))
     return dtype == 1 ? launch_counted<__nv_bfloat16>(p, batch, stream) : launch_counted<__half>(p, batch, stream);
   if (dtype == 1) return launch_typed<__nv_bfloat16>(p, batch, max_len, stream);
   return launch_typed<__half>(p, batch, max_len, stream);

@@ -301,3 +301,30 @@ def test_packed_rows_of_very_different_lengths(cuda_device, dtype):
     for max_len in (0, 1, 5000, 2 ** 40):
         again = tr.sample_compact_logits(ids, x, offsets, uniforms=u, top_p=0.9, max_len=max_len)
         assert all(torch.equal(a, b) for a, b in zip(again, got))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_long_rows_of_a_full_batch(cuda_device, dtype):
+    """148 rows of 70,000 tokens with settings per request (counted, one CTA
+    per row): every combination of filters, greedy, and rows of one value or
+    two, more of it than 16 bits count; then settings known at the call (rows
+    split over clusters)."""
+    dev = cuda_device
+    batch, vocab = 148, 70000
+    x = _logits(31, batch, vocab, dtype, dev)
+    x[5] = 1.5
+    x[6] = -0.75
+    x[7, ::2], x[7, 1::2] = 0.0, -0.0
+    x[8, 100:], x[8, :100] = -2.0, 2.0
+    x[9] = float("-inf")
+    x[10, 3::7] = float("nan")
+    x[11, 50000:50003] = float("inf")
+    u = _uniforms(32, batch, dev)
+    at = [SETTINGS[(b * 7) % len(SETTINGS)] for b in range(batch)]
+    full = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+    types = dict(temperature=torch.float32, top_k=torch.int32, top_p=torch.float32, min_p=torch.float32)
+    settings = {k: torch.tensor([{**full, **s}[k] for s in at], dtype=types[k], device=dev) for k in full}
+    got = tr.sample_logits(x, uniforms=u, **settings)
+    _check(got, x, u, settings)
+    for one in (dict(top_k=20), dict(min_p=0.05, temperature=0.9), dict(temperature=0.0), dict(top_k=700, top_p=0.9)):
+        _check(tr.sample_logits(x, uniforms=u, **one), x, u, one)

@@ -20,8 +20,9 @@
  *     the hidden dtype, gsp/triton_runtime.py:111; gsp/runtime.py:46-51 is a
  *     plain F.linear). fp32 runs on the row-sparse kernels only: the block and
  *     dense entry points given GSP_DTYPE_F32 run the row-sparse kernel (same
- *     outputs), and the sampler, adaptive and grouped entry points return
- *     GSP_ERR_UNSUPPORTED for it.
+ *     outputs), and the fused sampler, adaptive and grouped entry points
+ *     return GSP_ERR_UNSUPPORTED for it. gsp_int8_* and gsp_sample_* state
+ *     their own types.
  *   - `vocab_offset` shifts the token ids reported in top_index / compact ids,
  *     for a weight that is one contiguous row shard of a larger vocabulary.
  *   - Optional outputs may be NULL.

@@ -59,6 +59,14 @@ __device__ __forceinline__ int quantize_by_division(float x, float scale) {
   return (int)fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -127.f), 127.f);
 }
 
+// One value, by the reciprocal where that cannot round to another integer.
+__device__ __forceinline__ int8_t quantize_value(float x, const RowScale& r) {
+  constexpr float kMagic = 12582912.f;
+  const float t = fmaf(x, r.inverse, kMagic);
+  if (r.divide || fabsf(fmaf(x, r.inverse, kMagic - t)) > 0.4999f) return (int8_t)quantize_by_division(x, r.scale);
+  return r.zero ? (int8_t)0 : (int8_t)(__float_as_uint(t) & 0xffu);
+}
+
 template <typename T>
 __device__ __forceinline__ float element(const uint32_t* words, int i) {
   if constexpr (sizeof(T) == 4)

@@ -154,8 +154,7 @@ def _pack(legal):
 def _int8_rows(x):
     """The definition of quantize: scale = max |x| / 127, value = x / scale to the nearest (ties to even)."""
     x = x.float()
-    scale = x.abs().amax(1)
-    scale = scale / torch.full_like(scale, 127.0)  # divided: by a plain number torch multiplies with its reciprocal
+    scale = x.abs().amax(1) / 127.0
     q = torch.round(x / scale.unsqueeze(1))
     return torch.where(scale.unsqueeze(1) > 0, q, torch.zeros_like(q)).clamp_(-127, 127).to(torch.int8), scale
 
@@ -327,8 +326,7 @@ def exact(case, seed):
         return {"values": None, "scales": scales}
     if state["op"] == "project":
         h = state["h"].double()
-        amax = h.abs().max(dim=1, keepdim=True).values.float()
-        scale = (amax / torch.full_like(amax, 127.0)).double()
+        scale = (h.abs().max(dim=1, keepdim=True).values.float() / 127.0).double()
         q = torch.where(scale > 0, (h / scale).round(), torch.zeros_like(h))
         vocab = state["w"].shape[0]
         words = state["mask"].cpu().numpy().view(np.uint32)

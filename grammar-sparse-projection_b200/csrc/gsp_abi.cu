@@ -890,6 +890,10 @@ constexpr int32_t kMaxInt8Hidden = 131071;  // 128 * 128 * 131071 < 2^31: the in
 
 size_t int8_row_bytes(int32_t hidden_dim) { return ((size_t)hidden_dim + 15) / 16 * 16; }
 
+// A dtype argument without its GSP_SCALE_RECIPROCAL.
+int32_t type_of(int32_t dtype) { return dtype & ~GSP_SCALE_RECIPROCAL; }
+bool by_product(int32_t dtype) { return (dtype & GSP_SCALE_RECIPROCAL) != 0; }
+
 // The step's hidden states as int8 rows with scales: the caller's own, or raw
 // rows still to be quantised into the scratch buffer ([batch] rows of
 // int8_row_bytes, then [batch] scales). Everything is checked before anything
@@ -918,7 +922,8 @@ int32_t validate_int8(const char* fn, const void* hidden, int64_t hidden_row_str
     if (!hidden_scales) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: int8 hidden states need hidden_scales", fn);
     return GSP_OK;
   }
-  if (hidden_dtype != GSP_DTYPE_F16 && hidden_dtype != GSP_DTYPE_BF16 && hidden_dtype != GSP_DTYPE_F32)
+  if (type_of(hidden_dtype) != GSP_DTYPE_F16 && type_of(hidden_dtype) != GSP_DTYPE_BF16 &&
+      type_of(hidden_dtype) != GSP_DTYPE_F32)
     return fail(GSP_ERR_UNSUPPORTED, "%s: unknown hidden_dtype %d", fn, hidden_dtype);
   if (!scratch || scratch_bytes < gsp_int8_scratch_bytes(batch, hidden_dim))
     return fail(GSP_ERR_WORKSPACE, "%s: scratch has %zu bytes, needs %zu", fn, scratch ? scratch_bytes : (size_t)0,
@@ -948,7 +953,7 @@ int32_t gsp_quantize_rows_int8(const void* src, int64_t src_row_stride, int64_t 
                                int8_t* values, int64_t values_row_stride, float* scales, void* stream) {
   const char* fn = "gsp_quantize_rows_int8";
   if (rows < 0 || cols < 1) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: rows must be >= 0 and cols positive", fn);
-  if (dtype != GSP_DTYPE_F16 && dtype != GSP_DTYPE_BF16 && dtype != GSP_DTYPE_F32)
+  if (type_of(dtype) != GSP_DTYPE_F16 && type_of(dtype) != GSP_DTYPE_BF16 && type_of(dtype) != GSP_DTYPE_F32)
     return fail(GSP_ERR_UNSUPPORTED, "%s: dtype must be GSP_DTYPE_F16, GSP_DTYPE_BF16 or GSP_DTYPE_F32", fn);
   if (rows == 0) return GSP_OK;
   if (rows > INT32_MAX) return fail(GSP_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows", fn);
@@ -956,8 +961,8 @@ int32_t gsp_quantize_rows_int8(const void* src, int64_t src_row_stride, int64_t 
   if (!src || !values || !scales) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: src, values and scales are required", fn);
   if (rows > 1 && (src_row_stride < 0 || values_row_stride < cols))
     return fail(GSP_ERR_INVALID_ARGUMENT, "%s: negative src_row_stride or values_row_stride < cols", fn);
-  return cuda_status(launch_quantize_rows_int8(src, rows > 1 ? src_row_stride : cols, rows, cols, dtype, values,
-                                               rows > 1 ? values_row_stride : cols, scales,
+  return cuda_status(launch_quantize_rows_int8(src, rows > 1 ? src_row_stride : cols, rows, cols, type_of(dtype),
+                                               by_product(dtype), values, rows > 1 ? values_row_stride : cols, scales,
                                                static_cast<cudaStream_t>(stream)),
                      fn);
 }
@@ -987,7 +992,8 @@ int32_t gsp_int8_logits(int32_t route, const void* hidden, int64_t hidden_row_st
     p.hidden_scales = h.scales;
     p.raw_hidden = h.raw;
     p.raw_stride = h.raw_stride;
-    p.raw_dtype = hidden_dtype;
+    p.raw_dtype = type_of(hidden_dtype);
+    p.raw_by_product = by_product(hidden_dtype);
     p.weight_scales = weight_scales;
     p.logits = logits;
     p.logits_stride = batch > 1 ? logits_row_stride : vocab;
@@ -999,7 +1005,7 @@ int32_t gsp_int8_logits(int32_t route, const void* hidden, int64_t hidden_row_st
   }
   if (h.raw != nullptr) {
     const cudaError_t err =
-        launch_quantize_rows_int8(h.raw, h.raw_stride, batch, hidden_dim, hidden_dtype,
+        launch_quantize_rows_int8(h.raw, h.raw_stride, batch, hidden_dim, type_of(hidden_dtype), by_product(hidden_dtype),
                                   const_cast<int8_t*>(h.values), h.stride, const_cast<float*>(h.scales), s);
     if (err != cudaSuccess) return cuda_status(err, fn);
   }
@@ -1059,7 +1065,8 @@ int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t 
   p.hidden_scales = h.scales;
   p.raw_hidden = h.raw;
   p.raw_stride = h.raw_stride;
-  p.raw_dtype = hidden_dtype;
+  p.raw_dtype = type_of(hidden_dtype);
+  p.raw_by_product = by_product(hidden_dtype);
   p.weight_scales = weight_scales;
   p.compact = capacity > 0 ? compact_logits : nullptr;
   p.compact_ids = compact_ids;

@@ -55,6 +55,7 @@ struct RowSparseParams {
   const void* raw_hidden;
   int64_t raw_stride;
   int raw_dtype;
+  bool raw_by_product;  // scale = max |x| * fp32(1 / 127), else max |x| / 127
   // full logits [batch, vocab] (optional)
   void* logits;
   int64_t logits_stride;
@@ -226,9 +227,11 @@ cudaError_t launch_block_gemm(const BlockGemmParams& p, int dtype, cudaStream_t 
 // ---- int8 operands (out_dtype: 0 fp16, 1 bf16, 2 fp32 logits) ---------------
 cudaError_t launch_row_sparse_int8(const RowSparseParams& p, int out_dtype, cudaStream_t stream);
 cudaError_t launch_block_gemm_int8(const BlockGemmParams& p, int out_dtype, cudaStream_t stream);
-// Rows of `src` (dtype 0 fp16, 1 bf16, 2 fp32) to int8 values and one scale each.
+// Rows of `src` (dtype 0 fp16, 1 bf16, 2 fp32) to int8 values and one scale each
+// (by_product: max |x| * fp32(1 / 127), else max |x| / 127).
 cudaError_t launch_quantize_rows_int8(const void* src, int64_t src_stride, int64_t rows, int cols, int dtype,
-                                      int8_t* values, int64_t values_stride, float* scales, cudaStream_t stream);
+                                      bool by_product, int8_t* values, int64_t values_stride, float* scales,
+                                      cudaStream_t stream);
 
 // ---- sampling with temperature, top-k, min-p and top-p (filtered_sample.cu) --
 struct FilteredSampleParams {

@@ -1,8 +1,9 @@
 // Rows to int8 with one scale each (sm_100a), for the int8 head: the weight's
 // rows once, the step's hidden states before each projection.
 //
-//   scale = max |x| / 127 (fp32 division), value = x / scale rounded to the
-//   nearest integer, ties to even (fp32 division, then rounding), in -127..127.
+//   scale = max |x| / 127 (fp32 division; or max |x| * fp32(1 / 127), as the
+//   caller says), value = x / scale rounded to the nearest integer, ties to even
+//   (fp32 division, then rounding), in -127..127.
 //
 // A row of zeros has scale 0 and values 0. A row that holds an infinity or NaN
 // has scale NaN and values 0, so that everything computed from it is NaN.
@@ -44,7 +45,7 @@ __device__ __forceinline__ float group_max(uint32_t running, int gw, float* s_ma
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads)
     quantize_rows_kernel(const T* __restrict__ src, int64_t src_stride, int64_t rows, int cols, int8_t* values,
-                         int64_t values_stride, float* scales, int gw) {
+                         int64_t values_stride, float* scales, int gw, bool by_product) {
   __shared__ float s_max[kQuantWarps];
   // a projection launched behind this kernel may set itself up already
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(kQuantThreads)
     }
     for (int i = t + kHeld * nt; i < n; i += nt)
       running = vector_max<T>(running, ld_stream_v4(static_cast<const uint4*>(base) + i));
-    const RowScale r = row_scale(group_max<T>(running, gw, s_max));
+    const RowScale r = row_scale(group_max<T>(running, gw, s_max), by_product);
     if (live && t == 0) scales[row] = r.scale;
 #pragma unroll
     for (int c = 0; c < kHeld; ++c) {
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__(kQuantThreads)
       running = word_max<T>(word_max<T>(word_max<T>(word_max<T>(running, x0), x1), x2), x3);
     }
     for (; i < n; i += nt) running = word_max<T>(running, (uint32_t)__ldg(xb + i));
-    const RowScale r = row_scale(group_max<T>(running, gw, s_max));
+    const RowScale r = row_scale(group_max<T>(running, gw, s_max), by_product);
     if (live && t == 0) scales[row] = r.scale;
     for (i = t; i - t + 4 * nt <= n; i += 4 * nt) {
       float f[4];
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(kQuantThreads)
 }
 
 template <typename T>
-cudaError_t launch_typed(const void* src, int64_t src_stride, int64_t rows, int cols, int8_t* values,
+cudaError_t launch_typed(const void* src, int64_t src_stride, int64_t rows, int cols, bool by_product, int8_t* values,
                          int64_t values_stride, float* scales, cudaStream_t stream) {
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
@@ -122,19 +123,19 @@ cudaError_t launch_typed(const void* src, int64_t src_stride, int64_t rows, int 
   const unsigned grid = (unsigned)((rows + per_block - 1) / per_block);
   const T* s = static_cast<const T*>(src);
   if (vec)
-    quantize_rows_kernel<T, true><<<grid, kQuantThreads, 0, stream>>>(s, src_stride, rows, cols, values, values_stride, scales, gw);
+    quantize_rows_kernel<T, true><<<grid, kQuantThreads, 0, stream>>>(s, src_stride, rows, cols, values, values_stride, scales, gw, by_product);
   else
-    quantize_rows_kernel<T, false><<<grid, kQuantThreads, 0, stream>>>(s, src_stride, rows, cols, values, values_stride, scales, gw);
+    quantize_rows_kernel<T, false><<<grid, kQuantThreads, 0, stream>>>(s, src_stride, rows, cols, values, values_stride, scales, gw, by_product);
   return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_quantize_rows_int8(const void* src, int64_t src_stride, int64_t rows, int cols, int dtype,
-                                      int8_t* values, int64_t values_stride, float* scales, cudaStream_t stream) {
-  if (dtype == 2) return launch_typed<float>(src, src_stride, rows, cols, values, values_stride, scales, stream);
-  if (dtype == 1) return launch_typed<__nv_bfloat16>(src, src_stride, rows, cols, values, values_stride, scales, stream);
-  return launch_typed<__half>(src, src_stride, rows, cols, values, values_stride, scales, stream);
+                                      bool by_product, int8_t* values, int64_t values_stride, float* scales,
+                                      cudaStream_t stream) {
+  auto launch = dtype == 2 ? launch_typed<float> : dtype == 1 ? launch_typed<__nv_bfloat16> : launch_typed<__half>;
+  return launch(src, src_stride, rows, cols, by_product, values, values_stride, scales, stream);
 }
 
 }  // namespace gsp

@@ -2,8 +2,9 @@
 // row quantiser and the row-sparse kernels that quantise their hidden states
 // themselves (same bits):
 //
-//   scale = max |x| / 127 (fp32 division), value = x / scale rounded to the
-//   nearest integer, ties to even (fp32 division, then rounding), in -127..127.
+//   scale = max |x| / 127 (fp32 division; or max |x| * fp32(1 / 127), as the
+//   caller says), value = x / scale rounded to the nearest integer, ties to even
+//   (fp32 division, then rounding), in -127..127.
 //
 // The division: x * (1 / scale) is within 3 * 2^-24 relative of the quotient
 // (at most 2.3e-5 absolute), so their roundings to an integer differ only where
@@ -43,10 +44,14 @@ struct RowScale {
   bool divide;  // the inverse is not finite (a denormal scale)
 };
 
-__device__ __forceinline__ RowScale row_scale(float amax) {
+// by_product: the scale is the product with the rounded reciprocal of 127,
+// which torch takes on the GPU for amax / 127.0 (one step off the division's in
+// some rows).
+__device__ __forceinline__ RowScale row_scale(float amax, bool by_product) {
+  constexpr float kInverse127 = 1.f / 127.f;
   RowScale r;
   const bool finite = amax < INFINITY;  // false for NaN
-  r.scale = finite ? __fdiv_rn(amax, 127.f) : __int_as_float(0x7fc00000);
+  r.scale = !finite ? __int_as_float(0x7fc00000) : by_product ? __fmul_rn(amax, kInverse127) : __fdiv_rn(amax, 127.f);
   r.zero = !finite || !(r.scale > 0.f);
   r.inverse = r.zero ? 0.f : __fdiv_rn(1.f, r.scale);
   r.divide = !(r.inverse < INFINITY);

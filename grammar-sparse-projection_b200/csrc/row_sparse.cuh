@@ -794,7 +794,7 @@ struct RawRows<Int8Rows<Out>> {
     int i = tid;
     for (int b = 0; b < p.batch; ++b) {
       const uint32_t m = __reduce_max_sync(FULL_MASK, __float_as_uint(s_max[b * kWarps + (tid & (kWarps - 1))]));
-      const RowScale r = row_scale(__uint_as_float(m));
+      const RowScale r = row_scale(__uint_as_float(m), p.raw_by_product);
       if (tid == 0) s_tokens[b] = r.scale;
       for (; i < (b + 1) * rvec; i += kThreads)
         store_packed<Out>(static_cast<int8_t*>(s_h), i, quantize_vector<Out>(i == tid ? first : at(b, i), r));
@@ -1631,8 +1631,8 @@ cudaError_t launch_row_sparse_typed(const RowSparseParams& p0, cudaStream_t stre
   if constexpr (IsInt8Rows<T>::value) {
     if (p.raw_hidden != nullptr && !(use_staged && RawFit<T>::holds(p))) {
       err = launch_quantize_rows_int8(p.raw_hidden, p.raw_stride, p.batch, p.hidden_dim, p.raw_dtype,
-                                      static_cast<int8_t*>(const_cast<void*>(p.hidden)), p.hidden_stride,
-                                      const_cast<float*>(p.hidden_scales), stream);
+                                      p.raw_by_product, static_cast<int8_t*>(const_cast<void*>(p.hidden)),
+                                      p.hidden_stride, const_cast<float*>(p.hidden_scales), stream);
       if (err != cudaSuccess) return err;
       p.raw_hidden = nullptr;
     }

@@ -658,6 +658,7 @@ def grouped(hidden, weight, mask, logits=None, top_value=None, top_index=None, c
 # a captured memory fill zeroes the workspace at every replay, so graphs share none.
 # ---------------------------------------------------------------------------
 DTYPE_I8 = 3
+SCALE_RECIPROCAL = 0x100
 
 
 class _NoGuard:
@@ -714,18 +715,19 @@ def _address(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def quantize_rows_int8(x, values, scales) -> None:
+def quantize_rows_int8(x, values, scales, reciprocal: bool = False) -> None:
     """gsp_quantize_rows_int8: x [N, H] -> values int8 [N, H], scales float32 [N]."""
     index = x.get_device()
+    code = DTYPE_CODES[x.dtype] + (SCALE_RECIPROCAL if reciprocal else 0)
     with on_device(index):
         status = load().gsp_quantize_rows_int8(x.data_ptr(), x.stride(0), x.shape[0], x.shape[1],
-                                               DTYPE_CODES[x.dtype], values.data_ptr(), values.stride(0),
-                                               scales.data_ptr(), raw_stream(index))
+                                               code, values.data_ptr(), values.stride(0), scales.data_ptr(),
+                                               raw_stream(index))
     if status:
         _check(status, "gsp_quantize_rows_int8")
 
 
-def _int8_call(hidden, hidden_scales, weight, weight_scales, mask):
+def _int8_call(hidden, hidden_scales, weight, weight_scales, mask, reciprocal):
     """Arguments shared by gsp_int8_logits and gsp_int8_compact: the operands,
     (scratch, workspace, stream), and the tensors to keep until the launch."""
     device, index = hidden.device, hidden.get_device()
@@ -734,6 +736,7 @@ def _int8_call(hidden, hidden_scales, weight, weight_scales, mask):
     stream = raw_stream(index)
     if hidden_scales is None:
         code, scratch_bytes = DTYPE_CODES[hidden.dtype], _int8_scratch_bytes(batch, hidden_dim)
+        code += SCALE_RECIPROCAL if reciprocal else 0
     else:
         code, scratch_bytes = DTYPE_I8, 0
     ws, scratch = _int8_buffers(device, stream, batch, vocab, scratch_bytes)
@@ -744,10 +747,10 @@ def _int8_call(hidden, hidden_scales, weight, weight_scales, mask):
 
 
 def int8_logits(route: str, hidden, hidden_scales, weight, weight_scales, mask, out_dtype, logits=None,
-                top_value=None, top_index=None, top_key=None, vocab_offset: int = 0) -> None:
+                top_value=None, top_index=None, top_key=None, vocab_offset: int = 0, reciprocal: bool = False) -> None:
     """gsp_int8_logits; hidden_scales None: `hidden` is floating point and quantised by the call."""
     with on_device(hidden.get_device()):
-        args, tail, keep = _int8_call(hidden, hidden_scales, weight, weight_scales, mask)
+        args, tail, keep = _int8_call(hidden, hidden_scales, weight, weight_scales, mask, reciprocal)
         status = load().gsp_int8_logits(
             ROUTE_CODES[route], *args, DTYPE_CODES[out_dtype], vocab_offset, _address(logits),
             0 if logits is None else logits.stride(0), _address(top_value), _address(top_index), _address(top_key),
@@ -757,10 +760,10 @@ def int8_logits(route: str, hidden, hidden_scales, weight, weight_scales, mask, 
 
 
 def int8_compact(hidden, hidden_scales, weight, weight_scales, mask, out_dtype, compact_logits, compact_ids, offsets,
-                 top_value=None, top_index=None, top_key=None, vocab_offset: int = 0) -> None:
+                 top_value=None, top_index=None, top_key=None, vocab_offset: int = 0, reciprocal: bool = False) -> None:
     """gsp_int8_compact."""
     with on_device(hidden.get_device()):
-        args, tail, keep = _int8_call(hidden, hidden_scales, weight, weight_scales, mask)
+        args, tail, keep = _int8_call(hidden, hidden_scales, weight, weight_scales, mask, reciprocal)
         status = load().gsp_int8_compact(
             *args, DTYPE_CODES[out_dtype], vocab_offset, _address(compact_logits), compact_ids.data_ptr(),
             0 if compact_logits is None else compact_logits.numel(), offsets.data_ptr(), _address(top_value),

@@ -37,13 +37,18 @@ class QuantizedRows(NamedTuple):
     scales: torch.Tensor  # float32 [N]; row n stands for values[n] * scales[n]
 
 
-def quantize_rows_int8(x: torch.Tensor, *, out: QuantizedRows | None = None) -> QuantizedRows:
+def quantize_rows_int8(x: torch.Tensor, *, out: QuantizedRows | None = None,
+                       reciprocal: bool = False) -> QuantizedRows:
     """Rows of x [N, H] (float16, bfloat16 or float32) to int8: scale =
     max |x| / 127, value = x / scale to the nearest integer (ties to even).
 
     A row of zeros has scale 0; a row that holds an infinity or NaN has scale
     NaN and values 0, so logits computed from it are NaN. x may have any row
     stride; `out` reuses tensors (for a CUDA graph, or a preallocated head).
+
+    reciprocal: scale = max |x| times the fp32 reciprocal of 127, at most one
+    step from the division's. torch computes amax / 127.0 that way on the GPU, so
+    these are the values and scales of rows quantised by torch expressions there.
     """
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
@@ -63,7 +68,7 @@ def quantize_rows_int8(x: torch.Tensor, *, out: QuantizedRows | None = None) -> 
         if out.values.shape != x.shape or out.values.device != x.device:
             raise ValueError("out must hold [N, H] values on x's device")
     if x.shape[0]:
-        _native.quantize_rows_int8(x, out.values, out.scales)
+        _native.quantize_rows_int8(x, out.values, out.scales, reciprocal)
     return out
 
 
@@ -79,7 +84,7 @@ def _check_rows(rows, what: str) -> None:
         raise ValueError(f"{what} must be contiguous")
 
 
-def _inputs(hidden, weight, bitmask_gpu, out_dtype):
+def _inputs(hidden, weight, bitmask_gpu, out_dtype, reciprocal):
     """Checked operands: (hidden values [B, H], token scales or None, mask [B, words] or None, logits dtype)."""
     _check_rows(weight, "weight")
     if isinstance(hidden, torch.Tensor):
@@ -99,6 +104,8 @@ def _inputs(hidden, weight, bitmask_gpu, out_dtype):
         values, scales = hidden
         if out_dtype is None:
             raise ValueError("int8 hidden states need out_dtype")
+        if reciprocal:
+            raise ValueError("int8 hidden states have their scales already: no reciprocal")
         dtype = out_dtype
     _native.dtype_code(dtype)
     if values.get_device() != weight.values.get_device():
@@ -127,37 +134,41 @@ def _inputs(hidden, weight, bitmask_gpu, out_dtype):
 
 
 def int8_grammar_logits(hidden, weight: QuantizedRows, bitmask_gpu: torch.Tensor | None, *,
-                        route: str = "row-sparse", out_dtype: torch.dtype | None = None, return_logits: bool = True):
+                        route: str = "row-sparse", out_dtype: torch.dtype | None = None, return_logits: bool = True,
+                        reciprocal: bool = False):
     """Masked logits of the int8 head and the fused greedy top-1.
 
     hidden: [B, D] (or [D]) float16 / bfloat16 / float32, quantised per
     request by the call; or QuantizedRows (then out_dtype says the logits'
     type, otherwise it defaults to hidden's). bitmask_gpu None: every token is
-    legal. Returns (logits [B, V] or None, top_value float32 [B], top_index
-    int64 [B]); top_index equals logits.argmax(-1), ties to the lowest id.
+    legal. reciprocal: how the call takes the requests' scales
+    (quantize_rows_int8). Returns (logits [B, V] or None, top_value float32 [B],
+    top_index int64 [B]); top_index equals logits.argmax(-1), ties to the lowest
+    id.
     """
     if route not in ROUTES:
         raise ValueError(f"unknown route {route!r}")
-    values, scales, mask, dtype = _inputs(hidden, weight, bitmask_gpu, out_dtype)
+    values, scales, mask, dtype = _inputs(hidden, weight, bitmask_gpu, out_dtype, reciprocal)
     batch, vocab, dev = values.shape[0], weight.values.shape[0], values.device
     logits = torch.empty((batch, vocab), device=dev, dtype=dtype) if return_logits else None
     top_value = torch.empty(batch, device=dev, dtype=torch.float32)
     top_index = torch.empty(batch, device=dev, dtype=torch.int64)
     _native.int8_logits(route, values, scales, weight.values, weight.scales, mask, dtype, logits=logits,
-                        top_value=top_value, top_index=top_index)
+                        top_value=top_value, top_index=top_index, reciprocal=reciprocal)
     return logits, top_value, top_index
 
 
 def int8_compact_logits(hidden, weight: QuantizedRows, bitmask_gpu: torch.Tensor, *,
-                        out_dtype: torch.dtype | None = None, capacity: int | None = None):
+                        out_dtype: torch.dtype | None = None, capacity: int | None = None, reciprocal: bool = False):
     """Compact legal logits of the int8 head: (token_ids int64 [N], logits
     [N], offsets int64 [B+1]); request b owns positions offsets[b]:offsets[b+1],
     token ids ascending (bitmask_compact_logits of triton_runtime). Without
     `capacity`, the legal count is measured on the device first (one sync);
-    positions past the legal tokens are not written."""
+    positions past the legal tokens are not written. reciprocal: as for
+    int8_grammar_logits."""
     if bitmask_gpu is None:
         raise ValueError("bitmask_gpu must be CUDA int32")
-    values, scales, mask, dtype = _inputs(hidden, weight, bitmask_gpu, out_dtype)
+    values, scales, mask, dtype = _inputs(hidden, weight, bitmask_gpu, out_dtype, reciprocal)
     dev = values.device
     if capacity is None:
         capacity = int(sum(mask_stats(mask, weight.values.shape[0])["legal_counts"]))
@@ -167,5 +178,5 @@ def int8_compact_logits(hidden, weight: QuantizedRows, bitmask_gpu: torch.Tensor
     ids = torch.empty(max(capacity, 1), device=dev, dtype=torch.int64)
     offsets = torch.empty(values.shape[0] + 1, device=dev, dtype=torch.int64)
     _native.int8_compact(values, scales, weight.values, weight.scales, mask, dtype, logits[:capacity] if capacity else
-                         None, ids, offsets)
+                         None, ids, offsets, reciprocal=reciprocal)
     return ids[:capacity], logits[:capacity], offsets

@@ -67,6 +67,9 @@ extern "C" {
 #define GSP_DTYPE_BF16 1
 #define GSP_DTYPE_F32 2
 #define GSP_DTYPE_I8 3 /* hidden_dtype of the gsp_int8_* entries only */
+/* Added to the dtype of rows that a gsp_quantize_rows_int8 / gsp_int8_* call
+ * quantises: how their scale is taken. */
+#define GSP_SCALE_RECIPROCAL 0x100
 
 /* Rows of one vocabulary tile for the block and dense GEMM paths and for the
  * active-tile statistics. */
@@ -507,6 +510,9 @@ int32_t gsp_grouped_logits(const void* hidden, int64_t hidden_row_stride, const 
  * elements, 0 allowed; up to 2^30 columns) to int8 values and one scale each:
  *   scale = max |x| / 127 (fp32 division), value = x / scale (fp32 division)
  *   rounded to the nearest integer, ties to even.
+ * With GSP_SCALE_RECIPROCAL added to dtype (hidden_dtype): scale = max |x| times
+ * the fp32 reciprocal of 127, at most one step from the division's: what torch
+ * computes on the GPU for amax / 127.0, for the bits of rows quantised there.
  * A row of zeros has scale 0; a row holding an infinity or NaN has scale NaN
  * and values 0. Every gsp_int8_* call quantises fp hidden states this way.
  */

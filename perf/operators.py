@@ -216,15 +216,16 @@ def _run_own(state):
         sys.path.insert(0, root)
     from gsp import int8_head, triton_runtime
     if state["op"] == "quantize":
-        q = int8_head.quantize_rows_int8(state["x"])
+        q = int8_head.quantize_rows_int8(state["x"], reciprocal=True)  # as torch takes amax / 127.0 on the GPU
         return {"values": q.values, "scales": q.scales}
     if state["op"] == "project":
         weight = int8_head.QuantizedRows(state["w"], state["ws"])
         if state["route"] == "packed":
             ids, logits, offsets = int8_head.int8_compact_logits(state["h"], weight, state["mask"],
-                                                                 capacity=state["legal_count"])
+                                                                 capacity=state["legal_count"], reciprocal=True)
             return {"ids": ids, "logits": logits, "offsets": offsets}
-        logits, top, at = int8_head.int8_grammar_logits(state["h"], weight, state["mask"], route=state["route"])
+        logits, top, at = int8_head.int8_grammar_logits(state["h"], weight, state["mask"], route=state["route"],
+                                                        reciprocal=True)
         return {"logits": logits, "top": top, "at": at}
     if state["form"] == "packed":
         r = triton_runtime.sample_compact_logits(state["ids"], state["x"], state["offsets"], uniforms=state["u"],

@@ -732,7 +732,7 @@ __global__ void __launch_bounds__(Epilogue<T>::kThreads, 1)
     tmem_dealloc(tmem_base, c.tmem_cols);
   }
   if (*abort_flag) {
-    if (tid == 0 && p.error) atomicExch(p.error, 1);
+    if (tid == 0) report_error(p, 1);
     return;
   }
   // The workspace must be left zero-filled for the next call, whatever its
@@ -1019,6 +1019,7 @@ cudaError_t launch_block_gemm_typed(const BlockGemmParams& p0, cudaStream_t stre
     r.keys = p0.keys;
     r.ticket = p0.ticket;
     r.error = p0.error;
+    r.device_error = p0.device_error;
     r.peers = p0.peers;
     r.sample_index = p0.sample_index;
     r.sample_lse = p0.sample_lse;

@@ -890,6 +890,19 @@ constexpr int32_t kMaxInt8Hidden = 131071;  // 128 * 128 * 131071 < 2^31: the in
 
 size_t int8_row_bytes(int32_t hidden_dim) { return ((size_t)hidden_dim + 15) / 16 * 16; }
 
+// The device's error word of the int8 calls: the workspaces of captured calls are
+// cleared by every replay and those of other threads are not at hand, so a wait
+// given up is recorded here as well.
+__device__ int g_int8_error;
+DeviceAddress g_int8_error_at[kMaxDevices] = {};
+
+cudaError_t int8_error_word(int** out) {
+  void* ptr = nullptr;
+  const cudaError_t err = device_address(g_int8_error_at, &g_int8_error, &ptr);
+  *out = static_cast<int*>(ptr);
+  return err;
+}
+
 // A dtype argument without its GSP_SCALE_RECIPROCAL.
 int32_t type_of(int32_t dtype) { return dtype & ~GSP_SCALE_RECIPROCAL; }
 bool by_product(int32_t dtype) { return (dtype & GSP_SCALE_RECIPROCAL) != 0; }
@@ -984,6 +997,8 @@ int32_t gsp_int8_logits(int32_t route, const void* hidden, int64_t hidden_row_st
   const bool want_top = top_value || top_index || top_key;
   st = check_workspace(fn, want_top || tensor_core, workspace, workspace_bytes_, batch, vocab);
   if (st != GSP_OK) return st;
+  int* device_error = nullptr;
+  if (const cudaError_t err = int8_error_word(&device_error); err != cudaSuccess) return cuda_status(err, fn);
   const Int8Hidden h = int8_hidden(hidden, hidden_row_stride, hidden_dtype, hidden_scales, batch, hidden_dim, scratch);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (!tensor_core) {
@@ -995,6 +1010,7 @@ int32_t gsp_int8_logits(int32_t route, const void* hidden, int64_t hidden_row_st
     p.raw_dtype = type_of(hidden_dtype);
     p.raw_by_product = by_product(hidden_dtype);
     p.weight_scales = weight_scales;
+    p.device_error = device_error;
     p.logits = logits;
     p.logits_stride = batch > 1 ? logits_row_stride : vocab;
     p.top_value = top_value;
@@ -1033,6 +1049,7 @@ int32_t gsp_int8_logits(int32_t route, const void* hidden, int64_t hidden_row_st
   p.keys = w.keys;
   p.ticket = w.ticket;
   p.error = w.error;
+  p.device_error = device_error;
   p.tile_list = w.tile_list;
   p.tile_counts = w.tile_counts;
   p.dense = route == GSP_ROUTE_DENSE_MASK || bitmask == nullptr;
@@ -1059,6 +1076,8 @@ int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t 
   const bool want_top = top_value || top_index || top_key;
   st = check_workspace(fn, want_top, workspace, workspace_bytes_, batch, vocab);
   if (st != GSP_OK) return st;
+  int* device_error = nullptr;
+  if (const cudaError_t err = int8_error_word(&device_error); err != cudaSuccess) return cuda_status(err, fn);
   const Int8Hidden h = int8_hidden(hidden, hidden_row_stride, hidden_dtype, hidden_scales, batch, hidden_dim, scratch);
   RowSparseParams p = make_row_sparse(h.values, h.stride, weight, weight_row_stride, bitmask, bitmask_row_stride,
                                       batch, vocab, hidden_dim, vocab_offset);
@@ -1068,6 +1087,7 @@ int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t 
   p.raw_dtype = type_of(hidden_dtype);
   p.raw_by_product = by_product(hidden_dtype);
   p.weight_scales = weight_scales;
+  p.device_error = device_error;
   p.compact = capacity > 0 ? compact_logits : nullptr;
   p.compact_ids = compact_ids;
   p.capacity = capacity;
@@ -1077,6 +1097,22 @@ int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t 
   p.top_key = top_key;
   if (workspace) attach_workspace(p, workspace);
   return cuda_status(launch_row_sparse_int8(p, out_dtype, static_cast<cudaStream_t>(stream)), fn);
+}
+
+int32_t gsp_int8_error(int32_t* error, const int32_t* set_to, void* stream) {
+  const char* fn = "gsp_int8_error";
+  if (!error) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: error is NULL", fn);
+  *error = 0;
+  int* word = nullptr;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t err = int8_error_word(&word);
+  if (err == cudaSuccess) err = cudaMemcpyAsync(error, word, sizeof(*error), cudaMemcpyDeviceToHost, s);
+  if (err == cudaSuccess) err = cudaStreamSynchronize(s);
+  if (err == cudaSuccess && set_to && *set_to != *error) {
+    err = cudaMemcpyAsync(word, set_to, sizeof(*word), cudaMemcpyHostToDevice, s);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(s);
+  }
+  return cuda_status(err, fn);
 }
 
 // ---- sampling from logits -----------------------------------------------------

@@ -210,6 +210,13 @@ __device__ __forceinline__ typename DTypeTraits<T>::Acc dot_vec(uint4 w, uint4 h
   }
 }
 
+// Records a wait given up, or state found corrupt, in the call's error words.
+template <typename Params>
+__device__ __forceinline__ void report_error(const Params& p, int code) {
+  if (p.error) atomicExch(p.error, code);
+  if (p.device_error) atomicExch(p.device_error, code);
+}
+
 // Sums over the warp, in every lane (of two independent values: their shuffles
 // interleave).
 __device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(FULL_MASK, v); }

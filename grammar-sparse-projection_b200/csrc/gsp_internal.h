@@ -72,6 +72,7 @@ struct RowSparseParams {
   unsigned long long* keys;
   unsigned int* ticket;
   int* error;  // set non-zero when a bounded wait gave up (never cleared by kernels)
+  int* device_error;  // int8 operands: the device's word, set beside it (or nullptr)
   // cooperative kernel (all zero on entry and exit): per-CTA slice popcounts,
   // the number of CTAs that have published theirs, per-CTA "units listed"
   // flags (one per kFlagStride words, so pollers of different flags never
@@ -117,6 +118,7 @@ struct BlockGemmParams {
   unsigned long long* keys;
   unsigned int* ticket;
   int* error;
+  int* device_error;
   int32_t* tile_list;     // workspace: compacted active tile ids
   int32_t* tile_counts;   // workspace: per-builder-block active tile counts
   int dense;              // 1: every tile is projected (dense_masked_logits)
@@ -223,6 +225,15 @@ cudaError_t launch_merge_logsumexp(const float* lse, int parts, int batch, float
 cudaError_t launch_top1_from_keys(const int64_t* keys, int batch, float* top_value,
                                   int64_t* top_index, cudaStream_t stream);
 cudaError_t launch_block_gemm(const BlockGemmParams& p, int dtype, cudaStream_t stream);
+
+// Address of a device variable of this library on the current device, kept in
+// `known` (kMaxDevices entries of the variable's own) per device and CUDA context.
+constexpr int kMaxDevices = 128;
+struct DeviceAddress {
+  void* context;
+  void* ptr;
+};
+cudaError_t device_address(DeviceAddress* known, const void* variable, void** out);
 
 // ---- int8 operands (out_dtype: 0 fp16, 1 bf16, 2 fp32 logits) ---------------
 cudaError_t launch_row_sparse_int8(const RowSparseParams& p, int out_dtype, cudaStream_t stream);

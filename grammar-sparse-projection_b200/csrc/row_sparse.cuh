@@ -404,7 +404,7 @@ __device__ __forceinline__ void finalize_top1_polled(const RowSparseParams& p, u
     }
   }
   const bool failed = __syncthreads_or(late);
-  if (failed && tid == 0 && p.error) atomicExch(p.error, 4);
+  if (failed && tid == 0) report_error(p, 4);
   bool ok = !failed;
   if (p.peers.world > 1) ok = peer_exchange_keys(p.peers, s_keys, B, s_word, p.error) && ok;
   for (int b = tid; b < B; b += blockDim.x) store_top1(p.top_value, p.top_index, p.top_key, b, s_keys[b], ok);
@@ -1298,7 +1298,7 @@ __device__ __forceinline__ void coop_stream_round(const RowSparseParams& p, cons
     bad |= (b >= (uint32_t)p.batch) || (code - b * code_stride >= (uint32_t)p.vocab);
   }
   if (__syncthreads_or(bad)) {
-    if (tid == 0 && p.error) atomicExch(p.error, 2);
+    if (tid == 0) report_error(p, 2);
     return;
   }
   round_noise<kSample>(p, sample_smem(s_keys, p.batch), s_list, n, code_stride);
@@ -1450,7 +1450,7 @@ __global__ void __launch_bounds__(kThreads, 1) row_sparse_coop_kernel(const RowS
       __nanosleep(64);
     }
     if (v < (uint32_t)G) {
-      if (p.error) atomicExch(p.error, 1);
+      report_error(p, 1);
       s_misc[0] = 1;
     }
   }
@@ -1504,7 +1504,7 @@ __global__ void __launch_bounds__(kThreads, 1) row_sparse_coop_kernel(const RowS
       if (tid < G) {
         const uint32_t sb = s_base[tid], sc = s_cnt[tid];
         if (sc != 0u && sb < hi && sb + sc > lo && wait_flag(p.slice_ready + (size_t)tid * kFlagStride) == 0u) {
-          if (p.error) atomicExch(p.error, 1);
+          report_error(p, 1);
           s_misc[0] = 1;
         }
       }

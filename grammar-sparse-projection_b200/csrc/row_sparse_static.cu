@@ -91,36 +91,38 @@ CUcontext current_context() {
   return c;
 }
 
-constexpr int kMaxDevices = 128;
 std::mutex g_setup_mu;
-struct ScratchAddress {
-  CUcontext ctx;
-  void* ptr;
-};
-ScratchAddress g_scratch[kMaxDevices] = {};
+DeviceAddress g_scratch[kMaxDevices] = {};
 
-// Device address of g_static_scratch on the current device, looked up once per
-// device and context (a device whose context was reset and re-created gets a
-// fresh lookup: the old address belonged to the old context).
-cudaError_t scratch_on_current_device(void** out) {
+cudaError_t scratch_on_current_device(void** out) { return device_address(g_scratch, g_static_scratch, out); }
+
+}  // namespace
+
+// Looked up once per device and context (a device whose context was reset and
+// re-created gets a fresh lookup: the old address belonged to the old context).
+cudaError_t device_address(DeviceAddress* known, const void* variable, void** out) {
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
   const CUcontext ctx = current_context();
   std::lock_guard<std::mutex> lock(g_setup_mu);
-  if (g_scratch[dev].ptr == nullptr || ctx == nullptr || g_scratch[dev].ctx != ctx) {
+  if (known[dev].ptr == nullptr || ctx == nullptr || known[dev].context != ctx) {
     void* ptr = nullptr;
-    err = cudaGetSymbolAddress(&ptr, g_static_scratch);
+    // (the first call may be under stream capture: the lookup is no stream work)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if ((err = cudaThreadExchangeStreamCaptureMode(&mode)) != cudaSuccess) return err;
+    err = cudaGetSymbolAddress(&ptr, variable);
+    const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (err == cudaSuccess) err = back;
     if (err != cudaSuccess) return err;
-    g_scratch[dev].ptr = ptr;
-    g_scratch[dev].ctx = current_context();
+    known[dev].ptr = ptr;
+    known[dev].context = current_context();
   }
-  *out = g_scratch[dev].ptr;
+  *out = known[dev].ptr;
   return cudaSuccess;
 }
 
-}  // namespace
 }  // namespace gsp
 
 extern "C" int32_t gsp_row_sparse_logits_static(const void* hidden, int64_t hidden_row_stride,

@@ -106,6 +106,7 @@ SIGNATURES = {
                          _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp], _i32),
     "gsp_int8_compact": ([_vp, _i64, _i32, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i64,
                           _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp], _i32),
+    "gsp_int8_error": ([ctypes.POINTER(_i32), ctypes.POINTER(_i32), _vp], _i32),
     "gsp_sample_logits": ([_vp, _i64, _i32, _vp, _i64, _i32, _i32, _i64] + _FILTER_ARGS, _i32),
     "gsp_sample_compact": ([_vp, _vp, _vp, _i64, _i32, _i32, _i32] + _FILTER_ARGS, _i32),
 }
@@ -165,10 +166,12 @@ def dtype_code(dtype: torch.dtype) -> int:
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
 _ws_lock = threading.Lock()
 _thread = threading.local()
+_int8_resets: dict[int, int] = {}  # device index -> resets so far
 
 
 def _thread_buffers() -> dict:
-    """The calling thread's (workspace, scratch) of its int8 calls, by (device index, stream)."""
+    """The calling thread's (workspace, scratch, resets when last zeroed) of its
+    int8 calls, by (device index, stream)."""
     held = getattr(_thread, "buffers", None)
     if held is None:
         held = _thread.buffers = {}
@@ -189,26 +192,36 @@ def workspace(device: torch.device, batch: int, vocab: int) -> torch.Tensor:
 
 
 def reset_workspace(device: torch.device) -> None:
-    """Re-zeroes the current stream's workspaces (needed after a call whose
-    kernel reported an error through workspace_error)."""
+    """Re-zeroes the current stream's workspace and, before their next calls,
+    those of the device's int8 calls on all threads and streams (needed after a
+    call whose kernel reported an error through workspace_error)."""
     dev_index = device.index if device.index is not None else torch.cuda.current_device()
-    key = (dev_index, torch.cuda.current_stream(device).cuda_stream)
-    for ws in (_workspaces.get(key), _thread_buffers().get(key, (None, None))[0]):
-        if ws is not None:
-            ws.zero_()
+    ws = _workspaces.get((dev_index, torch.cuda.current_stream(device).cuda_stream))
+    if ws is not None:
+        ws.zero_()
+    _int8_error(dev_index, set_to=0)
+    with _ws_lock:
+        _int8_resets[dev_index] = _int8_resets.get(dev_index, 0) + 1
 
 
 def workspace_error(device: torch.device) -> int:
-    """Error word of the current stream's workspace, or of the calling thread's
-    own for int8 calls: non-zero after a kernel gave up a bounded wait (reads
-    the device, so it synchronises)."""
+    """Error word of the current stream's workspace, or of the device's int8
+    calls, captured or on whatever stream and thread, since the last
+    reset_workspace: non-zero after a kernel gave up a bounded wait (reads the
+    device, so it synchronises the current stream; int8 calls on other streams
+    must have ended to be seen)."""
     dev_index = device.index if device.index is not None else torch.cuda.current_device()
-    key = (dev_index, torch.cuda.current_stream(device).cuda_stream)
-    for ws in (_workspaces.get(key), _thread_buffers().get(key, (None, None))[0]):
-        word = 0 if ws is None else int(ws[4:8].view(torch.int32).item())
-        if word:
-            return word
-    return 0
+    ws = _workspaces.get((dev_index, torch.cuda.current_stream(device).cuda_stream))
+    word = 0 if ws is None else int(ws[4:8].view(torch.int32).item())
+    return word or _int8_error(dev_index)
+
+
+def _int8_error(dev_index: int, set_to: int | None = None) -> int:
+    """gsp_int8_error on the device's current stream."""
+    word, new = _i32(0), None if set_to is None else ctypes.byref(_i32(set_to))
+    with on_device(dev_index):
+        _check(load().gsp_int8_error(ctypes.byref(word), new, raw_stream(dev_index)), "gsp_int8_error")
+    return word.value
 
 
 def _require_cuda(*tensors: torch.Tensor) -> None:
@@ -703,12 +716,13 @@ def _int8_buffers(device: torch.device, stream: int, batch: int, vocab: int, scr
         return (torch.zeros(need, dtype=torch.uint8, device=device),
                 torch.empty(scratch_bytes, dtype=torch.uint8, device=device))
     held, key = _thread_buffers(), (device.index, stream)
-    buffers = held.get(key)
-    if buffers is None or buffers[0].numel() < need or buffers[1].numel() < scratch_bytes:
-        sizes = (64 * 1024, 64 * 1024) if buffers is None else tuple(2 * t.numel() for t in buffers)
+    buffers, resets = held.get(key), _int8_resets.get(device.index, 0)
+    stale = buffers is None or buffers[2] != resets
+    if stale or buffers[0].numel() < need or buffers[1].numel() < scratch_bytes:
+        sizes = (64 * 1024, 64 * 1024) if buffers is None else tuple((1 if stale else 2) * t.numel() for t in buffers[:2])
         buffers = held[key] = (torch.zeros(max(need, sizes[0]), dtype=torch.uint8, device=device),
-                               torch.empty(max(scratch_bytes, sizes[1]), dtype=torch.uint8, device=device))
-    return buffers
+                               torch.empty(max(scratch_bytes, sizes[1]), dtype=torch.uint8, device=device), resets)
+    return buffers[:2]
 
 
 def _address(t: torch.Tensor | None):

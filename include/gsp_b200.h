@@ -550,6 +550,15 @@ int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t 
                          float* top_value, int64_t* top_index, int64_t* top_key, void* scratch, size_t scratch_bytes,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* Reads the current device's error word of the gsp_int8_* calls: every such call,
+ * on any stream, host thread or workspace, captured ones included, records there
+ * the code that it leaves in its workspace's error word. set_to not NULL: the word
+ * is *set_to afterwards (0 clears it; nothing else does). After a non-zero word
+ * each workspace that the failed call may have used is re-zeroed before its next
+ * call. Synchronises `stream`; calls on other streams that are to be seen must have
+ * ended. */
+int32_t gsp_int8_error(int32_t* error, const int32_t* set_to, void* stream);
+
 /* ---- sampling from logits ------------------------------------------------------
  * One token per request from logits that a route of the head wrote (-inf on
  * illegal tokens), or from any logits with the packed bitmask (NULL: none), by

@@ -4,7 +4,7 @@
 // For one row with legal logits x_i (bit set, not NaN, not -inf), in the order
 // "falling logit, ties by rising position", and w_i = exp((x_i - max) / T):
 //   top-k   keep the first k                                  (k <= 0: all)
-//   min-p   keep w_i >= min_p                                 (min_p <= 0: all)
+//   min-p   keep w_i >= min_p           (min_p <= 0: all; above 1 it counts as 1)
 //   top-p   keep the shortest prefix with sum >= top_p * sum  (top_p >= 1: all)
 //   draw    the first kept i with w_1 + ... + w_i > u * (sum of the kept)
 // Each filter leaves a prefix of that order, so a kept set is a border key and

@@ -584,9 +584,10 @@ def sample_logits(logits: torch.Tensor, *, uniforms: torch.Tensor, temperature=1
     head writes (-inf on illegal tokens), or any logits with their bitmask;
     NaN and -inf are never drawn. In the order "falling logit, ties by rising
     id", with w = exp((x - max) / temperature): keep the first top_k (0: all),
-    of these w >= min_p, of these the shortest prefix with at least top_p of
-    the weight, and draw the first token whose running weight passes
-    uniforms[b] times the kept weight. Each setting is a number or a tensor
+    of these w >= min_p (above 1 it counts as 1: the largest logit and its
+    ties), of these the shortest prefix with at least top_p of the weight, and
+    draw the first token whose running weight passes uniforms[b] times the kept
+    weight. Each setting is a number or a tensor
     with one value per request (float32; top_k int32). Temperature 0 is greedy
     (largest logit, lowest id). The sums are exact, so equal calls give equal
     tokens, log-probabilities and counts. A request without a legal token

@@ -565,8 +565,9 @@ int32_t gsp_int8_error(int32_t* error, const int32_t* set_to, void* stream);
  * temperature, top-k, min-p and top-p from a given uniform number:
  *   legal tokens (bit set, not NaN, not -inf) in the order "falling logit, ties
  *   by rising id"; w = exp((x - max) / T);
- *   keep the first top_k (<= 0: all), of these w >= min_p (<= 0: all), of these
- *   the shortest prefix with sum >= top_p * sum (>= 1: all; at least one token);
+ *   keep the first top_k (<= 0: all), of these w >= min_p (<= 0: all; above 1
+ *   counts as 1: the largest logit and its ties), of these the shortest prefix
+ *   with sum >= top_p * sum (>= 1: all; at least one token);
  *   draw the first kept token with w_1 + ... + w_i > uniforms[b] * sum.
  * Outputs: token_ids [batch], logprobs [batch] (optional: log-probability among
  * the kept tokens), kept [batch] (optional: how many were kept). Sums are exact

@@ -368,7 +368,8 @@ def filtered_sample_reference(row, uniform: float, temperature: float = 1.0, top
     """Temperature, top-k, min-p, top-p and one draw on one row of logits, in
     float64: (position or 0, log-probability among the kept, number kept).
     NaN and -inf are not drawn; order: falling logit, ties by rising position.
-    The settings are the fp32 values a kernel receives."""
+    A min_p above 1 counts as 1: the largest logit and its ties. The settings
+    are the fp32 values a kernel receives."""
     x = np.asarray(row, dtype=np.float64)
     at = np.flatnonzero(x > -np.inf)  # NaN compares false
     if at.size == 0:
@@ -383,7 +384,7 @@ def filtered_sample_reference(row, uniform: float, temperature: float = 1.0, top
     if top_k > 0:
         score = score[:top_k]
     w = np.exp(score)
-    w = w[w >= m]
+    w = w[w >= min(m, 1.0)]
     upto = np.cumsum(w)
     if p < 1.0:
         w = w[:max(1, int(np.count_nonzero(upto - w < p * upto[-1])))]

@@ -47,7 +47,8 @@ __global__ void __launch_bounds__(kQuantThreads)
     quantize_rows_kernel(const T* __restrict__ src, int64_t src_stride, int64_t rows, int cols, int8_t* values,
                          int64_t values_stride, float* scales, int gw, bool by_product) {
   __shared__ float s_max[kQuantWarps];
-  // a projection launched behind this kernel may set itself up already
+  // a staged projection launched behind this kernel may have its CTAs in place
+  // already (it waits for this kernel's end before it does anything)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int per_block = kQuantWarps / gw;
   const int group = threadIdx.x / (32 * gw), t = threadIdx.x - group * 32 * gw, nt = 32 * gw;

@@ -178,7 +178,12 @@ RowSparseParams make_row_sparse(const void* hidden, int64_t hidden_row_stride, c
   return p;
 }
 
-void attach_workspace(RowSparseParams& p, void* workspace) {
+// (a workspace that the call does not need may be smaller than one that it does:
+// then it is not used)
+void attach_workspace(RowSparseParams& p, void* workspace, size_t bytes) {
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
+      bytes < row_sparse_workspace_bytes(p.batch, p.vocab))
+    return;
   const Workspace w = carve_workspace(workspace, p.batch, p.vocab);
   p.keys = w.keys;
   p.ticket = w.ticket;
@@ -219,7 +224,7 @@ int32_t projection_common(const char* fn, bool tensor_core, int dense, const voi
     p.top_value = top_value;
     p.top_index = top_index;
     p.top_key = top_key;
-    if (workspace) attach_workspace(p, workspace);
+    attach_workspace(p, workspace, workspace_bytes_);
     if (peers) p.peers = *peers;
     return cuda_status(launch_row_sparse(p, dtype, s), fn);
   }
@@ -347,7 +352,7 @@ int32_t gsp_row_sparse_compact(const void* hidden, int64_t hidden_row_stride, co
   p.top_value = top_value;
   p.top_index = top_index;
   p.top_key = top_key;
-  if (workspace) attach_workspace(p, workspace);
+  attach_workspace(p, workspace, workspace_bytes_);
   return cuda_status(launch_row_sparse(p, dtype, static_cast<cudaStream_t>(stream)), fn);
 }
 
@@ -445,7 +450,7 @@ static int32_t sample_common(const char* fn, int32_t route, const void* hidden, 
     p.top_value = top_value;
     p.top_index = top_index;
     p.top_key = top_key;
-    attach_workspace(p, workspace);
+    attach_workspace(p, workspace, workspace_bytes_);
     p.sample_index = sample_index;
     p.sample_lse = sample_logsumexp;
     p.sample_key = sample_key;
@@ -1016,7 +1021,7 @@ int32_t gsp_int8_logits(int32_t route, const void* hidden, int64_t hidden_row_st
     p.top_value = top_value;
     p.top_index = top_index;
     p.top_key = top_key;
-    if (workspace) attach_workspace(p, workspace);
+    attach_workspace(p, workspace, workspace_bytes_);
     return cuda_status(launch_row_sparse_int8(p, out_dtype, s), fn);
   }
   if (h.raw != nullptr) {
@@ -1095,7 +1100,7 @@ int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t 
   p.top_value = top_value;
   p.top_index = top_index;
   p.top_key = top_key;
-  if (workspace) attach_workspace(p, workspace);
+  attach_workspace(p, workspace, workspace_bytes_);
   return cuda_status(launch_row_sparse_int8(p, out_dtype, static_cast<cudaStream_t>(stream)), fn);
 }
 

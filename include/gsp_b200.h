@@ -28,7 +28,8 @@
  *   - Optional outputs may be NULL.
  *   - `workspace` must be at least gsp_workspace_bytes(batch, vocab) bytes,
  *     zero-filled once before first use; every call leaves it zero-filled
- *     again. Calls that run concurrently must not share one workspace.
+ *     again. Calls that run concurrently must not share one workspace. A
+ *     row-sparse call without a top-1 needs none, and does not use a smaller one.
  *     Exception: bytes 4..7 hold an int32 error word that kernels set (and
  *     never clear) when a bounded wait ran out instead of hanging: 1 a
  *     multi-CTA kernel's wait for its CTAs' counts, flags or pipeline stages,

@@ -14,8 +14,13 @@ hot path: full -inf-filled logits [V] plus the fused greedy top-1.
              kernel into pinned host memory, all inside the timed region;
   roofline   the row-sparse kernel's achieved legal-row bandwidth against the
              measured HBM copy bandwidth;
-  sweep      every density of the GEMV workload, uniform and clustered;
   cpu_baseline  the oracle's CPU restatement of the same step on host cores.
+
+One JSON line on stdout has these. The other sections (the sweep over densities,
+uniform and clustered; batched, mixed, sampler, graphed and grouped heads; the
+vocabulary-parallel head; the end-to-end step's parts) are one JSON line on
+stderr, {"sections": ...}: with them the stdout line was 23 KB long, and a reader
+that keeps the end of the output lost its beginning.
 
 Timing (one GPU): the K timed steps are captured in one CUDA graph and timed
 with CUDA events around its replay, so host launch overhead and per-step event
@@ -54,6 +59,30 @@ UNIT = "GB/s"
 VOCAB, HIDDEN = 248320, 2048
 DENSITIES = (0.0005, 0.005, 0.01, 0.10, 0.50, 1.0)
 FALLBACK_HBM_GBS = 6650.0
+
+
+# Kept off the stdout line.
+SECTIONS = ("sweep", "batched", "mixed", "vocab_parallel_head", "sampler", "graphed_head", "lane_groups")
+
+
+def rounded(v):
+    """v with its floats to six significant digits."""
+    if isinstance(v, dict):
+        return {k: rounded(x) for k, x in v.items()}
+    if isinstance(v, (list, tuple)):
+        return [rounded(x) for x in v]
+    return float(f"{v:.6g}") if isinstance(v, float) else v
+
+
+def split_line(line: dict) -> tuple[dict, dict]:
+    """(the stdout line, the sections for stderr) of a run's results."""
+    line, sections = dict(line), {}
+    for name in SECTIONS:
+        sections[name] = line.pop(name, None)
+    e2e = dict(line["e2e"])
+    sections["e2e"] = {k: e2e.pop(k) for k in ("breakdown", "what") if k in e2e}
+    line["e2e"] = e2e
+    return rounded(line), {k: v for k, v in sections.items() if v}
 
 
 def parse_args():
@@ -917,6 +946,8 @@ def main():
             "graphed_head": graphed,
             "lane_groups": groups,
         }
+        line, sections = split_line(line)
+        print(json.dumps({"sections": sections}), file=sys.stderr, flush=True)
         print(json.dumps(line), flush=True)
     if world > 1:
         xch.close()

@@ -1,0 +1,865 @@
+// Log probabilities of given tokens, entropy, logsumexp and the top alternatives
+// of logits rows, and their gradient (sm_100a).
+//
+// With x the legal logits of a row (bit set, not NaN, not -inf), T its
+// temperature, z = x / T, m = max x:
+//
+//   S = sum exp((x - m) / T),  A = sum exp((x - m) / T) (x - m) / T
+//   logprob_t = (x_t - m) / T - ln S       (-inf for a token that is not legal)
+//   entropy   = ln S - A / S               (0 for a row without a legal token)
+//   logsumexp = m / T + ln S
+//   top n     = the n legal tokens that come first by falling x, ties by rising id
+//
+//   dL/dx_j = (p_j (gL - sum_k g_k - gH (ln p_j + entropy)) + sum_k g_k [j = t_k]) / T
+//
+// Forward: one pass over the row, which is bound by its bytes. A row belongs to
+// one CTA, or to a cluster of CTAs whose shares are merged over distributed
+// shared memory when there are few rows. A thread keeps its own running (m, S, A)
+// in powers of two (d = (x - m) log2(e) / T, clamped at -200 so that an excluded
+// value adds exactly nothing) and compares a vector's maximum, two packed
+// instructions per four elements, with both m and the n-th alternative so far:
+// the two rare cases (a new maximum, a candidate) share that one test. All
+// threads start from the maximum of the CTA's first batch of vectors, and the
+// alternatives from the n-th largest of its 64 eight-lane maxima, so hardly any
+// vector takes the slow path after it. Candidates gather in a list, are ranked
+// by counting when it fills, and what does not fit is tried again against the
+// higher border: rows in rising order or of equal values cost time, not results.
+//
+// Sums run in fp32: a thread adds at most a few hundred terms, then a tree.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/gsp_b200.h"
+#include "gsp_common.cuh"
+#include "gsp_internal.h"
+
+namespace cg = cooperative_groups;
+
+namespace gsp {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kUnroll = 4;       // 16-byte vectors a thread has under way
+constexpr int kMaxTop = 64;      // alternatives
+constexpr int kListSize = 1024;  // candidates held at a time
+constexpr int kListFull = 96;    // candidates past n at which the list is ranked
+constexpr int kMaxClusterSize = 16;
+constexpr int kMaxTokens = 1024;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNothing = -200.f;  // exponent whose power of two is 0 in fp32
+
+struct LogprobParams {
+  const void* logits;
+  int64_t row_stride;
+  const uint32_t* mask;
+  int64_t mask_stride;
+  int vocab;               // row length (packed rows: ignored)
+  const int64_t* offsets;  // packed rows: [batch + 1], else nullptr
+  const int64_t* ids;      // packed rows: token id of each position, rising in a row
+  int64_t capacity;        // packed rows: positions that exist
+  float temperature;
+  const float* temperatures;
+  const int64_t* token_ids;  // [batch, tokens]
+  int tokens;
+  int top_n;
+  float* logprobs;      // [batch, tokens]
+  float* entropy;       // [batch] (optional)
+  float* logsumexp;     // [batch] (optional)
+  int64_t* top_ids;     // [batch, top_n]
+  float* top_logprobs;  // [batch, top_n]
+  float4* stats;        // [batch]: m, S, entropy, 1 / T (optional)
+};
+
+// One row as 16-byte vectors from an aligned base: vector i holds elements
+// i * kPerVec - phase and on; those before 0 and from len on are not the row's.
+struct Row {
+  const uint4* base;
+  int phase;
+  int64_t len;
+  const uint32_t* mask;
+  int64_t first;  // position of element 0 in the packed arrays
+};
+
+template <typename T>
+__device__ __forceinline__ void set_row(Row& r, const void* logits, int64_t start, int64_t len) {
+  using Bits = typename DTypeTraits<T>::Bits;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(static_cast<const Bits*>(logits) + start);
+  r.base = reinterpret_cast<const uint4*>(at & ~uintptr_t(15));
+  r.phase = (int)((at & 15) / sizeof(Bits));
+  r.len = len;
+  r.first = start;
+}
+
+template <typename T>
+__device__ __forceinline__ int64_t row_vectors(const Row& r) {
+  return r.len <= 0 ? 0 : (r.len + r.phase + DTypeTraits<T>::kPerVec - 1) / DTypeTraits<T>::kPerVec;
+}
+
+// Which of vector i's elements belong to the row and are legal.
+template <typename T, bool kMask>
+__device__ __forceinline__ uint32_t legal_bits(const Row& r, int64_t i) {
+  constexpr int kPer = DTypeTraits<T>::kPerVec;
+  const int64_t e0 = i * kPer - r.phase;
+  uint32_t bits = (1u << kPer) - 1u;
+  if constexpr (kMask) {
+    const int64_t w = e0 >> 5, nw = (r.len + 31) >> 5;
+    const int shift = (int)(e0 & 31);
+    const uint32_t lo = w >= 0 && w < nw ? __ldg(r.mask + w) : 0u;
+    const uint32_t hi = shift + kPer > 32 && w + 1 < nw ? __ldg(r.mask + w + 1) : 0u;
+    bits &= __funnelshift_r(lo, hi, shift);
+  }
+  if (e0 < 0) bits &= ~((1u << (int)(-e0)) - 1u);
+  if (e0 + kPer > r.len) bits &= r.len > e0 ? (1u << (int)(r.len - e0)) - 1u : 0u;
+  return bits;
+}
+
+// -inf in the elements whose bit is not set.
+template <typename T>
+__device__ __forceinline__ void exclude(uint4& v, uint32_t bits) {
+  constexpr int kPer = DTypeTraits<T>::kPerVec;
+  if (bits == (1u << kPer) - 1u) return;
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (sizeof(typename DTypeTraits<T>::Bits) == 2) {
+      const uint32_t two = bits >> (2 * k);
+      const uint32_t keep = ((two & 1u) ? 0x0000ffffu : 0u) | ((two & 2u) ? 0xffff0000u : 0u);
+      const uint32_t ninf = DTypeTraits<T>::kNegInfBits * 0x00010001u;
+      w[k] = (w[k] & keep) | (ninf & ~keep);
+    } else {
+      w[k] = ((bits >> k) & 1u) ? w[k] : 0xff800000u;
+    }
+  }
+  v = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Largest element; NaN counts as absent.
+template <typename T>
+__device__ __forceinline__ float vector_top(const uint4& v) {
+  if constexpr (std::is_same<T, float>::value) {
+    return fmaxf(fmaxf(fmaxf(__uint_as_float(v.x), -INFINITY), __uint_as_float(v.y)),
+                 fmaxf(fmaxf(__uint_as_float(v.z), -INFINITY), __uint_as_float(v.w)));
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* h = reinterpret_cast<const T2*>(&v);
+    const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    uint32_t w;
+    w = *reinterpret_cast<const uint32_t*>(&m);
+    const float2 f = DTypeTraits<T>::pair_to_float2(w);
+    return fmaxf(fmaxf(f.x, -INFINITY), f.y);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float2 element_pair(const uint4& v, int k) {  // elements 2k, 2k + 1
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (std::is_same<T, float>::value) return make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+  else return DTypeTraits<T>::pair_to_float2(w[k]);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two fp32 operations per instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 r, a, b;\n\t"
+      "mov.b64 {%0, %1}, r;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 r, a, b;\n\t"
+      "mov.b64 {%0, %1}, r;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 r, a, b, c;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
+// A thread's running maximum and sums relative to it, in two lanes each.
+struct Running {
+  float m;
+  float2 s, a;
+  // Moves the reference from m up to `to`: s 2^delta, a -> 2^delta (a + delta s).
+  __device__ __forceinline__ void raise(float to, float c) {
+    const float delta = fmaxf((m - to) * c, kNothing);
+    const float f = exp2_approx(delta);
+    a = make_float2(f * fmaf(delta, s.x, a.x), f * fmaf(delta, s.y, a.y));
+    s = make_float2(f * s.x, f * s.y);
+    m = to;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void accumulate(Running& r, const uint4& v, float c) {
+  const float2 neg = make_float2(-r.m, -r.m), cc = make_float2(c, c);
+#pragma unroll
+  for (int k = 0; k < DTypeTraits<T>::kPerVec / 2; ++k) {
+    float2 d = mul2(add2(element_pair<T>(v, k), neg), cc);
+    d = make_float2(fmaxf(d.x, kNothing), fmaxf(d.y, kNothing));  // (-inf, NaN and what is far below: nothing)
+    const float2 e = make_float2(exp2_approx(d.x), exp2_approx(d.y));
+    r.s = add2(r.s, e);
+    r.a = fma2(e, d, r.a);
+  }
+}
+
+struct Sums {
+  float m, s, a;
+};
+__device__ __forceinline__ Sums merge(Sums x, Sums y, float c) {
+  const float m = fmaxf(x.m, y.m);
+  const float dx = fmaxf((x.m - m) * c, kNothing), dy = fmaxf((y.m - m) * c, kNothing);
+  const float fx = exp2_approx(dx), fy = exp2_approx(dy);
+  return Sums{m, fx * x.s + fy * y.s, fx * fmaf(dx, x.s, x.a) + fy * fmaf(dy, y.s, y.a)};
+}
+
+struct Shared {
+  Sums part[kThreads / 32];
+  Sums total;  // this CTA's, read by the cluster
+  unsigned int ninf;
+  float group_top[kThreads / 8];
+  unsigned int count;
+  int listed;
+  unsigned long long border;
+  alignas(16) unsigned long long list[kListSize];
+  unsigned long long best[kMaxTop];
+};
+
+// The n largest of the list's keys, in falling order, at its front. Called by
+// the whole CTA between barriers of its own; afterwards s.border is the n-th.
+__device__ __forceinline__ void rank_list(Shared& s, int n) {
+  __syncthreads();
+  const int count = min((int)s.count, kListSize);
+  for (int t = threadIdx.x; t < count; t += kThreads) {
+    const unsigned long long key = s.list[t];
+    int rank = 0;
+    int j = 0;
+    for (; j + 2 <= count; j += 2) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&s.list[j]);
+      rank += (two.x > key) + (two.y > key);
+    }
+    if (j < count) rank += s.list[j] > key;
+    if (rank < n) s.best[rank] = key;
+  }
+  __syncthreads();
+  const int kept = min(count, n);
+  if ((int)threadIdx.x < kept) s.list[threadIdx.x] = s.best[threadIdx.x];
+  if (threadIdx.x == 0) {
+    s.count = (unsigned)kept;
+    s.listed = kept;
+    if (count >= n) s.border = s.best[n - 1];
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ float border_value(unsigned long long border) {
+  return border == 0ull ? -INFINITY : from_ordered_bits((uint32_t)(border >> 32));
+}
+
+// Of vector v's elements, those past the border.
+template <typename T>
+__device__ __forceinline__ uint32_t candidates(const uint4& v, float least) {
+  uint32_t found = 0u;
+#pragma unroll
+  for (int k = 0; k < DTypeTraits<T>::kPerVec / 2; ++k) {
+    const float2 x = element_pair<T>(v, k);
+    if (x.x >= least && x.x > -INFINITY) found |= 1u << (2 * k);
+    if (x.y >= least && x.y > -INFINITY) found |= 2u << (2 * k);
+  }
+  return found;
+}
+
+// Lists vector v's waiting elements; those that find no room stay waiting.
+template <typename T>
+__device__ __forceinline__ uint32_t list_candidates(Shared& s, const uint4& v, uint32_t waiting, int64_t e0,
+                                                    unsigned long long border, int limit, bool& full) {
+#pragma unroll
+  for (int j = 0; j < DTypeTraits<T>::kPerVec; ++j) {
+    if (!((waiting >> j) & 1u)) continue;
+    const float2 x = element_pair<T>(v, j / 2);
+    const unsigned long long key = top1_key(j & 1 ? x.y : x.x, (uint64_t)(e0 + j));
+    if (key > border) {
+      const unsigned at = atomicAdd(&s.count, 1u);
+      if ((int)at >= limit) full = true;
+      if (at >= (unsigned)kListSize) continue;
+      s.list[at] = key;
+    }
+    waiting &= ~(1u << j);
+  }
+  return waiting;
+}
+
+__device__ __forceinline__ bool valid_temperature(float t) { return t > 0.f && t < INFINITY; }
+
+// (x - m) / T - ln S; infinite maxima share the weight among themselves.
+__device__ __forceinline__ float logprob_of(float x, float m, float t, float log_s) {
+  if (!(x > -INFINITY)) return -INFINITY;  // (NaN too)
+  if (x == m) return -log_s;
+  return __fdiv_rn(x - m, t) - log_s;  // (m infinite: -inf)
+}
+
+template <typename T, bool kMask, bool kTop>
+__global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const LogprobParams p) {
+  using Bits = typename DTypeTraits<T>::Bits;
+  constexpr int kPer = DTypeTraits<T>::kPerVec;
+  __shared__ Shared s;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int64_t b = blockIdx.x / size;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  Row r;
+  if (p.offsets) {
+    int64_t lo = p.offsets[b], hi = p.offsets[b + 1];
+    lo = lo < 0 ? 0 : lo > p.capacity ? p.capacity : lo;
+    hi = hi > p.capacity ? p.capacity : hi;
+    set_row<T>(r, p.logits, lo, hi > lo ? hi - lo : 0);
+  } else {
+    set_row<T>(r, p.logits, b * p.row_stride, p.vocab);
+  }
+  r.mask = kMask ? p.mask + b * p.mask_stride : nullptr;
+  const float t = p.temperatures ? p.temperatures[b] : p.temperature;
+  const bool valid = valid_temperature(t);
+  const float c = fminf(kLog2e / t, 3e38f);
+  const int64_t nv = valid ? row_vectors<T>(r) : 0;
+  const int64_t lo = nv * rank / size, hi = nv * (rank + 1) / size;
+  const int n = p.top_n;
+
+  if (tid == 0) {
+    s.count = 0u;
+    s.listed = 0;
+    s.border = 0ull;
+    s.ninf = 0u;
+  }
+
+  uint4 v[kUnroll];
+  uint32_t bits[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t i = lo + u * kThreads + tid;
+    bits[u] = i < hi ? legal_bits<T, kMask>(r, i) : 0u;
+    v[u] = i < hi ? ld_stream_v4(r.base + i) : make_uint4(0u, 0u, 0u, 0u);
+  }
+
+  // the CTA's first batch: everyone's first maximum, and the first border
+  float top = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    exclude<T>(v[u], bits[u]);
+    bits[u] = (1u << kPer) - 1u;
+    top = fmaxf(top, vector_top<T>(v[u]));
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
+  if ((lane & 7) == 0) s.group_top[tid >> 3] = top;
+  __syncthreads();
+  {
+    const float x0 = s.group_top[lane], x1 = s.group_top[lane + 32];
+    float m = fmaxf(x0, x1);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, o));
+    top = m;
+    if (kTop && warp == 0) {  // the n-th largest of the 64: at least n elements are no smaller
+      int above0 = 0, above1 = 0;
+      for (int j = 0; j < kThreads / 8; ++j) {
+        const float y = s.group_top[j];
+        above0 += y > x0 || (y == x0 && j < lane);
+        above1 += y > x1 || (y == x1 && j < lane + 32);
+      }
+      if (above0 == n - 1) s.border = x0 > -INFINITY ? (unsigned long long)ordered_bits(x0) << 32 : 0ull;
+      if (above1 == n - 1) s.border = x1 > -INFINITY ? (unsigned long long)ordered_bits(x1) << 32 : 0ull;
+    }
+  }
+  unsigned long long border = 0ull;
+  float least = INFINITY;
+  if constexpr (kTop) {
+    __syncthreads();
+    border = s.border;
+    least = border_value(border);
+  }
+  Running run{top, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+
+  const int limit = n + kListFull;
+  for (int64_t i0 = lo; i0 < hi; i0 += kUnroll * kThreads) {
+    uint32_t waiting = 0u;  // candidates that found no room, by vector and element
+    bool full = false;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = i0 + u * kThreads + tid, after = i + kUnroll * kThreads;
+      uint4 now = v[u];
+      exclude<T>(now, bits[u]);
+      bits[u] = after < hi ? legal_bits<T, kMask>(r, after) : 0u;
+      v[u] = after < hi ? ld_stream_v4(r.base + after) : make_uint4(0u, 0u, 0u, 0u);
+      const float vt = vector_top<T>(now);
+      if (vt >= (kTop ? fminf(least, run.m) : run.m)) {
+        if (vt > run.m) run.raise(vt, c);
+        if (kTop && vt >= least)
+          waiting |= list_candidates<T>(s, now, candidates<T>(now, least), i * kPer - r.phase, border, limit, full)
+                     << (u * kPer);
+      }
+      accumulate<T>(run, now, c);
+    }
+    if constexpr (kTop) {
+      while (__syncthreads_or(full)) {  // (what finds no room is full as well)
+        rank_list(s, n);
+        border = s.border;
+        least = border_value(border);
+        full = false;
+#pragma unroll 1
+        for (int u = 0; waiting != 0u && u < kUnroll; ++u) {
+          const uint32_t mine = (waiting >> (u * kPer)) & ((1u << kPer) - 1u);
+          if (!mine) continue;
+          const int64_t i = i0 + u * kThreads + tid;
+          const uint32_t left = list_candidates<T>(s, ld_stream_v4(r.base + i), mine, i * kPer - r.phase, border, limit, full);
+          waiting = (waiting & ~(mine << (u * kPer))) | (left << (u * kPer));
+        }
+      }
+    }
+  }
+
+  // this CTA's sums
+  Sums mine = merge(Sums{run.m, run.s.x, run.a.x}, Sums{run.m, run.s.y, run.a.y}, c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    mine = merge(mine, Sums{__shfl_xor_sync(FULL_MASK, mine.m, o), __shfl_xor_sync(FULL_MASK, mine.s, o),
+                            __shfl_xor_sync(FULL_MASK, mine.a, o)}, c);
+  if (lane == 0) s.part[warp] = mine;
+  if constexpr (kTop) rank_list(s, n);
+  else __syncthreads();
+  if (warp == 0) {
+    mine = s.part[lane & (kThreads / 32 - 1)];
+#pragma unroll
+    for (int o = kThreads / 64; o > 0; o >>= 1)
+      mine = merge(mine, Sums{__shfl_xor_sync(FULL_MASK, mine.m, o), __shfl_xor_sync(FULL_MASK, mine.s, o),
+                              __shfl_xor_sync(FULL_MASK, mine.a, o)}, c);
+    if (lane == 0) s.total = mine;
+  }
+  if (size > 1) cluster.sync();
+  else __syncthreads();
+
+  // the cluster's, the same in every thread (merged in rank order)
+  Sums sum = *cluster.map_shared_rank(&s.total, 0);
+  for (int q = 1; q < size; ++q) sum = merge(sum, *cluster.map_shared_rank(&s.total, q), c);
+  if (sum.m == INFINITY) {  // infinite logits share the weight: S counts them
+    unsigned int found = 0u;
+    for (int64_t i = lo + tid; i < hi; i += kThreads) {
+      uint4 x = ld_stream_v4(r.base + i);
+      exclude<T>(x, legal_bits<T, kMask>(r, i));
+#pragma unroll
+      for (int k = 0; k < kPer / 2; ++k) {
+        const float2 f = element_pair<T>(x, k);
+        found += (f.x == INFINITY) + (f.y == INFINITY);
+      }
+    }
+    if (found) atomicAdd(&s.ninf, found);
+    if (size > 1) cluster.sync();
+    else __syncthreads();
+    unsigned int all = 0u;
+    for (int q = 0; q < size; ++q) all += *cluster.map_shared_rank(&s.ninf, q);
+    sum.s = (float)all;
+    sum.a = 0.f;
+  }
+
+  if (rank == 0) {
+    const bool some = sum.m > -INFINITY;
+    const float nan = __int_as_float(0x7fc00000);
+    const float log_s = !valid ? nan : some ? logf(sum.s) : 0.f;
+    const float entropy = !valid ? nan : some ? fmaxf(log_s - kLn2 * (sum.a / sum.s), 0.f) : 0.f;
+    if (tid == 0) {
+      if (p.entropy) p.entropy[b] = entropy;
+      if (p.logsumexp) p.logsumexp[b] = !valid ? nan : some ? __fdiv_rn(sum.m, t) + log_s : -INFINITY;
+      if (p.stats) p.stats[b] = make_float4(sum.m, sum.s, entropy, valid ? fminf(__fdiv_rn(1.f, t), 3e38f) : nan);
+    }
+    for (int k = tid; k < p.tokens; k += kThreads) {
+      const int64_t id = p.token_ids[b * p.tokens + k];
+      int64_t at = id;
+      if (p.offsets && id >= 0) {  // its place among the row's rising ids
+        int64_t a = 0, z = r.len;
+        while (a < z) {
+          const int64_t mid = (a + z) >> 1;
+          if (p.ids[r.first + mid] < id) a = mid + 1;
+          else z = mid;
+        }
+        at = a < r.len && p.ids[r.first + a] == id ? a : r.len;
+      }
+      float lp = -INFINITY;
+      if (id >= 0 && at < r.len && (!kMask || ((__ldg(r.mask + (at >> 5)) >> (at & 31)) & 1u)))
+        lp = logprob_of(DTypeTraits<T>::bits_to_float(__ldg(static_cast<const Bits*>(p.logits) + r.first + at)), sum.m, t,
+                        log_s);
+      p.logprobs[b * p.tokens + k] = !valid ? nan : id < 0 ? 0.f : lp;
+    }
+    if constexpr (kTop) {
+      // the CTAs' lists, each in falling order: a key's place is the number of larger ones
+      const int all = size * n;
+      for (int i = tid; i < all; i += kThreads) {
+        const int q = i / n, at = i - q * n;
+        if (at >= *cluster.map_shared_rank(&s.listed, q)) continue;
+        const unsigned long long key = cluster.map_shared_rank(s.list, q)[at];
+        int place = at;
+        for (int o = 0; o < size && place < n; ++o) {
+          if (o == q) continue;
+          const unsigned long long* other = cluster.map_shared_rank(s.list, o);
+          int a = 0, z = *cluster.map_shared_rank(&s.listed, o);
+          while (a < z) {  // larger keys come first
+            const int mid = (a + z) >> 1;
+            if (other[mid] > key) a = mid + 1;
+            else z = mid;
+          }
+          place += a;
+        }
+        if (place >= n) continue;
+        const int64_t at_row = key_index(key);
+        p.top_ids[b * n + place] = p.offsets ? p.ids[r.first + at_row] : at_row;
+        p.top_logprobs[b * n + place] = logprob_of(key_value(key), sum.m, t, log_s);
+      }
+      int listed = 0;
+      for (int q = 0; q < size; ++q) listed += *cluster.map_shared_rank(&s.listed, q);
+      for (int i = min(listed, n) + tid; i < n; i += kThreads) {
+        p.top_ids[b * n + i] = -1;
+        p.top_logprobs[b * n + i] = valid ? -INFINITY : nan;
+      }
+    }
+  }
+  if (size > 1) cluster.sync();  // (shared memory is read until here)
+}
+
+template <typename T, bool kMask, bool kTop>
+cudaError_t launch_forward(const LogprobParams& p, int batch, int size, cudaStream_t stream) {
+  auto k = token_logprobs_kernel<T, kMask, kTop>;
+  if (size > 8) {
+    const cudaError_t err = cudaFuncSetAttribute(reinterpret_cast<const void*>(k),
+                                                 cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (err != cudaSuccess) return err;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)batch * (unsigned)size);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k, p);
+}
+
+template <typename T>
+cudaError_t launch_typed(const LogprobParams& p, int batch, int64_t max_len, cudaStream_t stream) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  // CTAs per row: while the device has room for twice as many (two per SM) and
+  // each keeps a whole batch of vectors.
+  const int64_t batch_elements = (int64_t)kThreads * kUnroll * DTypeTraits<T>::kPerVec;
+  int size = 1;
+  while (size < kMaxClusterSize && (int64_t)batch * size * 2 <= 2 * (int64_t)num_sms(dev) &&
+         max_len > batch_elements / 2 * size)
+    size *= 2;
+  if (p.mask) return p.top_n ? launch_forward<T, true, true>(p, batch, size, stream)
+                             : launch_forward<T, true, false>(p, batch, size, stream);
+  return p.top_n ? launch_forward<T, false, true>(p, batch, size, stream)
+                 : launch_forward<T, false, false>(p, batch, size, stream);
+}
+
+// ---- gradient -------------------------------------------------------------------
+// Reads the logits once more and writes the gradient once; a CTA takes a batch of
+// vectors of one row. A given token's own term is added by a second store of the
+// CTA that holds its element, after a barrier: the element is computed again from
+// its logit, with every term that names it, and rounded once.
+struct LogprobGradParams {
+  const void* logits;
+  int64_t row_stride;
+  const uint32_t* mask;
+  int64_t mask_stride;
+  int vocab;
+  const int64_t* token_ids;
+  int tokens;
+  const float4* stats;
+  const float* grad_logprobs;   // [batch, tokens] (optional)
+  const float* grad_entropy;    // [batch] (optional)
+  const float* grad_logsumexp;  // [batch] (optional)
+  void* grad;
+  int64_t grad_stride;
+  int slices;
+};
+
+constexpr int kGradThreads = 256;
+
+struct RowGrad {
+  float m, c, inv_s, base, slope;
+  bool inf, none;
+  // p (base - gH ln p), without the factor 1 / T: with d = (x - m) log2(e) / T,
+  // p = 2^d / S and ln p = d ln 2 - ln S, whose ln S is part of `base`
+  __device__ __forceinline__ float at(float x) const {
+    float d = inf ? (x == m ? 0.f : -INFINITY) : (x - m) * c;
+    d = fmaxf(d, kNothing);  // (NaN, -inf: p = 0)
+    return exp2_approx(d) * inv_s * fmaf(slope, d, base);
+  }
+};
+
+template <typename T, bool kMask>
+__global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const LogprobGradParams p) {
+  using Bits = typename DTypeTraits<T>::Bits;
+  constexpr int kPer = DTypeTraits<T>::kPerVec;
+  __shared__ float s_sum;
+  const int tid = threadIdx.x;
+  const int64_t b = blockIdx.x / p.slices;
+  const int slice = (int)(blockIdx.x - b * p.slices);
+  Row r;
+  set_row<T>(r, p.logits, b * p.row_stride, p.vocab);
+  r.mask = kMask ? p.mask + b * p.mask_stride : nullptr;
+  const int64_t nv = row_vectors<T>(r);
+  const int64_t i0 = (int64_t)slice * kGradThreads * kUnroll, hi = min(nv, i0 + kGradThreads * kUnroll);
+  uint4 v[kUnroll];
+  uint32_t bits[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t i = i0 + u * kGradThreads + tid;
+    bits[u] = i < hi ? legal_bits<T, kMask>(r, i) : 0u;
+    v[u] = i < hi ? ld_stream_v4(r.base + i) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  const float4 st = p.stats[b];
+  const int64_t* ids = p.token_ids + b * p.tokens;
+  const float* g = p.grad_logprobs ? p.grad_logprobs + b * p.tokens : nullptr;
+  if (tid < 32) {
+    float sum = 0.f;
+    if (g)
+      for (int k = tid; k < p.tokens; k += 32) sum += ids[k] >= 0 ? g[k] : 0.f;
+    sum = warp_sum(sum);
+    if (tid == 0) s_sum = sum;
+  }
+  __syncthreads();
+  RowGrad row;
+  row.m = st.x;
+  row.c = fminf(kLog2e * st.w, 3e38f);
+  row.inv_s = __fdiv_rn(1.f, st.y);
+  const float gh = p.grad_entropy ? p.grad_entropy[b] : 0.f;
+  row.base = (p.grad_logsumexp ? p.grad_logsumexp[b] : 0.f) - s_sum + gh * (logf(st.y) - st.z);
+  row.slope = -gh * kLn2;
+  row.inf = st.x == INFINITY;
+  row.none = !(st.x > -INFINITY);
+
+  Bits* out = static_cast<Bits*>(p.grad) + b * p.grad_stride;
+  // (element 0 of the gradient's row lies as far into a 16-byte vector as the logits')
+  const bool same_phase = (reinterpret_cast<uintptr_t>(out - r.phase) & 15) == 0;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t i = i0 + u * kGradThreads + tid;
+    if (i >= hi) continue;
+    uint4 x = v[u];
+    exclude<T>(x, bits[u]);
+    float y[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer / 2; ++k) {
+      const float2 f = element_pair<T>(x, k);
+      y[2 * k] = f.x > -INFINITY && !row.none ? row.at(f.x) * st.w : 0.f;
+      y[2 * k + 1] = f.y > -INFINITY && !row.none ? row.at(f.y) * st.w : 0.f;
+    }
+    const int64_t e0 = i * kPer - r.phase;
+    if (same_phase && e0 >= 0 && e0 + kPer <= r.len) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(Bits) == 2)
+          w[k] = (uint32_t)DTypeTraits<T>::round_bits(y[2 * k]) | ((uint32_t)DTypeTraits<T>::round_bits(y[2 * k + 1]) << 16);
+        else
+          w[k] = __float_as_uint(y[k]);
+      }
+      *reinterpret_cast<uint4*>(out + e0) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (e0 + j >= 0 && e0 + j < r.len) out[e0 + j] = DTypeTraits<T>::round_bits(y[j]);
+    }
+  }
+  if (!g || row.none) return;
+  __syncthreads();  // the stores above come before those below
+  const int64_t first = i0 * kPer - r.phase, last = hi * kPer - r.phase;
+  for (int k = tid; k < p.tokens; k += kGradThreads) {
+    const int64_t id = ids[k];
+    if (id < 0 || id < first || id >= last || id >= r.len) continue;
+    if (kMask && !((__ldg(r.mask + (id >> 5)) >> (id & 31)) & 1u)) continue;
+    const float x = DTypeTraits<T>::bits_to_float(__ldg(static_cast<const Bits*>(p.logits) + r.first + id));
+    if (!(x > -INFINITY)) continue;
+    bool earlier = false;
+    for (int j = 0; j < k && !earlier; ++j) earlier = ids[j] == id;
+    if (earlier) continue;
+    float own = 0.f;
+    for (int j = k; j < p.tokens; ++j)
+      if (ids[j] == id) own += g[j];
+    out[id] = DTypeTraits<T>::round_bits((row.at(x) + own) * st.w);
+  }
+}
+
+template <typename T>
+cudaError_t launch_grad(LogprobGradParams p, int batch, cudaStream_t stream) {
+  // (one vector more than the length needs, for rows that start inside one)
+  const int64_t per_cta = (int64_t)kGradThreads * kUnroll;
+  const int64_t vectors = ((int64_t)p.vocab + DTypeTraits<T>::kPerVec - 1) / DTypeTraits<T>::kPerVec + 1;
+  const int64_t slices = (vectors + per_cta - 1) / per_cta, grid = slices * batch;
+  if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  p.slices = (int)slices;
+  if (p.mask) token_logprobs_grad_kernel<T, true><<<(unsigned)grid, kGradThreads, 0, stream>>>(p);
+  else token_logprobs_grad_kernel<T, false><<<(unsigned)grid, kGradThreads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+int32_t check(const char* fn, int32_t dtype, int32_t batch, const int64_t* token_ids, int32_t tokens) {
+  if (dtype != GSP_DTYPE_F16 && dtype != GSP_DTYPE_BF16 && dtype != GSP_DTYPE_F32)
+    return record_error(GSP_ERR_UNSUPPORTED, "%s: dtype must be GSP_DTYPE_F16, GSP_DTYPE_BF16 or GSP_DTYPE_F32", fn);
+  if (batch < 1 || batch > (1 << 26)) return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: batch must be in 1..2^26", fn);
+  if (tokens < 0 || tokens > kMaxTokens)
+    return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: tokens must be in 0..%d", fn, kMaxTokens);
+  if (tokens > 0 && !token_ids) return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: token_ids is required", fn);
+  return GSP_OK;
+}
+
+int32_t check_rows(const char* fn, const void* logits, int64_t row_stride, const int32_t* bitmask,
+                   int64_t bitmask_row_stride, int32_t batch, int32_t vocab) {
+  if (!logits) return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: logits is required", fn);
+  if (vocab < 1) return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: vocab must be positive", fn);
+  if (vocab > (1 << 30)) return record_error(GSP_ERR_UNSUPPORTED, "%s: vocab above 2^30", fn);
+  if (row_stride < 0) return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: negative logits_row_stride", fn);
+  const int64_t nw = ((int64_t)vocab + 31) / 32;
+  if (bitmask && (bitmask_row_stride < 0 || (batch > 1 && bitmask_row_stride != 0 && bitmask_row_stride < nw)))
+    return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: bitmask_row_stride must be 0 or >= ceil(vocab/32)", fn);
+  return GSP_OK;
+}
+
+int32_t forward(const char* fn, const LogprobParams& p, int32_t dtype, int32_t batch, int64_t max_len, void* stream) {
+  if (!p.temperatures && !(p.temperature > 0.f && p.temperature < INFINITY))
+    return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: temperature must be positive and finite", fn);
+  if (p.top_n < 0 || p.top_n > kMaxTop)
+    return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: top_n must be in 0..%d", fn, kMaxTop);
+  if (p.tokens > 0 && !p.logprobs) return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: logprobs is required", fn);
+  if (p.top_n > 0 && (!p.top_ids || !p.top_logprobs))
+    return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: top_ids and top_logprobs are required", fn);
+  if (reinterpret_cast<uintptr_t>(p.stats) & 15)
+    return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: stats must be 16-byte aligned", fn);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t err = dtype == GSP_DTYPE_F32    ? launch_typed<float>(p, batch, max_len, s)
+                          : dtype == GSP_DTYPE_BF16 ? launch_typed<__nv_bfloat16>(p, batch, max_len, s)
+                                                    : launch_typed<__half>(p, batch, max_len, s);
+  if (err == cudaSuccess) return GSP_OK;
+  return record_error(GSP_ERR_CUDA, "%s: %s (%s)", fn, cudaGetErrorName(err), cudaGetErrorString(err));
+}
+
+}  // namespace
+}  // namespace gsp
+
+using namespace gsp;
+
+extern "C" {
+
+int32_t gsp_token_logprobs(const void* logits, int64_t logits_row_stride, int32_t dtype, const int32_t* bitmask,
+                           int64_t bitmask_row_stride, int32_t batch, int32_t vocab, float temperature,
+                           const float* temperatures, const int64_t* token_ids, int32_t tokens, int32_t top_n,
+                           float* logprobs, float* entropy, float* logsumexp, int64_t* top_ids, float* top_logprobs,
+                           float* stats, void* stream) {
+  const char* fn = "gsp_token_logprobs";
+  int32_t st = check(fn, dtype, batch, token_ids, tokens);
+  if (st == GSP_OK) st = check_rows(fn, logits, logits_row_stride, bitmask, bitmask_row_stride, batch, vocab);
+  if (st != GSP_OK) return st;
+  LogprobParams p{};
+  p.logits = logits;
+  p.row_stride = batch > 1 ? logits_row_stride : 0;
+  p.mask = reinterpret_cast<const uint32_t*>(bitmask);
+  p.mask_stride = batch > 1 ? bitmask_row_stride : 0;
+  p.vocab = vocab;
+  p.temperature = temperature;
+  p.temperatures = temperatures;
+  p.token_ids = token_ids;
+  p.tokens = tokens;
+  p.top_n = top_n;
+  p.logprobs = logprobs;
+  p.entropy = entropy;
+  p.logsumexp = logsumexp;
+  p.top_ids = top_ids;
+  p.top_logprobs = top_logprobs;
+  p.stats = reinterpret_cast<float4*>(stats);
+  return forward(fn, p, dtype, batch, vocab, stream);
+}
+
+int32_t gsp_token_logprobs_compact(const void* compact_logits, const int64_t* compact_ids,
+                                   const int64_t* request_offsets, int64_t capacity, int32_t max_len, int32_t dtype,
+                                   int32_t batch, float temperature, const float* temperatures,
+                                   const int64_t* token_ids, int32_t tokens, int32_t top_n, float* logprobs,
+                                   float* entropy, float* logsumexp, int64_t* top_ids, float* top_logprobs,
+                                   void* stream) {
+  const char* fn = "gsp_token_logprobs_compact";
+  const int32_t st = check(fn, dtype, batch, token_ids, tokens);
+  if (st != GSP_OK) return st;
+  if (capacity < 0 || max_len < 0)
+    return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: capacity and max_len must not be negative", fn);
+  if (!request_offsets) return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: request_offsets is required", fn);
+  if (capacity > 0 && (!compact_logits || !compact_ids))
+    return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: compact_logits and compact_ids are required", fn);
+  LogprobParams p{};
+  p.logits = compact_logits;
+  p.ids = compact_ids;
+  p.offsets = request_offsets;
+  p.capacity = capacity;
+  p.temperature = temperature;
+  p.temperatures = temperatures;
+  p.token_ids = token_ids;
+  p.tokens = tokens;
+  p.top_n = top_n;
+  p.logprobs = logprobs;
+  p.entropy = entropy;
+  p.logsumexp = logsumexp;
+  p.top_ids = top_ids;
+  p.top_logprobs = top_logprobs;
+  return forward(fn, p, dtype, batch, max_len, stream);
+}
+
+int32_t gsp_token_logprobs_grad(const void* logits, int64_t logits_row_stride, int32_t dtype, const int32_t* bitmask,
+                                int64_t bitmask_row_stride, int32_t batch, int32_t vocab, const int64_t* token_ids,
+                                int32_t tokens, const float* stats, const float* grad_logprobs,
+                                const float* grad_entropy, const float* grad_logsumexp, void* grad_logits,
+                                int64_t grad_row_stride, void* stream) {
+  const char* fn = "gsp_token_logprobs_grad";
+  int32_t st = check(fn, dtype, batch, token_ids, tokens);
+  if (st == GSP_OK) st = check_rows(fn, logits, logits_row_stride, bitmask, bitmask_row_stride, batch, vocab);
+  if (st != GSP_OK) return st;
+  if (!stats || !grad_logits)
+    return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: stats and grad_logits are required", fn);
+  if (reinterpret_cast<uintptr_t>(stats) & 15)
+    return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: stats must be 16-byte aligned", fn);
+  if (batch > 1 && grad_row_stride < vocab)
+    return record_error(GSP_ERR_INVALID_ARGUMENT, "%s: grad_row_stride < vocab", fn);
+  LogprobGradParams p{};
+  p.logits = logits;
+  p.row_stride = batch > 1 ? logits_row_stride : 0;
+  p.mask = reinterpret_cast<const uint32_t*>(bitmask);
+  p.mask_stride = batch > 1 ? bitmask_row_stride : 0;
+  p.vocab = vocab;
+  p.token_ids = token_ids;
+  p.tokens = tokens;
+  p.stats = reinterpret_cast<const float4*>(stats);
+  p.grad_logprobs = tokens > 0 ? grad_logprobs : nullptr;
+  p.grad_entropy = grad_entropy;
+  p.grad_logsumexp = grad_logsumexp;
+  p.grad = grad_logits;
+  p.grad_stride = batch > 1 ? grad_row_stride : 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t err = dtype == GSP_DTYPE_F32    ? launch_grad<float>(p, batch, s)
+                          : dtype == GSP_DTYPE_BF16 ? launch_grad<__nv_bfloat16>(p, batch, s)
+                                                    : launch_grad<__half>(p, batch, s);
+  if (err == cudaSuccess) return GSP_OK;
+  return record_error(GSP_ERR_CUDA, "%s: %s (%s)", fn, cudaGetErrorName(err), cudaGetErrorString(err));
+}
+
+}  // extern "C"

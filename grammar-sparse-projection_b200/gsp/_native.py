@@ -109,6 +109,11 @@ SIGNATURES = {
     "gsp_int8_error": ([ctypes.POINTER(_i32), ctypes.POINTER(_i32), _vp], _i32),
     "gsp_sample_logits": ([_vp, _i64, _i32, _vp, _i64, _i32, _i32, _i64] + _FILTER_ARGS, _i32),
     "gsp_sample_compact": ([_vp, _vp, _vp, _i64, _i32, _i32, _i32] + _FILTER_ARGS, _i32),
+    "gsp_token_logprobs": ([_vp, _i64, _i32, _vp, _i64, _i32, _i32, _f32, _vp, _vp, _i32, _i32] + [_vp] * 7, _i32),
+    "gsp_token_logprobs_compact": ([_vp, _vp, _vp, _i64, _i32, _i32, _i32, _f32, _vp, _vp, _i32, _i32] + [_vp] * 6,
+                                   _i32),
+    "gsp_token_logprobs_grad": ([_vp, _i64, _i32, _vp, _i64, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64,
+                                 _vp], _i32),
 }
 
 ROUTE_CODES = {"row-sparse": 0, "block-sparse": 1, "dense-mask": 2}
@@ -818,6 +823,52 @@ def sample_compact(logits, ids, offsets, max_len: int, settings, uniforms, token
             uniforms.numel(), *_filter_args(settings, uniforms, token_ids, logprobs, kept), raw_stream(index))
     if status:
         _check(status, "gsp_sample_compact")
+
+
+def _temperature_args(temperature):
+    return (1.0, temperature.data_ptr()) if isinstance(temperature, torch.Tensor) else (temperature, None)
+
+
+def token_logprobs(logits, mask, temperature, token_ids, tokens: int, top_n: int, logprobs, entropy, logsumexp, top_ids,
+                   top_logprobs, stats=None) -> None:
+    """gsp_token_logprobs; logits [B, V] (row stride free), token_ids contiguous with `tokens` per row."""
+    index = logits.get_device()
+    with on_device(index):
+        status = load().gsp_token_logprobs(
+            logits.data_ptr(), logits.stride(0), DTYPE_CODES[logits.dtype], _address(mask),
+            0 if mask is None else mask.stride(0), logits.shape[0], logits.shape[1], *_temperature_args(temperature),
+            token_ids.data_ptr(), tokens, top_n, logprobs.data_ptr(), entropy.data_ptr(), logsumexp.data_ptr(),
+            top_ids.data_ptr(), top_logprobs.data_ptr(), _address(stats), raw_stream(index))
+    if status:
+        _check(status, "gsp_token_logprobs")
+
+
+def token_logprobs_compact(logits, ids, offsets, max_len: int, temperature, token_ids, tokens: int, top_n: int,
+                           logprobs, entropy, logsumexp, top_ids, top_logprobs) -> None:
+    """gsp_token_logprobs_compact; logits [N] and ids [N] packed by offsets [B + 1]."""
+    index = logits.get_device()
+    with on_device(index):
+        status = load().gsp_token_logprobs_compact(
+            logits.data_ptr(), ids.data_ptr(), offsets.data_ptr(), logits.numel(), max_len, DTYPE_CODES[logits.dtype],
+            offsets.shape[0] - 1, *_temperature_args(temperature), token_ids.data_ptr(), tokens, top_n,
+            logprobs.data_ptr(), entropy.data_ptr(), logsumexp.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr(),
+            raw_stream(index))
+    if status:
+        _check(status, "gsp_token_logprobs_compact")
+
+
+def token_logprobs_grad(logits, mask, token_ids, tokens: int, stats, grad_logprobs, grad_entropy, grad_logsumexp,
+                        grad) -> None:
+    """gsp_token_logprobs_grad into grad [B, V]."""
+    index = logits.get_device()
+    with on_device(index):
+        status = load().gsp_token_logprobs_grad(
+            logits.data_ptr(), logits.stride(0), DTYPE_CODES[logits.dtype], _address(mask),
+            0 if mask is None else mask.stride(0), logits.shape[0], logits.shape[1], token_ids.data_ptr(), tokens,
+            stats.data_ptr(), _address(grad_logprobs), _address(grad_entropy), _address(grad_logsumexp),
+            grad.data_ptr(), grad.stride(0), raw_stream(index))
+    if status:
+        _check(status, "gsp_token_logprobs_grad")
 
 
 def copy_bytes(dst: torch.Tensor, src: torch.Tensor, nbytes: int | None = None) -> None:

@@ -597,6 +597,50 @@ int32_t gsp_sample_compact(const void* compact_logits, const int64_t* compact_id
                            const float* top_ps, float min_p, const float* min_ps, const float* uniforms,
                            int64_t* token_ids, float* logprobs, int32_t* kept, void* stream);
 
+/* ---- log probabilities of given tokens -------------------------------------------
+ * From logits that a route of the head wrote (-inf on illegal tokens), or any logits
+ * with the packed bitmask (NULL: none), over the legal tokens (bit set, not NaN, not
+ * -inf) of each request, with x the logits, T the temperature, m = max x and
+ * S = sum exp((x - m) / T):
+ *   logprobs [batch, tokens]: (x_t - m) / T - ln S of the given token_ids
+ *     [batch, tokens] (at most 1,024 each); -inf for one that is not legal or not
+ *     below the vocabulary; a negative id stands for none and reports 0;
+ *   entropy [batch]: of the distribution; logsumexp [batch]: m / T + ln S;
+ *   top_ids, top_logprobs [batch, top_n] (top_n <= 64): the alternatives by falling
+ *     logit, ties by rising id; where fewer are legal, id -1 and -inf;
+ *   stats [batch, 4] (16-byte aligned): what gsp_token_logprobs_grad needs.
+ * Outputs but logprobs (tokens > 0) and the alternatives (top_n > 0) may be NULL.
+ * Sums are fp32. A request without a legal token reports -inf, entropy 0; infinite
+ * logits share the weight among themselves. temperatures (optional): one device
+ * value per request; a request whose value is not positive and finite reports NaN
+ * and ids -1. Row strides may be 0 (one row for all). No workspace.
+ * gsp_token_logprobs_compact: rows packed as for gsp_sample_compact, ids rising in a
+ * row. No counterpart in the reference, whose loop takes the argmax alone
+ * (benchmarks/qwen35_adaptive_paired.py:94). */
+int32_t gsp_token_logprobs(const void* logits, int64_t logits_row_stride, int32_t dtype, const int32_t* bitmask,
+                           int64_t bitmask_row_stride, int32_t batch, int32_t vocab, float temperature,
+                           const float* temperatures, const int64_t* token_ids, int32_t tokens, int32_t top_n,
+                           float* logprobs, float* entropy, float* logsumexp, int64_t* top_ids, float* top_logprobs,
+                           float* stats, void* stream);
+int32_t gsp_token_logprobs_compact(const void* compact_logits, const int64_t* compact_ids,
+                                   const int64_t* request_offsets, int64_t capacity, int32_t max_len, int32_t dtype,
+                                   int32_t batch, float temperature, const float* temperatures,
+                                   const int64_t* token_ids, int32_t tokens, int32_t top_n, float* logprobs,
+                                   float* entropy, float* logsumexp, int64_t* top_ids, float* top_logprobs,
+                                   void* stream);
+
+/* The gradient of the logits from those of logprobs, entropy and logsumexp (each
+ * optional, fp32), with the logits, bitmask and token_ids of the forward call and
+ * its stats; p_j the probability of token j:
+ *   dx_j = (p_j (gL - sum_k g_k - gH (ln p_j + entropy)) + sum_k g_k [j = t_k]) / T
+ * for legal j, 0 elsewhere and in rows without a legal token; negative ids take no
+ * part, a token named twice counts twice. Rounded once to dtype. Deterministic. */
+int32_t gsp_token_logprobs_grad(const void* logits, int64_t logits_row_stride, int32_t dtype, const int32_t* bitmask,
+                                int64_t bitmask_row_stride, int32_t batch, int32_t vocab, const int64_t* token_ids,
+                                int32_t tokens, const float* stats, const float* grad_logprobs,
+                                const float* grad_entropy, const float* grad_logsumexp, void* grad_logits,
+                                int64_t grad_row_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

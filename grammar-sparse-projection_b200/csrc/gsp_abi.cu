@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "../../include/gsp_b200.h"
+#include "fp8_head.cuh"
 #include "gsp_internal.h"
 
 namespace gsp {
@@ -1118,6 +1119,117 @@ int32_t gsp_int8_error(int32_t* error, const int32_t* set_to, void* stream) {
     if (err == cudaSuccess) err = cudaStreamSynchronize(s);
   }
   return cuda_status(err, fn);
+}
+
+// ---- fp8 head ---------------------------------------------------------------
+namespace {
+
+constexpr int32_t kMaxFp8Hidden = 32768;  // the row-sparse kernel keeps a hidden state in shared memory, in fp32
+
+struct Fp8Scratch {
+  size_t keys, tickets, values, scales_t, groups, counts, bits, total;
+  Fp8Scratch(int32_t batch, int32_t vocab, int32_t hidden_dim) {
+    const size_t b = (size_t)batch, nw = ((size_t)vocab + 31) / 32, blocks = ((size_t)hidden_dim + kBlock - 1) / kBlock;
+    const size_t builders = (nw + kListGroups - 1) / kListGroups;
+    keys = 0;
+    tickets = align256(8 * b);
+    values = tickets + align256(4 * b);
+    scales_t = values + align256(b * int8_row_bytes(hidden_dim));
+    groups = scales_t + align256(4 * b * blocks);
+    counts = groups + align256(4 * builders * kListGroups);
+    bits = counts + align256(4 * builders);
+    total = bits + align256(4 * ((nw + 31) / 32));
+  }
+};
+
+}  // namespace
+
+size_t gsp_fp8_scratch_bytes(int32_t batch, int32_t vocab, int32_t hidden_dim) {
+  if (batch < 1 || vocab < 1 || hidden_dim < 1) return 0;
+  return Fp8Scratch(batch, vocab, hidden_dim).total;
+}
+
+int32_t gsp_fp8_logits(int32_t route, const void* hidden, int64_t hidden_row_stride, int32_t hidden_dtype,
+                       const float* hidden_scales, int64_t hidden_scales_row_stride, const uint8_t* weight,
+                       int64_t weight_row_stride, const float* weight_scales, int64_t weight_scales_row_stride,
+                       const int32_t* bitmask, int64_t bitmask_row_stride, int32_t batch, int32_t vocab,
+                       int32_t hidden_dim, int32_t out_dtype, int64_t vocab_offset, void* logits,
+                       int64_t logits_row_stride, float* top_value, int64_t* top_index, int64_t* top_key,
+                       void* scratch, size_t scratch_bytes, void* stream) {
+  const char* fn = "gsp_fp8_logits";
+  if (route < GSP_ROUTE_ROW_SPARSE || route > GSP_ROUTE_DENSE_MASK)
+    return fail(GSP_ERR_INVALID_ARGUMENT, "%s: unknown route %d", fn, route);
+  const int32_t st = validate_projection(fn, hidden, hidden_row_stride, weight, weight_row_stride, bitmask,
+                                         bitmask_row_stride, batch, vocab, hidden_dim, out_dtype, logits,
+                                         logits_row_stride);
+  if (st != GSP_OK) return st;
+  if (hidden_dim > kMaxFp8Hidden)
+    return fail(GSP_ERR_UNSUPPORTED, "%s: hidden_dim above %d", fn, kMaxFp8Hidden);
+  const int blocks = (hidden_dim + kBlock - 1) / kBlock;
+  if (!weight_scales) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: weight_scales is required", fn);
+  if (vocab > kBlock && weight_scales_row_stride < blocks)
+    return fail(GSP_ERR_INVALID_ARGUMENT, "%s: weight_scales_row_stride < ceil(hidden_dim / 128)", fn);
+  const bool quantised = hidden_dtype == GSP_DTYPE_E4M3;
+  if (quantised) {
+    if (!hidden_scales) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: e4m3 hidden states need hidden_scales", fn);
+    if (batch > 1 && hidden_scales_row_stride < blocks)
+      return fail(GSP_ERR_INVALID_ARGUMENT, "%s: hidden_scales_row_stride < ceil(hidden_dim / 128)", fn);
+  } else if (hidden_dtype != GSP_DTYPE_F16 && hidden_dtype != GSP_DTYPE_BF16 && hidden_dtype != GSP_DTYPE_F32) {
+    return fail(GSP_ERR_UNSUPPORTED, "%s: unknown hidden_dtype %d", fn, hidden_dtype);
+  }
+  if (!logits && !top_value && !top_index && !top_key)
+    return fail(GSP_ERR_INVALID_ARGUMENT, "%s: no output is asked for", fn);
+  const Fp8Scratch room(batch, vocab, hidden_dim);
+  if (!scratch || scratch_bytes < room.total)
+    return fail(GSP_ERR_WORKSPACE, "%s: scratch has %zu bytes, needs %zu", fn, scratch ? scratch_bytes : (size_t)0,
+                room.total);
+  if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0)
+    return fail(GSP_ERR_WORKSPACE, "%s: scratch must be 16-byte aligned", fn);
+  int* device_error = nullptr;
+  if (const cudaError_t err = int8_error_word(&device_error); err != cudaSuccess) return cuda_status(err, fn);
+  char* at = static_cast<char*>(scratch);
+  Fp8Params p;
+  std::memset(&p, 0, sizeof(p));
+  if (quantised) {
+    p.hidden = static_cast<const uint8_t*>(hidden);
+    p.hidden_stride = batch > 1 ? hidden_row_stride : (int64_t)int8_row_bytes(hidden_dim);
+    p.hidden_scales = hidden_scales;
+    p.hidden_scales_stride = batch > 1 ? hidden_scales_row_stride : 0;
+  } else {
+    p.raw = hidden;
+    p.raw_stride = batch > 1 ? hidden_row_stride : 0;
+    p.raw_dtype = hidden_dtype;
+    p.hidden = reinterpret_cast<const uint8_t*>(at + room.values);
+    p.hidden_stride = (int64_t)int8_row_bytes(hidden_dim);
+  }
+  p.weight = weight;
+  p.weight_stride = vocab > 1 ? weight_row_stride : (int64_t)int8_row_bytes(hidden_dim);
+  p.weight_scales = weight_scales;
+  p.weight_scales_stride = vocab > kBlock ? weight_scales_row_stride : 0;
+  p.mask = reinterpret_cast<const uint32_t*>(bitmask);
+  p.mask_stride = batch > 1 ? bitmask_row_stride : 0;
+  p.batch = batch;
+  p.vocab = vocab;
+  p.hidden_dim = hidden_dim;
+  p.nw = (vocab + 31) / 32;
+  p.blocks = blocks;
+  p.vocab_offset = vocab_offset;
+  p.logits = logits;
+  p.logits_stride = batch > 1 ? logits_row_stride : vocab;
+  p.top_value = top_value;
+  p.top_index = top_index;
+  p.top_key = top_key;
+  p.keys = reinterpret_cast<unsigned long long*>(at + room.keys);
+  p.tickets = reinterpret_cast<unsigned int*>(at + room.tickets);
+  p.scales_t = reinterpret_cast<float*>(at + room.scales_t);
+  p.groups = reinterpret_cast<int32_t*>(at + room.groups);
+  p.group_counts = reinterpret_cast<int32_t*>(at + room.counts);
+  p.group_bits = reinterpret_cast<uint32_t*>(at + room.bits);
+  p.device_error = device_error;
+  p.dense = route == GSP_ROUTE_DENSE_MASK || bitmask == nullptr;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (route == GSP_ROUTE_ROW_SPARSE) return cuda_status(launch_fp8_row_sparse(p, out_dtype, s), fn);
+  return cuda_status(launch_fp8_tensor(p, out_dtype, s), fn);
 }
 
 // ---- sampling from logits -----------------------------------------------------

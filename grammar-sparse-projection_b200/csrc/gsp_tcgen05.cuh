@@ -55,6 +55,18 @@ __device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t a_desc, uint
       : "memory");
 }
 
+// The same with kind::f8f6f4: e4m3 operands, fp32 accumulation; 32 elements (32
+// bytes) of K per instruction.
+__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrives once on `bar` when every tcgen05 operation this thread issued so far
 // has completed.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
@@ -78,6 +90,14 @@ __host__ __device__ constexpr uint32_t tc_idesc_i8(uint32_t n) {
   return (2u << 4) |         // D format: S32
          (1u << 7) |         // A format: signed 8-bit
          (1u << 10) |        // B format: signed 8-bit
+         ((n >> 3) << 17) |  // N >> 3
+         ((128u >> 4) << 24);  // M >> 4
+}
+
+// Instruction descriptor of kind::f8f6f4 with fp32 accumulation, both operands
+// e4m3 (format code 0) and K-major, M = 128 (N a multiple of 16).
+__host__ __device__ constexpr uint32_t tc_idesc_e4m3(uint32_t n) {
+  return (1u << 4) |         // D format: F32
          ((n >> 3) << 17) |  // N >> 3
          ((128u >> 4) << 24);  // M >> 4
 }

@@ -109,6 +109,13 @@ SIGNATURES = {
     "gsp_int8_error": ([ctypes.POINTER(_i32), ctypes.POINTER(_i32), _vp], _i32),
     "gsp_sample_logits": ([_vp, _i64, _i32, _vp, _i64, _i32, _i32, _i64] + _FILTER_ARGS, _i32),
     "gsp_sample_compact": ([_vp, _vp, _vp, _i64, _i32, _i32, _i32] + _FILTER_ARGS, _i32),
+    "gsp_rms_norm": ([_vp, _i64, _vp, _i64, _vp, _i64, _i32, _f32, _i32, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp],
+                     _i32),
+    "gsp_quantize_rows_fp8": ([_vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp, _i64, _vp], _i32),
+    "gsp_quantize_weight_fp8": ([_vp, _i64, _i64, _i32, _i32, _vp, _i64, _vp, _i64, _vp], _i32),
+    "gsp_fp8_scratch_bytes": ([_i32, _i32, _i32], _sz),
+    "gsp_fp8_logits": ([_i32, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _i64,
+                        _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp], _i32),
     "gsp_token_logprobs": ([_vp, _i64, _i32, _vp, _i64, _i32, _i32, _f32, _vp, _vp, _i32, _i32] + [_vp] * 7, _i32),
     "gsp_token_logprobs_compact": ([_vp, _vp, _vp, _i64, _i32, _i32, _i32, _f32, _vp, _vp, _i32, _i32] + [_vp] * 6,
                                    _i32),
@@ -210,8 +217,8 @@ def reset_workspace(device: torch.device) -> None:
 
 
 def workspace_error(device: torch.device) -> int:
-    """Error word of the current stream's workspace, or of the device's int8
-    calls, captured or on whatever stream and thread, since the last
+    """Error word of the current stream's workspace, or of the device's int8 and
+    fp8 calls, captured or on whatever stream and thread, since the last
     reset_workspace: non-zero after a kernel gave up a bounded wait (reads the
     device, so it synchronises the current stream; int8 calls on other streams
     must have ended to be seen)."""
@@ -823,6 +830,65 @@ def sample_compact(logits, ids, offsets, max_len: int, settings, uniforms, token
             uniforms.numel(), *_filter_args(settings, uniforms, token_ids, logprobs, kept), raw_stream(index))
     if status:
         _check(status, "gsp_sample_compact")
+
+
+# ---------------------------------------------------------------------------
+# norm and fp8 head
+# ---------------------------------------------------------------------------
+DTYPE_E4M3 = 4
+
+
+def rms_norm(x, weight, residual, eps: float, residual_out, out, scales, out_code: int | None) -> None:
+    """gsp_rms_norm on rows x [N, H]; out_code None: the output has x's type."""
+    index = x.get_device()
+    code = DTYPE_CODES[x.dtype]
+    with on_device(index):
+        status = load().gsp_rms_norm(
+            x.data_ptr(), x.stride(0), _address(residual), 0 if residual is None else residual.stride(0),
+            _address(weight), x.shape[0], x.shape[1], eps, code, _address(residual_out),
+            0 if residual_out is None else residual_out.stride(0), code if out_code is None else out_code,
+            out.data_ptr(), out.stride(0), _address(scales),
+            0 if scales is None or scales.dim() == 1 else scales.stride(0), raw_stream(index))
+    if status:
+        _check(status, "gsp_rms_norm")
+
+
+def quantize_fp8(entry: str, x, values, scales) -> None:
+    """gsp_quantize_rows_fp8 / gsp_quantize_weight_fp8: x [N, H] -> values e4m3 [N, H], scales float32."""
+    index = x.get_device()
+    with on_device(index):
+        status = getattr(load(), entry)(x.data_ptr(), x.stride(0), x.shape[0], x.shape[1], DTYPE_CODES[x.dtype],
+                                        values.data_ptr(), values.stride(0), scales.data_ptr(), scales.stride(0),
+                                        raw_stream(index))
+    if status:
+        _check(status, entry)
+
+
+@functools.lru_cache(maxsize=1024)
+def _fp8_scratch_bytes(batch: int, vocab: int, hidden_dim: int) -> int:
+    return int(load().gsp_fp8_scratch_bytes(batch, vocab, hidden_dim))
+
+
+def fp8_logits(route: str, hidden, hidden_scales, weight, weight_scales, mask, out_dtype, logits=None, top_value=None,
+               top_index=None, top_key=None, vocab_offset: int = 0) -> None:
+    """gsp_fp8_logits; hidden_scales None: `hidden` is floating point and quantised by the call. The scratch is
+    the call's own (torch's allocator keeps it in stream order, and a captured call's in its graph's pool)."""
+    index = hidden.get_device()
+    batch, hidden_dim = hidden.shape
+    vocab = weight.shape[0]
+    with on_device(index):
+        need = _fp8_scratch_bytes(batch, vocab, hidden_dim)
+        scratch = torch.empty(need, dtype=torch.uint8, device=hidden.device)
+        status = load().gsp_fp8_logits(
+            ROUTE_CODES[route], hidden.data_ptr(), hidden.stride(0),
+            DTYPE_CODES[hidden.dtype] if hidden_scales is None else DTYPE_E4M3, _address(hidden_scales),
+            0 if hidden_scales is None else hidden_scales.stride(0), weight.data_ptr(), weight.stride(0),
+            weight_scales.data_ptr(), weight_scales.stride(0), _address(mask), 0 if mask is None else mask.stride(0),
+            batch, vocab, hidden_dim, DTYPE_CODES[out_dtype], vocab_offset, _address(logits),
+            0 if logits is None else logits.stride(0), _address(top_value), _address(top_index), _address(top_key),
+            scratch.data_ptr(), need, raw_stream(index))
+    if status:
+        _check(status, "gsp_fp8_logits")
 
 
 def _temperature_args(temperature):

@@ -67,7 +67,8 @@ extern "C" {
 #define GSP_DTYPE_F16 0
 #define GSP_DTYPE_BF16 1
 #define GSP_DTYPE_F32 2
-#define GSP_DTYPE_I8 3 /* hidden_dtype of the gsp_int8_* entries only */
+#define GSP_DTYPE_I8 3   /* hidden_dtype of the gsp_int8_* entries, out_dtype of gsp_rms_norm */
+#define GSP_DTYPE_E4M3 4 /* hidden_dtype of gsp_fp8_logits, out_dtype of gsp_rms_norm */
 /* Added to the dtype of rows that a gsp_quantize_rows_int8 / gsp_int8_* call
  * quantises: how their scale is taken. */
 #define GSP_SCALE_RECIPROCAL 0x100
@@ -551,9 +552,9 @@ int32_t gsp_int8_compact(const void* hidden, int64_t hidden_row_stride, int32_t 
                          float* top_value, int64_t* top_index, int64_t* top_key, void* scratch, size_t scratch_bytes,
                          void* workspace, size_t workspace_bytes, void* stream);
 
-/* Reads the current device's error word of the gsp_int8_* calls: every such call,
- * on any stream, host thread or workspace, captured ones included, records there
- * the code that it leaves in its workspace's error word. set_to not NULL: the word
+/* Reads the current device's error word of the gsp_int8_* and gsp_fp8_* calls: every
+ * such call, on any stream, host thread or workspace, captured ones included, records
+ * there the code that it leaves in its workspace's error word (gsp_fp8_*: there alone). set_to not NULL: the word
  * is *set_to afterwards (0 clears it; nothing else does). After a non-zero word
  * each workspace that the failed call may have used is re-zeroed before its next
  * call. Synchronises `stream`; calls on other streams that are to be seen must have
@@ -640,6 +641,67 @@ int32_t gsp_token_logprobs_grad(const void* logits, int64_t logits_row_stride, i
                                 int32_t tokens, const float* stats, const float* grad_logprobs,
                                 const float* grad_entropy, const float* grad_logsumexp, void* grad_logits,
                                 int64_t grad_row_stride, void* stream);
+
+/* ---- root-mean-square norm ---------------------------------------------------------
+ * The step before the head, rows of dtype (fp16, bf16 or fp32), in one pass:
+ *   h = x + residual, rounded to dtype, to residual_out (both or neither given);
+ *   y = h * (1 / sqrt(mean(h^2) + eps)) * weight in fp32 (weight [cols] of dtype,
+ *   NULL: 1), to out by out_dtype:
+ *     dtype           y rounded;
+ *     GSP_DTYPE_I8    int8 values and one scale per row by gsp_quantize_rows_int8's
+ *                     rule (scales [rows]): hidden of gsp_int8_logits;
+ *     GSP_DTYPE_E4M3  e4m3 values and one scale per 128 columns by
+ *                     gsp_quantize_rows_fp8's rule (scales [rows, ceil(cols / 128)],
+ *                     row stride in elements): hidden of gsp_fp8_logits.
+ * The 8-bit values are taken from y itself, not from its rounding. residual_out may
+ * be residual. x's and residual's row strides may be 0; up to 2^24 columns. The
+ * reference starts at the hidden states (gsp/triton_runtime.py:61-109). */
+int32_t gsp_rms_norm(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                     const void* weight, int64_t rows, int32_t cols, float eps, int32_t dtype, void* residual_out,
+                     int64_t residual_out_row_stride, int32_t out_dtype, void* out, int64_t out_row_stride, float* scales,
+                     int64_t scales_row_stride, void* stream);
+
+/* ---- fp8 head ----------------------------------------------------------------------
+ * The projection on a weight in e4m3 with one fp32 scale per block of 128 rows x 128
+ * columns, and hidden states in e4m3 with one scale per 128 columns of a request. No
+ * counterpart in the reference (its heads are fp16 / bf16 / fp32).
+ *
+ * Quantisers: blocks of `src` (fp16, bf16 or fp32; up to 2^24 columns) to values and
+ * one scale each, the last blocks of a row or column shorter:
+ *   scale = max |x| / 448 (fp32 division), value = x / scale (fp32 division) to the
+ *   nearest e4m3, ties to even.
+ * A block of zeros has scale 0; one that holds an infinity or NaN has scale NaN and
+ * values 0. gsp_quantize_rows_fp8: blocks of 1 x 128, scales [rows, ceil(cols / 128)];
+ * gsp_quantize_weight_fp8: of 128 x 128, scales [ceil(rows / 128), ceil(cols / 128)]. */
+int32_t gsp_quantize_rows_fp8(const void* src, int64_t src_row_stride, int64_t rows, int32_t cols, int32_t dtype,
+                              uint8_t* values, int64_t values_row_stride, float* scales, int64_t scales_row_stride,
+                              void* stream);
+int32_t gsp_quantize_weight_fp8(const void* src, int64_t src_row_stride, int64_t rows, int32_t cols, int32_t dtype,
+                                uint8_t* values, int64_t values_row_stride, float* scales, int64_t scales_row_stride,
+                                void* stream);
+
+/* Masked logits and fused greedy top-1 on any route (GSP_ROUTE_*):
+ *   y[b, v] = sum_j hs[b, j] ws[v / 128, j] sum_{k in block j} q[b, k] w[v, k]
+ * in fp32, rounded once to out_dtype (GSP_DTYPE_F16 / _BF16 / _F32). The routes add
+ * the products in their own order and agree to fp32 rounding.
+ * hidden_dtype GSP_DTYPE_E4M3: `hidden` holds e4m3 values with hidden_scales [batch,
+ * ceil(hidden_dim / 128)] (row stride in elements). Otherwise `hidden` is fp16 / bf16 /
+ * fp32, quantised by the call as gsp_quantize_rows_fp8 does. bitmask NULL (every token
+ * legal): the plain product, for the positions of a prompt on the dense route.
+ * hidden_dim <= 32,768. The tensor-core routes want 16-byte aligned rows (hidden_dim a
+ * multiple of 16) and, in block mode, vocabularies up to 1,048,576; they run the
+ * row-sparse kernel otherwise. scratch: gsp_fp8_scratch_bytes, 16-byte aligned, contents
+ * neither read nor preserved, one per concurrent call; it takes the place of a
+ * workspace. A bounded wait that ran out is recorded in the device's error word
+ * (gsp_int8_error). The other arguments are those of gsp_int8_logits. */
+size_t gsp_fp8_scratch_bytes(int32_t batch, int32_t vocab, int32_t hidden_dim);
+int32_t gsp_fp8_logits(int32_t route, const void* hidden, int64_t hidden_row_stride, int32_t hidden_dtype,
+                       const float* hidden_scales, int64_t hidden_scales_row_stride, const uint8_t* weight,
+                       int64_t weight_row_stride, const float* weight_scales, int64_t weight_scales_row_stride,
+                       const int32_t* bitmask, int64_t bitmask_row_stride, int32_t batch, int32_t vocab,
+                       int32_t hidden_dim, int32_t out_dtype, int64_t vocab_offset, void* logits,
+                       int64_t logits_row_stride, float* top_value, int64_t* top_index, int64_t* top_key,
+                       void* scratch, size_t scratch_bytes, void* stream);
 
 #ifdef __cplusplus
 }

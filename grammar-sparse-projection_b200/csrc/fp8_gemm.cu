@@ -21,7 +21,7 @@
 //   warp 0      TMA producer: the active groups' 32 rows x 128 bytes each, and the
 //               hidden states' rows x 128 bytes, 128-byte swizzle;
 //   warp 1      TMEM, and one lane's tcgen05.mma;
-//   warps 2-9   epilogue, two per TMEM lane quadrant, alternating groups.
+//   warps 4-11  epilogue, two per TMEM lane quadrant, alternating groups.
 //
 // A prologue kernel quantises (or turns round the scales of) the hidden states,
 // clears the top-1 keys, and in block mode lists the 32-row groups that hold a legal
@@ -46,8 +46,11 @@ namespace {
 constexpr int kChunkRows = 128;  // hidden states of a tile
 constexpr int kGroupRows = 32;
 constexpr uint32_t kGroupBytes = kGroupRows * kBlock;
-constexpr int kEpilogueWarps = 8;
-constexpr int kGemmThreads = 32 * (2 + kEpilogueWarps);
+constexpr int kEpilogueWarps = 8, kQuadWarps = kEpilogueWarps / 4;  // (kQuadWarps per TMEM lane quadrant)
+constexpr int kGemmThreads = 32 * (4 + kEpilogueWarps);  // (two of the first four warps only take part in the barriers)
+// Registers: 168 a thread at launch (384 threads); tiles of eight groups hand those
+// of the first four warps to the epilogue: 4 * 56 + 8 * 224 = 12 * 168.
+constexpr int kFewRegisters = 56, kManyRegisters = 224;
 constexpr int kMaxStages = 10;
 constexpr int kMaxAcc = 4;
 constexpr int kMaxBuilders = 256;  // prefix sums that fit the CTA's table: 2^20 tokens; past it they are searched in global memory
@@ -162,29 +165,39 @@ struct GemmLayout {
   }
 };
 
-// A tile: `n` groups from compacted position `pos` on, for chunk `chunk`.
-struct Tile {
-  int chunk, pos, n;
-};
-
-// The CTA's i-th tile; false past the last.
+// The CTA's tiles, one after another: `n` groups from compacted position `pos` on, for
+// chunk `chunk` (n 0: past the last). One chunk: an even share of the positions. Several:
+// (tile, chunk) pairs, chunks first, strided by the grid.
 template <int kGroups>
-__device__ __forceinline__ bool tile_of(int i, int total, int chunks, Tile& t) {
-  if (chunks == 1) {
-    const int lo = (int)((int64_t)total * blockIdx.x / gridDim.x), hi = (int)((int64_t)total * (blockIdx.x + 1) / gridDim.x);
-    t.chunk = 0;
-    t.pos = lo + i * kGroups;
-    t.n = min(kGroups, hi - t.pos);
-    return t.n > 0;
+struct Tiles {
+  int chunk, pos, n;
+  int end, chunks, tile_step, chunk_step;
+  __device__ __forceinline__ Tiles(int total, int chunks_) : chunks(chunks_) {
+    const int G = gridDim.x, cta = blockIdx.x;
+    if (chunks == 1) {
+      end = (int)((int64_t)total * (cta + 1) / G);
+      chunk = chunk_step = 0;
+      pos = (int)((int64_t)total * cta / G);
+      tile_step = kGroups;
+    } else {
+      end = total;
+      chunk = cta % chunks;
+      chunk_step = G % chunks;
+      pos = cta / chunks * kGroups;
+      tile_step = G / chunks * kGroups;
+    }
+    n = max(0, min(kGroups, end - pos));
   }
-  const int64_t item = (int64_t)blockIdx.x + (int64_t)i * gridDim.x;
-  const int64_t tile = item / chunks;
-  t.chunk = (int)(item - tile * chunks);
-  if (tile * kGroups >= total) return false;
-  t.pos = (int)(tile * kGroups);
-  t.n = min(kGroups, total - t.pos);
-  return true;
-}
+  __device__ __forceinline__ void next() {
+    pos += tile_step;
+    chunk += chunk_step;
+    if (chunk >= chunks) {  // (one chunk: never, chunk stays 0)
+      chunk -= chunks;
+      pos += kGroups;
+    }
+    n = max(0, min(kGroups, end - pos));
+  }
+};
 
 // Group (mask word) at compacted position `pos`.
 __device__ __forceinline__ int group_at(const Fp8Params& p, const int* s_prefix, int builders, int pos) {
@@ -229,53 +242,124 @@ __device__ __forceinline__ void fill_inactive(const Fp8Params& p, int ew, int la
   }
 }
 
-// One group's 32 logits of a request: masked, rounded, stored; the largest as a top-1 key.
+// A request's largest logit so far, as a thread has seen them (ids rising).
+struct Best {
+  float value;
+  unsigned long long key;
+  int row;
+};
+
+// 32 bytes, a whole sector, in one store (`at` 32-byte aligned).
+__device__ __forceinline__ void store_sector(void* at, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// Larger of two, NaN above all.
+__device__ __forceinline__ float max_nan(float a, float b) { return a > b || a != a ? a : b; }
+
+// One group's 32 logits of a request: rounded, masked, stored; and the largest of
+// them, whose place is sought only when it passes the largest so far.
 template <typename Out>
-__device__ __forceinline__ unsigned long long finish_group(const float (&y)[32], uint32_t legal, typename DTypeTraits<Out>::OutBits* out,
-                                                           bool vec, int left, int64_t first_id) {
+__device__ __forceinline__ void finish_group(const float2 (&acc)[16], uint32_t legal, typename DTypeTraits<Out>::OutBits* out,
+                                             bool vec, int left, int64_t first_id, bool want_top, Best& best) {
   using OutBits = typename DTypeTraits<Out>::OutBits;
-  uint32_t best = 0u;  // (ordered bits: a NaN is the largest, as for the other heads)
-  int at = -1;
-  OutBits bits[32];
+  float top;
+  if constexpr (sizeof(OutBits) == 2) {
+    using Out2 = typename std::conditional<std::is_same<Out, __half>::value, __half2, __nv_bfloat162>::type;
+    uint32_t w[16];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const OutBits r = DTypeTraits<Out>::round_bits(y[j]);
-    const bool ok = (legal >> j) & 1u;
-    bits[j] = ok ? r : (OutBits)DTypeTraits<Out>::kNegInfBits;
-    const uint32_t o = ordered_bits(DTypeTraits<Out>::bits_to_float(r));
-    if (ok && o > best) {
-      best = o;
-      at = j;
+    for (int k = 0; k < 16; ++k) {
+      Out2 two;
+      if constexpr (std::is_same<Out, __half>::value) two = __floats2half2_rn(acc[k].x, acc[k].y);
+      else two = __floats2bfloat162_rn(acc[k].x, acc[k].y);
+      w[k] = *reinterpret_cast<const uint32_t*>(&two);
     }
-  }
-  if (out) {
-    if (vec && left >= 32) {
-      constexpr int kPer = 16 / (int)sizeof(OutBits);
+    if (legal != 0xffffffffu) {
+      const uint32_t ninf = DTypeTraits<Out>::kNegInfBits * 0x00010001u;
+      // bits 2k and 2k + 1 to the tops of a word's halves, whose signs spread over them
+      const uint32_t lo = (legal & 0xffffu) | (legal << 15), hi = (legal >> 16) | ((legal >> 1) & 0xffff8000u);
 #pragma unroll
-      for (int k = 0; k < 32 / kPer; ++k) {
-        uint32_t w[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if constexpr (sizeof(OutBits) == 2) w[q] = (uint32_t)bits[k * 8 + 2 * q] | ((uint32_t)bits[k * 8 + 2 * q + 1] << 16);
-          else w[q] = bits[k * 4 + q];
-        }
-        reinterpret_cast<uint4*>(out)[k] = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int k = 0; k < 16; ++k) {
+        const uint32_t keep = spread_half_signs((k < 8 ? lo : hi) << (15 - 2 * (k & 7)));
+        w[k] = (w[k] & keep) | (ninf & ~keep);
       }
-    } else {
+    }
+    if (out) {
+      if (vec && left >= 32) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < left) out[j] = bits[j];
+        for (int k = 0; k < 2; ++k) store_sector(out + 16 * k, &w[8 * k]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j < left) out[j] = (OutBits)(w[j / 2] >> (16 * (j & 1)));
+      }
+    }
+    if (!want_top) return;
+    Out2 m[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) m[k] = *reinterpret_cast<const Out2*>(&w[k]);
+#pragma unroll
+    for (int h = 8; h >= 1; h >>= 1) {
+#pragma unroll
+      for (int k = 0; k < h; ++k) m[k] = __hmax2_nan(m[k], m[k + h]);
+    }
+    const float2 two = DTypeTraits<Out>::pair_to_float2(*reinterpret_cast<const uint32_t*>(&m[0]));
+    top = max_nan(two.x, two.y);
+    if (!(top <= best.value)) {  // larger, or NaN
+      // even elements that equal it in the low half, odd ones in the high half (NaN: those unordered with themselves)
+      const uint32_t top_bits = (uint32_t)DTypeTraits<Out>::round_bits(top) * 0x00010001u;
+      const Out2 same = *reinterpret_cast<const Out2*>(&top_bits);
+      uint32_t equal = 0u;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const Out2 x = *reinterpret_cast<const Out2*>(&w[k]);
+        equal |= (top != top ? __hneu2_mask(x, x) : __heq2_mask(x, same)) & (0x00010001u << k);
+      }
+      const int even = __ffs(equal & 0xffffu), odd = __ffs(equal >> 16);  // (from 1; 0: none)
+      const int at = min(even ? 2 * even - 2 : 32, odd ? 2 * odd - 1 : 32);
+      const unsigned long long key = top1_key(top, (uint64_t)(first_id + at));
+      if (key > best.key) best.key = key;
+      best.value = top;
+    }
+  } else {
+    float y[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = (legal >> j) & 1u ? (j & 1 ? acc[j / 2].y : acc[j / 2].x) : -INFINITY;
+    if (out) {
+      if (vec && left >= 32) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) store_sector(out + 8 * k, reinterpret_cast<const uint32_t*>(&y[8 * k]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j < left) out[j] = __float_as_uint(y[j]);
+      }
+    }
+    if (!want_top) return;
+    top = y[0];
+#pragma unroll
+    for (int j = 1; j < 32; ++j) top = max_nan(top, y[j]);
+    if (!(top <= best.value)) {
+      int at = -1;
+#pragma unroll
+      for (int j = 31; j >= 0; --j)
+        if (y[j] == top || (y[j] != y[j] && top != top)) at = j;
+      const unsigned long long key = top1_key(top, (uint64_t)(first_id + at));
+      if (key > best.key) best.key = key;
+      best.value = top;
     }
   }
-  return at < 0 ? 0ull : top1_key(from_ordered_bits(best), (uint64_t)(first_id + at));
 }
 
 template <typename Out, int kGroups>
 __global__ void __launch_bounds__(kGemmThreads, 1)
-    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_w4,
+                    const __grid_constant__ CUtensorMap tmap_x,
                     const __grid_constant__ Fp8Params p, const GemmConfig c) {
   using OutBits = typename DTypeTraits<Out>::OutBits;
-  constexpr int kUnits = kGroups / 2;               // groups of an epilogue warp
+  constexpr int kUnits = kGroups / kQuadWarps;      // groups of an epilogue warp
   constexpr int kAcc = 512 / (kGroupRows * kGroups);  // accumulators: all of TMEM
   constexpr uint32_t kAccCols = kGroupRows * kGroups;
   static_assert(kAcc <= kMaxAcc, "accumulator barriers");
@@ -299,6 +383,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_w4);
     tma_prefetch_desc(&tmap_x);
     for (int s = 0; s < c.stages; ++s) {
       mbar_init(full + s, 1);
@@ -306,7 +391,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
     for (int a = 0; a < kAcc; ++a) {
       mbar_init(tfull + a, 1);
-      mbar_init(tempty + a, 2 * (uint32_t)quads);
+      mbar_init(tempty + a, kQuadWarps * (uint32_t)quads);
     }
     fence_mbar_init();
     s_misc[0] = 0;
@@ -340,16 +425,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const uint32_t tmem_base = *s_tmem;
   const int total = s_misc[2];
 
+  if (warp < 4) {
+    if constexpr (kGroups == 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+  }
   if (warp == 0) {
     if (lane == 0) {
       uint32_t parity = 1, issued = 0;
       int s = 0;
-      Tile t;
-      for (int i = 0; !*abort_flag && tile_of<kGroups>(i, total, c.chunks, t); ++i) {
+      for (Tiles<kGroups> t(total, c.chunks); t.n > 0 && !*abort_flag; t.next()) {
         int row[kGroups];
+        bool whole[kGroups / 4];  // four groups side by side: one copy
 #pragma unroll
         for (int g = 0; g < kGroups; ++g)
           row[g] = g < t.n ? group_at(p, s_prefix, c.builders, t.pos + g) * kGroupRows : 0;
+#pragma unroll
+        for (int h = 0; h < kGroups / 4; ++h) whole[h] = 4 * h + 4 <= t.n && row[4 * h + 3] - row[4 * h] == 3 * kGroupRows;
         const uint32_t bytes = (uint32_t)t.n * kGroupBytes + (uint32_t)c.xrows * kBlock;
         for (int kb = 0; kb < p.blocks; ++kb) {
           if (!mbar_wait(empty + s, parity, abort_flag)) {
@@ -359,8 +449,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           mbar_arrive_expect_tx(full + s, bytes);
           unsigned char* w = s_w + (size_t)s * GemmLayout<kGroups>::kWBytes;
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g)
-            if (g < t.n) tma_load_2d(w + g * kGroupBytes, &tmap_w, kb * kBlock, row[g], full + s);
+          for (int h = 0; h < kGroups / 4; ++h) {
+            if (whole[h]) {
+              tma_load_2d(w + 4 * h * kGroupBytes, &tmap_w4, kb * kBlock, row[4 * h], full + s);
+            } else {
+#pragma unroll
+              for (int g = 4 * h; g < 4 * h + 4; ++g)
+                if (g < t.n) tma_load_2d(w + g * kGroupBytes, &tmap_w, kb * kBlock, row[g], full + s);
+            }
+          }
           tma_load_2d(s_x + (size_t)s * c.xrows * kBlock, &tmap_x, kb * kBlock, t.chunk * kChunkRows, full + s);
           ++issued;
           if (++s == c.stages) {
@@ -380,9 +477,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const uint32_t x_step = ((uint32_t)c.xrows * kBlock) >> 4, w_step = GemmLayout<kGroups>::kWBytes >> 4;
       uint32_t parity = 0, last_parity = 0, it = 0;
       int s = 0, last_stage = -1;
-      Tile t;
       bool ok = true;
-      for (int i = 0; ok && !*abort_flag && tile_of<kGroups>(i, total, c.chunks, t); ++i) {
+      for (Tiles<kGroups> t(total, c.chunks); ok && t.n > 0 && !*abort_flag; t.next()) {
         const uint32_t idesc = tc_idesc_e4m3((uint32_t)(t.n * kGroupRows));
         for (int kb = 0; kb < p.blocks; ++kb, ++it) {
           const uint32_t acc = it % kAcc, use = it / kAcc;
@@ -408,52 +504,75 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
       if (last_stage >= 0) mbar_wait(empty + last_stage, last_parity, nullptr);  // all tensor-core work is done
     }
-  } else {
-    const int ew = warp - 2, q = warp & 3, half = ew >> 2;
+  } else if (warp >= 4) {
+    if constexpr (kGroups == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+    const int ew = warp - 4, q = warp & 3, part = ew >> 2;
     if (!p.dense && p.logits) fill_inactive<Out>(p, ew, lane);
-    constexpr int kVec = 16 / (int)sizeof(OutBits);
-    const bool vec = (reinterpret_cast<uintptr_t>(p.logits) & 15) == 0 && p.logits_stride % kVec == 0;
-    unsigned long long best = 0ull;  // of request `best_row`
-    int best_row = -1;
+    constexpr int kSector = 32 / (int)sizeof(OutBits);
+    const bool vec = (reinterpret_cast<uintptr_t>(p.logits) & 31) == 0 && p.logits_stride % kSector == 0;
+    Best best{-INFINITY, 0ull, -1};
     const auto flush = [&]() {
-      if (best != 0ull && best > *(volatile unsigned long long*)(p.keys + best_row)) atomicMax(p.keys + best_row, best);
-      best = 0ull;
+      if (best.key != 0ull && best.key > *(volatile unsigned long long*)(p.keys + best.row)) atomicMax(p.keys + best.row, best.key);
     };
     uint32_t it = 0;
-    Tile t;
     bool ok = q < quads;
-    for (int i = 0; ok && tile_of<kGroups>(i, total, c.chunks, t); ++i) {
+    Tiles<kGroups> t(total, c.chunks);
+    // The next tile's groups, mask words and first scales are loaded while a tile is
+    // worked on: nothing else would hide their latency (2 us a tile).
+    int group_next[kUnits];
+    uint32_t legal_next[kUnits];
+    float ws_next[kUnits], hs_next[4];
+    const auto load_hs = [&](int row, int kb) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        hs_next[j] = row < p.batch && kb + j < p.blocks ? p.scales_t[(int64_t)(kb + j) * p.batch + row] : 0.f;
+    };
+    const auto load_ws = [&](int group, int kb) {
+      return kb + lane < p.blocks ? __ldg(p.weight_scales + (int64_t)(group >> 2) * p.weight_scales_stride + kb + lane) : 0.f;
+    };
+    const auto load_tile = [&]() {  // of t; its hidden states' scales come with load_hs
+      const int row = t.chunk * kChunkRows + q * 32 + lane;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int g = kQuadWarps * u + part;
+        group_next[u] = g < t.n ? group_at(p, s_prefix, c.builders, t.pos + g) : 0;
+        legal_next[u] = 0u;
+        if (g < t.n && row < p.batch)
+          legal_next[u] = p.mask ? __ldg(p.mask + (int64_t)row * p.mask_stride + group_next[u]) : 0xffffffffu;
+        ws_next[u] = load_ws(group_next[u], 0);
+      }
+    };
+    if (ok) {
+      load_tile();
+      load_hs(t.chunk * kChunkRows + q * 32 + lane, 0);
+    }
+    while (ok && t.n > 0) {
       const int b = t.chunk * kChunkRows + q * 32 + lane;
       const bool mine = b < p.batch;
+      const int mine_n = (t.n - part + kQuadWarps - 1) / kQuadWarps;  // groups part, part + 2, ...
       int group[kUnits];
       uint32_t legal[kUnits];
       float2 acc[kUnits][16];
+      float hs[4], ws[kUnits];
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
-        const int g = 2 * u + half;
-        group[u] = g < t.n ? group_at(p, s_prefix, c.builders, t.pos + g) : 0;
-        legal[u] = 0u;
-        if (g < t.n && mine)
-          legal[u] = tail_clip(p.mask ? __ldg(p.mask + (int64_t)b * p.mask_stride + group[u]) : 0xffffffffu, group[u], p.vocab);
+        group[u] = group_next[u];
+        legal[u] = tail_clip(legal_next[u], group[u], p.vocab);
+        ws[u] = ws_next[u];
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[u][j] = make_float2(0.f, 0.f);
       }
-      // scales: the request's, four blocks ahead; the groups', a lane each for 32 blocks
-      float hs[4], hs_next[4], ws[kUnits];
-      const auto load_hs = [&](int kb, float (&v)[4]) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          v[j] = mine && kb + j < p.blocks ? p.scales_t[(int64_t)(kb + j) * p.batch + b] : 0.f;
-      };
-      load_hs(0, hs_next);
+      t.next();
+      load_tile();
+      const int b_next = t.chunk * kChunkRows + q * 32 + lane;
       for (int kb0 = 0; ok && kb0 < p.blocks; kb0 += 4) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) hs[j] = hs_next[j];
-        load_hs(kb0 + 4, hs_next);
-        if ((kb0 & 31) == 0) {
+        if (kb0 + 4 < p.blocks) load_hs(b, kb0 + 4);
+        else load_hs(b_next, 0);  // the next tile's
+        if (kb0 != 0 && (kb0 & 31) == 0) {
 #pragma unroll
-          for (int u = 0; u < kUnits; ++u)
-            ws[u] = kb0 + lane < p.blocks ? __ldg(p.weight_scales + (int64_t)(group[u] >> 2) * p.weight_scales_stride + kb0 + lane) : 0.f;
+          for (int u = 0; u < kUnits; ++u) ws[u] = load_ws(group[u], kb0);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -466,18 +585,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           ok = __all_sync(FULL_MASK, ok);
           if (!ok) break;
           tc_fence_after_sync();
-          const uint32_t col = tmem_base + ((uint32_t)(q * 32) << 16) + a * kAccCols + (uint32_t)half * kGroupRows;
+          const uint32_t col = tmem_base + ((uint32_t)(q * 32) << 16) + a * kAccCols + (uint32_t)part * kGroupRows;
+          // (all of the warp's groups, whether the tile has them: their sums are not used)
 #pragma unroll
-          for (int u = 0; u < kUnits; ++u) {
-            const float w = __shfl_sync(FULL_MASK, ws[u], (kb0 + j) & 31);
-            if (2 * u + half < t.n) {
-              uint32_t v[32];
-              tmem_ld32(col + (uint32_t)(2 * u) * kGroupRows, v);
-              tmem_ld_wait();
-              const float f = hs[j] * w;
+          for (int u = 0; u < kUnits; u += 2) {
+            uint32_t v[2][32];
+            tmem_ld_2x32(col + (uint32_t)(kQuadWarps * u) * kGroupRows, col + (uint32_t)(kQuadWarps * (u + 1)) * kGroupRows,
+                         v[0], v[1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float f = hs[j] * __shfl_sync(FULL_MASK, ws[u + e], (kb0 + j) & 31);
 #pragma unroll
               for (int k = 0; k < 16; ++k)
-                acc[u][k] = fma2(make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), make_float2(f, f), acc[u][k]);
+                acc[u + e][k] = fma2(make_float2(__uint_as_float(v[e][2 * k]), __uint_as_float(v[e][2 * k + 1])),
+                                     make_float2(f, f), acc[u + e][k]);
             }
           }
           tc_fence_before_sync();
@@ -487,23 +608,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
       }
       if (!ok) break;
-      if (want_top && mine && b != best_row) {
+      if (want_top && mine && b != best.row) {
         flush();
-        best_row = b;
+        best = Best{-INFINITY, 0ull, b};
       }
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
-        if (2 * u + half >= t.n || !mine) continue;
-        float y[32];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          y[2 * k] = acc[u][k].x;
-          y[2 * k + 1] = acc[u][k].y;
-        }
+        if (u >= mine_n || !mine) continue;
         const int v0 = group[u] * kGroupRows;
         OutBits* out = p.logits ? static_cast<OutBits*>(p.logits) + b * p.logits_stride + v0 : nullptr;
-        const unsigned long long key = finish_group<Out>(y, legal[u], out, vec, p.vocab - v0, p.vocab_offset + v0);
-        best = key > best ? key : best;
+        finish_group<Out>(acc[u], legal[u], out, vec, p.vocab - v0, p.vocab_offset + v0, want_top, best);
       }
     }
     if (want_top) flush();
@@ -591,8 +705,9 @@ cudaError_t launch_gemm(const Fp8Params& p, GemmConfig c, int dev, cudaStream_t 
   c.stages = kMaxStages;
   while (c.stages > 2 && GemmLayout<kGroups>(c).total + 1024 > (uint32_t)optin) --c.stages;
   const size_t smem = GemmLayout<kGroups>(c).total + 1024;
-  CUtensorMap tw, tx;
+  CUtensorMap tw, tw4, tx;
   if (!make_map(&tw, p.weight, (uint64_t)p.vocab, (uint64_t)p.hidden_dim, (uint64_t)p.weight_stride, kGroupRows) ||
+      !make_map(&tw4, p.weight, (uint64_t)p.vocab, (uint64_t)p.hidden_dim, (uint64_t)p.weight_stride, 4 * kGroupRows) ||
       !make_map(&tx, p.hidden, (uint64_t)p.batch, (uint64_t)p.hidden_dim, (uint64_t)p.hidden_stride, (uint32_t)c.xrows))
     return cudaErrorInvalidValue;
   auto k = fp8_gemm_kernel<Out, kGroups>;
@@ -608,7 +723,7 @@ cudaError_t launch_gemm(const Fp8Params& p, GemmConfig c, int dev, cudaStream_t 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, tw, tx, p, c);
+  return cudaLaunchKernelEx(&cfg, k, tw, tw4, tx, p, c);
 }
 
 template <typename Out>

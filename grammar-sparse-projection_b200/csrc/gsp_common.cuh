@@ -101,6 +101,13 @@ struct DTypeTraits<Int8Rows<Out>> {
   static __device__ __forceinline__ float bits_to_float(OutBits u) { return DTypeTraits<Out>::bits_to_float(u); }
 };
 
+// All ones in the halves of a word whose top bit (15, 31) is set.
+__device__ __forceinline__ uint32_t spread_half_signs(uint32_t x) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(r) : "r"(x));  // (a selector's top bit takes the byte's sign)
+  return r;
+}
+
 // Order-preserving map float -> uint32 (total order on non-NaN values).
 // +0 and -0 are canonicalised so that they compare equal, as in torch.argmax.
 __device__ __forceinline__ uint32_t ordered_bits(float f) {

@@ -46,14 +46,19 @@ namespace {
 constexpr int kChunkRows = 128;  // hidden states of a tile
 constexpr int kGroupRows = 32;
 constexpr uint32_t kGroupBytes = kGroupRows * kBlock;
-constexpr int kEpilogueWarps = 8, kQuadWarps = kEpilogueWarps / 4;  // (kQuadWarps per TMEM lane quadrant)
+// Eight epilogue warps, two per TMEM lane quadrant. Sixteen, with half the groups each,
+// took longer (128 x 262,144 x 8,192: 477 us against 414): what a stage costs a warp
+// besides its sums is then paid twice as often.
+constexpr int kEpilogueWarps = 8, kQuadWarps = kEpilogueWarps / 4;
 constexpr int kGemmThreads = 32 * (4 + kEpilogueWarps);  // (two of the first four warps only take part in the barriers)
-// Registers: 168 a thread at launch (384 threads); tiles of eight groups hand those
-// of the first four warps to the epilogue: 4 * 56 + 8 * 224 = 12 * 168.
+// Registers: 168 a thread at launch (384 threads); the first four warps hand theirs to the
+// epilogue: 4 * 56 + 8 * 224 = 12 * 168.
 constexpr int kFewRegisters = 56, kManyRegisters = 224;
 constexpr int kMaxStages = 10;
 constexpr int kMaxAcc = 4;
 constexpr int kMaxBuilders = 256;  // prefix sums that fit the CTA's table: 2^20 tokens; past it they are searched in global memory
+
+constexpr int kAhead = 2, kScaleRing = 4;  // vectors of four scales that a thread loads ahead, and keeps
 
 struct GemmConfig {
   int chunks;  // of kChunkRows hidden states
@@ -86,7 +91,7 @@ __device__ __forceinline__ void quantize_hidden(const Fp8Params& p, int64_t firs
 #pragma unroll
     for (int k = 0; k < kE / 4; ++k) w[k] = to_e4m3(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3], s);
     U::store_bytes(values + row * p.hidden_stride, i, p.hidden_dim, w);
-    if (i % U::kLanes == 0) p.scales_t[(int64_t)(i / U::kLanes) * p.batch + row] = s.scale;
+    if (i % U::kLanes == 0) p.scales[(int64_t)row * p.scales_stride + i / U::kLanes] = s.scale;
   }
 }
 
@@ -110,9 +115,9 @@ __global__ void __launch_bounds__(kPrologueThreads) fp8_prologue_kernel(const __
     } else {
       const int64_t total = (int64_t)p.batch * p.blocks;
       for (int64_t at = first; at < total; at += step) {
-        const int kb = (int)(at / p.batch);
-        const int64_t row = at - (int64_t)kb * p.batch;
-        p.scales_t[at] = __ldg(p.hidden_scales + row * p.hidden_scales_stride + kb);
+        const int64_t row = at / p.blocks;
+        const int kb = (int)(at - row * p.blocks);
+        p.scales[row * p.scales_stride + kb] = __ldg(p.hidden_scales + row * p.hidden_scales_stride + kb);
       }
     }
     return;
@@ -153,14 +158,15 @@ __global__ void __launch_bounds__(kPrologueThreads) fp8_prologue_kernel(const __
 template <int kGroups>
 struct GemmLayout {
   static constexpr uint32_t kWBytes = kGroups * kGroupBytes;
-  uint32_t x, bars, tmem, misc, prefix, total;
+  uint32_t x, bars, tmem, misc, scales, prefix, total;
   __host__ __device__ GemmLayout(const GemmConfig& c) {
     x = (uint32_t)c.stages * kWBytes;
     // (the MMA reads 128 rows of a stage's hidden states, loaded or not)
     bars = x + (uint32_t)(c.stages - 1) * (uint32_t)c.xrows * kBlock + kChunkRows * kBlock;
     tmem = bars + 8 * (2 * kMaxStages + 2 * kMaxAcc);
     misc = tmem + 16;
-    prefix = misc + 16;
+    scales = misc + 16;  // of the hidden states: a ring of vectors per epilogue thread
+    prefix = scales + 16 * kScaleRing * 32 * kEpilogueWarps;
     total = prefix + 4 * (kMaxBuilders + 1);
   }
 };
@@ -262,10 +268,13 @@ __device__ __forceinline__ float max_nan(float a, float b) { return a > b || a !
 // One group's 32 logits of a request: rounded, masked, stored; and the largest of
 // them, whose place is sought only when it passes the largest so far.
 template <typename Out>
-__device__ __forceinline__ void finish_group(const float2 (&acc)[16], uint32_t legal, typename DTypeTraits<Out>::OutBits* out,
+__device__ __forceinline__ void finish_group(const unsigned long long (&sums)[16], uint32_t legal, typename DTypeTraits<Out>::OutBits* out,
                                              bool vec, int left, int64_t first_id, bool want_top, Best& best) {
   using OutBits = typename DTypeTraits<Out>::OutBits;
   float top;
+  float2 acc[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) acc[k] = unpack2(sums[k]);
   if constexpr (sizeof(OutBits) == 2) {
     using Out2 = typename std::conditional<std::is_same<Out, __half>::value, __half2, __nv_bfloat162>::type;
     uint32_t w[16];
@@ -426,10 +435,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int total = s_misc[2];
 
   if (warp < 4) {
-    if constexpr (kGroups == 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
   }
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t parity = 1, issued = 0;
       int s = 0;
       for (Tiles<kGroups> t(total, c.chunks); t.n > 0 && !*abort_flag; t.next()) {
@@ -472,17 +481,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint64_t x_desc = tc_desc_sw128(s_x), w_desc = tc_desc_sw128(s_w);
       const uint32_t x_step = ((uint32_t)c.xrows * kBlock) >> 4, w_step = GemmLayout<kGroups>::kWBytes >> 4;
-      uint32_t parity = 0, last_parity = 0, it = 0;
+      uint32_t parity = 0, last_parity = 0, acc = 0, acc_parity = 1;  // (a fresh `tempty` lets parity 1 pass)
       int s = 0, last_stage = -1;
       bool ok = true;
       for (Tiles<kGroups> t(total, c.chunks); ok && t.n > 0 && !*abort_flag; t.next()) {
         const uint32_t idesc = tc_idesc_e4m3((uint32_t)(t.n * kGroupRows));
-        for (int kb = 0; kb < p.blocks; ++kb, ++it) {
-          const uint32_t acc = it % kAcc, use = it / kAcc;
-          if ((use > 0 && !mbar_wait(tempty + acc, (use - 1) & 1u, abort_flag)) || !mbar_wait(full + s, parity, abort_flag)) {
+        for (int kb = 0; kb < p.blocks; ++kb) {
+          if (!mbar_wait(tempty + acc, acc_parity, abort_flag) || !mbar_wait(full + s, parity, abort_flag)) {
             *abort_flag = 1;
             ok = false;
             break;
@@ -494,6 +502,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           for (int k = 0; k < kBlock / 32; ++k) tc_mma_f8(d, xd + 2ull * k, wd + 2ull * k, idesc, k != 0);
           tc_commit(empty + s);
           tc_commit(tfull + acc);
+          if (++acc == kAcc) {
+            acc = 0;
+            acc_parity ^= 1u;
+          }
           last_stage = s;
           last_parity = parity;
           if (++s == c.stages) {
@@ -505,7 +517,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       if (last_stage >= 0) mbar_wait(empty + last_stage, last_parity, nullptr);  // all tensor-core work is done
     }
   } else if (warp >= 4) {
-    if constexpr (kGroups == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
     const int ew = warp - 4, q = warp & 3, part = ew >> 2;
     if (!p.dense && p.logits) fill_inactive<Out>(p, ew, lane);
     constexpr int kSector = 32 / (int)sizeof(OutBits);
@@ -514,18 +526,40 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const auto flush = [&]() {
       if (best.key != 0ull && best.key > *(volatile unsigned long long*)(p.keys + best.row)) atomicMax(p.keys + best.row, best.key);
     };
-    uint32_t it = 0;
+    const uint32_t acc_base = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)part * kGroupRows;
+    uint32_t a = 0, parity = 0, slot = 0;
     bool ok = q < quads;
     Tiles<kGroups> t(total, c.chunks);
     // The next tile's groups, mask words and first scales are loaded while a tile is
     // worked on: nothing else would hide their latency (2 us a tile).
     int group_next[kUnits];
     uint32_t legal_next[kUnits];
-    float ws_next[kUnits], hs_next[4];
-    const auto load_hs = [&](int row, int kb) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        hs_next[j] = row < p.batch && kb + j < p.blocks ? p.scales_t[(int64_t)(kb + j) * p.batch + row] : 0.f;
+    float ws_next[kUnits];
+    // The scales of the thread's hidden state, four stages a vector, come through shared
+    // memory: registers that wait for a load cannot be passed on in a loop.
+    float4* s_scale = reinterpret_cast<float4*>(smem + L.scales) + (tid - 128);
+    constexpr uint32_t kSlot = 32 * kEpilogueWarps, kSlots = kScaleRing * kSlot;
+    Tiles<kGroups> ahead = t;
+    const float* ahead_src;
+    int ahead_left;  // stages of that tile
+    bool ahead_valid;
+    uint32_t ahead_slot = 0;
+    const auto scales_of = [&]() {
+      const int row = ahead.chunk * kChunkRows + q * 32 + lane;
+      ahead_valid = ahead.n > 0 && row < p.batch;
+      ahead_src = p.scales + (ahead_valid ? (int64_t)row * p.scales_stride : 0);
+      ahead_left = p.blocks;
+    };
+    scales_of();
+    const auto load_scales = [&]() {
+      cp_async16(s_scale + ahead_slot, ahead_src, ahead_valid);
+      cp_async_commit();
+      ahead_slot = (ahead_slot + kSlot) & (kSlots - 1);
+      ahead_src += 4;
+      if ((ahead_left -= 4) <= 0) {
+        ahead.next();
+        scales_of();
+      }
     };
     const auto load_ws = [&](int group, int kb) {
       return kb + lane < p.blocks ? __ldg(p.weight_scales + (int64_t)(group >> 2) * p.weight_scales_stride + kb + lane) : 0.f;
@@ -544,7 +578,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     };
     if (ok) {
       load_tile();
-      load_hs(t.chunk * kChunkRows + q * 32 + lane, 0);
+      for (int j = 0; j < kAhead; ++j) load_scales();
     }
     while (ok && t.n > 0) {
       const int b = t.chunk * kChunkRows + q * 32 + lane;
@@ -552,61 +586,67 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int mine_n = (t.n - part + kQuadWarps - 1) / kQuadWarps;  // groups part, part + 2, ...
       int group[kUnits];
       uint32_t legal[kUnits];
-      float2 acc[kUnits][16];
-      float hs[4], ws[kUnits];
+      unsigned long long acc[kUnits][16];  // pairs of fp32 sums
+      float ws[kUnits], ws_later[kUnits];
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         group[u] = group_next[u];
         legal[u] = tail_clip(legal_next[u], group[u], p.vocab);
         ws[u] = ws_next[u];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) acc[u][j] = make_float2(0.f, 0.f);
+        for (int j = 0; j < 16; ++j) acc[u][j] = 0ull;
       }
       t.next();
       load_tile();
-      const int b_next = t.chunk * kChunkRows + q * 32 + lane;
-      for (int kb0 = 0; ok && kb0 < p.blocks; kb0 += 4) {
+#pragma unroll 1
+      for (int kb = 0; kb < p.blocks; ++kb) {
+        if ((kb & 3) == 0) {
+          if (kb != 0) slot = (slot + kSlot) & (kSlots - 1);
+          load_scales();
+          cp_async_wait<kAhead>();
+          if ((kb & 31) == 0) {  // the groups' scales: a lane each for 32 stages, the next 32 under way
 #pragma unroll
-        for (int j = 0; j < 4; ++j) hs[j] = hs_next[j];
-        if (kb0 + 4 < p.blocks) load_hs(b, kb0 + 4);
-        else load_hs(b_next, 0);  // the next tile's
-        if (kb0 != 0 && (kb0 & 31) == 0) {
-#pragma unroll
-          for (int u = 0; u < kUnits; ++u) ws[u] = load_ws(group[u], kb0);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (!ok || kb0 + j >= p.blocks) break;
-          const uint32_t a = it % kAcc;
-          if (!mbar_wait(tfull + a, (it / kAcc) & 1u, abort_flag)) {
-            if (lane == 0) *abort_flag = 1;
-            ok = false;
-          }
-          ok = __all_sync(FULL_MASK, ok);
-          if (!ok) break;
-          tc_fence_after_sync();
-          const uint32_t col = tmem_base + ((uint32_t)(q * 32) << 16) + a * kAccCols + (uint32_t)part * kGroupRows;
-          // (all of the warp's groups, whether the tile has them: their sums are not used)
-#pragma unroll
-          for (int u = 0; u < kUnits; u += 2) {
-            uint32_t v[2][32];
-            tmem_ld_2x32(col + (uint32_t)(kQuadWarps * u) * kGroupRows, col + (uint32_t)(kQuadWarps * (u + 1)) * kGroupRows,
-                         v[0], v[1]);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float f = hs[j] * __shfl_sync(FULL_MASK, ws[u + e], (kb0 + j) & 31);
-#pragma unroll
-              for (int k = 0; k < 16; ++k)
-                acc[u + e][k] = fma2(make_float2(__uint_as_float(v[e][2 * k]), __uint_as_float(v[e][2 * k + 1])),
-                                     make_float2(f, f), acc[u + e][k]);
+            for (int u = 0; u < kUnits; ++u) {
+              if (kb != 0) ws[u] = ws_later[u];
+              ws_later[u] = load_ws(group[u], kb + 32);
             }
           }
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(tempty + a);
-          ++it;
+        }
+        const float h = reinterpret_cast<const float*>(s_scale + slot)[kb & 3];
+        unsigned long long ff[kUnits];
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          const uint32_t f = __float_as_uint(h * __shfl_sync(FULL_MASK, ws[u], kb & 31));
+          ff[u] = pack2(f, f);
+        }
+        if (!mbar_wait(tfull + a, parity, abort_flag)) *abort_flag = 1;  // (seen below)
+        tc_fence_after_sync();
+        __syncwarp();
+        const uint32_t col = acc_base + a * kAccCols;
+        // (all of the warp's groups, whether the tile has them: their sums are not used)
+#pragma unroll
+        for (int u = 0; u < kUnits; u += 2) {
+          uint32_t v[2][32];
+          tmem_ld_2x32(col + (uint32_t)(kQuadWarps * u) * kGroupRows, col + (uint32_t)(kQuadWarps * (u + 1)) * kGroupRows,
+                       v[0], v[1]);
+          if (u + 2 >= kUnits) {  // all read: the accumulator is free
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tempty + a);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[u + e][k] = fma2(pack2(v[e][2 * k], v[e][2 * k + 1]), ff[u + e], acc[u + e][k]);
+          }
+        }
+        if (++a == kAcc) {
+          a = 0;
+          parity ^= 1u;
         }
       }
+      slot = (slot + kSlot) & (kSlots - 1);
+      ok = !__any_sync(FULL_MASK, *abort_flag != 0);
       if (!ok) break;
       if (want_top && mine && b != best.row) {
         flush();
@@ -621,6 +661,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
     }
     if (want_top) flush();
+    cp_async_wait<0>();
   }
 
   tc_fence_before_sync();

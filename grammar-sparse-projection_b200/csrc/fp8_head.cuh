@@ -36,7 +36,8 @@ struct Fp8Params {
   // scratch of this call (contents undefined on entry)
   unsigned long long* keys;  // [batch] running top-1 keys, zeroed by the prologue
   unsigned int* tickets;     // [batch] (tensor-core kernel: the first only), zeroed by the prologue
-  float* scales_t;           // [blocks, batch]: the hidden states' scales, one block of columns a row
+  float* scales;             // [batch, scales_stride]: the hidden states' scales
+  int scales_stride;         // blocks rounded up to 4: rows of whole 16-byte vectors
   int32_t* groups;           // active 32-row vocabulary groups, kListGroups slots a builder block
   int32_t* group_counts;     // per builder block
   uint32_t* group_bits;      // the active groups as bits

@@ -19,8 +19,8 @@ namespace {
 constexpr int kBlock = 128;  // columns (and, of a weight, rows) that share a scale
 
 struct BlockScale {
-  float scale;
-  bool zero;
+  float scale, below, above;  // the scale's reciprocal, less and more 2^-21 of it
+  bool zero, divide;          // divide: the reciprocal is not finite (a denormal scale)
 };
 
 // magnitude: the largest |x| as fp32 bits (infinities and NaN above every finite value).
@@ -30,16 +30,28 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t magnitude) {
   const bool finite = amax < INFINITY;  // false for NaN
   s.scale = finite ? __fdiv_rn(amax, 448.f) : __int_as_float(0x7fc00000);
   s.zero = !finite || !(s.scale > 0.f);
+  const float inverse = __frcp_rn(s.scale);
+  s.below = inverse * (1.f - 0x1p-21f);
+  s.above = inverse * (1.f + 0x1p-21f);
+  s.divide = !(s.above < INFINITY);
   return s;
 }
 
-// Four values as four e4m3 bytes.
+__device__ __forceinline__ uint32_t e4m3_pair_of(float a, float b) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+// Four values as four e4m3 bytes. The quotients lie between the products with the two
+// reciprocals (each within 3 * 2^-24 of its exact value); where both products round to
+// one e4m3, and rounding is monotonic, so do the quotients, and that is nearly always.
+// Else they are divided out.
 __device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d, const BlockScale& s) {
   if (s.zero) return 0u;
-  const float2 lo = make_float2(__fdiv_rn(a, s.scale), __fdiv_rn(b, s.scale));
-  const float2 hi = make_float2(__fdiv_rn(c, s.scale), __fdiv_rn(d, s.scale));
-  return (uint32_t)__nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3) |
-         ((uint32_t)__nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3) << 16);
+  const uint32_t lo = e4m3_pair_of(a * s.below, b * s.below) | (e4m3_pair_of(c * s.below, d * s.below) << 16);
+  const uint32_t hi = e4m3_pair_of(a * s.above, b * s.above) | (e4m3_pair_of(c * s.above, d * s.above) << 16);
+  if (lo == hi && !s.divide) return lo;
+  return e4m3_pair_of(__fdiv_rn(a, s.scale), __fdiv_rn(b, s.scale)) |
+         (e4m3_pair_of(__fdiv_rn(c, s.scale), __fdiv_rn(d, s.scale)) << 16);
 }
 
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }

@@ -1127,15 +1127,15 @@ namespace {
 constexpr int32_t kMaxFp8Hidden = 32768;  // the row-sparse kernel keeps a hidden state in shared memory, in fp32
 
 struct Fp8Scratch {
-  size_t keys, tickets, values, scales_t, groups, counts, bits, total;
+  size_t keys, tickets, values, scales, groups, counts, bits, total;
   Fp8Scratch(int32_t batch, int32_t vocab, int32_t hidden_dim) {
     const size_t b = (size_t)batch, nw = ((size_t)vocab + 31) / 32, blocks = ((size_t)hidden_dim + kBlock - 1) / kBlock;
     const size_t builders = (nw + kListGroups - 1) / kListGroups;
     keys = 0;
     tickets = align256(8 * b);
     values = tickets + align256(4 * b);
-    scales_t = values + align256(b * int8_row_bytes(hidden_dim));
-    groups = scales_t + align256(4 * b * blocks);
+    scales = values + align256(b * int8_row_bytes(hidden_dim));
+    groups = scales + align256(4 * b * ((blocks + 3) / 4 * 4));
     counts = groups + align256(4 * builders * kListGroups);
     bits = counts + align256(4 * builders);
     total = bits + align256(4 * ((nw + 31) / 32));
@@ -1221,7 +1221,8 @@ int32_t gsp_fp8_logits(int32_t route, const void* hidden, int64_t hidden_row_str
   p.top_key = top_key;
   p.keys = reinterpret_cast<unsigned long long*>(at + room.keys);
   p.tickets = reinterpret_cast<unsigned int*>(at + room.tickets);
-  p.scales_t = reinterpret_cast<float*>(at + room.scales_t);
+  p.scales = reinterpret_cast<float*>(at + room.scales);
+  p.scales_stride = (blocks + 3) / 4 * 4;
   p.groups = reinterpret_cast<int32_t*>(at + room.groups);
   p.group_counts = reinterpret_cast<int32_t*>(at + room.counts);
   p.group_bits = reinterpret_cast<uint32_t*>(at + room.bits);

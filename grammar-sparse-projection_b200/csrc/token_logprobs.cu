@@ -82,6 +82,7 @@ struct Row {
   int64_t len;
   const uint32_t* mask;
   int64_t first;  // position of element 0 in the packed arrays
+  int last;       // vector that holds the last element
 };
 
 template <typename T>
@@ -92,47 +93,49 @@ __device__ __forceinline__ void set_row(Row& r, const void* logits, int64_t star
   r.phase = (int)((at & 15) / sizeof(Bits));
   r.len = len;
   r.first = start;
+  r.last = len > 0 ? (int)((len + r.phase + DTypeTraits<T>::kPerVec - 1) / DTypeTraits<T>::kPerVec) - 1 : -1;
 }
 
-template <typename T>
-__device__ __forceinline__ int64_t row_vectors(const Row& r) {
-  return r.len <= 0 ? 0 : (r.len + r.phase + DTypeTraits<T>::kPerVec - 1) / DTypeTraits<T>::kPerVec;
-}
-
-// Which of vector i's elements belong to the row and are legal.
+// Which of vector i's elements belong to the row and are legal. Rows that start on a
+// vector read the vector's own bits alone.
 template <typename T, bool kMask>
-__device__ __forceinline__ uint32_t legal_bits(const Row& r, int64_t i) {
+__device__ __forceinline__ uint32_t legal_bits(const Row& r, int i) {
   constexpr int kPer = DTypeTraits<T>::kPerVec;
-  const int64_t e0 = i * kPer - r.phase;
   uint32_t bits = (1u << kPer) - 1u;
   if constexpr (kMask) {
-    const int64_t w = e0 >> 5, nw = (r.len + 31) >> 5;
-    const int shift = (int)(e0 & 31);
-    const uint32_t lo = w >= 0 && w < nw ? __ldg(r.mask + w) : 0u;
-    const uint32_t hi = shift + kPer > 32 && w + 1 < nw ? __ldg(r.mask + w + 1) : 0u;
-    bits &= __funnelshift_r(lo, hi, shift);
+    if (r.phase == 0) {
+      const uint32_t byte = __ldg(reinterpret_cast<const uint8_t*>(r.mask) + (kPer == 8 ? i : i >> 1));
+      bits &= kPer == 8 ? byte : byte >> (4 * (i & 1));
+    } else {
+      const int e0 = i * kPer - r.phase, w = e0 >> 5, shift = e0 & 31, nw = (int)((r.len + 31) >> 5);
+      const uint32_t lo = w >= 0 ? __ldg(r.mask + w) : 0u;
+      const uint32_t hi = shift + kPer > 32 && w + 1 < nw ? __ldg(r.mask + w + 1) : 0u;
+      bits &= __funnelshift_r(lo, hi, shift);
+    }
   }
-  if (e0 < 0) bits &= ~((1u << (int)(-e0)) - 1u);
-  if (e0 + kPer > r.len) bits &= r.len > e0 ? (1u << (int)(r.len - e0)) - 1u : 0u;
+  if (i == r.last || i == 0) {  // (the row's edges)
+    const int e0 = i * kPer - r.phase, left = (int)r.len - e0;
+    if (e0 < 0) bits &= ~((1u << -e0) - 1u);
+    if (left < kPer) bits &= (1u << left) - 1u;
+  }
   return bits;
 }
 
 // -inf in the elements whose bit is not set.
 template <typename T>
 __device__ __forceinline__ void exclude(uint4& v, uint32_t bits) {
-  constexpr int kPer = DTypeTraits<T>::kPerVec;
-  if (bits == (1u << kPer) - 1u) return;
   uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (sizeof(typename DTypeTraits<T>::Bits) == 2) {
+    // bits 2k and 2k + 1 to the tops of a word's halves, whose signs spread over them
+    const uint32_t z = bits | (bits << 15), ninf = DTypeTraits<T>::kNegInfBits * 0x00010001u;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if constexpr (sizeof(typename DTypeTraits<T>::Bits) == 2) {
-      const uint32_t two = bits >> (2 * k);
-      const uint32_t keep = ((two & 1u) ? 0x0000ffffu : 0u) | ((two & 2u) ? 0xffff0000u : 0u);
-      const uint32_t ninf = DTypeTraits<T>::kNegInfBits * 0x00010001u;
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t keep = spread_half_signs(z << (15 - 2 * k));
       w[k] = (w[k] & keep) | (ninf & ~keep);
-    } else {
-      w[k] = ((bits >> k) & 1u) ? w[k] : 0xff800000u;
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = ((bits >> k) & 1u) ? w[k] : 0xff800000u;
   }
   v = make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -206,14 +209,16 @@ __device__ __forceinline__ Sums merge(Sums x, Sums y, float c) {
 
 struct Shared {
   Sums part[kThreads / 32];
-  Sums total;  // this CTA's, read by the cluster
-  unsigned int ninf;
+  Sums total[kMaxClusterSize];  // every CTA's, written by them
+  unsigned int ninf, all_ninf[kMaxClusterSize];
   float group_top[kThreads / 8];
   unsigned int count;
   int listed;
   unsigned long long border;
   alignas(16) unsigned long long list[kListSize];
   unsigned long long best[kMaxTop];
+  // CTA 0's: the lists of all (n keys each in falling order, 0: none), written by them
+  alignas(16) unsigned long long all[kMaxClusterSize * kMaxTop];
 };
 
 // The n largest of the list's keys, in falling order, at its front. Called by
@@ -262,7 +267,7 @@ __device__ __forceinline__ uint32_t candidates(const uint4& v, float least) {
 
 // Lists vector v's waiting elements; those that find no room stay waiting.
 template <typename T>
-__device__ __forceinline__ uint32_t list_candidates(Shared& s, const uint4& v, uint32_t waiting, int64_t e0,
+__device__ __forceinline__ uint32_t list_candidates(Shared& s, const uint4& v, uint32_t waiting, int e0,
                                                     unsigned long long border, int limit, bool& full) {
 #pragma unroll
   for (int j = 0; j < DTypeTraits<T>::kPerVec; ++j) {
@@ -293,8 +298,11 @@ template <typename T, bool kMask, bool kTop>
 __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const LogprobParams p) {
   using Bits = typename DTypeTraits<T>::Bits;
   constexpr int kPer = DTypeTraits<T>::kPerVec;
+  constexpr uint32_t kAll = (1u << kPer) - 1u;
   __shared__ Shared s;
   cg::cluster_group cluster = cg::this_cluster();
+  // (nothing is written to a CTA's shared memory before it runs)
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t b = blockIdx.x / size;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -312,8 +320,8 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
   const float t = p.temperatures ? p.temperatures[b] : p.temperature;
   const bool valid = valid_temperature(t);
   const float c = fminf(kLog2e / t, 3e38f);
-  const int64_t nv = valid ? row_vectors<T>(r) : 0;
-  const int64_t lo = nv * rank / size, hi = nv * (rank + 1) / size;
+  const int nv = valid ? r.last + 1 : 0;
+  const int lo = (int)((int64_t)nv * rank / size), hi = (int)((int64_t)nv * (rank + 1) / size);
   const int n = p.top_n;
 
   if (tid == 0) {
@@ -327,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
   uint32_t bits[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t i = lo + u * kThreads + tid;
+    const int i = lo + u * kThreads + tid;
     bits[u] = i < hi ? legal_bits<T, kMask>(r, i) : 0u;
     v[u] = i < hi ? ld_stream_v4(r.base + i) : make_uint4(0u, 0u, 0u, 0u);
   }
@@ -337,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     exclude<T>(v[u], bits[u]);
-    bits[u] = (1u << kPer) - 1u;
+    bits[u] = kAll;
     top = fmaxf(top, vector_top<T>(v[u]));
   }
 #pragma unroll
@@ -371,14 +379,14 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
   Running run{top, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 
   const int limit = n + kListFull;
-  for (int64_t i0 = lo; i0 < hi; i0 += kUnroll * kThreads) {
+  for (int i0 = lo; i0 < hi; i0 += kUnroll * kThreads) {
     uint32_t waiting = 0u;  // candidates that found no room, by vector and element
     bool full = false;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int64_t i = i0 + u * kThreads + tid, after = i + kUnroll * kThreads;
+      const int i = i0 + u * kThreads + tid, after = i + kUnroll * kThreads;
       uint4 now = v[u];
-      exclude<T>(now, bits[u]);
+      if (kMask || bits[u] != kAll) exclude<T>(now, bits[u]);
       bits[u] = after < hi ? legal_bits<T, kMask>(r, after) : 0u;
       v[u] = after < hi ? ld_stream_v4(r.base + after) : make_uint4(0u, 0u, 0u, 0u);
       const float vt = vector_top<T>(now);
@@ -400,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
         for (int u = 0; waiting != 0u && u < kUnroll; ++u) {
           const uint32_t mine = (waiting >> (u * kPer)) & ((1u << kPer) - 1u);
           if (!mine) continue;
-          const int64_t i = i0 + u * kThreads + tid;
+          const int i = i0 + u * kThreads + tid;
           const uint32_t left = list_candidates<T>(s, ld_stream_v4(r.base + i), mine, i * kPer - r.phase, border, limit, full);
           waiting = (waiting & ~(mine << (u * kPer))) | (left << (u * kPer));
         }
@@ -423,17 +431,27 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
     for (int o = kThreads / 64; o > 0; o >>= 1)
       mine = merge(mine, Sums{__shfl_xor_sync(FULL_MASK, mine.m, o), __shfl_xor_sync(FULL_MASK, mine.s, o),
                               __shfl_xor_sync(FULL_MASK, mine.a, o)}, c);
-    if (lane == 0) s.total = mine;
+    if (lane == 0) s.part[0] = mine;
   }
-  if (size > 1) cluster.sync();
-  else __syncthreads();
-
+  __syncthreads();
+  // to the other CTAs' shared memory (all of them run: the barrier at the start): what a
+  // CTA would have to fetch takes it 15 us for 16 lists of 20
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (size > 1) {
+    if (tid < size) cluster.map_shared_rank(s.total, tid)[rank] = s.part[0];
+    if (kTop && tid < n) cluster.map_shared_rank(s.all, 0)[rank * n + tid] = tid < s.listed ? s.list[tid] : 0ull;
+    cluster.sync();
+  } else {
+    if (tid == 0) s.total[0] = s.part[0];
+    if (kTop && tid < n) s.all[tid] = tid < s.listed ? s.list[tid] : 0ull;
+    __syncthreads();
+  }
   // the cluster's, the same in every thread (merged in rank order)
-  Sums sum = *cluster.map_shared_rank(&s.total, 0);
-  for (int q = 1; q < size; ++q) sum = merge(sum, *cluster.map_shared_rank(&s.total, q), c);
+  Sums sum = s.total[0];
+  for (int q = 1; q < size; ++q) sum = merge(sum, s.total[q], c);
   if (sum.m == INFINITY) {  // infinite logits share the weight: S counts them
     unsigned int found = 0u;
-    for (int64_t i = lo + tid; i < hi; i += kThreads) {
+    for (int i = lo + tid; i < hi; i += kThreads) {
       uint4 x = ld_stream_v4(r.base + i);
       exclude<T>(x, legal_bits<T, kMask>(r, i));
 #pragma unroll
@@ -443,10 +461,12 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
       }
     }
     if (found) atomicAdd(&s.ninf, found);
+    __syncthreads();
+    if (tid == 0) cluster.map_shared_rank(s.all_ninf, 0)[rank] = s.ninf;
     if (size > 1) cluster.sync();
     else __syncthreads();
     unsigned int all = 0u;
-    for (int q = 0; q < size; ++q) all += *cluster.map_shared_rank(&s.ninf, q);
+    for (int q = 0; q < size; ++q) all += s.all_ninf[q];  // (CTA 0's are all there)
     sum.s = (float)all;
     sum.a = 0.f;
   }
@@ -480,18 +500,17 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
       p.logprobs[b * p.tokens + k] = !valid ? nan : id < 0 ? 0.f : lp;
     }
     if constexpr (kTop) {
-      // the CTAs' lists, each in falling order: a key's place is the number of larger ones
-      const int all = size * n;
-      for (int i = tid; i < all; i += kThreads) {
-        const int q = i / n, at = i - q * n;
-        if (at >= *cluster.map_shared_rank(&s.listed, q)) continue;
-        const unsigned long long key = cluster.map_shared_rank(s.list, q)[at];
-        int place = at;
+      // a key's place is the number of larger ones, counted in the lists one by one
+      for (int i = tid; i < size * n; i += kThreads) {
+        const unsigned long long key = s.all[i];
+        const int q = i / n;
+        if (key == 0ull) continue;
+        int place = i - q * n;
         for (int o = 0; o < size && place < n; ++o) {
           if (o == q) continue;
-          const unsigned long long* other = cluster.map_shared_rank(s.list, o);
-          int a = 0, z = *cluster.map_shared_rank(&s.listed, o);
-          while (a < z) {  // larger keys come first
+          const unsigned long long* other = s.all + o * n;
+          int a = 0, z = n;
+          while (a < z) {  // larger keys come first, and none (0) last
             const int mid = (a + z) >> 1;
             if (other[mid] > key) a = mid + 1;
             else z = mid;
@@ -504,14 +523,14 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
         p.top_logprobs[b * n + place] = logprob_of(key_value(key), sum.m, t, log_s);
       }
       int listed = 0;
-      for (int q = 0; q < size; ++q) listed += *cluster.map_shared_rank(&s.listed, q);
+      for (int i = lane; i < size * n; i += 32) listed += s.all[i] != 0ull;
+      listed = warp_sum(listed);
       for (int i = min(listed, n) + tid; i < n; i += kThreads) {
         p.top_ids[b * n + i] = -1;
         p.top_logprobs[b * n + i] = valid ? -INFINITY : nan;
       }
     }
   }
-  if (size > 1) cluster.sync();  // (shared memory is read until here)
 }
 
 template <typename T, bool kMask, bool kTop>
@@ -601,13 +620,12 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
   Row r;
   set_row<T>(r, p.logits, b * p.row_stride, p.vocab);
   r.mask = kMask ? p.mask + b * p.mask_stride : nullptr;
-  const int64_t nv = row_vectors<T>(r);
-  const int64_t i0 = (int64_t)slice * kGradThreads * kUnroll, hi = min(nv, i0 + kGradThreads * kUnroll);
+  const int nv = r.last + 1, i0 = slice * kGradThreads * kUnroll, hi = min(nv, i0 + kGradThreads * kUnroll);
   uint4 v[kUnroll];
   uint32_t bits[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t i = i0 + u * kGradThreads + tid;
+    const int i = i0 + u * kGradThreads + tid;
     bits[u] = i < hi ? legal_bits<T, kMask>(r, i) : 0u;
     v[u] = i < hi ? ld_stream_v4(r.base + i) : make_uint4(0u, 0u, 0u, 0u);
   }
@@ -637,10 +655,10 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
   const bool same_phase = (reinterpret_cast<uintptr_t>(out - r.phase) & 15) == 0;
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t i = i0 + u * kGradThreads + tid;
+    const int i = i0 + u * kGradThreads + tid;
     if (i >= hi) continue;
     uint4 x = v[u];
-    exclude<T>(x, bits[u]);
+    if (kMask || bits[u] != (1u << kPer) - 1u) exclude<T>(x, bits[u]);
     float y[kPer];
 #pragma unroll
     for (int k = 0; k < kPer / 2; ++k) {
@@ -648,7 +666,7 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
       y[2 * k] = f.x > -INFINITY && !row.none ? row.at(f.x) * st.w : 0.f;
       y[2 * k + 1] = f.y > -INFINITY && !row.none ? row.at(f.y) * st.w : 0.f;
     }
-    const int64_t e0 = i * kPer - r.phase;
+    const int e0 = i * kPer - r.phase;
     if (same_phase && e0 >= 0 && e0 + kPer <= r.len) {
       uint32_t w[4];
 #pragma unroll
@@ -667,7 +685,7 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
   }
   if (!g || row.none) return;
   __syncthreads();  // the stores above come before those below
-  const int64_t first = i0 * kPer - r.phase, last = hi * kPer - r.phase;
+  const int64_t first = (int64_t)i0 * kPer - r.phase, last = (int64_t)hi * kPer - r.phase;
   for (int k = tid; k < p.tokens; k += kGradThreads) {
     const int64_t id = ids[k];
     if (id < 0 || id < first || id >= last || id >= r.len) continue;

@@ -30,7 +30,8 @@ __device__ __forceinline__ BlockScale block_scale(uint32_t magnitude) {
   const bool finite = amax < INFINITY;  // false for NaN
   s.scale = finite ? __fdiv_rn(amax, 448.f) : __int_as_float(0x7fc00000);
   s.zero = !finite || !(s.scale > 0.f);
-  const float inverse = __frcp_rn(s.scale);
+  float inverse;  // (within 2^-23; a denormal scale's is infinite)
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(s.scale));
   s.below = inverse * (1.f - 0x1p-21f);
   s.above = inverse * (1.f + 0x1p-21f);
   s.divide = !(s.above < INFINITY);
@@ -42,7 +43,7 @@ __device__ __forceinline__ uint32_t e4m3_pair_of(float a, float b) {
 }
 
 // Four values as four e4m3 bytes. The quotients lie between the products with the two
-// reciprocals (each within 3 * 2^-24 of its exact value); where both products round to
+// reciprocals (each within 2^-22 of its exact value); where both products round to
 // one e4m3, and rounding is monotonic, so do the quotients, and that is nearly always.
 // Else they are divided out.
 __device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d, const BlockScale& s) {
@@ -83,21 +84,49 @@ struct Units {
   static __device__ __forceinline__ int column(int unit, int j) {
     return kVec ? unit * kElems + j : (unit >> 5) * kBlock + (unit & 31) + 32 * j;
   }
+  // A unit as it is held: a vector in the row's type, or four fp32 values.
+  static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[kElems]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (!kVec || sizeof(Bits) == 4) {
+        f[k] = __uint_as_float(w[k]);
+      } else {
+        const float2 two = DTypeTraits<T>::pair_to_float2(w[k]);
+        f[2 * k] = two.x;
+        f[2 * k + 1] = two.y;
+      }
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[kElems]) {  // rounded to the row's type
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (sizeof(Bits) == 4) w[k] = __float_as_uint(f[k]);
+      else if constexpr (!kVec) w[k] = __float_as_uint(DTypeTraits<T>::bits_to_float(DTypeTraits<T>::round_bits(f[k])));
+      else w[k] = (uint32_t)DTypeTraits<T>::round_bits(f[2 * k]) | ((uint32_t)DTypeTraits<T>::round_bits(f[2 * k + 1]) << 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ uint4 load_packed(const Bits* row, int unit, int cols) {
+    if constexpr (kVec) return ld_stream_v4(reinterpret_cast<const uint4*>(row) + unit);
+    float f[kElems];
+    load(row, unit, cols, f);
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  static __device__ __forceinline__ void store_packed(Bits* row, int unit, int cols, const uint4& v) {
+    if constexpr (kVec) {
+      reinterpret_cast<uint4*>(row)[unit] = v;
+    } else {
+      float f[kElems];
+      unpack(v, f);
+      store(row, unit, cols, f);
+    }
+  }
   // (elements past the row are 0)
   static __device__ __forceinline__ void load(const Bits* row, int unit, int cols, float (&f)[kElems]) {
     if constexpr (kVec) {
-      const uint4 v = ld_stream_v4(reinterpret_cast<const uint4*>(row) + unit);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (sizeof(Bits) == 4) {
-          f[k] = __uint_as_float(w[k]);
-        } else {
-          const float2 two = DTypeTraits<T>::pair_to_float2(w[k]);
-          f[2 * k] = two.x;
-          f[2 * k + 1] = two.y;
-        }
-      }
+      unpack(ld_stream_v4(reinterpret_cast<const uint4*>(row) + unit), f);
     } else {
 #pragma unroll
       for (int j = 0; j < kElems; ++j) {
@@ -108,13 +137,7 @@ struct Units {
   }
   static __device__ __forceinline__ void store(Bits* row, int unit, int cols, const float (&f)[kElems]) {
     if constexpr (kVec) {
-      uint32_t w[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (sizeof(Bits) == 4) w[k] = __float_as_uint(f[k]);
-        else w[k] = (uint32_t)DTypeTraits<T>::round_bits(f[2 * k]) | ((uint32_t)DTypeTraits<T>::round_bits(f[2 * k + 1]) << 16);
-      }
-      reinterpret_cast<uint4*>(row)[unit] = make_uint4(w[0], w[1], w[2], w[3]);
+      reinterpret_cast<uint4*>(row)[unit] = pack(f);
     } else {
 #pragma unroll
       for (int j = 0; j < kElems; ++j) {

@@ -73,9 +73,9 @@ __device__ __forceinline__ uint32_t to_int8(float a, float b, float c, float d, 
          (((uint32_t)quantize_value(c, s) & 0xffu) << 16) | (((uint32_t)quantize_value(d, s) & 0xffu) << 24);
 }
 
-// kHeld: units a thread holds.
-template <typename T, bool kVec, int kOut, int kHeld, int kThreads>
-__global__ void __launch_bounds__(kThreads) rms_norm_kernel(const __grid_constant__ NormParams p) {
+// kHeld: units a thread holds, in the row's type. kLong: rows may be longer than that.
+template <typename T, bool kVec, int kOut, int kHeld, int kThreads, int kThreadsPerSm, bool kLong>
+__global__ void __launch_bounds__(kThreads, kThreadsPerSm / kThreads) rms_norm_kernel(const __grid_constant__ NormParams p) {
   using U = Units<T, kVec>;
   using Bits = typename U::Bits;
   constexpr int kE = U::kElems;
@@ -92,16 +92,17 @@ __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const __grid_constan
   const Bits* weight = static_cast<const Bits*>(p.weight);
   const int n = live ? U::count(cols) : 0;
 
-  // h of a unit, written to the residual stream the first time
-  const auto sum_of = [&](int i, float (&h)[kE]) {
-    U::load(x, i, cols, h);
-    if (res) {
-      float r[kE];
-      U::load(res, i, cols, r);
+  // h of a unit: with a residual their rounded sum, which the residual stream takes
+  const auto sum_of = [&](int i, const uint4& v) {
+    if (!res) return v;
+    float a[kE], b[kE];
+    U::unpack(v, a);
+    U::unpack(U::load_packed(res, i, cols), b);
 #pragma unroll
-      for (int j = 0; j < kE; ++j) h[j] = DTypeTraits<T>::bits_to_float(DTypeTraits<T>::round_bits(h[j] + r[j]));
-      U::store(res_out, i, cols, h);
-    }
+    for (int j = 0; j < kE; ++j) a[j] += b[j];
+    const uint4 h = U::pack(a);
+    U::store_packed(res_out, i, cols, h);
+    return h;
   };
   const auto again = [&](int i, float (&h)[kE]) {  // (this thread's own store, or the input)
     if (!res) {
@@ -114,30 +115,29 @@ __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const __grid_constan
       h[j] = c < cols ? DTypeTraits<T>::bits_to_float(*(volatile const Bits*)(res_out + c)) : 0.f;
     }
   };
+  const auto squares_of = [&](const uint4& v) {
+    float f[kE], sum = 0.f;
+    U::unpack(v, f);
+#pragma unroll
+    for (int j = 0; j < kE; ++j) sum = fmaf(f[j], f[j], sum);
+    return sum;
+  };
 
-  float h[kHeld][kE];
+  uint4 held[kHeld];
 #pragma unroll
   for (int c = 0; c < kHeld; ++c) {
     const int i = t + c * nt;
-    if (i < n) {
-      sum_of(i, h[c]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kE; ++j) h[c][j] = 0.f;
-    }
+    held[c] = i < n ? U::load_packed(x, i, cols) : make_uint4(0u, 0u, 0u, 0u);
   }
   float squares = 0.f;
 #pragma unroll
   for (int c = 0; c < kHeld; ++c) {
-#pragma unroll
-    for (int j = 0; j < kE; ++j) squares = fmaf(h[c][j], h[c][j], squares);
+    const int i = t + c * nt;
+    if (i < n) held[c] = sum_of(i, held[c]);
+    squares += squares_of(held[c]);
   }
-  for (int i = t + kHeld * nt; i < n; i += nt) {
-    float more[kE], part = 0.f;
-    sum_of(i, more);
-#pragma unroll
-    for (int j = 0; j < kE; ++j) part = fmaf(more[j], more[j], part);
-    squares += part;
+  if constexpr (kLong) {
+    for (int i = t + kHeld * nt; i < n; i += nt) squares += squares_of(sum_of(i, U::load_packed(x, i, cols)));
   }
   // (each thread's part of the mean: the sum over the row of squares near fp32's largest would pass it)
   const float mean = over_group<false>(__fdiv_rn(squares, (float)cols), gw, s_sum);
@@ -146,14 +146,8 @@ __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const __grid_constan
   const auto normed = [&](int i, float (&v)[kE]) {  // h -> y
     if (weight) {
       float w[kE];
-      if constexpr (kVec) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(weight) + i);
-        const uint32_t word[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int j = 0; j < kE; ++j) w[j] = element<T>(word, j);
-      } else {
-        U::load(weight, i, cols, w);
-      }
+      if constexpr (kVec) U::unpack(__ldg(reinterpret_cast<const uint4*>(weight) + i), w);
+      else U::load(weight, i, cols, w);
 #pragma unroll
       for (int j = 0; j < kE; ++j) v[j] = v[j] * by * w[j];
     } else {
@@ -161,63 +155,52 @@ __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const __grid_constan
       for (int j = 0; j < kE; ++j) v[j] = v[j] * by;
     }
   };
-  // (lanes past the row take part in the blocks' maxima, with zeros)
-  const int upper = (n + 31) & ~31;
+  // every unit of the thread's, as y
+  const auto each = [&](auto&& use) {
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c) {
+      const int i = t + c * nt;
+      float v[kE];
+      U::unpack(held[c], v);
+      if (i < n) normed(i, v);
+      use(i, v);
+    }
+    if constexpr (kLong) {
+      for (int i = t + kHeld * nt; i < ((n + 31) & ~31); i += nt) {  // (whole warps)
+        float v[kE];
+        if (i < n) {
+          again(i, v);
+          normed(i, v);
+        }
+        use(i, v);
+      }
+    }
+  };
 
   if constexpr (kOut == kSame) {
     Bits* out = static_cast<Bits*>(p.out) + at * p.out_stride;
-#pragma unroll
-    for (int c = 0; c < kHeld; ++c) {
-      const int i = t + c * nt;
-      if (i >= n) continue;
-      normed(i, h[c]);
-      U::store(out, i, cols, h[c]);
-    }
-    for (int i = t + kHeld * nt; i < n; i += nt) {
-      float v[kE];
-      again(i, v);
-      normed(i, v);
-      U::store(out, i, cols, v);
-    }
+    each([&](int i, const float (&v)[kE]) {
+      if (i < n) U::store(out, i, cols, v);
+    });
   } else if constexpr (kOut == kInt8) {
     uint8_t* out = static_cast<uint8_t*>(p.out) + at * p.out_stride;
     uint32_t top = 0u;
-#pragma unroll
-    for (int c = 0; c < kHeld; ++c) {
-      const int i = t + c * nt;
-      if (i >= n) continue;
-      normed(i, h[c]);
-      top = max(top, U::magnitude(h[c]));
-    }
-    for (int i = t + kHeld * nt; i < n; i += nt) {
-      float v[kE];
-      again(i, v);
-      normed(i, v);
-      top = max(top, U::magnitude(v));
-    }
+    each([&](int i, const float (&v)[kE]) {
+      if (i < n) top = max(top, U::magnitude(v));
+    });
     const RowScale scale = row_scale(over_group<true>(__uint_as_float(top), gw, s_max), false);
     if (live && t == 0) p.scales[row] = scale.scale;
-    const auto put = [&](int i, const float (&v)[kE]) {
+    each([&](int i, const float (&v)[kE]) {
+      if (i >= n) return;
       uint32_t w[kE / 4];
 #pragma unroll
       for (int k = 0; k < kE / 4; ++k) w[k] = to_int8(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3], scale);
       U::store_bytes(out, i, cols, w);
-    };
-#pragma unroll
-    for (int c = 0; c < kHeld; ++c) {
-      const int i = t + c * nt;
-      if (i < n) put(i, h[c]);
-    }
-    for (int i = t + kHeld * nt; i < n; i += nt) {
-      float v[kE];
-      again(i, v);
-      normed(i, v);
-      put(i, v);
-    }
+    });
   } else {
     uint8_t* out = static_cast<uint8_t*>(p.out) + at * p.out_stride;
     float* scales = p.scales + at * p.scales_stride;
-    const auto put = [&](int i, const float (&v)[kE]) {  // all lanes of the warp
+    each([&](int i, const float (&v)[kE]) {  // (lanes past the row take part in the blocks' maxima)
       const BlockScale s = block_scale(lanes_max<U::kLanes>(i < n ? U::magnitude(v) : 0u));
       if (i >= n) return;
       uint32_t w[kE / 4];
@@ -225,22 +208,7 @@ __global__ void __launch_bounds__(kThreads) rms_norm_kernel(const __grid_constan
       for (int k = 0; k < kE / 4; ++k) w[k] = to_e4m3(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3], s);
       U::store_bytes(out, i, cols, w);
       if (i % U::kLanes == 0) scales[i / U::kLanes] = s.scale;
-    };
-#pragma unroll
-    for (int c = 0; c < kHeld; ++c) {
-      const int i = t + c * nt;
-      if (i >= upper) continue;
-      if (i < n) normed(i, h[c]);
-      put(i, h[c]);
-    }
-    for (int i = t + kHeld * nt; i < upper; i += nt) {
-      float v[kE];
-      if (i < n) {
-        again(i, v);
-        normed(i, v);
-      }
-      put(i, v);
-    }
+    });
   }
 }
 
@@ -250,25 +218,23 @@ cudaError_t launch_norm(NormParams p, cudaStream_t stream) {
   const cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   constexpr int kE = Units<T, kVec>::kElems;
-  // Warps per row: as few as hold it in 32 registers a thread; with few rows more,
-  // while the SMs have room and a thread has more than 8.
+  // Warps per row: 8 values a thread, from 8,192 columns on 16 and 32: a row is soon done,
+  // and most of the SM's threads are resident. Rows of few warps share a CTA.
   const int64_t units = kVec ? p.cols / kE : ((int64_t)p.cols + kBlock - 1) / kBlock * 32;
   int gw = 1;
-  while (gw < 16 && (units * kE > (int64_t)32 * gw * 32 ||
-                     (units * kE > (int64_t)32 * gw * 8 && p.rows * gw < (int64_t)num_sms(dev) * 8)))
-    gw *= 2;
+  while (gw < 16 && units * kE > (int64_t)32 * gw * 8) gw *= 2;
   p.group_warps = gw;
-  const int64_t floats = (units + 32 * gw - 1) / (32 * gw) * kE;
-  const int threads = gw == 16 ? 512 : 256;
+  const int threads = std::max(256, 32 * gw);
   const int64_t per_cta = threads / 32 / gw, grid = (p.rows + per_cta - 1) / per_cta;
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  if (gw == 16) {
-    if (floats <= 8) rms_norm_kernel<T, kVec, kOut, 8 / kE, 512><<<(unsigned)grid, 512, 0, stream>>>(p);
-    else rms_norm_kernel<T, kVec, kOut, 32 / kE, 512><<<(unsigned)grid, 512, 0, stream>>>(p);
-  } else {
-    if (floats <= 8) rms_norm_kernel<T, kVec, kOut, 8 / kE, 256><<<(unsigned)grid, 256, 0, stream>>>(p);
-    else rms_norm_kernel<T, kVec, kOut, 32 / kE, 256><<<(unsigned)grid, 256, 0, stream>>>(p);
-  }
+  const unsigned g = (unsigned)grid;
+  const int64_t floats = units * kE, row_threads = 32 * gw;
+  const auto run = [&](auto kernel) { kernel<<<g, (unsigned)threads, 0, stream>>>(p); };
+  if (threads == 256) run(rms_norm_kernel<T, kVec, kOut, 8 / kE, 256, 1536, false>);
+  else if (floats <= row_threads * 8) run(rms_norm_kernel<T, kVec, kOut, 8 / kE, 512, 1536, false>);
+  else if (floats <= row_threads * 16) run(rms_norm_kernel<T, kVec, kOut, 16 / kE, 512, 1536, false>);
+  else if (floats <= row_threads * 32) run(rms_norm_kernel<T, kVec, kOut, 32 / kE, 512, 1024, false>);
+  else run(rms_norm_kernel<T, kVec, kOut, 32 / kE, 512, 1024, true>);
   return cudaGetLastError();
 }
 

@@ -21,9 +21,9 @@
 // the two rare cases (a new maximum, a candidate) share that one test. All
 // threads start from the maximum of the CTA's first batch of vectors, and the
 // alternatives from the n-th largest of its 64 eight-lane maxima, so hardly any
-// vector takes the slow path after it. Candidates gather in a list, are ranked
-// by counting when it fills, and what does not fit is tried again against the
-// higher border: rows in rising order or of equal values cost time, not results.
+// vector takes the slow path after it. Candidates gather in a list that is ranked by
+// counting each time the row read has doubled; a list that overflows (rows in rising
+// order, equal values) is made again with a barrier for every vector: time, not results.
 //
 // Sums run in fp32: a thread adds at most a few hundred terms, then a tree.
 #include <cooperative_groups.h>
@@ -45,7 +45,6 @@ constexpr int kThreads = 512;
 constexpr int kUnroll = 4;       // 16-byte vectors a thread has under way
 constexpr int kMaxTop = 64;      // alternatives
 constexpr int kListSize = 1024;  // candidates held at a time
-constexpr int kListFull = 96;    // candidates past n at which the list is ranked
 constexpr int kMaxClusterSize = 16;
 constexpr int kMaxTokens = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -170,32 +169,88 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// The exponents d = (x - m) c of a vector's elements, in pairs, none below kNothing
+// (-inf, NaN and what is far below: nothing). Halves are held back at `floor` before they
+// are widened: a value of the type at or below m + kNothing / c, two in each word.
+template <typename T>
+struct Exponents {
+  unsigned long long neg, by;
+  uint32_t floor;
+  bool deep;  // the type has no such value (a maximum near its lowest): held back in fp32
+  __device__ __forceinline__ void set(float m, float c) {
+    neg = pack2(-m, -m);
+    by = pack2(c, c);
+    // (a maximum so large that the difference is lost in it: the number below it, whose
+    // weight is nothing as well)
+    float low = m + kNothing / c;
+    if (!(low < m)) low = m > 0.f ? __uint_as_float(__float_as_uint(m) - 1u) : __uint_as_float(__float_as_uint(m) + 1u);
+    floor = 0u;
+    deep = true;
+    if constexpr (std::is_same<T, __half>::value) {
+      deep = !(low >= -65504.f);
+      floor = (uint32_t)__half_as_ushort(__float2half_rd(low)) * 0x00010001u;
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      deep = !(low >= -3.3895313892515355e38f);
+      floor = (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rd(low)) * 0x00010001u;
+    }
+  }
+  template <bool kDeep>
+  __device__ __forceinline__ unsigned long long at(const uint4& v, int k) const {  // of elements 2k, 2k + 1
+    if constexpr (kDeep) {
+      const float2 x = element_pair<T>(v, k);
+      const float2 d = unpack2(mul2(add2(pack2(x.x, x.y), neg), by));
+      return pack2(fmaxf(d.x, kNothing), fmaxf(d.y, kNothing));
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      const T2 held = __hmax2(*reinterpret_cast<const T2*>(&w[k]), *reinterpret_cast<const T2*>(&floor));
+      const float2 x = DTypeTraits<T>::pair_to_float2(*reinterpret_cast<const uint32_t*>(&held));
+      return mul2(add2(pack2(x.x, x.y), neg), by);
+    }
+  }
+};
+
 // A thread's running maximum and sums relative to it, in two lanes each.
+template <typename T>
 struct Running {
   float m;
-  float2 s, a;
+  unsigned long long s, a;
+  Exponents<T> d;
+  __device__ __forceinline__ void start(float top, float c) {
+    m = top;
+    s = a = 0ull;
+    d.set(m, c);
+  }
   // Moves the reference from m up to `to`: s 2^delta, a -> 2^delta (a + delta s).
   __device__ __forceinline__ void raise(float to, float c) {
     const float delta = fmaxf((m - to) * c, kNothing);
     const float f = exp2_approx(delta);
-    a = make_float2(f * fmaf(delta, s.x, a.x), f * fmaf(delta, s.y, a.y));
-    s = make_float2(f * s.x, f * s.y);
+    a = mul2(pack2(f, f), fma2(pack2(delta, delta), s, a));
+    s = mul2(pack2(f, f), s);
     m = to;
+    d.set(m, c);
+  }
+  __device__ __forceinline__ void add(const uint4& v) {
+    if constexpr (!std::is_same<T, float>::value) {
+      if (!d.deep) {
+        add_as<false>(v);
+        return;
+      }
+    }
+    add_as<true>(v);
+  }
+  template <bool kDeep>
+  __device__ __forceinline__ void add_as(const uint4& v) {
+#pragma unroll
+    for (int k = 0; k < DTypeTraits<T>::kPerVec / 2; ++k) {
+      const unsigned long long dd = d.template at<kDeep>(v, k);
+      const float2 one = unpack2(dd);
+      const unsigned long long e = pack2(exp2_approx(one.x), exp2_approx(one.y));
+      s = add2(s, e);
+      a = fma2(e, dd, a);
+    }
   }
 };
-
-template <typename T>
-__device__ __forceinline__ void accumulate(Running& r, const uint4& v, float c) {
-  const float2 neg = make_float2(-r.m, -r.m), cc = make_float2(c, c);
-#pragma unroll
-  for (int k = 0; k < DTypeTraits<T>::kPerVec / 2; ++k) {
-    float2 d = mul2(add2(element_pair<T>(v, k), neg), cc);
-    d = make_float2(fmaxf(d.x, kNothing), fmaxf(d.y, kNothing));  // (-inf, NaN and what is far below: nothing)
-    const float2 e = make_float2(exp2_approx(d.x), exp2_approx(d.y));
-    r.s = add2(r.s, e);
-    r.a = fma2(e, d, r.a);
-  }
-}
 
 struct Sums {
   float m, s, a;
@@ -213,7 +268,7 @@ struct Shared {
   unsigned int ninf, all_ninf[kMaxClusterSize];
   float group_top[kThreads / 8];
   unsigned int count;
-  int listed;
+  int listed, overflow;
   unsigned long long border;
   alignas(16) unsigned long long list[kListSize];
   unsigned long long best[kMaxTop];
@@ -265,10 +320,10 @@ __device__ __forceinline__ uint32_t candidates(const uint4& v, float least) {
   return found;
 }
 
-// Lists vector v's waiting elements; those that find no room stay waiting.
+// Lists vector v's waiting elements past the border; those that find no room stay waiting.
 template <typename T>
 __device__ __forceinline__ uint32_t list_candidates(Shared& s, const uint4& v, uint32_t waiting, int e0,
-                                                    unsigned long long border, int limit, bool& full) {
+                                                    unsigned long long border) {
 #pragma unroll
   for (int j = 0; j < DTypeTraits<T>::kPerVec; ++j) {
     if (!((waiting >> j) & 1u)) continue;
@@ -276,13 +331,42 @@ __device__ __forceinline__ uint32_t list_candidates(Shared& s, const uint4& v, u
     const unsigned long long key = top1_key(j & 1 ? x.y : x.x, (uint64_t)(e0 + j));
     if (key > border) {
       const unsigned at = atomicAdd(&s.count, 1u);
-      if ((int)at >= limit) full = true;
       if (at >= (unsigned)kListSize) continue;
       s.list[at] = key;
     }
     waiting &= ~(1u << j);
   }
   return waiting;
+}
+
+// The n largest keys of the vectors lo .. hi - 1 when the list has not held the
+// candidates (rows in rising order, or of equal values): a vector a thread and time, what
+// finds no room tried again against the border of what is listed.
+template <typename T, bool kMask>
+__device__ __noinline__ void list_again(Shared& s, const Row& r, int lo, int hi, int n) {
+  constexpr int kPer = DTypeTraits<T>::kPerVec;
+  if (threadIdx.x == 0) {
+    s.count = 0u;
+    if (s.border != 0ull) s.border -= 1ull;  // (the key on the border is to be found again)
+  }
+  __syncthreads();
+  for (int i0 = lo; i0 < hi; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    uint32_t waiting = 0u;
+    unsigned long long border = s.border;
+    if (i < hi) {
+      v = ld_stream_v4(r.base + i);
+      exclude<T>(v, legal_bits<T, kMask>(r, i));
+      waiting = candidates<T>(v, border_value(border));
+    }
+    for (;;) {
+      if (waiting) waiting = list_candidates<T>(s, v, waiting, i * kPer - r.phase, border);
+      if (!__syncthreads_or(waiting != 0u)) break;
+      rank_list(s, n);
+      border = s.border;
+    }
+  }
 }
 
 __device__ __forceinline__ bool valid_temperature(float t) { return t > 0.f && t < INFINITY; }
@@ -326,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
 
   if (tid == 0) {
     s.count = 0u;
-    s.listed = 0;
+    s.listed = s.overflow = 0;
     s.border = 0ull;
     s.ninf = 0u;
   }
@@ -376,12 +460,10 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
     border = s.border;
     least = border_value(border);
   }
-  Running run{top, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  Running<T> run;
+  run.start(top, c);
 
-  const int limit = n + kListFull;
-  for (int i0 = lo; i0 < hi; i0 += kUnroll * kThreads) {
-    uint32_t waiting = 0u;  // candidates that found no room, by vector and element
-    bool full = false;
+  for (int i0 = lo, batch = 0; i0 < hi; i0 += kUnroll * kThreads, ++batch) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int i = i0 + u * kThreads + tid, after = i + kUnroll * kThreads;
@@ -392,32 +474,27 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
       const float vt = vector_top<T>(now);
       if (vt >= (kTop ? fminf(least, run.m) : run.m)) {
         if (vt > run.m) run.raise(vt, c);
-        if (kTop && vt >= least)
-          waiting |= list_candidates<T>(s, now, candidates<T>(now, least), i * kPer - r.phase, border, limit, full)
-                     << (u * kPer);
+        if (kTop && vt >= least && list_candidates<T>(s, now, candidates<T>(now, least), i * kPer - r.phase, border))
+          s.overflow = 1;
       }
-      accumulate<T>(run, now, c);
+      if (vt > -INFINITY) run.add(now);
     }
-    if constexpr (kTop) {
-      while (__syncthreads_or(full)) {  // (what finds no room is full as well)
-        rank_list(s, n);
-        border = s.border;
-        least = border_value(border);
-        full = false;
-#pragma unroll 1
-        for (int u = 0; waiting != 0u && u < kUnroll; ++u) {
-          const uint32_t mine = (waiting >> (u * kPer)) & ((1u << kPer) - 1u);
-          if (!mine) continue;
-          const int i = i0 + u * kThreads + tid;
-          const uint32_t left = list_candidates<T>(s, ld_stream_v4(r.base + i), mine, i * kPer - r.phase, border, limit, full);
-          waiting = (waiting & ~(mine << (u * kPer))) | (left << (u * kPer));
-        }
-      }
+    // After 1, 2, 4, ... batches the list is ranked and the border with it: each doubling
+    // of what has been read brings about n candidates more.
+    if (kTop && (batch & (batch + 1)) == 0 && i0 + kUnroll * kThreads < hi) {
+      rank_list(s, n);
+      border = s.border;
+      least = border_value(border);
     }
+  }
+  if constexpr (kTop) {
+    __syncthreads();
+    if (s.overflow) list_again<T, kMask>(s, r, lo, hi, n);
   }
 
   // this CTA's sums
-  Sums mine = merge(Sums{run.m, run.s.x, run.a.x}, Sums{run.m, run.s.y, run.a.y}, c);
+  const float2 run_s = unpack2(run.s), run_a = unpack2(run.a);
+  Sums mine = merge(Sums{run.m, run_s.x, run_a.x}, Sums{run.m, run_s.y, run_a.y}, c);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
     mine = merge(mine, Sums{__shfl_xor_sync(FULL_MASK, mine.m, o), __shfl_xor_sync(FULL_MASK, mine.s, o),
@@ -597,15 +674,15 @@ struct LogprobGradParams {
 
 constexpr int kGradThreads = 256;
 
+// y = p (base - gH ln p) / T: with d = (x - m) log2(e) / T, p = 2^d / S and
+// ln p = d ln 2 - ln S, so y = 2^d (first + slope d) with the factors folded in.
 struct RowGrad {
-  float m, c, inv_s, base, slope;
-  bool inf, none;
-  // p (base - gH ln p), without the factor 1 / T: with d = (x - m) log2(e) / T,
-  // p = 2^d / S and ln p = d ln 2 - ln S, whose ln S is part of `base`
+  float m, c, first, slope, inv_t;
+  bool inf;  // infinite logits share the weight; the others have none
   __device__ __forceinline__ float at(float x) const {
     float d = inf ? (x == m ? 0.f : -INFINITY) : (x - m) * c;
     d = fmaxf(d, kNothing);  // (NaN, -inf: p = 0)
-    return exp2_approx(d) * inv_s * fmaf(slope, d, base);
+    return exp2_approx(d) * fmaf(slope, d, first);
   }
 };
 
@@ -642,13 +719,18 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
   __syncthreads();
   RowGrad row;
   row.m = st.x;
+  row.inv_t = st.w;
   row.c = fminf(kLog2e * st.w, 3e38f);
-  row.inv_s = __fdiv_rn(1.f, st.y);
-  const float gh = p.grad_entropy ? p.grad_entropy[b] : 0.f;
-  row.base = (p.grad_logsumexp ? p.grad_logsumexp[b] : 0.f) - s_sum + gh * (logf(st.y) - st.z);
-  row.slope = -gh * kLn2;
+  const float gh = p.grad_entropy ? p.grad_entropy[b] : 0.f, share = __fdiv_rn(1.f, st.y) * st.w;
+  row.first = ((p.grad_logsumexp ? p.grad_logsumexp[b] : 0.f) - s_sum + gh * (logf(st.y) - st.z)) * share;
+  row.slope = -gh * kLn2 * share;
   row.inf = st.x == INFINITY;
-  row.none = !(st.x > -INFINITY);
+  const bool none = !(st.x > -INFINITY);
+  Exponents<T> exponents;
+  exponents.set(st.x, row.c);
+  constexpr bool kDeep = std::is_same<T, float>::value;
+  const bool plain = !none && !row.inf && (kDeep || !exponents.deep);  // (else element by element)
+  const unsigned long long first2 = pack2(row.first, row.first), slope2 = pack2(row.slope, row.slope);
 
   Bits* out = static_cast<Bits*>(p.grad) + b * p.grad_stride;
   // (element 0 of the gradient's row lies as far into a 16-byte vector as the logits')
@@ -662,19 +744,32 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
     float y[kPer];
 #pragma unroll
     for (int k = 0; k < kPer / 2; ++k) {
-      const float2 f = element_pair<T>(x, k);
-      y[2 * k] = f.x > -INFINITY && !row.none ? row.at(f.x) * st.w : 0.f;
-      y[2 * k + 1] = f.y > -INFINITY && !row.none ? row.at(f.y) * st.w : 0.f;
+      float2 two;
+      if (plain) {
+        const unsigned long long d = exponents.template at<kDeep>(x, k);
+        const float2 one = unpack2(d);
+        two = unpack2(mul2(pack2(exp2_approx(one.x), exp2_approx(one.y)), fma2(slope2, d, first2)));
+      } else {
+        const float2 f = element_pair<T>(x, k);
+        two = make_float2(none || !(f.x > -INFINITY) ? 0.f : row.at(f.x), none || !(f.y > -INFINITY) ? 0.f : row.at(f.y));
+      }
+      y[2 * k] = two.x;
+      y[2 * k + 1] = two.y;
     }
     const int e0 = i * kPer - r.phase;
     if (same_phase && e0 >= 0 && e0 + kPer <= r.len) {
       uint32_t w[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if constexpr (sizeof(Bits) == 2)
-          w[k] = (uint32_t)DTypeTraits<T>::round_bits(y[2 * k]) | ((uint32_t)DTypeTraits<T>::round_bits(y[2 * k + 1]) << 16);
-        else
+        if constexpr (std::is_same<T, __half>::value) {
+          const __half2 h = __floats2half2_rn(y[2 * k], y[2 * k + 1]);
+          w[k] = *reinterpret_cast<const uint32_t*>(&h);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(y[2 * k], y[2 * k + 1]);
+          w[k] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
           w[k] = __float_as_uint(y[k]);
+        }
       }
       *reinterpret_cast<uint4*>(out + e0) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
@@ -683,7 +778,7 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
         if (e0 + j >= 0 && e0 + j < r.len) out[e0 + j] = DTypeTraits<T>::round_bits(y[j]);
     }
   }
-  if (!g || row.none) return;
+  if (!g || none) return;
   __syncthreads();  // the stores above come before those below
   const int64_t first = (int64_t)i0 * kPer - r.phase, last = (int64_t)hi * kPer - r.phase;
   for (int k = tid; k < p.tokens; k += kGradThreads) {
@@ -698,7 +793,7 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
     float own = 0.f;
     for (int j = k; j < p.tokens; ++j)
       if (ids[j] == id) own += g[j];
-    out[id] = DTypeTraits<T>::round_bits((row.at(x) + own) * st.w);
+    out[id] = DTypeTraits<T>::round_bits(fmaf(own, st.w, row.at(x)));
   }
 }
 

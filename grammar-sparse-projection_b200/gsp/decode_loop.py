@@ -16,8 +16,11 @@ Per step, as the reference does it:
      by temperature, top-k, top-p and min-p) and given to the matcher
      (accept_token), which must accept it.
 
-Beyond the reference's heads, head="int8" projects with the weight quantised
-to int8 once (gsp.int8_head) on the route the reference rule picks.
+Beyond the reference's heads, head="int8" and head="fp8" project with the weight
+quantised once (gsp.int8_head, gsp.fp8_head) on the route the reference rule
+picks; with fused_norm=True the model's last norm hands them its 8-bit rows
+(gsp.norm). run(..., logprobs=n) records each taken token's log-probability
+with the entropy and n alternatives (gsp.logprobs).
 
 The reference drives Qwen3.5-2B from Hugging Face. Any model works here: the
 loop needs only `step(tokens) -> hidden [B, H]` and the LM-head weight
@@ -34,7 +37,9 @@ import time
 
 import torch
 
-from . import int8_head
+from . import fp8_head, int8_head
+from . import logprobs as token_logprobs
+from . import norm
 from . import triton_runtime as tr
 from .graphed import GraphedGrammarHead
 
@@ -116,12 +121,19 @@ class TinyDecoder(torch.nn.Module):
         self.position = torch.zeros(batch, dtype=torch.long, device=self.embed.device)
 
     @torch.inference_mode()
-    def step(self, tokens: torch.Tensor) -> torch.Tensor:
+    def step(self, tokens: torch.Tensor, quantize: str | None = None):
+        """quantize "int8" / "fp8": the final norm, the last block's addition included,
+        is gsp.norm.rms_norm's and its 8-bit rows (QuantizedRows / Fp8Rows) are returned."""
         x = self.embed[tokens] + self.pos[self.position.clamp_max(self.pos.shape[0] - 1)]
+        update = None
         for up, down in zip(self.up, self.down):
-            x = x + torch.nn.functional.gelu(self._rms(x) @ up) @ down
+            x = x if update is None else x + update
+            update = torch.nn.functional.gelu(self._rms(x) @ up) @ down
         self.position += 1
-        return self._rms(x).contiguous()
+        if quantize is not None:
+            return norm.rms_norm(x if update is None else update, residual=None if update is None else x,
+                                 quantize=quantize).output
+        return self._rms(x if update is None else x + update).contiguous()
 
 
 @dataclasses.dataclass
@@ -131,9 +143,10 @@ class StepRecord:
     routes: str
     full_word_fraction: list[float]
     head_us: float
+    logprobs: list[dict] | None = None  # per request: logprob, entropy, top [(token id, logprob), ...]
 
 
-HEAD_MODES = ("adaptive", "dense", "fused-top1", "graphed", "int8")
+HEAD_MODES = ("adaptive", "dense", "fused-top1", "graphed", "int8", "fp8")
 
 
 class GrammarDecodeLoop:
@@ -141,24 +154,30 @@ class GrammarDecodeLoop:
     request and this library's head. `model` has reset(batch) and
     step(tokens [B] on the device) -> hidden [B, H]; `weight` is the LM head
     [V, H]; `vocab` a SyntheticVocabulary (or any object with tokenizer_info()
-    and stop_id)."""
+    and stop_id). fused_norm (heads "int8" and "fp8"): the model's
+    step(tokens, quantize=head) returns the 8-bit rows the head takes."""
 
-    def __init__(self, model, weight: torch.Tensor, vocab, *, head: str = "adaptive", policy: str = "reference"):
+    def __init__(self, model, weight: torch.Tensor, vocab, *, head: str = "adaptive", policy: str = "reference",
+                 fused_norm: bool = False):
         import xgrammar as xgr
         if head not in HEAD_MODES:
             raise ValueError(f"head must be one of {HEAD_MODES}")
+        if fused_norm and head not in ("int8", "fp8"):
+            raise ValueError('fused_norm is for the heads "int8" and "fp8"')
+        self.fused_norm = fused_norm
         self.model, self.weight, self.vocab = model, weight, vocab
         self.head, self.policy = head, policy
         self.compiler = xgr.GrammarCompiler(vocab.tokenizer_info())
         self._graphed = None
         self.weight_int8 = int8_head.quantize_rows_int8(weight) if head == "int8" else None
+        self.weight_fp8 = fp8_head.quantize_weight_fp8(weight) if head == "fp8" else None
 
     def new_matchers(self, schemas) -> list:
         import xgrammar as xgr
         return [xgr.GrammarMatcher(self.compiler.compile_json_schema(
             s if isinstance(s, str) else json.dumps(s))) for s in schemas]
 
-    def _project(self, hidden: torch.Tensor, mask_cpu: torch.Tensor, mask_gpu: torch.Tensor, fractions):
+    def _project(self, hidden, mask_cpu: torch.Tensor, mask_gpu: torch.Tensor, fractions):
         """Returns (logits [B, V] or None, next greedy tokens [B] on the device, route string)."""
         if self.head == "graphed":  # mask_cpu is the head's own pinned staging buffer
             head = self._graphed
@@ -169,9 +188,12 @@ class GrammarDecodeLoop:
         if self.head == "dense":
             logits = tr.dense_masked_logits(hidden, self.weight, mask_gpu)
             return logits, logits.argmax(-1), "dense-mask"
-        if self.head == "int8":
-            route = tr._reference_route(hidden.shape[0], fractions, 0.80)
-            logits, _, top_index = int8_head.int8_grammar_logits(hidden, self.weight_int8, mask_gpu, route=route)
+        if self.head in ("int8", "fp8"):
+            route = tr._reference_route(mask_gpu.shape[0], fractions, 0.80)
+            project, weight = ((int8_head.int8_grammar_logits, self.weight_int8) if self.head == "int8" else
+                               (fp8_head.fp8_grammar_logits, self.weight_fp8))
+            logits, _, top_index = project(hidden, weight, mask_gpu, route=route,
+                                           out_dtype=self.weight.dtype if self.fused_norm else None)
             return logits, top_index, route
         if self.head == "fused-top1":
             route = tr._reference_route(hidden.shape[0], fractions, 0.80)
@@ -182,19 +204,31 @@ class GrammarDecodeLoop:
         logits = logits.reshape(hidden.shape[0], -1)
         return logits, logits.argmax(-1), route
 
+    @staticmethod
+    def _worth(r) -> list[dict]:
+        rows = zip(r.logprobs.tolist(), r.entropy.tolist(), r.top_ids.tolist(), r.top_logprobs.tolist())
+        return [{"logprob": lp, "entropy": entropy, "top": [(i, x) for i, x in zip(ids, top) if i >= 0]}
+                for lp, entropy, ids, top in rows]
+
     def run(self, schemas, *, targets: list[list[int]] | None = None, max_steps: int = 64, on_step=None,
-            sampling: dict | None = None, generator: torch.Generator | None = None):
+            sampling: dict | None = None, generator: torch.Generator | None = None, logprobs: int | None = None):
         """Decodes one request per schema. With `targets` (token ids per
         request) the loop is teacher-forced, as the reference's is; without,
         it takes the greedy token, or with `sampling` (settings of
         triton_runtime.sample_logits: temperature, top_k, top_p, min_p) a draw
         from the masked logits, its uniform numbers from `generator` (a CUDA
-        generator; one per request and step). Finished requests (matcher terminated) keep
+        generator; one per request and step). logprobs: record with each step the
+        taken tokens' log-probabilities under softmax(logits / temperature) over
+        the legal tokens (temperature: sampling's, 1 for greedy), the entropy and
+        that many alternatives. Finished requests (matcher terminated) keep
         an all-legal mask and are not advanced. on_step(step, hidden, mask_cpu,
         logits, tokens, route) is called before the tokens are accepted.
         Returns (token ids per request, list of StepRecord)."""
         if sampling is not None and targets is not None:
             raise ValueError("a teacher-forced run takes its targets: no sampling")
+        temperature = (sampling or {}).get("temperature", 1.0)
+        if not isinstance(temperature, torch.Tensor) and temperature == 0.0:
+            temperature = 1.0
         batch = len(schemas)
         matchers = self.new_matchers(schemas)
         vocab = self.weight.shape[0]
@@ -220,7 +254,7 @@ class GrammarDecodeLoop:
                 else:
                     m.fill_next_token_bitmask(mask_cpu, b)
             fractions = tr.full_word_fraction_cpu(mask_cpu)
-            hidden = self.model.step(prev)
+            hidden = self.model.step(prev, quantize=self.head) if self.fused_norm else self.model.step(prev)
             t0 = time.perf_counter()
             logits, greedy, route = self._project(hidden, mask_cpu, mask_gpu, fractions)
             if sampling is not None:
@@ -236,6 +270,10 @@ class GrammarDecodeLoop:
                     tokens.append(int(greedy[b] if sampling is None else drawn[b]))
             if on_step is not None:
                 on_step(step, hidden, mask_cpu, logits, greedy, route)
+            worth = None
+            if logprobs is not None:
+                taken = torch.tensor(tokens, dtype=torch.long, device=self.weight.device)
+                worth = self._worth(token_logprobs.token_logprobs(logits, taken, temperature=temperature, top_n=logprobs))
             for b, m in enumerate(matchers):
                 if done[b] or (targets is not None and step >= len(targets[b])):
                     continue
@@ -244,7 +282,7 @@ class GrammarDecodeLoop:
                 out[b].append(tokens[b])
                 if m.is_terminated():
                     done[b] = True
-            records.append(StepRecord(step, tokens, route, list(fractions), head_us))
+            records.append(StepRecord(step, tokens, route, list(fractions), head_us, worth))
             prev = torch.tensor(tokens, dtype=torch.long, device=self.weight.device)
             if all(done):
                 break

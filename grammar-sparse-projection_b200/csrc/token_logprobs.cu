@@ -20,7 +20,7 @@
 // instructions per four elements, with both m and the n-th alternative so far:
 // the two rare cases (a new maximum, a candidate) share that one test. All
 // threads start from the maximum of the CTA's first batch of vectors, and the
-// alternatives from the n-th largest of its 64 eight-lane maxima, so hardly any
+// alternatives from the n-th largest of its lanes' maxima in 64 groups, so hardly any
 // vector takes the slow path after it. Candidates gather in a list that is ranked by
 // counting each time the row read has doubled; a list that overflows (rows in rising
 // order, equal values) is made again with a barrier for every vector: time, not results.
@@ -41,11 +41,13 @@ namespace cg = cooperative_groups;
 namespace gsp {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kMaxThreads = 512;
+constexpr int kGroups = 64;      // groups of lanes whose maxima place the first border
+constexpr int kParts = 8;        // lanes that count for one key
 constexpr int kUnroll = 4;       // 16-byte vectors a thread has under way
 constexpr int kMaxTop = 64;      // alternatives
 constexpr int kListSize = 1024;  // candidates held at a time
-constexpr int kMaxClusterSize = 16;
+constexpr int kMaxClusterSize = 8;
 constexpr int kMaxTokens = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -230,17 +232,8 @@ struct Running {
     m = to;
     d.set(m, c);
   }
-  __device__ __forceinline__ void add(const uint4& v) {
-    if constexpr (!std::is_same<T, float>::value) {
-      if (!d.deep) {
-        add_as<false>(v);
-        return;
-      }
-    }
-    add_as<true>(v);
-  }
   template <bool kDeep>
-  __device__ __forceinline__ void add_as(const uint4& v) {
+  __device__ __forceinline__ void add(const uint4& v) {
 #pragma unroll
     for (int k = 0; k < DTypeTraits<T>::kPerVec / 2; ++k) {
       const unsigned long long dd = d.template at<kDeep>(v, k);
@@ -263,10 +256,10 @@ __device__ __forceinline__ Sums merge(Sums x, Sums y, float c) {
 }
 
 struct Shared {
-  Sums part[kThreads / 32];
+  Sums part[kMaxThreads / 32];
   Sums total[kMaxClusterSize];  // every CTA's, written by them
   unsigned int ninf, all_ninf[kMaxClusterSize];
-  float group_top[kThreads / 8];
+  float group_top[kGroups];
   unsigned int count;
   int listed, overflow;
   unsigned long long border;
@@ -276,21 +269,27 @@ struct Shared {
   alignas(16) unsigned long long all[kMaxClusterSize * kMaxTop];
 };
 
-// The n largest of the list's keys, in falling order, at its front. Called by
-// the whole CTA between barriers of its own; afterwards s.border is the n-th.
+// Sum over the kParts neighbouring lanes of a key.
+__device__ __forceinline__ int over_parts(int v) {
+#pragma unroll
+  for (int o = 1; o < kParts; o <<= 1) v += __shfl_xor_sync(FULL_MASK, v, o);
+  return v;
+}
+
+// The n largest of the list's keys, in falling order, at its front: a key's place is the
+// number of larger ones, which kParts lanes count. Called by the whole CTA between
+// barriers of its own; afterwards s.border is the n-th.
+template <int kThreads>
 __device__ __forceinline__ void rank_list(Shared& s, int n) {
   __syncthreads();
-  const int count = min((int)s.count, kListSize);
-  for (int t = threadIdx.x; t < count; t += kThreads) {
-    const unsigned long long key = s.list[t];
+  const int count = min((int)s.count, kListSize), part = threadIdx.x % kParts;
+  for (int t0 = 0; t0 < count; t0 += kThreads / kParts) {
+    const int t = t0 + threadIdx.x / kParts;
+    const unsigned long long key = t < count ? s.list[t] : ~0ull;
     int rank = 0;
-    int j = 0;
-    for (; j + 2 <= count; j += 2) {
-      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(&s.list[j]);
-      rank += (two.x > key) + (two.y > key);
-    }
-    if (j < count) rank += s.list[j] > key;
-    if (rank < n) s.best[rank] = key;
+    for (int j = part; j < count; j += kParts) rank += s.list[j] > key;
+    rank = over_parts(rank);
+    if (part == 0 && t < count && rank < n) s.best[rank] = key;
   }
   __syncthreads();
   const int kept = min(count, n);
@@ -342,7 +341,7 @@ __device__ __forceinline__ uint32_t list_candidates(Shared& s, const uint4& v, u
 // The n largest keys of the vectors lo .. hi - 1 when the list has not held the
 // candidates (rows in rising order, or of equal values): a vector a thread and time, what
 // finds no room tried again against the border of what is listed.
-template <typename T, bool kMask>
+template <typename T, bool kMask, int kThreads>
 __device__ __noinline__ void list_again(Shared& s, const Row& r, int lo, int hi, int n) {
   constexpr int kPer = DTypeTraits<T>::kPerVec;
   if (threadIdx.x == 0) {
@@ -363,7 +362,7 @@ __device__ __noinline__ void list_again(Shared& s, const Row& r, int lo, int hi,
     for (;;) {
       if (waiting) waiting = list_candidates<T>(s, v, waiting, i * kPer - r.phase, border);
       if (!__syncthreads_or(waiting != 0u)) break;
-      rank_list(s, n);
+      rank_list<kThreads>(s, n);
       border = s.border;
     }
   }
@@ -378,11 +377,12 @@ __device__ __forceinline__ float logprob_of(float x, float m, float t, float log
   return __fdiv_rn(x - m, t) - log_s;  // (m infinite: -inf)
 }
 
-template <typename T, bool kMask, bool kTop>
-__global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const LogprobParams p) {
+template <typename T, bool kMask, bool kTop, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kernel(const LogprobParams p) {
   using Bits = typename DTypeTraits<T>::Bits;
   constexpr int kPer = DTypeTraits<T>::kPerVec;
   constexpr uint32_t kAll = (1u << kPer) - 1u;
+  constexpr int kGroupLanes = kThreads / kGroups;
   __shared__ Shared s;
   cg::cluster_group cluster = cg::this_cluster();
   // (nothing is written to a CTA's shared memory before it runs)
@@ -433,24 +433,28 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
     top = fmaxf(top, vector_top<T>(v[u]));
   }
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
-  if ((lane & 7) == 0) s.group_top[tid >> 3] = top;
+  for (int o = 1; o < kGroupLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, o));
+  if (lane % kGroupLanes == 0) s.group_top[tid / kGroupLanes] = top;
   __syncthreads();
   {
-    const float x0 = s.group_top[lane], x1 = s.group_top[lane + 32];
-    float m = fmaxf(x0, x1);
+    float m = fmaxf(s.group_top[lane], s.group_top[lane + 32]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL_MASK, m, o));
     top = m;
-    if (kTop && warp == 0) {  // the n-th largest of the 64: at least n elements are no smaller
-      int above0 = 0, above1 = 0;
-      for (int j = 0; j < kThreads / 8; ++j) {
-        const float y = s.group_top[j];
-        above0 += y > x0 || (y == x0 && j < lane);
-        above1 += y > x1 || (y == x1 && j < lane + 32);
+    if constexpr (kTop) {  // the n-th largest of the 64: at least n elements are no smaller
+#pragma unroll
+      for (int g0 = 0; g0 < kGroups; g0 += kThreads / kParts) {
+        const int g = g0 + tid / kParts;
+        const float x = s.group_top[g];
+        int above = 0;
+#pragma unroll
+        for (int j = tid % kParts; j < kGroups; j += kParts) {
+          const float y = s.group_top[j];
+          above += y > x || (y == x && j < g);
+        }
+        above = over_parts(above);
+        if (above == n - 1 && tid % kParts == 0 && x > -INFINITY) s.border = (unsigned long long)ordered_bits(x) << 32;
       }
-      if (above0 == n - 1) s.border = x0 > -INFINITY ? (unsigned long long)ordered_bits(x0) << 32 : 0ull;
-      if (above1 == n - 1) s.border = x1 > -INFINITY ? (unsigned long long)ordered_bits(x1) << 32 : 0ull;
     }
   }
   unsigned long long border = 0ull;
@@ -464,32 +468,47 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
   run.start(top, c);
 
   for (int i0 = lo, batch = 0; i0 < hi; i0 += kUnroll * kThreads, ++batch) {
+    float most = -INFINITY;  // of the batch's vectors
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int i = i0 + u * kThreads + tid, after = i + kUnroll * kThreads;
-      uint4 now = v[u];
-      if (kMask || bits[u] != kAll) exclude<T>(now, bits[u]);
-      bits[u] = after < hi ? legal_bits<T, kMask>(r, after) : 0u;
-      v[u] = after < hi ? ld_stream_v4(r.base + after) : make_uint4(0u, 0u, 0u, 0u);
-      const float vt = vector_top<T>(now);
-      if (vt >= (kTop ? fminf(least, run.m) : run.m)) {
-        if (vt > run.m) run.raise(vt, c);
-        if (kTop && vt >= least && list_candidates<T>(s, now, candidates<T>(now, least), i * kPer - r.phase, border))
-          s.overflow = 1;
+      if (kMask || bits[u] != kAll) exclude<T>(v[u], bits[u]);
+      most = fmaxf(most, vector_top<T>(v[u]));
+    }
+    if (most >= (kTop ? fminf(least, run.m) : run.m)) {  // rarely
+      if (most > run.m) run.raise(most, c);
+      if (kTop && most >= least) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const uint32_t found = candidates<T>(v[u], least);
+          if (found && list_candidates<T>(s, v[u], found, (i0 + u * kThreads + tid) * kPer - r.phase, border)) s.overflow = 1;
+        }
       }
-      if (vt > -INFINITY) run.add(now);
+    }
+    const bool some = most > -INFINITY;
+    if (some && (std::is_same<T, float>::value || run.d.deep)) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) run.template add<true>(v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int after = i0 + (kUnroll + u) * kThreads + tid;
+      if constexpr (!std::is_same<T, float>::value) {
+        if (some && !run.d.deep) run.template add<false>(v[u]);
+      }
+      bits[u] = after < hi ? legal_bits<T, kMask>(r, after) : 0u;
+      if (after < hi) v[u] = ld_stream_v4(r.base + after);
     }
     // After 1, 2, 4, ... batches the list is ranked and the border with it: each doubling
     // of what has been read brings about n candidates more.
     if (kTop && (batch & (batch + 1)) == 0 && i0 + kUnroll * kThreads < hi) {
-      rank_list(s, n);
+      rank_list<kThreads>(s, n);
       border = s.border;
       least = border_value(border);
     }
   }
   if constexpr (kTop) {
     __syncthreads();
-    if (s.overflow) list_again<T, kMask>(s, r, lo, hi, n);
+    if (s.overflow) list_again<T, kMask, kThreads>(s, r, lo, hi, n);
   }
 
   // this CTA's sums
@@ -500,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
     mine = merge(mine, Sums{__shfl_xor_sync(FULL_MASK, mine.m, o), __shfl_xor_sync(FULL_MASK, mine.s, o),
                             __shfl_xor_sync(FULL_MASK, mine.a, o)}, c);
   if (lane == 0) s.part[warp] = mine;
-  if constexpr (kTop) rank_list(s, n);
+  if constexpr (kTop) rank_list<kThreads>(s, n);
   else __syncthreads();
   if (warp == 0) {
     mine = s.part[lane & (kThreads / 32 - 1)];
@@ -512,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
   }
   __syncthreads();
   // to the other CTAs' shared memory (all of them run: the barrier at the start): what a
-  // CTA would have to fetch takes it 15 us for 16 lists of 20
+  // CTA would have to fetch took it 15 us for 16 lists of 20
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (size > 1) {
     if (tid < size) cluster.map_shared_rank(s.total, tid)[rank] = s.part[0];
@@ -577,24 +596,26 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
       p.logprobs[b * p.tokens + k] = !valid ? nan : id < 0 ? 0.f : lp;
     }
     if constexpr (kTop) {
-      // a key's place is the number of larger ones, counted in the lists one by one
-      for (int i = tid; i < size * n; i += kThreads) {
-        const unsigned long long key = s.all[i];
-        const int q = i / n;
-        if (key == 0ull) continue;
-        int place = i - q * n;
-        for (int o = 0; o < size && place < n; ++o) {
-          if (o == q) continue;
-          const unsigned long long* other = s.all + o * n;
-          int a = 0, z = n;
-          while (a < z) {  // larger keys come first, and none (0) last
-            const int mid = (a + z) >> 1;
-            if (other[mid] > key) a = mid + 1;
-            else z = mid;
+      // a key's place is the number of larger ones, counted in the other lists one by one
+      for (int i0 = 0; i0 < size * n; i0 += kThreads / kParts) {
+        const int i = i0 + tid / kParts, q = i / n;
+        const unsigned long long key = i < size * n ? s.all[i] : 0ull;
+        int place = 0;
+        if (key != 0ull) {
+          for (int o = tid % kParts; o < size; o += kParts) {
+            if (o == q) continue;
+            const unsigned long long* other = s.all + o * n;
+            int a = 0, z = n;
+            while (a < z) {  // larger keys come first, and none (0) last
+              const int mid = (a + z) >> 1;
+              if (other[mid] > key) a = mid + 1;
+              else z = mid;
+            }
+            place += a;
           }
-          place += a;
         }
-        if (place >= n) continue;
+        place = over_parts(place) + i - q * n;
+        if (key == 0ull || place >= n || tid % kParts != 0) continue;
         const int64_t at_row = key_index(key);
         p.top_ids[b * n + place] = p.offsets ? p.ids[r.first + at_row] : at_row;
         p.top_logprobs[b * n + place] = logprob_of(key_value(key), sum.m, t, log_s);
@@ -610,14 +631,9 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Logpr
   }
 }
 
-template <typename T, bool kMask, bool kTop>
+template <typename T, bool kMask, bool kTop, int kThreads>
 cudaError_t launch_forward(const LogprobParams& p, int batch, int size, cudaStream_t stream) {
-  auto k = token_logprobs_kernel<T, kMask, kTop>;
-  if (size > 8) {
-    const cudaError_t err = cudaFuncSetAttribute(reinterpret_cast<const void*>(k),
-                                                 cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (err != cudaSuccess) return err;
-  }
+  auto k = token_logprobs_kernel<T, kMask, kTop, kThreads>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)batch * (unsigned)size);
   cfg.blockDim = dim3(kThreads);
@@ -632,22 +648,31 @@ cudaError_t launch_forward(const LogprobParams& p, int batch, int size, cudaStre
   return cudaLaunchKernelEx(&cfg, k, p);
 }
 
+template <typename T, bool kMask, bool kTop>
+cudaError_t launch_shaped(const LogprobParams& p, int batch, int64_t max_len, cudaStream_t stream) {
+  int dev = 0;
+  const cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  const int sms = num_sms(dev);
+  // Many rows: a CTA of 256 threads each, four on an SM, so that one's start and end pass
+  // while the others read (1,999 x 151,936 bf16: 132 us, two of 512 threads 151).
+  if (batch >= 4 * sms) return launch_forward<T, kMask, kTop, 256>(p, batch, 1, stream);
+  // Few: CTAs of 512 threads, as many for a row as keep half a batch of vectors each while
+  // the device holds them all, two on an SM; and no more than 8, past which the cluster's
+  // barriers cost what the shorter shares gain (one row of 248,320, 20 alternatives: 8 and
+  // 16 alike, 4 take a fifth longer).
+  const int64_t half = (int64_t)kMaxThreads * kUnroll * DTypeTraits<T>::kPerVec / 2;
+  int size = 1;
+  while (size < kMaxClusterSize && (int64_t)batch * size * 2 <= 2 * (int64_t)sms && max_len > half * size) size *= 2;
+  return launch_forward<T, kMask, kTop, 512>(p, batch, size, stream);
+}
+
 template <typename T>
 cudaError_t launch_typed(const LogprobParams& p, int batch, int64_t max_len, cudaStream_t stream) {
-  int dev = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err != cudaSuccess) return err;
-  // CTAs per row: while the device has room for twice as many (two per SM) and
-  // each keeps a whole batch of vectors.
-  const int64_t batch_elements = (int64_t)kThreads * kUnroll * DTypeTraits<T>::kPerVec;
-  int size = 1;
-  while (size < kMaxClusterSize && (int64_t)batch * size * 2 <= 2 * (int64_t)num_sms(dev) &&
-         max_len > batch_elements / 2 * size)
-    size *= 2;
-  if (p.mask) return p.top_n ? launch_forward<T, true, true>(p, batch, size, stream)
-                             : launch_forward<T, true, false>(p, batch, size, stream);
-  return p.top_n ? launch_forward<T, false, true>(p, batch, size, stream)
-                 : launch_forward<T, false, false>(p, batch, size, stream);
+  if (p.mask) return p.top_n ? launch_shaped<T, true, true>(p, batch, max_len, stream)
+                             : launch_shaped<T, true, false>(p, batch, max_len, stream);
+  return p.top_n ? launch_shaped<T, false, true>(p, batch, max_len, stream)
+                 : launch_shaped<T, false, false>(p, batch, max_len, stream);
 }
 
 // ---- gradient -------------------------------------------------------------------
@@ -742,19 +767,22 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
     uint4 x = v[u];
     if (kMask || bits[u] != (1u << kPer) - 1u) exclude<T>(x, bits[u]);
     float y[kPer];
+    if (plain) {
 #pragma unroll
-    for (int k = 0; k < kPer / 2; ++k) {
-      float2 two;
-      if (plain) {
+      for (int k = 0; k < kPer / 2; ++k) {
         const unsigned long long d = exponents.template at<kDeep>(x, k);
         const float2 one = unpack2(d);
-        two = unpack2(mul2(pack2(exp2_approx(one.x), exp2_approx(one.y)), fma2(slope2, d, first2)));
-      } else {
-        const float2 f = element_pair<T>(x, k);
-        two = make_float2(none || !(f.x > -INFINITY) ? 0.f : row.at(f.x), none || !(f.y > -INFINITY) ? 0.f : row.at(f.y));
+        const float2 two = unpack2(mul2(pack2(exp2_approx(one.x), exp2_approx(one.y)), fma2(slope2, d, first2)));
+        y[2 * k] = two.x;
+        y[2 * k + 1] = two.y;
       }
-      y[2 * k] = two.x;
-      y[2 * k + 1] = two.y;
+    } else {
+#pragma unroll
+      for (int k = 0; k < kPer / 2; ++k) {
+        const float2 f = element_pair<T>(x, k);
+        y[2 * k] = none || !(f.x > -INFINITY) ? 0.f : row.at(f.x);
+        y[2 * k + 1] = none || !(f.y > -INFINITY) ? 0.f : row.at(f.y);
+      }
     }
     const int e0 = i * kPer - r.phase;
     if (same_phase && e0 >= 0 && e0 + kPer <= r.len) {

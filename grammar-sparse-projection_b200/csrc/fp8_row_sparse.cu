@@ -3,7 +3,7 @@
 //
 //   y[b, v] = sum_kb ws[v / 128, kb] sum_{k in block kb} (hs[b, kb] q[b, k]) w[v, k]
 //
-// A request has `parts` CTAs (all SMs' worth over the batch). Each ranks the request's
+// A request has `parts` CTAs (one or two SMs' worth over the batch). Each ranks the request's
 // whole mask (one pass over its words, a prefix over the threads), takes an even share
 // of the legal rows by rank, and streams them: a warp holds four rows, 16 bytes of each
 // a lane, converts them to fp32 and multiplies with the hidden state, which lies in
@@ -12,6 +12,10 @@
 // goes to the illegal tokens of an even share of the words. Bound by the legal rows'
 // bytes where they are many, by latency (mask, list, rows, one after another) where
 // they are few.
+//
+// Measured (device): one request, 248,320 x 2,048 fp16 at 1% 12-13 us (floor 0.9: launch of
+// the clearing kernel, mask, prefix, list, rows, merge), 32 requests at 1% 57 us (24), one
+// request at 20% 45 us (16).
 //
 // Hidden states that are not quantised yet are quantised here, each CTA its request's.
 // The request's top-1 merges in scratch keys; its last CTA stores it.
@@ -97,7 +101,7 @@ __device__ __forceinline__ float dot16(const uint4& w, const float4 (&x)[4]) {
 }
 
 template <typename Out, bool kVec>
-__global__ void __launch_bounds__(kThreads) fp8_row_sparse_kernel(const __grid_constant__ Fp8Params p, int parts) {
+__global__ void __launch_bounds__(kThreads, 2) fp8_row_sparse_kernel(const __grid_constant__ Fp8Params p, int parts) {
   using OutBits = typename DTypeTraits<Out>::OutBits;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int s_warp[kWarps], s_list[kListRows];
@@ -110,11 +114,18 @@ __global__ void __launch_bounds__(kThreads) fp8_row_sparse_kernel(const __grid_c
   float* s_x = reinterpret_cast<float*>(smem);
   const auto word_at = [&](int w) { return tail_clip(mask ? __ldg(mask + w) : 0xffffffffu, w, p.vocab); };
 
-  // ranks: thread t has the words [w0, w1)
-  const int per = (nw + kThreads - 1) / kThreads, w0 = min(nw, tid * per), w1 = min(nw, w0 + per);
-  int count = 0;
-#pragma unroll 8
-  for (int w = w0; w < w1; ++w) count += __popc(word_at(w));
+  // ranks: thread t has the words [w0, w1), whole 16-byte vectors of them
+  const int per = (nw + 4 * kThreads - 1) / (4 * kThreads) * 4, w0 = min(nw, tid * per), w1 = min(nw, w0 + per);
+  int count = 0, w = w0;
+  if (mask && (reinterpret_cast<uintptr_t>(mask) & 15) == 0) {
+#pragma unroll 4
+    for (; w + 4 <= w1; w += 4) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(mask + w));
+      count += __popc(tail_clip(q.x, w, p.vocab)) + __popc(tail_clip(q.y, w + 1, p.vocab)) +
+               __popc(tail_clip(q.z, w + 2, p.vocab)) + __popc(tail_clip(q.w, w + 3, p.vocab));
+    }
+  }
+  for (; w < w1; ++w) count += __popc(word_at(w));
   int incl = count;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -168,14 +179,17 @@ __global__ void __launch_bounds__(kThreads) fp8_row_sparse_kernel(const __grid_c
     }
     __syncthreads();
     const int n = r1 - r0;
-    for (int i = warp * kRows; i < n; i += kWarps * kRows) {
+    // (few rows: one or two a warp, so that all warps have some)
+    const int share = min(kRows, (n + kWarps - 1) / kWarps);
+    for (int i = warp * share; i < n; i += kWarps * share) {
+      const int live = min(share, n - i);
       int row[kRows];
       const uint8_t* w[kRows];
       const float* ws[kRows];
       float acc[kRows];
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        row[r] = s_list[min(i + r, n - 1)];
+        row[r] = s_list[min(i + r, n - 1)];  // (past `live`: not read)
         w[r] = p.weight + (int64_t)row[r] * p.weight_stride;
         ws[r] = p.weight_scales + (int64_t)(row[r] >> 7) * p.weight_scales_stride;
         acc[r] = 0.f;
@@ -190,8 +204,8 @@ __global__ void __launch_bounds__(kThreads) fp8_row_sparse_kernel(const __grid_c
             const int v = v0 + 32 * h + lane;
 #pragma unroll
             for (int r = 0; r < kRows; ++r) {
-              q[h][r] = v < nvec ? ld_stream_v4(reinterpret_cast<const uint4*>(w[r]) + v) : make_uint4(0u, 0u, 0u, 0u);
-              scale[h][r] = v < nvec ? __ldg(ws[r] + (v >> 3)) : 0.f;
+              q[h][r] = v < nvec && r < live ? ld_stream_v4(reinterpret_cast<const uint4*>(w[r]) + v) : make_uint4(0u, 0u, 0u, 0u);
+              scale[h][r] = v < nvec && r < live ? __ldg(ws[r] + (v >> 3)) : 0.f;
             }
           }
 #pragma unroll
@@ -200,7 +214,8 @@ __global__ void __launch_bounds__(kThreads) fp8_row_sparse_kernel(const __grid_c
             if (v >= nvec) continue;
             const float4 x[4] = {x4[v], x4[nvec + v], x4[2 * nvec + v], x4[3 * nvec + v]};
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) acc[r] = fmaf(dot16(q[h][r], x), scale[h][r], acc[r]);
+            for (int r = 0; r < kRows; ++r)
+              if (r < live) acc[r] = fmaf(dot16(q[h][r], x), scale[h][r], acc[r]);
           }
         }
       } else {
@@ -210,7 +225,7 @@ __global__ void __launch_bounds__(kThreads) fp8_row_sparse_kernel(const __grid_c
           for (int j = 0; j < 4; ++j) {
             const int k = kb * kBlock + lane + 32 * j;
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) q[j][r] = k < p.hidden_dim ? (uint32_t)__ldg(w[r] + k) : 0u;
+            for (int r = 0; r < kRows; ++r) q[j][r] = k < p.hidden_dim && r < live ? (uint32_t)__ldg(w[r] + k) : 0u;
           }
           float x[4];
 #pragma unroll
@@ -231,7 +246,7 @@ __global__ void __launch_bounds__(kThreads) fp8_row_sparse_kernel(const __grid_c
       for (int r = 0; r < kRows; ++r) acc[r] = warp_sum(acc[r]);
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        if (lane != r || i + r >= n) continue;
+        if (lane != r || r >= live) continue;
         const OutBits bits = DTypeTraits<Out>::round_bits(acc[r]);
         if (logits) logits[row[r]] = bits;
         const unsigned long long key = top1_key(DTypeTraits<Out>::bits_to_float(bits), (uint64_t)(p.vocab_offset + row[r]));
@@ -265,8 +280,10 @@ cudaError_t launch(const Fp8Params& p, cudaStream_t stream) {
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   const int sms = num_sms(dev);
-  // CTAs of a request: two per SM over the batch, at least 64 mask words each
-  int parts = std::max(1, 2 * sms / p.batch);
+  // CTAs of a request, at least 64 mask words each: one per SM over a batch of up to 8,
+  // whose time is that of ranking the masks (8 x 248,320 x 2,048 at 1%: 23.6 us, two per SM
+  // 25.4), two per SM over a larger one (32: 59.7 and 57.4 us)
+  int parts = std::max(1, (p.batch <= 8 ? 1 : 2) * sms / p.batch);
   parts = std::min(parts, std::max(1, p.nw / 64));
   if ((int64_t)p.batch * parts > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const bool keys = parts > 1 && (p.top_value || p.top_index || p.top_key);

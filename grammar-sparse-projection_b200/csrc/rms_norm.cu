@@ -13,11 +13,14 @@
 // The 8-bit outputs are taken from y in fp32: rounding it to T first, as a norm
 // followed by a quantiser does, would add half a step of T.
 //
-// One pass over memory, which bounds it (2 + 2 read, 2 + 1 written per element of a
-// 16-bit row with residual and 8-bit output): 1 to 16 warps hold a row's h in
-// registers, and the squares, the row's maximum and the blocks' maxima are reduced
-// from there. With few rows more warps share a row, until the SMs are filled. What
-// of a row is past the registers (over 16,384 columns) is read again.
+// One pass over memory (2 + 2 read, 2 + 1 written per element of a 16-bit row with
+// residual and 8-bit output): 1 to 16 warps hold a row's h in registers, and the squares,
+// the row's maximum and the blocks' maxima are reduced from there. What of a row is past
+// the registers (over 16,384 columns) is read again.
+//
+// Measured, 16,384 x 8,192 bf16 with residual: rounded output 204 us (5.3 TB/s, 81% of
+// measured), e4m3 221 us (4.2 TB/s; floor 146), int8 250 us: with an 8-bit output the
+// instructions of the quantisation bound it beside memory. 64 x 2,048: 2.9-3.3 us, a launch.
 #include <algorithm>
 #include <cmath>
 

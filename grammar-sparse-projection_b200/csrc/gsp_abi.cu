@@ -1211,7 +1211,7 @@ int32_t gsp_fp8_logits(int32_t route, const void* hidden, int64_t hidden_row_str
   p.batch = batch;
   p.vocab = vocab;
   p.hidden_dim = hidden_dim;
-  p.nw = (vocab + 31) / 32;
+  p.nw = (int)(((int64_t)vocab + 31) / 32);
   p.blocks = blocks;
   p.vocab_offset = vocab_offset;
   p.logits = logits;

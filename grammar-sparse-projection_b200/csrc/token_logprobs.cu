@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
     int64_t lo = p.offsets[b], hi = p.offsets[b + 1];
     lo = lo < 0 ? 0 : lo > p.capacity ? p.capacity : lo;
     hi = hi > p.capacity ? p.capacity : hi;
-    set_row<T>(r, p.logits, lo, hi > lo ? hi - lo : 0);
+    set_row<T>(r, p.logits, lo, hi > lo ? min(hi - lo, (int64_t)1 << 30) : 0);  // (vectors are counted in 32 bits)
   } else {
     set_row<T>(r, p.logits, b * p.row_stride, p.vocab);
   }

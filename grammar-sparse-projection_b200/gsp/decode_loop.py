@@ -227,7 +227,9 @@ class GrammarDecodeLoop:
         if sampling is not None and targets is not None:
             raise ValueError("a teacher-forced run takes its targets: no sampling")
         temperature = (sampling or {}).get("temperature", 1.0)
-        if not isinstance(temperature, torch.Tensor) and temperature == 0.0:
+        if isinstance(temperature, torch.Tensor):
+            temperature = torch.where(temperature > 0, temperature, 1.0)
+        elif temperature == 0.0:
             temperature = 1.0
         batch = len(schemas)
         matchers = self.new_matchers(schemas)

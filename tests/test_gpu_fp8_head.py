@@ -87,6 +87,24 @@ def test_routes_match_64_bits(cuda_device, shape, dtype):
     assert _native.workspace_error(cuda_device) == 0
 
 
+@pytest.mark.parametrize("shape", [(2, 300, 32768), (3, 1048609, 16), (140, 1048609, 16), (1, 129, 33), (260, 40, 128)])
+def test_largest_hidden_size_and_vocabularies_past_the_list(cuda_device, shape):
+    """The widest hidden state that shared memory takes; vocabularies whose active groups are not listed (the block
+    route then takes the legal rows); sizes below a vector, a block and a tile."""
+    batch, vocab, hidden = shape
+    h, weight = _case(7, batch, vocab, hidden, torch.bfloat16, cuda_device)
+    rows = F.quantize_rows_fp8(h)
+    exact, size = _exact(rows, weight)
+    legal = torch.zeros(batch, vocab, dtype=torch.bool)
+    legal[:, ::97], legal[0, -1] = True, True
+    words = torch.zeros(batch, (vocab + 31) // 32 * 32, dtype=torch.uint8)
+    words[:, :vocab] = legal
+    mask = torch.from_numpy(np.packbits(words.numpy(), axis=1, bitorder="little").view(np.int32).copy()).to(cuda_device)
+    for route in tr.ROUTES:
+        _check(F.fp8_grammar_logits(h, weight, mask, route=route), exact, size, legal, torch.bfloat16, (hidden + 127) // 128)
+    assert _native.workspace_error(cuda_device) == 0
+
+
 @pytest.mark.parametrize("batch", [1, 17, 200])
 @pytest.mark.parametrize("route", tr.ROUTES)
 def test_masks_without_a_token_wide_masks_and_no_logits(cuda_device, route, batch):

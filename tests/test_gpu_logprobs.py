@@ -191,6 +191,21 @@ def test_strides_and_alignment(cuda_device, dtype):
     _check(one, wide[:1, 1:1 + vocab], ids[:1], 1.0, 1)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("batch", [300, 700])
+def test_many_rows_with_lists_that_overflow(cuda_device, batch, dtype):
+    """Rows in rising order and of equal values among ordinary ones, a CTA each (of 512 and of 256 threads)."""
+    vocab = 16411
+    x = _logits(61, batch, vocab, dtype)
+    x[5] = torch.linspace(-30, 30, vocab).to(dtype)
+    x[7] = 1.5
+    x[9, ::2] = -math.inf
+    ids = _some_ids(3, batch, vocab, 2)
+    for top_n in (0, 64):
+        r = L.token_logprobs(x.to(cuda_device), ids.to(cuda_device), temperature=0.9, top_n=top_n)
+        _check(r, x, ids, 0.9, top_n)
+
+
 def test_no_given_tokens(cuda_device):
     x = _logits(3, 4, 5000, torch.bfloat16)
     ids = torch.empty(4, 0, dtype=torch.int64)

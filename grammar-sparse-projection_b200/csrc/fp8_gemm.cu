@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     bool ok = q < quads;
     Tiles<kGroups> t(total, c.chunks);
     // The next tile's groups, mask words and first scales are loaded while a tile is
-    // worked on: nothing else would hide their latency (2 us a tile).
+    // worked on: nothing else would hide their latency.
     int group_next[kUnits];
     uint32_t legal_next[kUnits];
     float ws_next[kUnits];
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const auto load_ws = [&](int group, int kb) {
       return kb + lane < p.blocks ? __ldg(p.weight_scales + (int64_t)(group >> 2) * p.weight_scales_stride + kb + lane) : 0.f;
     };
-    const auto load_tile = [&]() {  // of t; its hidden states' scales come with load_hs
+    const auto load_tile = [&]() {  // of t; its hidden states' scales come with load_scales
       const int row = t.chunk * kChunkRows + q * 32 + lane;
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {

@@ -47,15 +47,6 @@ struct Fp8Params {
 
 constexpr int kListGroups = 128;  // mask words of a builder block
 
-template <typename T>
-struct OutCode;
-template <>
-struct OutCode<__half> { static constexpr int value = 0; };
-template <>
-struct OutCode<__nv_bfloat16> { static constexpr int value = 1; };
-template <>
-struct OutCode<float> { static constexpr int value = 2; };
-
 // out_dtype: 0 fp16, 1 bf16, 2 fp32 logits.
 cudaError_t launch_fp8_row_sparse(const Fp8Params& p, int out_dtype, cudaStream_t stream);
 cudaError_t launch_fp8_tensor(const Fp8Params& p, int out_dtype, cudaStream_t stream);

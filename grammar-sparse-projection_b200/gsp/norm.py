@@ -59,14 +59,16 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
     if rows.shape[0] >= 2 ** 31 or rows.shape[1] > MAX_COLUMNS:  # (the C entries take 32-bit sizes)
         raise ValueError("x may hold up to 2^31 - 1 rows of 2^24 columns")
     _native.dtype_code(x.dtype)
-    _check_rows(rows, rows, "x")
     count, cols = rows.shape
+    if cols > 1 and rows.stride(1) != 1:
+        raise ValueError("x must be contiguous along its rows")
     if weight is not None and (weight.device != x.device or weight.dtype != x.dtype or weight.shape != (cols,)
                                or not weight.is_contiguous()):
         raise ValueError("weight must be a contiguous tensor [H] of x's type and device")
     if not 0.0 <= eps < float("inf"):
         raise ValueError("eps must be finite and not negative")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         raise ValueError("rms_norm has no gradient: call it without tensors that require one, or under torch.no_grad()")
     if residual is not None:
         residual = residual.unsqueeze(0) if one_row and residual.dim() == 1 else residual

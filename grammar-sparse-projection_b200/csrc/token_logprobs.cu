@@ -58,6 +58,7 @@ constexpr int kMaxTokens = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNothing = -200.f;  // exponent whose power of two is 0 in fp32
+constexpr float kFurthest = -1e30f;  // no exponent of a half is below it
 
 struct LogprobParams {
   const void* logits;
@@ -179,12 +180,15 @@ __device__ __forceinline__ float exp2_approx(float x) {
 
 // The exponents d = (x - m) c of a vector's elements, in pairs, none below kNothing
 // (-inf, NaN and what is far below: nothing). Halves are held back at `floor` before they
-// are widened: a value of the type at or below m + kNothing / c, two in each word.
+// are widened: a value of the type at or below m + kNothing / c, two in each word. Where m
+// is large the next such value may lie far below that (at the largest bf16 one step is
+// 1.3e36), so far that its exponent would pass fp32 and 0 times it be NaN: then, too, the
+// exponents are held back in fp32.
 template <typename T>
 struct Exponents {
   unsigned long long neg, by;
   uint32_t floor;
-  bool deep;  // the type has no such value (a maximum near its lowest): held back in fp32
+  bool deep;  // the type has no such value (a maximum near its lowest), or one too far: held back in fp32
   __device__ __forceinline__ void set(float m, float c) {
     neg = pack2(-m, -m);
     by = pack2(c, c);
@@ -194,12 +198,18 @@ struct Exponents {
     if (!(low < m)) low = m > 0.f ? __uint_as_float(__float_as_uint(m) - 1u) : __uint_as_float(__float_as_uint(m) + 1u);
     floor = 0u;
     deep = true;
-    if constexpr (std::is_same<T, __half>::value) {
-      deep = !(low >= -65504.f);
-      floor = (uint32_t)__half_as_ushort(__float2half_rd(low)) * 0x00010001u;
-    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      deep = !(low >= -3.3895313892515355e38f);
-      floor = (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rd(low)) * 0x00010001u;
+    if constexpr (!std::is_same<T, float>::value) {
+      float held;  // the floor's value (-inf where the type has none)
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half h = __float2half_rd(low);
+        floor = (uint32_t)__half_as_ushort(h) * 0x00010001u;
+        held = __half2float(h);
+      } else {
+        const __nv_bfloat16 h = __float2bfloat16_rd(low);
+        floor = (uint32_t)__bfloat16_as_ushort(h) * 0x00010001u;
+        held = __bfloat162float(h);
+      }
+      deep = !((held - m) * c >= kFurthest);
     }
   }
   template <bool kDeep>
@@ -577,7 +587,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
     const bool some = sum.m > -INFINITY;
     const float nan = __int_as_float(0x7fc00000);
     const float log_s = !valid ? nan : some ? logf(sum.s) : 0.f;
-    const float entropy = !valid ? nan : some ? fmaxf(log_s - kLn2 * (sum.a / sum.s), 0.f) : 0.f;
+    const float rounded = log_s - kLn2 * (sum.a / sum.s);
+    const float entropy = !valid ? nan : some && !(rounded < 0.f) ? rounded : 0.f;
     if (tid == 0) {
       if (p.entropy) p.entropy[b] = entropy;
       if (p.logsumexp) p.logsumexp[b] = !valid ? nan : some ? __fdiv_rn(sum.m, t) + log_s : -INFINITY;

@@ -1,0 +1,61 @@
+"""GPU tests of the log probabilities on rows with the largest and lowest values of their type, at temperatures down to
+1e-37, against the 64-bit restatement of test_gpu_logprobs (and within its bounds)."""
+import math
+
+import pytest
+import torch
+
+from gsp import logprobs as L
+from test_gpu_logprobs import DTYPES, _check, _error, _logits, _pack
+
+pytestmark = pytest.mark.gpu
+
+VOCAB = 20011
+
+
+def _rows(dtype):
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    every = torch.arange(VOCAB)
+    bell = lambda seed: _logits(seed, 1, VOCAB, torch.float32)[0]  # noqa: E731
+    rows = [
+        torch.where(every % 3 == 0, high, low),                           # extremes, side by side
+        bell(1).index_fill_(0, torch.tensor([77]), high),                 # a forced token among ordinary logits
+        bell(2).index_fill_(0, torch.tensor([5, 77, VOCAB - 1]), high),   # several
+        torch.full((VOCAB,), low).index_fill_(0, torch.tensor([VOCAB - 2]), 1.0),
+        torch.full((VOCAB,), low),
+        torch.full((VOCAB,), high),
+        bell(3).index_fill_(0, torch.tensor([77]), high / 4).index_fill_(0, every[::5], math.nan),
+        bell(4).index_fill_(0, every[::2], -math.inf).index_fill_(0, torch.tensor([4001]), high / 64),
+        torch.where(every % 7 == 0, 0.0, -0.0),
+        torch.full((VOCAB,), -math.inf),
+        bell(5).index_fill_(0, torch.tensor([77, 78]), math.inf),
+        torch.linspace(-40.0, 40.0, VOCAB),
+    ]
+    return torch.stack(rows).to(dtype)
+
+
+def _ids(batch):
+    return torch.stack([torch.full((batch,), i) for i in (0, 77, VOCAB - 2, VOCAB - 1)], 1).contiguous()
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("temperature", [1.0, 0.05, 1e-3, 1e-6, 1e-37])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_forward(cuda_device, dtype, temperature, masked):
+    x = _rows(dtype)
+    ids = _ids(len(x))
+    legal = torch.rand(x.shape, generator=torch.Generator().manual_seed(9)) < 0.6 if masked else None
+    mask = _pack(legal).to(cuda_device) if masked else None
+    r = L.token_logprobs(x.to(cuda_device), ids.to(cuda_device), bitmask_gpu=mask, temperature=temperature, top_n=5)
+    _check(r, x, ids, temperature, 5, legal)
+
+
+def test_entropy_of_tied_largest_values(cuda_device):
+    """ln of their number, however large they are and however low the temperature."""
+    for dtype in DTYPES:
+        x = _rows(dtype)[[0, 2, 5]]
+        ids = torch.zeros(3, dtype=torch.int64, device=cuda_device)
+        for temperature in (0.005, 1e-6, 1e-37):
+            r = L.token_logprobs(x.to(cuda_device), ids, temperature=temperature)
+            want = torch.tensor([(VOCAB + 2) // 3, 3, VOCAB], dtype=torch.float64).log()
+            assert (r.entropy.double().cpu() - want).abs().max() <= 2 * _error(VOCAB) * (1 + math.log(VOCAB) + 1)

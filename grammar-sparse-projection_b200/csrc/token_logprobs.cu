@@ -189,6 +189,7 @@ struct Exponents {
   unsigned long long neg, by;
   uint32_t floor;
   bool deep;  // the type has no such value (a maximum near its lowest), or one too far: held back in fp32
+  float lowest;  // no exponent is below it
   __device__ __forceinline__ void set(float m, float c) {
     neg = pack2(-m, -m);
     by = pack2(c, c);
@@ -198,6 +199,7 @@ struct Exponents {
     if (!(low < m)) low = m > 0.f ? __uint_as_float(__float_as_uint(m) - 1u) : __uint_as_float(__float_as_uint(m) + 1u);
     floor = 0u;
     deep = true;
+    lowest = kNothing;
     if constexpr (!std::is_same<T, float>::value) {
       float held;  // the floor's value (-inf where the type has none)
       if constexpr (std::is_same<T, __half>::value) {
@@ -209,7 +211,9 @@ struct Exponents {
         floor = (uint32_t)__bfloat16_as_ushort(h) * 0x00010001u;
         held = __bfloat162float(h);
       }
-      deep = !((held - m) * c >= kFurthest);
+      const float d = (held - m) * c;
+      deep = !(d >= kFurthest);
+      if (!deep) lowest = d;
     }
   }
   template <bool kDeep>
@@ -725,7 +729,8 @@ struct RowGrad {
   __device__ __forceinline__ float at(float x) const {
     float d = inf ? (x == m ? 0.f : -INFINITY) : (x - m) * c;
     d = fmaxf(d, kNothing);  // (NaN, -inf: p = 0)
-    return exp2_approx(d) * fmaf(slope, d, first);
+    const float e = exp2_approx(d);
+    return e > 0.f ? e * fmaf(slope, d, first) : 0.f;  // (the factor may be infinite)
   }
 };
 
@@ -772,7 +777,9 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
   Exponents<T> exponents;
   exponents.set(st.x, row.c);
   constexpr bool kDeep = std::is_same<T, float>::value;
-  const bool plain = !none && !row.inf && (kDeep || !exponents.deep);  // (else element by element)
+  // (else element by element: where a factor passes fp32, 0 times it would be NaN)
+  const bool plain = !none && !row.inf && (kDeep || !exponents.deep) &&
+                     fabsf(row.first) + fabsf(row.slope * exponents.lowest) < INFINITY;
   const unsigned long long first2 = pack2(row.first, row.first), slope2 = pack2(row.slope, row.slope);
 
   Bits* out = static_cast<Bits*>(p.grad) + b * p.grad_stride;

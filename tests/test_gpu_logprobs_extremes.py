@@ -1,12 +1,16 @@
-"""GPU tests of the log probabilities on rows with the largest and lowest values of their type, at temperatures down to
-1e-37, against the 64-bit restatement of test_gpu_logprobs (and within its bounds)."""
+"""GPU tests of the log probabilities and their gradient on rows with the largest and lowest values of their type, at
+temperatures down to 1e-37, against the 64-bit restatement of test_gpu_logprobs (and within its bounds).
+
+Beyond those bounds a gradient's weight 2^d below 2^-126 is taken as 0, so a probability may be off by 2^-126 more;
+what rounds past the largest number of the output's type is infinite.
+"""
 import math
 
 import pytest
 import torch
 
 from gsp import logprobs as L
-from test_gpu_logprobs import DTYPES, _check, _error, _logits, _pack
+from test_gpu_logprobs import DTYPES, STEP, _check, _error, _logits, _pack, _reference
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +63,45 @@ def test_entropy_of_tied_largest_values(cuda_device):
             r = L.token_logprobs(x.to(cuda_device), ids, temperature=temperature)
             want = torch.tensor([(VOCAB + 2) // 3, 3, VOCAB], dtype=torch.float64).log()
             assert (r.entropy.double().cpu() - want).abs().max() <= 2 * _error(VOCAB) * (1 + math.log(VOCAB) + 1)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("temperature", [1.0, 0.05, 0.005, 1e-3, 1e-6, 1e-37])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradient(cuda_device, dtype, temperature, masked):
+    x = _rows(dtype)
+    batch = len(x)
+    ids = _ids(batch)
+    legal = torch.ones(x.shape, dtype=torch.bool)
+    mask = None
+    if masked:
+        legal = torch.rand(x.shape, generator=torch.Generator().manual_seed(9)) < 0.6
+        mask = _pack(legal).to(cuda_device)
+    g = torch.Generator().manual_seed(6)
+    gp, gh, gl = torch.randn(batch, 4, generator=g), torch.ones(batch), torch.randn(batch, generator=g)
+    _, entropy, _, _, _, p = _reference(x, ids, temperature, 0, legal)
+    own = torch.zeros_like(p).scatter_add_(1, ids, gp.double())
+    absolute = torch.zeros_like(p).scatter_add_(1, ids, gp.double().abs())
+    lnp = torch.where(p > 0, p.log(), 0.0)
+    there = legal & (x > -math.inf)  # (NaN is not)
+    info, t = torch.finfo(dtype), float(torch.tensor(temperature, dtype=torch.float32))
+    for gh_, gl_ in ((gh.double(), gl.double()), (torch.zeros(batch).double(), torch.zeros(batch).double())):
+        leaf = x.to(cuda_device).requires_grad_(True)
+        r = L.token_logprobs(leaf, ids.to(cuda_device), bitmask_gpu=mask, temperature=temperature)
+        if gh_.any():
+            (grad,) = torch.autograd.grad((r.logprobs, r.entropy, r.logsumexp), leaf,
+                                          [v.to(cuda_device) for v in (gp, gh, gl)])
+        else:  # (the log probabilities' alone)
+            (grad,) = torch.autograd.grad(r.logprobs, leaf, gp.to(cuda_device))
+        got = grad.double().cpu()
+        want = p * (gl_.unsqueeze(1) - gp.double().sum(1, keepdim=True) - gh_.unsqueeze(1) * (lnp + entropy.unsqueeze(1))) + own
+        want = torch.where(there, want, 0.0) / t
+        size = (p + 2.0 ** -126) * (gl_.abs().unsqueeze(1) + gp.double().abs().sum(1, keepdim=True)
+                                    + gh_.unsqueeze(1) * (lnp.abs() + entropy.unsqueeze(1) + 1))
+        flushed = 2.0 ** -126 * (size / (p + 2.0 ** -126))
+        bound = (size * 4 * _error(VOCAB) + flushed + absolute * 8 * STEP) / t + want.abs() * info.eps / 2 + info.tiny * info.eps
+        assert not got.isnan().any()
+        assert (got[~there] == 0).all()
+        past = want.abs() + bound >= info.max  # may have rounded to infinity
+        assert ((got - want).abs() <= bound)[~past].all(), ((got - want).abs() / bound)[~past].max()
+        assert (got * want.sign() >= info.max * (1 - 2 * info.eps))[want.abs() - bound >= info.max].all()

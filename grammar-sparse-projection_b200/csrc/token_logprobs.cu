@@ -774,6 +774,7 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
   row.slope = -gh * kLn2 * share;
   row.inf = st.x == INFINITY;
   const bool none = !(st.x > -INFINITY);
+  const float nothing = st.w != st.w ? st.w : 0.f;  // (a temperature that is not valid: NaN, as the row reports)
   Exponents<T> exponents;
   exponents.set(st.x, row.c);
   constexpr bool kDeep = std::is_same<T, float>::value;
@@ -805,8 +806,8 @@ __global__ void __launch_bounds__(kGradThreads) token_logprobs_grad_kernel(const
 #pragma unroll
       for (int k = 0; k < kPer / 2; ++k) {
         const float2 f = element_pair<T>(x, k);
-        y[2 * k] = none || !(f.x > -INFINITY) ? 0.f : row.at(f.x);
-        y[2 * k + 1] = none || !(f.y > -INFINITY) ? 0.f : row.at(f.y);
+        y[2 * k] = !(f.x > -INFINITY) ? 0.f : none ? nothing : row.at(f.x);
+        y[2 * k + 1] = !(f.y > -INFINITY) ? 0.f : none ? nothing : row.at(f.y);
       }
     }
     const int e0 = i * kPer - r.phase;

@@ -101,8 +101,10 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, *, bitmask_gpu
 
     logprobs, entropy and logsumexp carry gradients to the logits when these
     require them (once; not to the temperature); top_logprobs does not: pass the
-    ids as token_ids for that. Sums are fp32 and in a fixed order, so equal calls
-    give equal bits. Asynchronous on the current stream, capturable.
+    ids as token_ids for that. A token that is not legal counts in them as one of
+    probability 0 (as with logits filled with -inf); a row whose temperature is
+    not valid has NaN on its legal tokens. Sums are fp32 and in a fixed order, so
+    equal calls give equal bits. Asynchronous on the current stream, capturable.
     """
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")

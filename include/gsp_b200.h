@@ -634,8 +634,10 @@ int32_t gsp_token_logprobs_compact(const void* compact_logits, const int64_t* co
  * optional, fp32), with the logits, bitmask and token_ids of the forward call and
  * its stats; p_j the probability of token j:
  *   dx_j = (p_j (gL - sum_k g_k - gH (ln p_j + entropy)) + sum_k g_k [j = t_k]) / T
- * for legal j, 0 elsewhere and in rows without a legal token; negative ids take no
- * part, a token named twice counts twice. Rounded once to dtype. Deterministic. */
+ * for legal j (NaN in a row whose temperature is not positive and finite), 0 elsewhere
+ * and in rows without a legal token; negative ids take no part, every other one counts in
+ * sum_k g_k (one that is not legal as a token of probability 0), a token named twice
+ * counts twice. Rounded once to dtype. Deterministic. */
 int32_t gsp_token_logprobs_grad(const void* logits, int64_t logits_row_stride, int32_t dtype, const int32_t* bitmask,
                                 int64_t bitmask_row_stride, int32_t batch, int32_t vocab, const int64_t* token_ids,
                                 int32_t tokens, const float* stats, const float* grad_logprobs,

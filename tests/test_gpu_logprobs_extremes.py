@@ -105,3 +105,20 @@ def test_gradient(cuda_device, dtype, temperature, masked):
         past = want.abs() + bound >= info.max  # may have rounded to infinity
         assert ((got - want).abs() <= bound)[~past].all(), ((got - want).abs() / bound)[~past].max()
         assert (got * want.sign() >= info.max * (1 - 2 * info.eps))[want.abs() - bound >= info.max].all()
+
+
+def test_gradient_of_rows_whose_temperature_is_not_valid(cuda_device):
+    """NaN like what they report, and 0 on illegal tokens."""
+    x = _logits(1, 5, 300, torch.float32)
+    legal = torch.rand(5, 300, generator=torch.Generator().manual_seed(2)) < 0.5
+    legal[:, 0] = True
+    t = torch.tensor([1.0, 0.0, -1.0, math.nan, math.inf], device=cuda_device)
+    for dtype in DTYPES:
+        leaf = x.to(dtype).to(cuda_device).requires_grad_(True)
+        r = L.token_logprobs(leaf, torch.zeros(5, dtype=torch.int64, device=cuda_device), temperature=t,
+                             bitmask_gpu=_pack(legal).to(cuda_device))
+        for loss in (r.logprobs.sum(), r.entropy.sum()):
+            (grad,) = torch.autograd.grad(loss, leaf, retain_graph=True)
+            grad = grad.cpu()
+            assert torch.isfinite(grad[0]).all() and (grad[~legal] == 0).all()
+            assert grad[1:][legal[1:]].isnan().all()

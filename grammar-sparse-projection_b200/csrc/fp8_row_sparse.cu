@@ -249,7 +249,9 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_row_sparse_kernel(const __gri
         if (lane != r || r >= live) continue;
         const OutBits bits = DTypeTraits<Out>::round_bits(acc[r]);
         if (logits) logits[row[r]] = bits;
-        const unsigned long long key = top1_key(DTypeTraits<Out>::bits_to_float(bits), (uint64_t)(p.vocab_offset + row[r]));
+        const float value = DTypeTraits<Out>::bits_to_float(bits);
+        if (value == -INFINITY) continue;  // (rounded to what illegal tokens have: no key, as on the other routes)
+        const unsigned long long key = top1_key(value, (uint64_t)(p.vocab_offset + row[r]));
         best = key > best ? key : best;
       }
     }

@@ -1,5 +1,5 @@
-"""GPU tests of the fp8 head's top-1 where every legal logit rounds to -inf. Integers and copies of logits: no
-tolerance."""
+"""GPU tests of the fp8 head's top-1 keys and vocabulary offset (a weight that is one row shard of a larger
+vocabulary), and of its top-1 where every legal logit rounds to -inf. Integers and copies of logits: no tolerance."""
 import math
 
 import numpy as np
@@ -14,6 +14,42 @@ from oracle import gsp_oracle as O
 pytestmark = pytest.mark.gpu
 
 DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [(5, 6016, 64), (40, 4000, 30), (200, 4000, 256)])
+def test_shards_merge_to_the_whole(cuda_device, dtype, case):
+    batch, vocab, hidden = case
+    dev, cut = cuda_device, 2048  # whole mask words and blocks
+    g = torch.Generator().manual_seed(vocab)
+    w = (torch.randn(vocab, hidden, generator=g) * 0.02)
+    w[cut:cut + 128] = w[cut - 128:cut] * 8  # the largest logits, the same on both sides of the border
+    w[cut - 128:cut] *= 8
+    weight = F.quantize_weight_fp8(w.to(dev))
+    rows = F.quantize_rows_fp8(torch.randn(batch, hidden, generator=g).to(dev))
+    counts = [vocab // 7] * (batch - 2) + [0, vocab]
+    mask = torch.from_numpy(O.make_batch_mask(np.random.default_rng(vocab), batch, vocab, counts)).to(dev)
+    mask[:batch - 2, (cut - 128) // 32:(cut + 128) // 32] = -1
+    for route in tr.ROUTES:
+        for words in (mask, None):
+            logits, value, token = F.fp8_grammar_logits(rows, weight, words, route=route, out_dtype=dtype)
+            keys, parts = [], []
+            for lo, hi in ((0, cut), (cut, vocab)):
+                key = torch.empty(batch, dtype=torch.int64, device=dev)
+                part = torch.empty(batch, hi - lo, dtype=dtype, device=dev)
+                some = None if words is None else words[:, lo // 32:(hi + 31) // 32].contiguous()
+                _native.fp8_logits(route, rows.values, rows.scales, weight.values[lo:hi],
+                                   weight.scales[lo // 128:(hi + 127) // 128], some, dtype, logits=part, top_key=key,
+                                   vocab_offset=lo)
+                keys.append(key)
+                parts.append(part)
+            assert torch.equal(torch.cat(parts, 1), logits)
+            merged_value = torch.empty(batch, device=dev)
+            merged_token = torch.empty(batch, dtype=torch.int64, device=dev)
+            _native.top1_from_keys(torch.maximum(*keys), merged_value, merged_token)
+            assert torch.equal(merged_value, value) and torch.equal(merged_token, token)
+            assert torch.equal(token.cpu(), logits.float().cpu().argmax(1))
+    assert _native.workspace_error(dev) == 0
 
 
 @pytest.mark.parametrize("batch", [4, 150])

@@ -1125,6 +1125,7 @@ int32_t gsp_int8_error(int32_t* error, const int32_t* set_to, void* stream) {
 namespace {
 
 constexpr int32_t kMaxFp8Hidden = 32768;  // the row-sparse kernel keeps a hidden state in shared memory, in fp32
+constexpr int32_t kMaxFp8Vocab = 1 << 30;  // it counts legal rows, 2,048 at a time, in 32 bits: past 2^31 - 2,048 it would not end
 
 struct Fp8Scratch {
   size_t keys, tickets, values, scales, groups, counts, bits, total;
@@ -1165,6 +1166,7 @@ int32_t gsp_fp8_logits(int32_t route, const void* hidden, int64_t hidden_row_str
   if (st != GSP_OK) return st;
   if (hidden_dim > kMaxFp8Hidden)
     return fail(GSP_ERR_UNSUPPORTED, "%s: hidden_dim above %d", fn, kMaxFp8Hidden);
+  if (vocab > kMaxFp8Vocab) return fail(GSP_ERR_UNSUPPORTED, "%s: vocab above 2^30", fn);
   const int blocks = (hidden_dim + kBlock - 1) / kBlock;
   if (!weight_scales) return fail(GSP_ERR_INVALID_ARGUMENT, "%s: weight_scales is required", fn);
   if (vocab > kBlock && weight_scales_row_stride < blocks)

@@ -31,6 +31,7 @@ __all__ = ["Fp8Rows", "Fp8Weight", "quantize_rows_fp8", "quantize_weight_fp8", "
 
 BLOCK = 128
 MAX_HIDDEN = 32768  # the row-sparse kernel keeps a hidden state in shared memory
+MAX_VOCAB = 2 ** 30  # and counts legal rows in 32 bits
 MAX_COLUMNS = 2 ** 24
 
 
@@ -123,8 +124,8 @@ def _inputs(hidden, weight, bitmask_gpu, out_dtype):
     batch, width = values.shape
     if batch < 1 or vocab < 1 or hidden_dim < 1:
         raise ValueError("hidden and weight must have at least one row and column")
-    if batch >= 2 ** 31 or vocab >= 2 ** 31:  # (the C entries take 32-bit sizes)
-        raise ValueError("hidden and weight may hold up to 2^31 - 1 rows")
+    if batch >= 2 ** 31 or vocab > MAX_VOCAB:  # (the C entries take 32-bit sizes)
+        raise ValueError("hidden may hold up to 2^31 - 1 rows, weight up to 2^30")
     if width != hidden_dim:
         raise ValueError("hidden dimension mismatch")
     if hidden_dim > MAX_HIDDEN:

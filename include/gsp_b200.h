@@ -692,7 +692,7 @@ int32_t gsp_quantize_weight_fp8(const void* src, int64_t src_row_stride, int64_t
  * legal): the plain product, for the positions of a prompt on the dense route.
  * A request whose logits are all -inf, illegal or rounded to it, has top value -inf,
  * index 0 and the lowest key, on every route.
- * hidden_dim <= 32,768. The tensor-core routes want 16-byte aligned rows (hidden_dim a
+ * hidden_dim <= 32,768, vocab <= 2^30. The tensor-core routes want 16-byte aligned rows (hidden_dim a
  * multiple of 16) and, in block mode, vocabularies up to 1,048,576; they run the
  * row-sparse kernel otherwise. scratch: gsp_fp8_scratch_bytes, 16-byte aligned, contents
  * neither read nor preserved, one per concurrent call; it takes the place of a

@@ -126,6 +126,8 @@ def _inputs(hidden, weight, bitmask_gpu, out_dtype):
         raise ValueError("hidden and weight must have at least one row and column")
     if batch >= 2 ** 31 or vocab > MAX_VOCAB:  # (the C entries take 32-bit sizes)
         raise ValueError("hidden may hold up to 2^31 - 1 rows, weight up to 2^30")
+    if batch * ((vocab + 31) // 32 * 32) >= 2 ** 32:
+        raise ValueError("a call may have up to 2^32 - 1 logits (the vocabulary in whole mask words): project in parts")
     if width != hidden_dim:
         raise ValueError("hidden dimension mismatch")
     if hidden_dim > MAX_HIDDEN:
@@ -156,8 +158,9 @@ def fp8_grammar_logits(hidden, weight: Fp8Weight, bitmask_gpu: torch.Tensor | No
     otherwise it defaults to hidden's), as gsp.norm.rms_norm writes them.
     bitmask_gpu None: every token is legal. Returns (logits [B, V] or None,
     top_value float32 [B], top_index int64 [B]); top_index equals
-    logits.argmax(-1), ties to the lowest id. Asynchronous, capturable; each call
-    has scratch of its own.
+    logits.argmax(-1), ties to the lowest id. A call takes up to 2^32 - 1 logits
+    (28,268 positions of 151,936 tokens) of up to 2^30 tokens. No gradient.
+    Asynchronous, capturable; each call has scratch of its own.
     """
     if route not in ROUTES:
         raise ValueError(f"unknown route {route!r}")

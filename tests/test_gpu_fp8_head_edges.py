@@ -1,5 +1,6 @@
 """GPU tests of the fp8 head's top-1 keys and vocabulary offset (a weight that is one row shard of a larger
-vocabulary), and of its top-1 where every legal logit rounds to -inf. Integers and copies of logits: no tolerance."""
+vocabulary), of its top-1 where every legal logit rounds to -inf, and of the number of logits. Integers and copies
+of logits: no tolerance."""
 import math
 
 import numpy as np
@@ -78,3 +79,16 @@ def test_top1_where_legal_logits_round_to_minus_infinity(cuda_device, batch):
         _native.fp8_logits(route, h.half(), None, weight.values, weight.scales, mask, torch.float16, top_key=key)
         found.append(key)
     assert torch.equal(found[0], found[1]) and torch.equal(found[0], found[2])
+
+
+def test_logits_past_the_limit_are_refused(cuda_device):
+    """More than 2^32 - 1 logits, whole mask words counted."""
+    dev = cuda_device
+    h = torch.zeros(65536, 1, device=dev)
+    for vocab in (65536, 65505):
+        weight = F.Fp8Weight(torch.zeros(vocab, 1, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
+                             torch.zeros(512, 1, device=dev))
+        before = torch.cuda.memory_allocated()
+        with pytest.raises(ValueError, match="2\\^32"):
+            F.fp8_grammar_logits(h, weight, None, route="dense-mask")
+        assert torch.cuda.memory_allocated() == before

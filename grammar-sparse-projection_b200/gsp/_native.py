@@ -709,6 +709,27 @@ def raw_stream(index: int) -> int:
     return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
+def rows_meet(a, b) -> bool:
+    """Whether a and b, tensors [N, H] that are contiguous along their rows, have a byte in common."""
+    (a0, na, wa, sa), (b0, nb, wb, sb) = (
+        (t.data_ptr(), t.shape[0], t.shape[1] * t.element_size(), t.stride(0) * t.element_size()) for t in (a, b))
+    if not na or not nb or a0 >= b0 + (nb - 1) * sb + wb or b0 >= a0 + (na - 1) * sa + wa:
+        return False
+    if sa == sb >= max(wa, wb):  # row i + q of b begins (k + q) sa + r bytes past row i of a
+        k, r = divmod(b0 - a0, sa)
+        return (r < wa and -nb < k < na) or (sa - r < wb and -nb < k + 1 < na)
+
+    def run_meets(first, last):  # bytes first .. last - 1: the first row of b that ends past `first`
+        j = max(0, (first - wb - b0) // sb + 1) if sb else 0
+        return j < nb and b0 + j * sb < last
+
+    if na == 1 or sa <= wa:  # no gaps between a's rows
+        return run_meets(a0, a0 + (na - 1) * sa + wa)
+    if nb == 1 or sb <= wb or nb < na:
+        return rows_meet(b, a)
+    return any(run_meets(a0 + i * sa, a0 + i * sa + wa) for i in range(na))
+
+
 @functools.lru_cache(maxsize=1024)
 def _workspace_bytes(batch: int, vocab: int) -> int:
     return int(load().gsp_workspace_bytes(batch, vocab))

@@ -67,6 +67,8 @@ def _quantize(entry, kind, x, out, scale_rows):
         _check_values(out, "out")
         if out.values.shape != x.shape or out.scales.shape != shape or out.values.device != x.device:
             raise ValueError("out must hold [N, H] values and their blocks' scales on x's device")
+        if any(_native.rows_meet(a, b) for a, b in ((x, out[0]), (x, out[1]), (out[0], out[1]))):
+            raise ValueError("out must not overlap x or itself")
     if x.shape[0]:
         _native.quantize_fp8(entry, x, out.values, out.scales)
     return out

@@ -45,8 +45,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
     (quantize_rows_fp8's rule). The 8-bit values are taken from y itself, not from
     its rounding to x's type, so they may differ by a step from a norm followed by
     a quantiser. weight [H] of x's type (None: 1). residual_out: where h goes;
-    may be `residual` itself. No gradient: tensors that require one are refused
-    while gradients are recorded.
+    may be `residual` or `x` itself, but share no part of their memory otherwise.
+    No gradient: tensors that require one are refused while gradients are recorded.
     """
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
@@ -80,6 +80,12 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
             _check_rows(residual_out, rows, "residual_out")
             if count > 1 and residual_out.stride(0) < cols:
                 raise ValueError("residual_out must not overlap itself")
+            for t in (rows, residual):
+                same = residual_out.data_ptr() == t.data_ptr() and (count == 1 or residual_out.stride(0) == t.stride(0))
+                if not same and _native.rows_meet(residual_out, t):
+                    raise ValueError("residual_out may be x or residual, but must not overlap a part of them")
+            if weight is not None and _native.rows_meet(residual_out, weight.unsqueeze(0)):
+                raise ValueError("residual_out must not overlap weight")
     elif residual_out is not None:
         raise ValueError("residual_out without residual")
     dev = x.device

@@ -656,8 +656,9 @@ int32_t gsp_token_logprobs_grad(const void* logits, int64_t logits_row_stride, i
  *                     gsp_quantize_rows_fp8's rule (scales [rows, ceil(cols / 128)],
  *                     row stride in elements): hidden of gsp_fp8_logits.
  * The 8-bit values are taken from y itself, not from its rounding. residual_out may
- * be residual. x's and residual's row strides may be 0; up to 2^24 columns. The
- * reference starts at the hidden states (gsp/triton_runtime.py:61-109). */
+ * be residual or x; otherwise no output overlaps an input or another output. x's and
+ * residual's row strides may be 0; up to 2^24 columns. The reference starts at the
+ * hidden states (gsp/triton_runtime.py:61-109). */
 int32_t gsp_rms_norm(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
                      const void* weight, int64_t rows, int32_t cols, float eps, int32_t dtype, void* residual_out,
                      int64_t residual_out_row_stride, int32_t out_dtype, void* out, int64_t out_row_stride, float* scales,
@@ -673,7 +674,8 @@ int32_t gsp_rms_norm(const void* x, int64_t x_row_stride, const void* residual, 
  *   scale = max |x| / 448 (fp32 division), value = x / scale (fp32 division) to the
  *   nearest e4m3, ties to even.
  * A block of zeros has scale 0; one that holds an infinity or NaN has scale NaN and
- * values 0. gsp_quantize_rows_fp8: blocks of 1 x 128, scales [rows, ceil(cols / 128)];
+ * values 0. Outputs overlap neither src nor one another. gsp_quantize_rows_fp8: blocks of
+ * 1 x 128, scales [rows, ceil(cols / 128)];
  * gsp_quantize_weight_fp8: of 128 x 128, scales [ceil(rows / 128), ceil(cols / 128)]. */
 int32_t gsp_quantize_rows_fp8(const void* src, int64_t src_row_stride, int64_t rows, int32_t cols, int32_t dtype,
                               uint8_t* values, int64_t values_row_stride, float* scales, int64_t scales_row_stride,

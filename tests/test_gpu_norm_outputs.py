@@ -1,0 +1,52 @@
+"""GPU tests of what the norm and the quantisers write into tensors that the caller gives: overlaps that would be read
+after they are written."""
+import pytest
+import torch
+
+from gsp import fp8_head as F
+from gsp import norm
+
+pytestmark = pytest.mark.gpu
+
+
+def test_residual_out_may_be_an_input_but_not_a_part_of_one(cuda_device):
+    n, h = 9, 256
+    buffer = torch.randn(n, 3 * h + 8, generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    x, residual = buffer[:, :h], buffer[:, h:2 * h]
+    want = norm.rms_norm(x.clone(), residual=residual.clone())
+    for out in (residual, x, buffer[:, 2 * h:3 * h]):  # rows between the inputs' rows share no element with them
+        kept = buffer.clone()
+        r = norm.rms_norm(x, residual=residual, residual_out=out)
+        assert r.residual.data_ptr() == out.data_ptr()
+        assert torch.equal(r.residual, want.residual) and torch.equal(r.output, want.output)
+        buffer.copy_(kept)
+    flat = buffer.view(-1)
+    weight = flat[5:5 + h]
+    with pytest.raises(ValueError, match="overlap"):
+        norm.rms_norm(torch.zeros(n, h, device=cuda_device), weight, residual=torch.zeros(n, h, device=cuda_device),
+                      residual_out=flat[:n * h].view(n, h))
+    for out in (buffer[:, 8:h + 8], buffer[:, h - 1:2 * h - 1], flat[:n * h].view(n, h), flat[h:h + n * h].view(n, h),
+                flat[1:1 + n * (2 * h)].view(n, 2 * h)[:, :h]):
+        with pytest.raises(ValueError, match="overlap"):
+            norm.rms_norm(x, residual=residual, residual_out=out)
+    one = torch.zeros(2 * h, device=cuda_device)
+    with pytest.raises(ValueError, match="overlap"):
+        norm.rms_norm(one[:h], residual=one[h:], residual_out=one[1:h + 1])
+    norm.rms_norm(one[:h], residual=one[h:], residual_out=one[:h])
+    norm.rms_norm(one.view(2, h)[:1], residual=one.view(2, h)[1:], residual_out=one.view(1, 2 * h)[:, :h])
+    assert torch.equal(buffer, kept)
+
+
+def test_quantised_outputs_must_not_overlap(cuda_device):
+    n, h = 64, 256
+    raw = torch.zeros(4 * n * h, dtype=torch.uint8, device=cuda_device)
+    x = raw[:2 * n * h].view(torch.float16).view(n, h)
+    values = torch.empty(n, h, dtype=torch.float8_e4m3fn, device=cuda_device)
+    scales = torch.empty(n, 2, device=cuda_device)
+    inside = raw[n * h:2 * n * h].view(torch.float8_e4m3fn).view(n, h)
+    beside = raw[2 * n * h:3 * n * h].view(torch.float8_e4m3fn).view(n, h)
+    for bad in (F.Fp8Rows(inside, scales), F.Fp8Rows(values, raw[:n * 8].view(torch.float32).view(n, 2)),
+                F.Fp8Rows(beside, raw[2 * n * h:2 * n * h + n * 8].view(torch.float32).view(n, 2))):
+        with pytest.raises(ValueError, match="overlap"):
+            F.quantize_rows_fp8(x, out=bad)
+    F.quantize_rows_fp8(x, out=F.Fp8Rows(beside, scales))

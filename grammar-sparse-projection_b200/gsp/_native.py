@@ -730,6 +730,14 @@ def rows_meet(a, b) -> bool:
     return any(run_meets(a0 + i * sa, a0 + i * sa + wa) for i in range(na))
 
 
+def written(*tensors) -> None:
+    """Raises the versions of tensors given by the caller that a kernel has written, so that an autograd graph which
+    saved one refuses its changed values."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 @functools.lru_cache(maxsize=1024)
 def _workspace_bytes(batch: int, vocab: int) -> int:
     return int(load().gsp_workspace_bytes(batch, vocab))

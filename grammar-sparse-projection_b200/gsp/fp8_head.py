@@ -60,7 +60,8 @@ def _quantize(entry, kind, x, out, scale_rows):
         raise ValueError("x may hold up to 2^31 - 1 rows of 2^24 columns")
     _native.dtype_code(x.dtype)
     shape = (scale_rows, _blocks(x.shape[1]))
-    if out is None:
+    given = out is not None
+    if not given:
         out = kind(torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device),
                    torch.empty(shape, dtype=torch.float32, device=x.device))
     else:
@@ -71,6 +72,8 @@ def _quantize(entry, kind, x, out, scale_rows):
             raise ValueError("out must not overlap x or itself")
     if x.shape[0]:
         _native.quantize_fp8(entry, x, out.values, out.scales)
+        if given:
+            _native.written(*out)
     return out
 
 

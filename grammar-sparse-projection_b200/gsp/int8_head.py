@@ -59,7 +59,8 @@ def quantize_rows_int8(x: torch.Tensor, *, out: QuantizedRows | None = None,
     if x.shape[0] >= 2 ** 31 or x.shape[1] > 2 ** 30:  # (the C entries take 32-bit sizes)
         raise ValueError("x may hold up to 2^31 - 1 rows of 2^30 columns")
     _native.dtype_code(x.dtype)
-    if out is None:
+    given = out is not None
+    if not given:
         device = x.device
         out = QuantizedRows(torch.empty(x.shape, dtype=torch.int8, device=device),
                             torch.empty(x.shape[0], dtype=torch.float32, device=device))
@@ -69,6 +70,8 @@ def quantize_rows_int8(x: torch.Tensor, *, out: QuantizedRows | None = None,
             raise ValueError("out must hold [N, H] values on x's device")
     if x.shape[0]:
         _native.quantize_rows_int8(x, out.values, out.scales, reciprocal)
+        if given:
+            _native.written(*out)
     return out
 
 

@@ -68,12 +68,14 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
     if not 0.0 <= eps < float("inf"):
         raise ValueError("eps must be finite and not negative")
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+                                    or (residual is not None and residual.requires_grad)
+                                    or (residual_out is not None and residual_out.requires_grad)):
         raise ValueError("rms_norm has no gradient: call it without tensors that require one, or under torch.no_grad()")
     if residual is not None:
         residual = residual.unsqueeze(0) if one_row and residual.dim() == 1 else residual
         _check_rows(residual, rows, "residual")
-        if residual_out is None:
+        given = residual_out is not None
+        if not given:
             residual_out = torch.empty(rows.shape, dtype=x.dtype, device=x.device)
         else:
             residual_out = residual_out.unsqueeze(0) if one_row and residual_out.dim() == 1 else residual_out
@@ -101,4 +103,6 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
         output, code = Fp8Rows(values, scales), _native.DTYPE_E4M3
     if count:
         _native.rms_norm(rows, weight, residual, eps, residual_out, values, scales, code)
+        if residual is not None and given:
+            _native.written(residual_out)
     return NormResult(output, residual_out[0] if residual_out is not None and one_row else residual_out)

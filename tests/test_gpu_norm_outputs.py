@@ -1,9 +1,10 @@
 """GPU tests of what the norm and the quantisers write into tensors that the caller gives: overlaps that would be read
-after they are written."""
+after they are written, and the tensors' versions, which autograd goes by."""
 import pytest
 import torch
 
 from gsp import fp8_head as F
+from gsp import int8_head as I
 from gsp import norm
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +51,26 @@ def test_quantised_outputs_must_not_overlap(cuda_device):
         with pytest.raises(ValueError, match="overlap"):
             F.quantize_rows_fp8(x, out=bad)
     F.quantize_rows_fp8(x, out=F.Fp8Rows(beside, scales))
+
+
+def test_versions_of_written_tensors(cuda_device):
+    """A graph that saved a tensor which a call writes into refuses to go backward with the changed values."""
+    x = torch.randn(4, 256, device=cuda_device)
+    leaf = torch.randn(4, 256, device=cuda_device, requires_grad=True)
+    stream = leaf * 2
+    loss = (stream * stream).sum()  # saves the stream
+    with torch.no_grad():
+        norm.rms_norm(x, residual=stream, residual_out=stream)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    for quantise in (F.quantize_rows_fp8, F.quantize_weight_fp8, I.quantize_rows_int8):
+        out = quantise(x)
+        before = [t._version for t in out]
+        quantise(x, out=out)
+        assert all(t._version > v for t, v in zip(out, before))
+    with torch.inference_mode():  # (tensors without a version)
+        stream = torch.randn(4, 256, device=cuda_device)
+        norm.rms_norm(x, residual=stream, residual_out=stream)
+        F.quantize_rows_fp8(x, out=F.quantize_rows_fp8(x))
+    with pytest.raises(ValueError, match="gradient"):
+        norm.rms_norm(x, residual=x, residual_out=leaf * 2)

@@ -12,6 +12,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libgsp_b200.so")
@@ -728,6 +729,13 @@ def rows_meet(a, b) -> bool:
     if nb == 1 or sb <= wb or nb < na:
         return rows_meet(b, a)
     return any(run_meets(a0 + i * sa, a0 + i * sa + wa) for i in range(na))
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether one of the tensors (or None) carries a tangent of torch's forward-mode differentiation."""
+    if forward_ad._current_level < 0:  # (outside every dual_level, as nearly always)
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def written(*tensors) -> None:

@@ -48,7 +48,7 @@ def _check_tokens(token_ids, batch, device, temperature, top_n) -> int:
         if (temperature.device != device or temperature.dtype != torch.float32 or temperature.shape != (batch,)
                 or not temperature.is_contiguous()):
             raise ValueError("temperature must be a number or a contiguous float32 tensor with one value per request")
-        if temperature.requires_grad and torch.is_grad_enabled():
+        if (temperature.requires_grad and torch.is_grad_enabled()) or _native.has_tangent(temperature):
             raise ValueError("there is no gradient of the temperature")
     elif not 0.0 < temperature < float("inf"):
         raise ValueError("temperature must be positive and finite")
@@ -100,7 +100,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, *, bitmask_gpu
     lowest id. A row without a legal token reports -inf, entropy 0, ids -1.
 
     logprobs, entropy and logsumexp carry gradients to the logits when these
-    require them (once; not to the temperature); top_logprobs does not: pass the
+    require them (backward, once; not to the temperature); top_logprobs does not: pass the
     ids as token_ids for that. A token that is not legal counts in them as one of
     probability 0 (as with logits filled with -inf); a row whose temperature is
     not valid has NaN on its legal tokens. Sums are fp32 and in a fixed order, so
@@ -117,6 +117,8 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, *, bitmask_gpu
     if vocab > 1 and rows.stride(1) != 1:
         raise ValueError("logits must be contiguous along the vocabulary")
     _native.dtype_code(rows.dtype)
+    if _native.has_tangent(rows):
+        raise ValueError("there is no forward-mode gradient")
     tokens = _check_tokens(token_ids, batch, rows.device, temperature, top_n)
     mask = bitmask_gpu
     if mask is not None:
@@ -146,7 +148,7 @@ def compact_token_logprobs(packed_ids: torch.Tensor, logits: torch.Tensor, offse
     read, whatever the offsets say. No gradient: the packed projections have none."""
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
-    if logits.requires_grad and torch.is_grad_enabled():
+    if (logits.requires_grad and torch.is_grad_enabled()) or _native.has_tangent(logits):
         raise ValueError("packed logits have no gradient: take token_logprobs on vocabulary-shaped ones")
     if logits.dim() != 1 or packed_ids.shape != logits.shape:
         raise ValueError("packed_ids and logits must have shape [N]")

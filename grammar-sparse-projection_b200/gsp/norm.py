@@ -46,7 +46,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
     its rounding to x's type, so they may differ by a step from a norm followed by
     a quantiser. weight [H] of x's type (None: 1). residual_out: where h goes;
     may be `residual` or `x` itself, but share no part of their memory otherwise.
-    No gradient: tensors that require one are refused while gradients are recorded.
+    No gradient: tensors that require one are refused while gradients are recorded,
+    and those with a forward-mode tangent.
     """
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
@@ -71,6 +72,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, *, residual: t
                                     or (residual is not None and residual.requires_grad)
                                     or (residual_out is not None and residual_out.requires_grad)):
         raise ValueError("rms_norm has no gradient: call it without tensors that require one, or under torch.no_grad()")
+    if _native.has_tangent(x, weight, residual):
+        raise ValueError("rms_norm has no forward-mode gradient")
     if residual is not None:
         residual = residual.unsqueeze(0) if one_row and residual.dim() == 1 else residual
         _check_rows(residual, rows, "residual")

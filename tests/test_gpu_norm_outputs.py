@@ -1,10 +1,12 @@
 """GPU tests of what the norm and the quantisers write into tensors that the caller gives: overlaps that would be read
-after they are written, and the tensors' versions, which autograd goes by."""
+after they are written, and the tensors' versions, which autograd goes by. And that forward-mode gradients, which the norm and
+the log probabilities do not have, are refused."""
 import pytest
 import torch
 
 from gsp import fp8_head as F
 from gsp import int8_head as I
+from gsp import logprobs as L
 from gsp import norm
 
 pytestmark = pytest.mark.gpu
@@ -74,3 +76,18 @@ def test_versions_of_written_tensors(cuda_device):
         F.quantize_rows_fp8(x, out=F.quantize_rows_fp8(x))
     with pytest.raises(ValueError, match="gradient"):
         norm.rms_norm(x, residual=x, residual_out=leaf * 2)
+
+
+def test_forward_mode_gradients_are_refused(cuda_device):
+    x = torch.randn(2, 64, device=cuda_device)
+    ids = torch.zeros(2, dtype=torch.int64, device=cuda_device)
+    offsets = torch.tensor([0, 30, 64], device=cuda_device)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: norm.rms_norm(dual), lambda: norm.rms_norm(x, dual[0]), lambda: norm.rms_norm(x, residual=dual),
+                     lambda: L.token_logprobs(dual, ids), lambda: L.compact_token_logprobs(torch.arange(64, device=cuda_device), dual[0], offsets, ids),
+                     lambda: L.token_logprobs(x, ids, temperature=dual[0, :2])):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+        norm.rms_norm(x)  # (no dual among its tensors)
+        L.token_logprobs(x, ids)

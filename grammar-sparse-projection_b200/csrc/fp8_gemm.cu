@@ -29,8 +29,12 @@
 // before their first accumulator.
 //
 // Measured (device, the prologue included): 64 x 151,936 x 1,024 bf16 48 us (floor 27),
-// 128 x 262,144 x 8,192 402-427 us (343), 32 requests x 248,320 x 2,048 at 5% in runs 105 us
-// (66), 2,048 positions x 151,936 x 1,024 515-650 us (by bytes 121, by e4m3 products 191).
+// 32 requests x 248,320 x 2,048 at 5% in runs 105 us (66), 128 x 262,144 x 8,192 384-434 us on
+// one state, 495-536 in turn over several (343: power and L2), 2,048 positions x 151,936 x
+// 1,024 512-534 us eagerly on one state, 558-575 over several, 565-822 recorded in graphs (by
+// bytes 121, by e4m3 products 191). Rows of logits that are not whole 32-byte sectors are
+// stored an element at a time: 64 x 50,257 x 1,024 49 us, 50,272 20; 1,376 x 81,758 x 256 fp16
+// 1,148 us, 81,760 118.
 // Copies and tensor cores alone, without the epilogue, take 30, 334 and 240 us of these:
 // what bounds the kernel is the epilogue warps' time a stage, 870 clocks for 128 columns
 // (TMEM loads 100, the sums 265, scales and barriers the rest), and a tile's rounding and
@@ -64,7 +68,7 @@ constexpr int kGemmThreads = 32 * (4 + kEpilogueWarps);  // (two of the first fo
 constexpr int kFewRegisters = 56, kManyRegisters = 224;
 constexpr int kMaxStages = 10;
 constexpr int kMaxAcc = 4;
-constexpr int kMaxBuilders = 256;  // prefix sums that fit the CTA's table: 2^20 tokens; past it they are searched in global memory
+constexpr int kMaxBuilders = 256;  // prefix sums that fit the CTA's table: 2^20 tokens; past it the row-sparse kernel takes the block route
 
 constexpr int kAhead = 2, kScaleRing = 4;  // vectors of four scales that a thread loads ahead, and keeps
 

@@ -149,14 +149,6 @@ int32_t status(const char* fn, cudaError_t err) {
 }
 
 }  // namespace
-
-cudaError_t launch_quantize_rows_fp8(const void* src, int64_t src_stride, int64_t rows, int cols, int dtype,
-                                     uint8_t* values, int64_t values_stride, float* scales, int64_t scales_stride,
-                                     cudaStream_t stream) {
-  auto launch = dtype == 2 ? launch_rows<float> : dtype == 1 ? launch_rows<__nv_bfloat16> : launch_rows<__half>;
-  return launch(src, src_stride, rows, cols, values, values_stride, scales, scales_stride, stream);
-}
-
 }  // namespace gsp
 
 using namespace gsp;
@@ -169,8 +161,9 @@ int32_t gsp_quantize_rows_fp8(const void* src, int64_t src_row_stride, int64_t r
   const char* fn = "gsp_quantize_rows_fp8";
   const int32_t st = check(fn, src, src_row_stride, rows, cols, dtype, values, values_row_stride, scales, scales_row_stride);
   if (st != GSP_OK || rows == 0) return st;
-  return status(fn, launch_quantize_rows_fp8(src, src_row_stride, rows, cols, dtype, values, values_row_stride, scales,
-                                             scales_row_stride, static_cast<cudaStream_t>(stream)));
+  auto launch = dtype == 2 ? launch_rows<float> : dtype == 1 ? launch_rows<__nv_bfloat16> : launch_rows<__half>;
+  return status(fn, launch(src, src_row_stride, rows, cols, values, values_row_stride, scales, scales_row_stride,
+                           static_cast<cudaStream_t>(stream)));
 }
 
 int32_t gsp_quantize_weight_fp8(const void* src, int64_t src_row_stride, int64_t rows, int32_t cols, int32_t dtype,

@@ -244,11 +244,6 @@ cudaError_t launch_quantize_rows_int8(const void* src, int64_t src_stride, int64
                                       bool by_product, int8_t* values, int64_t values_stride, float* scales,
                                       cudaStream_t stream);
 
-// Rows of `src` (dtype 0 fp16, 1 bf16, 2 fp32) to e4m3 values and a scale per 128 columns.
-cudaError_t launch_quantize_rows_fp8(const void* src, int64_t src_stride, int64_t rows, int cols, int dtype,
-                                     uint8_t* values, int64_t values_stride, float* scales, int64_t scales_stride,
-                                     cudaStream_t stream);
-
 // ---- sampling with temperature, top-k, min-p and top-p (filtered_sample.cu) --
 struct FilteredSampleParams {
   const void* logits;

@@ -221,8 +221,8 @@ cudaError_t launch_norm(NormParams p, cudaStream_t stream) {
   const cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   constexpr int kE = Units<T, kVec>::kElems;
-  // Warps per row: 8 values a thread, from 8,192 columns on 16 and 32: a row is soon done,
-  // and most of the SM's threads are resident. Rows of few warps share a CTA.
+  // Warps per row: 8 values a thread, past 4,096 columns 16, past 8,192 32: a row is soon
+  // done, and most of the SM's threads are resident. Rows of few warps share a CTA.
   const int64_t units = kVec ? p.cols / kE : ((int64_t)p.cols + kBlock - 1) / kBlock * 32;
   int gw = 1;
   while (gw < 16 && units * kE > (int64_t)32 * gw * 8) gw *= 2;

@@ -25,13 +25,16 @@
 // counting each time the row read has doubled; a list that overflows (rows in rising
 // order, equal values) is made again with a barrier for every vector: time, not results.
 //
-// Measured (device): 1,999 x 151,936 bf16, four tokens a row, 132 us (4.6 TB/s, 71% of
-// measured; a thread issues about 12 instructions an element, 70% of what an SM can);
-// 128 x 248,320 bf16 with masks and five alternatives 42 us (floor 10.5: 16 instructions
-// an element, and 40 of 148 SMs have half the work of the others); one row of 248,320 with
-// 20 alternatives 14 us, 7 of them the alternatives' rankings and barriers.
+// Measured (device): 1,999 x 151,936 bf16, four tokens a row, 132-135 us (4.5 TB/s, 70% of
+// measured; issue slots 65% busy, the exponentials' pipe 54%, the rest waits for loads);
+// 128 x 248,320 bf16 with masks and five alternatives 42 us (floor 10.5: issue slots 44%
+// busy; what waits, waits for loads and, a third as often, at the rankings' barriers; 40 of
+// 148 SMs have half the work of the others); one row of 248,320 with 20 alternatives 14 us,
+// 7 of them the alternatives' rankings and barriers.
 //
-// Sums run in fp32: a thread adds at most a few hundred terms, then a tree.
+// Sums run in fp32: a thread adds a row's terms over 512 (CTAs of 256 threads) or over 1,024
+// times the row's CTAs in each of two sums, 300 at 151,936 tokens and 131,072 at 2^30, then
+// a tree.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -144,8 +144,8 @@ def compact_token_logprobs(packed_ids: torch.Tensor, logits: torch.Tensor, offse
     offsets int64 [B+1]) as bitmask_compact_logits and int8_compact_logits return
     them, ids rising in a row; token_ids are vocabulary ids, and so are the
     alternatives'. max_len, the longest row expected (default: twice the mean),
-    only picks the launch shape. Positions past the end of the arrays are not
-    read, whatever the offsets say. No gradient: the packed projections have none."""
+    only picks the launch shape. Positions past the end of the arrays, or past a
+    row's 2^30th, are not read, whatever the offsets say. No gradient: the packed projections have none."""
     if not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor")
     if (logits.requires_grad and torch.is_grad_enabled()) or _native.has_tangent(logits):

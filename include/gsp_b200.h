@@ -616,7 +616,7 @@ int32_t gsp_sample_compact(const void* compact_logits, const int64_t* compact_id
  * value per request; a request whose value is not positive and finite reports NaN
  * and ids -1. Row strides may be 0 (one row for all). No workspace.
  * gsp_token_logprobs_compact: rows packed as for gsp_sample_compact, ids rising in a
- * row. No counterpart in the reference, whose loop takes the argmax alone
+ * row, up to 2^30 of them. No counterpart in the reference, whose loop takes the argmax alone
  * (benchmarks/qwen35_adaptive_paired.py:94). */
 int32_t gsp_token_logprobs(const void* logits, int64_t logits_row_stride, int32_t dtype, const int32_t* bitmask,
                            int64_t bitmask_row_stride, int32_t batch, int32_t vocab, float temperature,

@@ -397,7 +397,8 @@ __device__ __forceinline__ bool valid_temperature(float t) { return t > 0.f && t
 __device__ __forceinline__ float logprob_of(float x, float m, float t, float log_s) {
   if (!(x > -INFINITY)) return -INFINITY;  // (NaN too)
   if (x == m) return -log_s;
-  return __fdiv_rn(x - m, t) - log_s;  // (m infinite: -inf)
+  if (m - x == INFINITY) return 2.f * __fdiv_rn(0.5f * x - 0.5f * m, t) - log_s;  // (the lowest value beside the largest)
+  return __fdiv_rn(x - m, t) - log_s;
 }
 
 template <typename T, bool kMask, bool kTop, int kThreads>

@@ -54,6 +54,17 @@ def test_forward(cuda_device, dtype, temperature, masked):
     _check(r, x, ids, temperature, 5, legal)
 
 
+@pytest.mark.parametrize("temperature", [1.5, 5.0, 1e3, 1e30])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lowest_beside_largest_values_at_high_temperatures(cuda_device, dtype, temperature):
+    """A difference that passes fp32 before it is divided, and not afterwards."""
+    x = _rows(dtype)
+    ids = _ids(len(x))
+    ids[:, 1] = 1  # (the lowest value of the first row)
+    r = L.token_logprobs(x.to(cuda_device), ids.to(cuda_device), temperature=temperature, top_n=5)
+    _check(r, x, ids, temperature, 5)
+
+
 def test_entropy_of_tied_largest_values(cuda_device):
     """ln of their number, however large they are and however low the temperature."""
     for dtype in DTYPES:
